@@ -98,6 +98,24 @@ class DecodeArgs(C.Structure):
                 ("workspace", C.c_void_p), ("workspace_bytes", C.c_size_t)]
 
 
+I64x2 = C.c_int64 * 2
+
+
+class PackedAttnArgs(C.Structure):
+    _fields_ = [(name, C.c_void_p) for name in ("q", "k", "v", "o", "cu_seqlens", "sink", "stat", "o_rest")] + \
+               [(name, C.c_int) for name in ("sequences", "tokens", "H", "Hkv", "D", "n")] + \
+               [("c", C.c_float), ("zero_tail", C.c_int), ("q_stride", I64x2), ("k_stride", I64x2), ("v_stride", I64x2),
+                ("o_stride", I64x2), ("workspace", C.c_void_p), ("workspace_bytes", C.c_size_t), ("status", C.c_void_p)]
+
+
+class PagedAttnArgs(C.Structure):
+    _fields_ = [(name, C.c_void_p) for name in ("q", "k_pages", "v_pages", "o", "block_table", "kv_lens", "cu_seqlens", "sink")] + \
+               [(name, C.c_int) for name in ("sequences", "tokens", "H", "Hkv", "D", "pages", "page_size", "table_width", "n")] + \
+               [("c", C.c_float), ("zero_tail", C.c_int), ("table_stride", C.c_int64), ("q_stride", I64x2), ("k_stride", I64x3),
+                ("v_stride", I64x3), ("o_stride", I64x2), ("workspace", C.c_void_p), ("workspace_bytes", C.c_size_t),
+                ("status", C.c_void_p)]
+
+
 class HeadArgs(C.Structure):
     _fields_ = [("h", C.c_void_p), ("e", C.c_void_p), ("targets", C.c_void_p), ("l_out", C.c_void_p),
                 ("zt_out", C.c_void_p), ("N", C.c_int), ("d", C.c_int), ("V_local", C.c_int),
@@ -135,6 +153,10 @@ SYMBOLS = {
     "alg_decode_workspace_bytes": (C.c_size_t, [C.POINTER(DecodeArgs)]),
     "alg_attn_decode": (C.c_int, [C.POINTER(DecodeArgs), C.c_void_p]),
     "alg_attn_decode_status": (C.c_int, [C.POINTER(DecodeArgs), C.c_void_p, C.c_void_p]),
+    "alg_packed_attn_workspace_bytes": (C.c_size_t, [C.POINTER(PackedAttnArgs)]),
+    "alg_packed_attn_fwd": (C.c_int, [C.POINTER(PackedAttnArgs), C.c_void_p]),
+    "alg_paged_attn_workspace_bytes": (C.c_size_t, [C.POINTER(PagedAttnArgs)]),
+    "alg_paged_attn_fwd": (C.c_int, [C.POINTER(PagedAttnArgs), C.c_void_p]),
     "alg_head_workspace_bytes": (C.c_size_t, [C.POINTER(HeadArgs)]),
     "alg_head_fwd": (C.c_int, [C.POINTER(HeadArgs), C.c_void_p]),
     "alg_head_fwd_static": (C.c_int, [C.POINTER(HeadArgs), C.c_void_p]),

@@ -1,0 +1,110 @@
+// Attention over sequences of different lengths: what the plan, the kernels and the C entry points share.
+//
+// Queries lie packed, (tokens, heads, D), sequence s in rows [cu[s], cu[s + 1]); keys and values lie packed beside them or in the
+// pages of a cache.  G = H / Hkv query heads share a key head, and a 128-row query tile holds G heads of 128 / G
+// consecutive tokens, row r = token r / G, head r % G, so that a tile's K and V tiles serve the whole group and a chunk of a
+// few tokens still fills rows.  Token i of the Lq at the end of a sequence of Lk keys sees keys [0, i + Lk - Lq].
+//
+// Lengths are device memory, which the host never reads: a plan kernel ahead of the attention turns them into a list of work items,
+// longest first, which the persistent CTAs of the attention kernel take from a counter.  What the lengths say is
+// clamped to the tensors' extents, so that no value in them leads outside.
+#pragma once
+
+#include "common.cuh"
+
+namespace alg {
+
+struct RaggedSeqs {
+  const int* cu;            // (S + 1), or nullptr: one token a sequence
+  const int* kv_lens;       // (S), or nullptr: keys lie packed like the queries, Lk = Lq
+  int S, tokens;            // tokens: rows of the packed tensors
+  int kv_capacity;          // no sequence has more keys than this
+};
+
+// first row and number of the sequence's packed rows, number of its keys
+__device__ __forceinline__ void ragged_lengths(const RaggedSeqs& q, int s, int& row0, int& Lq, int& Lk) {
+  if (q.cu != nullptr) {
+    row0 = min(max(__ldg(q.cu + s), 0), q.tokens);
+    Lq = min(max(__ldg(q.cu + s + 1), row0), q.tokens) - row0;
+  } else {
+    row0 = s;
+    Lq = 1;
+  }
+  Lk = q.kv_lens != nullptr ? min(max(__ldg(q.kv_lens + s), 0), q.kv_capacity) : Lq;
+}
+
+// 128-key tiles that the tokens up to `end` (exclusive, of this sequence) see: one at least, so that a token that sees nothing
+// still has an item that writes its row
+__device__ __forceinline__ int ragged_tiles(int Lq, int Lk, int end) {
+  const int visible = Lk - Lq + min(end, Lq);
+  return visible > 0 ? (visible + 127) >> 7 : 1;
+}
+
+struct __align__(16) RaggedItem {
+  int row0, Lq, Lk, seq;    // the sequence
+  int t0;                   // first token of the block, counted in the sequence
+  int k0, nk;               // key tiles [k0, k0 + nk)
+  int slot;                 // < 0: the whole item; else this part's slot (times Hkv, plus the head)
+};
+struct __align__(16) RaggedCombo {   // an item that is cut along the keys, for the kernel that adds its parts up
+  int row0, Lq, Lk, t0;
+  int slot, parts, pad0, pad1;
+};
+struct __align__(16) RaggedHeader {
+  int items, combos;        // entries of the lists
+  int counter;              // next (item, head) to be taken
+  int pad;
+};
+
+// Workspace of a forward call: header | items | combos | prefix of the sequences' blocks | slots.
+struct RaggedPlan {
+  RaggedHeader* header;
+  RaggedItem* items;
+  RaggedCombo* combos;
+  int* prefix;              // (S + 1)
+  float* slots;             // parts' accumulators, (slot, head, 256 rows, D + 4)
+  int max_items, max_combos, max_slots;   // slots: of one head
+  int block_tokens;         // tokens of an item: two tiles of 128 / G
+  int heads;                // Hkv
+  int sms;
+};
+
+// A list of (sequence, 128-row block), longest first, for the backward kernels: [0, n) by the queries ahead of a key block,
+// [n, 2 n) by the keys behind a query block.
+struct RaggedBlocks {
+  RaggedHeader* header;     // items: entries of each list
+  int4* list;               // (row0, L, first row of the block, sequence)
+  int* prefix;
+  int max_items;
+};
+
+struct Strides2 { int64_t t, h; };
+
+struct RaggedParams {
+  RaggedSeqs seqs;
+  RaggedPlan plan;
+  const void* q;
+  const void* k;            // (tokens, Hkv, D) packed, or the pages
+  const void* v;
+  void* o;
+  void* o_lo;               // what the rounding to o left over, dense (tokens, H, D), or nullptr
+  float* stat;              // (H, tokens): a with p = (rho(x) a)^n, or nullptr
+  const float* sink;
+  Strides2 qs, ks, vs, os;
+  int64_t k_page, v_page;   // page strides (paged)
+  const int* table;         // (S, table_width) page numbers, or nullptr: packed keys
+  int64_t table_stride;
+  int table_width, page, log2_page, pages;
+  int H, Hkv, G, D, log2n;
+  int tile_tokens;          // 128 / G
+  float scale, inv_c;
+  int zero_tail;            // rows of no sequence are written as zeros
+  int* status;
+};
+
+size_t ragged_plan_bytes(int S, int tokens, int Hkv, int G, int D, bool may_split);
+void ragged_plan_carve(RaggedPlan* plan, void* workspace, int S, int tokens, int Hkv, int G, int D, bool may_split);
+int launch_ragged_plan(const RaggedSeqs& seqs, const RaggedPlan& plan, int G, cudaStream_t stream);
+int launch_ragged_attention(const RaggedParams& p, cudaStream_t stream);
+
+}  // namespace alg

@@ -1,0 +1,149 @@
+// C entry points of the attention over packed sequences and paged caches: argument checks, workspace, kernel choice.
+#include <limits.h>
+#include <math.h>
+
+#include "common.cuh"
+#include "launchers.h"
+#include "ragged.cuh"
+
+namespace alg {
+namespace {
+
+bool aligned16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15) == 0; }
+
+// Rows of `count` vectors must start on 16-byte boundaries, apart from one another; a single one may have any stride, which is
+// replaced by one the copies accept.
+bool stride_ok(int64_t* s, int64_t count, int64_t dense) {
+  if (count <= 1) { *s = dense; return true; }
+  return *s > 0 && *s % 8 == 0 && *s < (int64_t(1) << 38);
+}
+bool strides_ok(Strides2* s, const int64_t given[2], int64_t rows, int64_t heads, int D) {
+  *s = {given[0], given[1]};
+  return stride_ok(&s->t, rows, int64_t(heads) * D) && stride_ok(&s->h, heads, D);
+}
+
+int check_link(const char* what, int H, int Hkv, int D, int n, float c) {
+  if (D != 64 && D != 128) { set_error("%s: head_dim must be 64 or 128, got %d", what, D); return ALG_ERR_UNSUPPORTED; }
+  if (n < 2 || n > 32 || ilog2_exact(n) < 0) { set_error("%s: n must be a power of two in [2, 32], got %d", what, n); return ALG_ERR_INVALID; }
+  if (!(c > 0.0f) || !isfinite(c)) { set_error("%s: scale c must be positive and finite", what); return ALG_ERR_INVALID; }
+  if (H < 1 || Hkv < 1 || H % Hkv != 0 || H / Hkv > 128) {
+    set_error("%s: query heads must be a multiple of the key heads, up to 128 times as many (got %d and %d)", what, H, Hkv);
+    return ALG_ERR_INVALID;
+  }
+  return ALG_OK;
+}
+
+// Items are cut along the keys only where that can pay: keys for at least two parts, and blocks too few to keep every CTA busy.
+bool may_split(int64_t keys, int tokens, int H, int Hkv) {
+  const int64_t blocks = tokens / (2 * (128 / (H / Hkv))) + 1;
+  return keys > 16 * 128 && blocks * Hkv < int64_t(8) * sm_count();
+}
+
+}  // namespace
+}  // namespace alg
+
+using namespace alg;
+
+extern "C" {
+
+size_t alg_packed_attn_workspace_bytes(const alg_packed_attn_args* a) {
+  if (a == nullptr || a->H < 1 || a->Hkv < 1 || a->H % a->Hkv != 0 || a->H / a->Hkv > 128 || a->tokens < 0 || a->sequences < 0) return 0;
+  return ragged_plan_bytes(a->sequences, a->tokens, a->Hkv, a->H / a->Hkv, a->D, may_split(a->tokens, a->tokens, a->H, a->Hkv));
+}
+
+int alg_packed_attn_fwd(const alg_packed_attn_args* a, void* stream_) {
+  cudaStream_t stream = static_cast<cudaStream_t>(stream_);
+  if (a == nullptr || a->q == nullptr || a->k == nullptr || a->v == nullptr || a->o == nullptr || a->cu_seqlens == nullptr) {
+    set_error("packed attention: null tensor argument");
+    return ALG_ERR_INVALID;
+  }
+  if (int rc = check_link("packed attention", a->H, a->Hkv, a->D, a->n, a->c)) return rc;
+  if (a->tokens < 0 || a->sequences < 0) { set_error("packed attention: negative extent"); return ALG_ERR_INVALID; }
+  if ((a->stat == nullptr) != (a->o_rest == nullptr)) { set_error("packed attention: stat and o_rest come as a pair"); return ALG_ERR_INVALID; }
+  RaggedParams p{};
+  if (!strides_ok(&p.qs, a->q_stride, a->tokens, a->H, a->D) || !strides_ok(&p.ks, a->k_stride, a->tokens, a->Hkv, a->D) ||
+      !strides_ok(&p.vs, a->v_stride, a->tokens, a->Hkv, a->D) || !strides_ok(&p.os, a->o_stride, a->tokens, a->H, a->D) ||
+      !aligned16(a->q) || !aligned16(a->k) || !aligned16(a->v) || !aligned16(a->o) || !aligned16(a->o_rest)) {
+    set_error("packed attention: rows must start on 16-byte boundaries and lie apart");
+    return ALG_ERR_INVALID;
+  }
+  const size_t need = alg_packed_attn_workspace_bytes(a);
+  if (a->workspace == nullptr || a->workspace_bytes < need || !aligned16(a->workspace)) {
+    set_error("packed attention: workspace of %zu bytes (16-byte aligned) required, got %zu", need, a->workspace_bytes);
+    return ALG_ERR_WORKSPACE;
+  }
+  if (a->tokens == 0) return ALG_OK;
+  p.G = a->H / a->Hkv;
+  ragged_plan_carve(&p.plan, a->workspace, a->sequences, a->tokens, a->Hkv, p.G, a->D, may_split(a->tokens, a->tokens, a->H, a->Hkv));
+  p.seqs = {a->cu_seqlens, nullptr, a->sequences, a->tokens, a->tokens};
+  p.q = a->q; p.k = a->k; p.v = a->v; p.o = a->o; p.o_lo = a->o_rest; p.stat = a->stat; p.sink = a->sink;
+  p.H = a->H; p.Hkv = a->Hkv; p.D = a->D; p.log2n = ilog2_exact(a->n);
+  p.tile_tokens = 128 / p.G;
+  p.scale = float(1.0 / (sqrt(double(a->D)) * double(a->c)));
+  p.inv_c = 1.0f / a->c;
+  p.zero_tail = a->zero_tail != 0;
+  p.status = a->status;
+  return launch_ragged_attention(p, stream);
+}
+
+static int paged_checks(const alg_paged_attn_args* a, const char* what) {
+  if (a->tokens < 0 || a->sequences < 0 || a->pages < 1 || a->table_width < 0) { set_error("%s: bad extents", what); return ALG_ERR_INVALID; }
+  if (a->page_size < 16 || a->page_size > 32768 || ilog2_exact(a->page_size) < 0) {
+    set_error("%s: pages of a power of two of tokens, at least 16, got %d", what, a->page_size);
+    return ALG_ERR_UNSUPPORTED;
+  }
+  if (int64_t(a->table_width) * a->page_size > INT_MAX - 4096) { set_error("%s: a sequence's pages hold more keys than 2^31", what); return ALG_ERR_INVALID; }
+  if (a->table_width > 0 && a->sequences > 1 && a->table_stride < a->table_width) { set_error("%s: rows of the block table overlap", what); return ALG_ERR_INVALID; }
+  if (a->cu_seqlens == nullptr && a->tokens != a->sequences) { set_error("%s: without cu_seqlens every sequence has one token", what); return ALG_ERR_INVALID; }
+  return ALG_OK;
+}
+
+size_t alg_paged_attn_workspace_bytes(const alg_paged_attn_args* a) {
+  if (a == nullptr || a->H < 1 || a->Hkv < 1 || a->H % a->Hkv != 0 || a->H / a->Hkv > 128 || a->tokens < 0 || a->sequences < 0) return 0;
+  return ragged_plan_bytes(a->sequences, a->tokens, a->Hkv, a->H / a->Hkv, a->D,
+                           may_split(int64_t(a->table_width) * a->page_size, a->tokens, a->H, a->Hkv));
+}
+
+int alg_paged_attn_fwd(const alg_paged_attn_args* a, void* stream_) {
+  cudaStream_t stream = static_cast<cudaStream_t>(stream_);
+  if (a == nullptr || a->q == nullptr || a->k_pages == nullptr || a->v_pages == nullptr || a->o == nullptr || a->kv_lens == nullptr ||
+      a->block_table == nullptr) {
+    set_error("paged attention: null tensor argument");
+    return ALG_ERR_INVALID;
+  }
+  if (int rc = check_link("paged attention", a->H, a->Hkv, a->D, a->n, a->c)) return rc;
+  if (int rc = paged_checks(a, "paged attention")) return rc;
+  RaggedParams p{};
+  int64_t kp = a->k_stride[0], vp = a->v_stride[0];
+  const int64_t page_elems = int64_t(a->page_size) * a->Hkv * a->D;
+  if (!strides_ok(&p.qs, a->q_stride, a->tokens, a->H, a->D) || !strides_ok(&p.ks, a->k_stride + 1, a->page_size, a->Hkv, a->D) ||
+      !strides_ok(&p.vs, a->v_stride + 1, a->page_size, a->Hkv, a->D) || !strides_ok(&p.os, a->o_stride, a->tokens, a->H, a->D) ||
+      !stride_ok(&kp, a->pages, page_elems) || !stride_ok(&vp, a->pages, page_elems) || !aligned16(a->q) || !aligned16(a->k_pages) ||
+      !aligned16(a->v_pages) || !aligned16(a->o)) {
+    set_error("paged attention: rows must start on 16-byte boundaries and lie apart");
+    return ALG_ERR_INVALID;
+  }
+  const size_t need = alg_paged_attn_workspace_bytes(a);
+  if (a->workspace == nullptr || a->workspace_bytes < need || !aligned16(a->workspace)) {
+    set_error("paged attention: workspace of %zu bytes (16-byte aligned) required, got %zu", need, a->workspace_bytes);
+    return ALG_ERR_WORKSPACE;
+  }
+  if (a->tokens == 0) return ALG_OK;
+  const int64_t keys = int64_t(a->table_width) * a->page_size;
+  p.G = a->H / a->Hkv;
+  ragged_plan_carve(&p.plan, a->workspace, a->sequences, a->tokens, a->Hkv, p.G, a->D, may_split(keys, a->tokens, a->H, a->Hkv));
+  p.seqs = {a->cu_seqlens, a->kv_lens, a->sequences, a->tokens, int(keys)};
+  p.q = a->q; p.k = a->k_pages; p.v = a->v_pages; p.o = a->o; p.sink = a->sink;
+  p.k_page = kp; p.v_page = vp;
+  p.table = a->block_table; p.table_stride = a->table_stride; p.table_width = a->table_width;
+  p.page = a->page_size; p.log2_page = ilog2_exact(a->page_size); p.pages = a->pages;
+  p.H = a->H; p.Hkv = a->Hkv; p.D = a->D; p.log2n = ilog2_exact(a->n);
+  p.tile_tokens = 128 / p.G;
+  p.scale = float(1.0 / (sqrt(double(a->D)) * double(a->c)));
+  p.inv_c = 1.0f / a->c;
+  p.zero_tail = a->zero_tail != 0 && a->cu_seqlens != nullptr;
+  p.status = a->status;
+  return launch_ragged_attention(p, stream);
+}
+
+}  // extern "C"

@@ -1,0 +1,801 @@
+// Causal asinh-power attention over sequences of different lengths, grouped heads, keys packed or in pages: tcgen05.
+//
+//   w_ij = rho(x_ij)^n, x = q.k / (sqrt(D) c), j <= i + Lk - Lq;  l_i = rho(b/c)^n + sum_j w_ij;  o_i = sum_j w_ij v_j / l_i
+//
+// The arithmetic per tile is that of attn_sm100.cu: S = Q K^T as 128 x 128 products, (y + sqrt(kappa + y^2))^n on packed fp32
+// straight from tensor memory (Q carries the power of two of the score scale), P back over S, O += P V with P from tensor
+// memory.  What is different:
+//   - work comes from a list made on the device (ragged.cuh, ragged_plan.cu), taken from a counter, and handed round the CTA
+//     through a small ring;
+//   - a query tile's rows are G heads of 128 / G tokens;
+//   - K and V tiles come from packed rows (a tile reads on into the next sequence) or page by page through the block table.
+//     Keys past the sequence's end are masked by the causal limit, but 0 times the NaN or infinity that a
+//     foreign V row may hold is NaN: one warp zeroes those rows of a sequence's last V tile in shared memory;
+//   - any scores: a warp whose 32 rows have all |x| <= x_fast in a tile takes the tile unshifted (x_fast keeps the weights within
+//     2^+-64 and the cancellation of y + sqrt(kappa + y^2) below 2e-4); a larger score, or a NaN, sends the warp to the max-shifted
+//     form with the cancellation-free rho for the rest of the item.  So no pass over q and k decides beforehand.
+//
+// Roles: warp 0 takes the work and runs the TMA loads, warp 1 issues the MMAs, warp 2 scales Q in shared memory, warp 3 clears the
+// foreign V rows, warps 4..7 and 8..11 weigh query tile 0 and 1, a thread a row.  An item of one tile runs as tile 1.
+// HILO (training): the weights go to the second product as two bf16 halves and the output is stored as two, since the
+// gradient of the sinks is a float32 sum of what the output's rounding would leave of its digits.
+//
+// Every mbarrier wait is bounded; a wait that runs out reports ALG_DEV_TIMEOUT.
+#include "common.cuh"
+#include "launchers.h"
+#include "ragged.cuh"
+#include "sm100_ptx.cuh"
+
+#include <math.h>
+
+#include <algorithm>
+
+namespace alg {
+namespace {
+
+using namespace sm100;
+
+constexpr int BQ = 128, BKEY = 128;
+constexpr int FIRST_WEIGHT_WARP = 4, NTHREADS = 384;
+constexpr int PANEL_BYTES = 128 * 128;          // 128 rows x 64 bf16, one swizzle-128B panel
+constexpr uint32_t TMEM_COLS = 512;
+constexpr int MAX_NKV = 10, RING = 3;
+constexpr int ITEM_READERS = 11;                // warps 1..11
+
+template <int D> struct Cfg {
+  static constexpr int PANELS = D / 64;
+  static constexpr int TILE_BYTES = PANELS * PANEL_BYTES;
+  static constexpr int NKV = (D == 128) ? 5 : 10;           // K/V ring depth (tiles)
+  static constexpr int KV_OFF = 2 * TILE_BYTES;             // behind the two Q tiles
+  static constexpr int CTL_OFF = KV_OFF + NKV * TILE_BYTES;
+  static constexpr uint32_t S_COL = 0, O_COL = 256;         // S_w at 128 w (P_w inside it), O_w at O_COL + D w
+  static constexpr uint32_t IDESC_S = make_idesc_bf16(BQ, BKEY, 0, 0);
+  static constexpr uint32_t IDESC_PV = make_idesc_bf16(BQ, D, 0, 1);   // V is [key][d]: MN-major B
+};
+
+// What a work item is to the roles.
+struct Work {
+  int row0, Lq, Lk, seq;
+  int head;                       // key head
+  int tok0, tok1;                 // first token (in the sequence) of query tile 0 / 1
+  int k0, n0, n1;                 // first key tile; key tiles of query tile 0 (0: it has none in this item) and 1 (< 0: no more work)
+  int has0;                       // query tile 0 has tokens
+  int slot;                       // < 0: whole
+};
+
+struct __align__(16) Control {
+  uint64_t q_full[2], q_ready[2], q_free[2], kv_full[MAX_NKV], kv_empty[MAX_NKV];
+  uint64_t s_full[2], p_half[2], p_full[2], o_full[2], o_free[2];
+  uint64_t v_here, v_clean, work_full[RING], work_empty[RING];
+  Work work[RING];
+  uint32_t tmem_base;
+  int abort_flag;
+};
+
+template <int D> constexpr size_t smem_bytes() { return size_t(Cfg<D>::CTL_OFF) + sizeof(Control) + 1024; }
+static_assert(smem_bytes<128>() <= 232448 && smem_bytes<64>() <= 232448, "shared memory budget of one CTA");
+
+struct ScoreScale {
+  float pow2;      // 2^e: applied to Q in shared memory
+  float m;         // x = m y
+  float kappa;     // 1 / m^2
+  float inv_m;     // every weight is (rho(x) / m)^n
+  float y_fast;    // x_fast / m
+};
+
+template <int LOG2N> __device__ __forceinline__ float2 power2(float2 t, int log2n) {
+  if (LOG2N > 0) {
+#pragma unroll
+    for (int k = 0; k < LOG2N; ++k) t = __fmul2_rn(t, t);
+  } else {
+    for (int k = 0; k < log2n; ++k) t = __fmul2_rn(t, t);
+  }
+  return t;
+}
+
+// 32 weights of this thread's row into bf16 pairs, hi and (HILO) what the rounding left over
+template <bool HILO>
+__device__ __forceinline__ void pack4(float2 t0, float2 t1, int i, uint32_t* packed) {
+  const uint32_t h0 = pack_bf16(t0.x, t0.y), h1 = pack_bf16(t1.x, t1.y);
+  packed[i >> 1] = h0;
+  packed[(i >> 1) + 1] = h1;
+  if (HILO) {
+    packed[16 + (i >> 1)] = pack_bf16(t0.x - __uint_as_float(h0 << 16), t0.y - __uint_as_float(h0 & 0xffff0000u));
+    packed[16 + (i >> 1) + 1] = pack_bf16(t1.x - __uint_as_float(h1 << 16), t1.y - __uint_as_float(h1 & 0xffff0000u));
+  }
+}
+template <bool HILO> __device__ __forceinline__ void store_packed(uint32_t taddr, const uint32_t* packed) {
+  if (HILO) tmem_st_32x32(taddr, packed);
+  else tmem_st_32x16(taddr, packed);
+}
+
+// Unshifted: 32 scores y -> (y + sqrt(kappa + y^2))^n.  `lim`: the last visible column of this row, counted from column 0 of the 32.
+template <int LOG2N, bool MASK, bool HILO>
+__device__ __forceinline__ void weigh(const uint32_t* s, float kappa, int log2n, int lim, float2& la, float2& lb, uint32_t* packed) {
+  const float2 kp = make_float2(kappa, kappa);
+#pragma unroll
+  for (int i = 0; i < 32; i += 4) {
+    const float2 y0 = make_float2(__uint_as_float(s[i]), __uint_as_float(s[i + 1]));
+    const float2 y1 = make_float2(__uint_as_float(s[i + 2]), __uint_as_float(s[i + 3]));
+    const float2 rad0 = __ffma2_rn(y0, y0, kp), rad1 = __ffma2_rn(y1, y1, kp);
+    const float2 rs0 = make_float2(rsqrt_approx(rad0.x), rsqrt_approx(rad0.y));
+    const float2 rs1 = make_float2(rsqrt_approx(rad1.x), rsqrt_approx(rad1.y));
+    float2 t0 = power2<LOG2N>(__ffma2_rn(rad0, rs0, y0), log2n), t1 = power2<LOG2N>(__ffma2_rn(rad1, rs1, y1), log2n);
+    if (MASK) {
+      t0.x = (i <= lim) ? t0.x : 0.f;     t0.y = (i + 1 <= lim) ? t0.y : 0.f;
+      t1.x = (i + 2 <= lim) ? t1.x : 0.f; t1.y = (i + 3 <= lim) ? t1.y : 0.f;
+    }
+    la = __fadd2_rn(la, t0);
+    lb = __fadd2_rn(lb, t1);
+    pack4<HILO>(t0, t1, i, packed);
+  }
+}
+
+// Shifted: (rho(x) sigma)^n with the cancellation-free rho, x = m y; sigma = rho(-reference) / m.
+template <bool HILO>
+__device__ __forceinline__ void weigh_shifted(const uint32_t* s, float m, float sigma, int log2n, int lim, float2& la, float2& lb,
+                                              uint32_t* packed) {
+#pragma unroll
+  for (int i = 0; i < 32; i += 4) {
+    float t[4];
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+      const float x = __uint_as_float(s[i + e]) * m, rad = fmaf(x, x, 1.0f);
+      float T = fmaf(rad, rsqrt_approx(rad), fabsf(x));
+      T = rad < 3.0e38f ? T : 2.0f * fabsf(x);           // x^2 past the range: sqrt(1 + x^2) = |x|
+      t[e] = pow2n_rt((x >= 0.f ? T : __fdividef(1.0f, T)) * sigma, log2n);
+      t[e] = (i + e <= lim) ? t[e] : 0.f;
+    }
+    const float2 t0 = make_float2(t[0], t[1]), t1 = make_float2(t[2], t[3]);
+    la = __fadd2_rn(la, t0);
+    lb = __fadd2_rn(lb, t1);
+    pack4<HILO>(t0, t1, i, packed);
+  }
+}
+// the same rho for a single value, whose square may leave the range too
+__device__ __forceinline__ float rho_any(float x) {
+  const float rad = fmaf(x, x, 1.0f);
+  const float T = rad < 3.0e38f ? fmaf(rad, rsqrt_approx(rad), fabsf(x)) : 2.0f * fabsf(x);
+  return x >= 0.0f ? T : __fdividef(1.0f, T);
+}
+
+__device__ __forceinline__ void signal_weights(uint64_t* bar) {
+  tmem_st_wait();
+  tc_fence_before();
+  mbar_arrive(bar);
+}
+
+// A tile of this thread's row, 32 columns at a time, the next load in flight while a block is weighed; `block(regs, b)` leaves
+// the packed weights of block b.
+template <bool HILO, class Block>
+__device__ __forceinline__ void weigh_tile(uint32_t s_taddr, uint64_t* p_half, uint64_t* p_full, Block&& block) {
+  uint32_t a[32], b[32], packed[HILO ? 32 : 16];
+  tmem_ld_32x32(s_taddr, a);
+  tmem_ld_wait_for(a);
+  tmem_ld_32x32(s_taddr + 32, b);
+  block(a, 0, packed);
+  store_packed<HILO>(s_taddr, packed);
+  tmem_ld_wait_for(b);
+  tmem_ld_32x32(s_taddr + 64, a);
+  block(b, 32, packed);
+  store_packed<HILO>(s_taddr + 32, packed);
+  signal_weights(p_half);
+  tmem_ld_wait_for(a);
+  tmem_ld_32x32(s_taddr + 96, b);
+  block(a, 64, packed);
+  store_packed<HILO>(s_taddr + 64, packed);
+  tmem_ld_wait_for(b);
+  block(b, 96, packed);
+  store_packed<HILO>(s_taddr + 96, packed);
+  signal_weights(p_full);
+}
+
+__device__ __forceinline__ float max3_abs_nan(float a, float b, float c) {      // NaN if one of them is
+  float r;
+  asm("max.NaN.abs.f32 %0, %1, %2, %3;" : "=f"(r) : "f"(a), "f"(b), "f"(c));
+  return r;
+}
+// Largest |y| of the row's visible scores, NaN if one is NaN.  Only what the row sees counts: which form its weights take, and
+// with it their rounding, must not depend on a neighbouring sequence.
+template <bool MASK>
+__device__ __forceinline__ float tile_abs_max(uint32_t s_taddr, int lim) {
+  uint32_t a[32], b[32];
+  float m[4] = {0.f, 0.f, 0.f, 0.f};
+  auto scan = [&](const uint32_t* s, int c) {
+#pragma unroll
+    for (int i = 0; i < 32; i += 2) {
+      const float y0 = !MASK || c + i <= lim ? __uint_as_float(s[i]) : 0.f, y1 = !MASK || c + i + 1 <= lim ? __uint_as_float(s[i + 1]) : 0.f;
+      m[(i >> 1) & 3] = max3_abs_nan(m[(i >> 1) & 3], y0, y1);
+    }
+  };
+  tmem_ld_32x32(s_taddr, a);
+  tmem_ld_32x32(s_taddr + 32, b);
+  tmem_ld_wait_for(a);
+  scan(a, 0);
+  tmem_ld_wait_for(b);                                  // complete already: orders the reads of b
+  tmem_ld_32x32(s_taddr + 64, a);
+  scan(b, 32);
+  tmem_ld_32x32(s_taddr + 96, b);
+  tmem_ld_wait_for(a);
+  scan(a, 64);
+  tmem_ld_wait_for(b);
+  scan(b, 96);
+  return max3_abs_nan(max3_abs_nan(m[0], m[1], m[2]), m[3], 0.f);
+}
+// largest visible x of the row (NaN ignored: its weight will be NaN whatever the reference); -inf if there is none
+__device__ __forceinline__ float tile_row_max(uint32_t s_taddr, float m, int lim) {
+  float top = -INFINITY;
+#pragma unroll 1
+  for (int c = 0; c < 128; c += 32) {
+    uint32_t a[32];
+    tmem_ld_32x32(s_taddr + c, a);
+    tmem_ld_wait_for(a);
+#pragma unroll
+    for (int i = 0; i < 32; ++i) top = (c + i <= lim) ? fmaxf(top, __uint_as_float(a[i]) * m) : top;
+  }
+  return top;
+}
+
+template <int NKV> struct RingCursor {
+  int slot = 0;
+  uint32_t phase = 0;
+  __device__ __forceinline__ void next() { if (++slot == NKV) { slot = 0; phase ^= 1u; } }
+};
+
+template <int D, int LOG2N, bool HILO, bool PAGED>
+__global__ void __launch_bounds__(NTHREADS, 1)
+ragged_attn_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant__ CUtensorMap tm_k,
+                   const __grid_constant__ CUtensorMap tm_v, const __grid_constant__ RaggedParams p, const ScoreScale sc) {
+  using C = Cfg<D>;
+  extern __shared__ unsigned char smem_raw[];
+  unsigned char* smem = reinterpret_cast<unsigned char*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
+  Control* ctl = reinterpret_cast<Control*>(smem + C::CTL_OFF);
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+
+  if (threadIdx.x == 0) {
+    for (int w = 0; w < 2; ++w) {
+      mbar_init(&ctl->q_full[w], 1); mbar_init(&ctl->q_ready[w], 1); mbar_init(&ctl->q_free[w], 1);
+      mbar_init(&ctl->s_full[w], 1); mbar_init(&ctl->p_half[w], 128); mbar_init(&ctl->p_full[w], 128);
+      mbar_init(&ctl->o_full[w], 1); mbar_init(&ctl->o_free[w], 128);
+    }
+    for (int i = 0; i < C::NKV; ++i) { mbar_init(&ctl->kv_full[i], 1); mbar_init(&ctl->kv_empty[i], 1); }
+    for (int i = 0; i < RING; ++i) { mbar_init(&ctl->work_full[i], 1); mbar_init(&ctl->work_empty[i], ITEM_READERS); }
+    mbar_init(&ctl->v_here, 1); mbar_init(&ctl->v_clean, 1);
+    ctl->abort_flag = 0;
+    fence_barrier_init();
+    tma_prefetch_desc(&tm_q); tma_prefetch_desc(&tm_k); tma_prefetch_desc(&tm_v);
+  }
+  if (warp == 1) {
+    tmem_alloc(&ctl->tmem_base, TMEM_COLS);
+    tmem_relinquish();
+  }
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+  griddep_wait();                                       // the plan, and q, k, v of the kernels ahead
+  const uint32_t tmem_base = ctl->tmem_base;
+  const BoundedWait bw{&ctl->abort_flag, 1000000000ull};
+  const int TT = p.tile_tokens;
+
+  // the k-th work item of this CTA; false at the end of the work or of the waiting
+  auto work_at = [&](int k, Work& w) -> bool {
+    if (!__all_sync(0xffffffffu, bw.wait(&ctl->work_full[k % RING], uint32_t(k / RING) & 1u))) return false;
+    w = ctl->work[k % RING];
+    return w.n1 >= 0;
+  };
+  auto work_done = [&](int k) {
+    __syncwarp();
+    if (lane == 0) mbar_arrive(&ctl->work_empty[k % RING]);
+  };
+
+  if (warp == 0) {
+    if (lane == 0) {
+      const int total = p.plan.header->items * p.Hkv;
+      // the next item: the CTA's own number first, then from the counter; shown to the other roles.  It is asked for when the loads of
+      // the item before have been issued, which is as late as can be without a pause, so that longest-first holds to the end
+      auto fetch = [&](int k, Work& w) -> bool {
+        if (k >= RING && !bw.wait(&ctl->work_empty[k % RING], uint32_t(k / RING - 1) & 1u)) return false;
+        const int next = k == 0 ? int(blockIdx.x) : int(gridDim.x) + atomicAdd(&p.plan.header->counter, 1);
+        w.n1 = -1;
+        if (next < total) {
+          const RaggedItem it = p.plan.items[next / p.Hkv];
+          w.head = next % p.Hkv;
+          w.row0 = it.row0; w.Lq = it.Lq; w.Lk = it.Lk; w.seq = it.seq; w.k0 = it.k0; w.slot = it.slot; w.n1 = it.nk;
+          const bool two = it.Lq - it.t0 > TT;
+          w.has0 = two ? 1 : 0;
+          w.tok0 = it.t0;
+          w.tok1 = two ? it.t0 + TT : it.t0;
+          w.n0 = two ? min(max(ragged_tiles(it.Lq, it.Lk, it.t0 + TT) - it.k0, 0), it.nk) : 0;
+        }
+        ctl->work[k % RING] = w;
+        mbar_arrive(&ctl->work_full[k % RING]);
+        return w.n1 >= 0;
+      };
+      RingCursor<C::NKV> cur;
+      int items0 = 0;                                   // items in which query tile 0 took part
+      Work w;
+      bool ok = true;
+      for (int k = 0; ok && fetch(k, w); ++k) {
+        auto load_kv = [&](int idx) {                   // K_0, V_0, K_1, V_1, ... of this item
+          const int buf = cur.slot;
+          if (!bw.wait(&ctl->kv_empty[buf], cur.phase ^ 1u)) return false;
+          const CUtensorMap* tm = (idx & 1) ? &tm_v : &tm_k;
+          unsigned char* dst = smem + C::KV_OFF + buf * C::TILE_BYTES;
+          const int key0 = (w.k0 + (idx >> 1)) * BKEY;
+          if (PAGED) {
+            const int rows = min(p.page, BKEY), live = min(BKEY, w.Lk - key0);      // keys of the tile that the sequence has
+            const int loads = live > 0 ? (live + rows - 1) / rows : 0;
+            mbar_arrive_expect_tx(&ctl->kv_full[buf], uint32_t(loads * rows) * (D * 2));
+            const int* pages = p.table + w.seq * p.table_stride;
+            for (int i = 0; i < loads; ++i) {
+              const int key = key0 + i * rows;
+              const int number = __ldg(pages + (key >> p.log2_page));    // outside the pool: the copy fills zeros
+              for (int pn = 0; pn < C::PANELS; ++pn)
+                tma_load_5d(dst + pn * PANEL_BYTES + i * rows * 128, tm, &ctl->kv_full[buf], 0, key & (p.page - 1), pn, w.head, number);
+            }
+          } else {
+            mbar_arrive_expect_tx(&ctl->kv_full[buf], C::TILE_BYTES);
+            tma_load_4d(dst, tm, &ctl->kv_full[buf], 0, w.row0 + key0, 0, w.head);
+          }
+          cur.next();
+          return true;
+        };
+        auto load_q = [&](int t) {                      // after the previous item's last S_t has read the tile
+          if (t == 0 && w.n0 == 0) return true;
+          const int before = t == 0 ? items0 : k;
+          if (before > 0 && !bw.wait(&ctl->q_free[t], uint32_t(before - 1) & 1u)) return false;
+          mbar_arrive_expect_tx(&ctl->q_full[t], uint32_t(p.G * TT) * (D * 2));
+          for (int pn = 0; pn < C::PANELS; ++pn)
+            tma_load_4d(smem + t * C::TILE_BYTES + pn * PANEL_BYTES, &tm_q, &ctl->q_full[t], 0, w.head * p.G,
+                        w.row0 + (t == 0 ? w.tok0 : w.tok1), pn);
+          return true;
+        };
+        if (k == 0) ok = load_q(0) && load_kv(0) && load_q(1) && load_kv(1);
+        else ok = load_kv(0) && load_q(0) && load_kv(1) && load_q(1);
+        for (int idx = 2; idx < 2 * w.n1 && ok; ++idx) ok = load_kv(idx);
+        if (w.n0 > 0) ++items0;
+      }
+    }
+  } else if (warp == 1) {
+    const uint32_t q_addr = smem_u32(smem), kv_addr = smem_u32(smem + C::KV_OFF);
+    using Cur = RingCursor<C::NKV>;
+    Cur cur;
+    int t0 = 0, t1 = 0, items0 = 0, cleans = 0;         // score tiles of query tile 0 / 1 in earlier items; items of tile 0
+    auto wait_all = [&](uint64_t* bar, uint32_t parity) { return __all_sync(0xffffffffu, bw.wait(bar, parity)) != 0; };
+    auto kv_wait = [&](const Cur& c) { return wait_all(&ctl->kv_full[c.slot], c.phase); };
+    const uint32_t q_lo0 = sw128_desc_lo(q_addr, 16), k_lo0 = sw128_desc_lo(kv_addr, 16), v_lo0 = sw128_desc_lo(kv_addr, PANEL_BYTES);
+    auto issue_s = [&](int t, int slot) {               // S_t = Q_t K^T
+      const uint32_t qa = q_lo0 + t * (C::TILE_BYTES >> 4), ka = k_lo0 + slot * (C::TILE_BYTES >> 4);
+#pragma unroll
+      for (int ks = 0; ks < D / 16; ++ks) {
+        const uint32_t off = ((ks >> 2) * PANEL_BYTES + (ks & 3) * 32) >> 4;
+        umma_f16_ss_parts(tmem_base + C::S_COL + t * 128, qa + off, SW128_DESC_HI, ka + off, SW128_DESC_HI, C::IDESC_S, ks != 0 ? 1u : 0u);
+      }
+    };
+    auto issue_pv = [&](int t, int slot, int h64, bool first) {   // O_t += P_t V for the first or second 64 keys
+      const uint32_t va = v_lo0 + slot * (C::TILE_BYTES >> 4);
+#pragma unroll
+      for (int part = 0; part < (HILO ? 2 : 1); ++part)
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {                   // 16 keys = 8 packed columns of P a step; 32 columns hold 32 keys' hi | lo
+          const int ks = 4 * h64 + i;
+          umma_f16_ts_parts(tmem_base + C::O_COL + t * D, tmem_base + C::S_COL + t * 128 + (ks >> 1) * 32 + (ks & 1) * 8 + part * 16,
+                            va + ks * (2048 >> 4), SW128_DESC_HI, C::IDESC_PV, (first && ks == 0 && part == 0) ? 0u : 1u);
+        }
+    };
+    // P of query tile t, tile j of nt, then the next scores into its place
+    auto serve = [&](int t, int j, int nt, int before, int items, int v_slot, int k_slot) -> bool {
+      if (!wait_all(&ctl->p_half[t], uint32_t(before + j) & 1u)) return false;
+      if (j == 0 && items > 0 && !wait_all(&ctl->o_free[t], uint32_t(items - 1) & 1u)) return false;   // the last output has been read
+      tc_fence_after();
+      if (elect_one()) issue_pv(t, v_slot, 0, j == 0);
+      __syncwarp();
+      if (!wait_all(&ctl->p_full[t], uint32_t(before + j) & 1u)) return false;
+      tc_fence_after();
+      if (elect_one()) {
+        issue_pv(t, v_slot, 1, false);
+        if (j + 1 < nt) { issue_s(t, k_slot); umma_commit(&ctl->s_full[t]); }    // behind P V: may overwrite P
+        else umma_commit(&ctl->o_full[t]);
+      }
+      __syncwarp();
+      return true;
+    };
+    Work w;
+    bool ok = true;
+    int k = 0;
+    for (; ok && work_at(k, w); ++k) {
+      work_done(k);
+      const int n0 = w.n0, n1 = w.n1;
+      const bool foreign = (w.k0 + n1) * BKEY > w.Lk;   // the last V tile has rows of no key of this sequence
+      if ((n0 > 0 && !wait_all(&ctl->q_ready[0], uint32_t(items0) & 1u)) || !kv_wait(cur)) { ok = false; break; }
+      tc_fence_after();
+      if (n0 > 0 && elect_one()) { issue_s(0, cur.slot); umma_commit(&ctl->s_full[0]); }
+      __syncwarp();
+      if (!wait_all(&ctl->q_ready[1], uint32_t(k) & 1u)) { ok = false; break; }
+      tc_fence_after();
+      if (elect_one()) { issue_s(1, cur.slot); umma_commit(&ctl->s_full[1]); }
+      __syncwarp();
+      cur.next();
+      for (int j = 0; j < n1 && ok; ++j) {
+        const Cur vc = cur;                             // V_j
+        cur.next();
+        const Cur kc = cur;                             // K_{j+1}
+        if (j + 1 < n1) cur.next();
+        if (!kv_wait(vc) || (j + 1 < n1 && !kv_wait(kc))) { ok = false; break; }
+        if (foreign && j + 1 == n1) {                   // the weights of this step take longer than the clearing
+          if (lane == 0) mbar_arrive(&ctl->v_here);
+          if (!wait_all(&ctl->v_clean, uint32_t(cleans) & 1u)) { ok = false; break; }
+        }
+        if (j < n0 && !serve(0, j, n0, t0, items0, vc.slot, kc.slot)) { ok = false; break; }
+        if (!serve(1, j, n1, t1, k, vc.slot, kc.slot)) { ok = false; break; }
+      }
+      t0 += n0; t1 += n1;
+      if (n0 > 0) ++items0;
+      if (foreign) ++cleans;
+    }
+  } else if (warp == 2) {
+    // Q scaler: multiplies a landed Q tile by 2^e where it lies
+    const __nv_bfloat162 f2 = __float2bfloat162_rn(sc.pow2);
+    Work w;
+    int items0 = 0;
+    bool ok = true;
+    for (int k = 0; ok && work_at(k, w); ++k) {
+      work_done(k);
+      for (int t = 0; t < 2 && ok; ++t) {
+        if (t == 0 && w.n0 == 0) continue;
+        if (!__all_sync(0xffffffffu, bw.wait(&ctl->q_full[t], uint32_t(t == 0 ? items0 : k) & 1u))) { ok = false; break; }
+        if (sc.pow2 != 1.0f) {
+          uint4* tile = reinterpret_cast<uint4*>(smem + t * C::TILE_BYTES);
+#pragma unroll 8
+          for (int i = lane; i < C::TILE_BYTES / 16; i += 32) {
+            uint4 v = tile[i];
+            __nv_bfloat162* h = reinterpret_cast<__nv_bfloat162*>(&v);
+            h[0] = __hmul2(h[0], f2); h[1] = __hmul2(h[1], f2); h[2] = __hmul2(h[2], f2); h[3] = __hmul2(h[3], f2);
+            tile[i] = v;
+          }
+          fence_async_shared();
+        }
+        __syncwarp();
+        if (lane == 0) mbar_arrive(&ctl->q_ready[t]);
+      }
+      if (w.n0 > 0) ++items0;
+    }
+  } else if (warp == 3) {
+    // zeroes the rows of a sequence's last V tile that hold none of its keys
+    Work w;
+    int slot = 0, cleans = 0;                           // ring slot of the item's first tile
+    bool ok = true;
+    for (int k = 0; ok && work_at(k, w); ++k) {
+      work_done(k);
+      const int live = max(w.Lk - (w.k0 + w.n1 - 1) * BKEY, 0);
+      if (live < BKEY) {
+        if (!__all_sync(0xffffffffu, bw.wait(&ctl->v_here, uint32_t(cleans) & 1u))) { ok = false; break; }
+        unsigned char* tile = smem + C::KV_OFF + (slot + 2 * w.n1 - 1) % C::NKV * C::TILE_BYTES;
+        const uint4 zero = make_uint4(0u, 0u, 0u, 0u);
+        for (int pn = 0; pn < C::PANELS; ++pn) {
+          uint4* panel = reinterpret_cast<uint4*>(tile + pn * PANEL_BYTES);
+          for (int i = live * 8 + lane; i < 1024; i += 32) panel[i] = zero;
+        }
+        fence_async_shared();
+        __syncwarp();
+        if (lane == 0) mbar_arrive(&ctl->v_clean);
+        ++cleans;
+      }
+      slot = (slot + 2 * w.n1) % C::NKV;
+    }
+    if (p.zero_tail) {                                  // rows of no sequence: before the first, behind the last
+      const int S = p.seqs.S;
+      const int first = min(max(__ldg(p.seqs.cu), 0), p.seqs.tokens), end = min(max(__ldg(p.seqs.cu + S), first), p.seqs.tokens);
+      const int none = first + p.seqs.tokens - end;
+      for (int64_t i = blockIdx.x; i < int64_t(none) * p.H; i += gridDim.x) {
+        const int at = int(i / p.H), h = int(i % p.H), row = at < first ? at : end + at - first;
+        if (lane < D / 8)
+          *reinterpret_cast<uint4*>(static_cast<__nv_bfloat16*>(p.o) + row * p.os.t + h * p.os.h + lane * 8) = make_uint4(0u, 0u, 0u, 0u);
+      }
+    }
+  } else {
+    const int t = (warp - FIRST_WEIGHT_WARP) >> 2;      // query tile
+    const int quarter = warp & 3;
+    const int r = quarter * 32 + lane;                  // row of the tile
+    const uint32_t lane_sel = uint32_t(quarter * 32) << 16;
+    const uint32_t s_taddr = tmem_base + lane_sel + C::S_COL + t * 128;
+    const uint32_t o_taddr = tmem_base + lane_sel + C::O_COL + t * D;
+    const int tok_r = r / p.G, g_r = r - tok_r * p.G;   // token and head of this row
+    // the "scores there" barriers of tile 1, served second in every step, tell that V of the step before and K of this one are read
+    const bool releaser = quarter == 0 && lane == 0;
+    RingCursor<C::NKV> rel;
+    int tiles = 0, items = 0;                           // of this group, in earlier items
+    Work w;
+    bool ok = true;
+    for (int k = 0; ok && work_at(k, w); ++k) {
+      const int nk = t == 0 ? w.n0 : w.n1;
+      const int tok = (t == 0 ? w.tok0 : w.tok1) + tok_r;
+      const bool live = tok_r < TT && tok < w.Lq && (t == 1 || w.has0 != 0);
+      const int limit = live ? w.Lk - w.Lq + tok - w.k0 * BKEY : -1;             // last visible key, from the item's first on
+      const int limit0 = w.Lk - w.Lq + (t == 0 ? w.tok0 : w.tok1) - w.k0 * BKEY; // of the tile's first row
+      const int head = w.head * p.G + g_r;
+      float l = 0.f, m_run = 0.f;                       // weights are (rho(x) rho(-m_run) / m)^n: unshifted at first
+      const bool whole_sink = live && p.sink != nullptr && w.k0 == 0;
+      bool shifted = false;                             // the warp's form
+      if (whole_sink) {
+        const float b = p.sink[head] * p.inv_c;
+        if (!(fabsf(b) <= sc.y_fast * sc.m)) m_run = b;
+        l = pow2n_rt(rho_any(b) * (m_run != 0.f ? rho_any(-m_run) : 1.0f) * sc.inv_m, p.log2n);
+      }
+      shifted = __any_sync(0xffffffffu, m_run != 0.f);
+      float2 la = make_float2(0.f, 0.f), lb = make_float2(0.f, 0.f);
+      for (int j = 0; j < nk && ok; ++j) {
+        if (!__all_sync(0xffffffffu, bw.wait(&ctl->s_full[t], uint32_t(tiles + j) & 1u))) { ok = false; break; }
+        tc_fence_after();
+        if (releaser) {
+          if (t == 1) {
+            if (j > 0) { mbar_arrive(&ctl->kv_empty[rel.slot]); rel.next(); }    // V_{j-1}
+            mbar_arrive(&ctl->kv_empty[rel.slot]); rel.next();                   // K_j
+          }
+          if (j == nk - 1) mbar_arrive(&ctl->q_free[t]);
+        }
+        const int lim = limit - j * BKEY;
+        const bool masked = limit0 - j * BKEY < BKEY - 1;                        // uniform over the group
+        if (!shifted) {
+          const float top = masked ? tile_abs_max<true>(s_taddr, lim) : tile_abs_max<false>(s_taddr, lim);
+          shifted = __any_sync(0xffffffffu, live && !(top <= sc.y_fast));
+        }
+        if (!shifted) {
+          const int warp_lim = masked ? __reduce_max_sync(0xffffffffu, lim) : 0;
+          if (masked) weigh_tile<HILO>(s_taddr, &ctl->p_half[t], &ctl->p_full[t], [&](const uint32_t* s, int c, uint32_t* packed) {
+            if (c <= warp_lim) {
+              weigh<LOG2N, true, HILO>(s, sc.kappa, p.log2n, lim - c, la, lb, packed);
+            } else {                                    // the block lies beyond what any row of the warp sees
+#pragma unroll
+              for (int i = 0; i < (HILO ? 32 : 16); ++i) packed[i] = 0u;
+            }
+          });
+          else weigh_tile<HILO>(s_taddr, &ctl->p_half[t], &ctl->p_full[t], [&](const uint32_t* s, int c, uint32_t* packed) {
+            weigh<LOG2N, false, HILO>(s, sc.kappa, p.log2n, 0, la, lb, packed);
+          });
+        } else {
+          l += (la.x + la.y) + (lb.x + lb.y);
+          la = make_float2(0.f, 0.f); lb = make_float2(0.f, 0.f);
+          // the reference moves to the row's largest score so far; with nothing weighed yet it may also fall
+          const float top = tile_row_max(s_taddr, sc.m, lim);
+          float m_new = m_run;
+          if (lim >= 0 && top > -INFINITY) m_new = l > 0.f ? fmaxf(m_run, top) : top;
+          const float alpha = m_new != m_run ? pow2n_rt(rho_any(m_run) * rho_any(-m_new), p.log2n) : 1.0f;
+          // O of the earlier tiles is at rest (these scores were issued behind their product): rescale it where a reference moved
+          if (__any_sync(0xffffffffu, j > 0 && alpha != 1.0f)) {
+            const float a_row = j > 0 ? alpha : 1.0f;
+#pragma unroll 1
+            for (int c = 0; c < D; c += 32) {
+              uint32_t o[32];
+              tmem_ld_32x32(o_taddr + c, o);
+              tmem_ld_wait_for(o);
+#pragma unroll
+              for (int i = 0; i < 32; ++i) o[i] = __float_as_uint(a_row == 0.f ? 0.f : __uint_as_float(o[i]) * a_row);
+              tmem_st_32x32(o_taddr + c, o);
+            }
+            tmem_st_wait();
+          }
+          if (l > 0.f) l *= alpha;
+          m_run = m_new;
+          const float sigma = rho_any(-m_run) * sc.inv_m;
+          weigh_tile<HILO>(s_taddr, &ctl->p_half[t], &ctl->p_full[t], [&](const uint32_t* s, int c, uint32_t* packed) {
+            weigh_shifted<HILO>(s, sc.m, sigma, p.log2n, lim - c, la, lb, packed);
+          });
+        }
+      }
+      if (!ok) break;
+      tiles += nk;
+      l += (la.x + la.y) + (lb.x + lb.y);
+      const bool partial = w.slot >= 0;
+      float* dst = nullptr;
+      if (partial && (t == 1 || w.has0)) {
+        dst = p.plan.slots + ((int64_t(w.slot) * p.Hkv + w.head) * 256 + t * BQ + r) * (D + 4);
+        *reinterpret_cast<float4*>(dst + D) = make_float4(nk > 0 && live ? l : 0.f, m_run, 0.f, 0.f);
+      }
+      if (nk > 0) {
+        if (!__all_sync(0xffffffffu, bw.wait(&ctl->o_full[t], uint32_t(items) & 1u))) { ok = false; break; }
+        ++items;
+        if (releaser && t == 1) { mbar_arrive(&ctl->kv_empty[rel.slot]); rel.next(); }     // the item's last V tile
+        tc_fence_after();
+        const float inv = l != 0.f ? 1.0f / l : 0.f;    // a row that sees nothing: zero
+        const int64_t row = int64_t(w.row0) + tok;
+        __nv_bfloat16* orow = static_cast<__nv_bfloat16*>(p.o) + row * p.os.t + head * p.os.h;
+        __nv_bfloat16* lrow = HILO ? static_cast<__nv_bfloat16*>(p.o_lo) + (row * p.H + head) * D : nullptr;
+#pragma unroll 1
+        for (int c = 0; c < D; c += 32) {
+          uint32_t o[32];
+          tmem_ld_32x32(o_taddr + c, o);
+          tmem_ld_wait_for(o);
+          if (c == D - 32) {                            // O is in registers: the next item may overwrite it
+            tc_fence_before();
+            mbar_arrive(&ctl->o_free[t]);
+          }
+          if (partial) {
+#pragma unroll
+            for (int i = 0; i < 8; ++i)
+              *reinterpret_cast<uint4*>(dst + c + 4 * i) = make_uint4(o[4 * i], o[4 * i + 1], o[4 * i + 2], o[4 * i + 3]);
+            continue;
+          }
+          if (!live) continue;
+          if (l == 0.f) {
+#pragma unroll
+            for (int i = 0; i < 32; ++i) o[i] = 0u;
+          }
+          uint32_t packed[HILO ? 32 : 16];
+#pragma unroll
+          for (int i = 0; i < 32; i += 4)
+            pack4<HILO>(make_float2(__uint_as_float(o[i]) * inv, __uint_as_float(o[i + 1]) * inv),
+                        make_float2(__uint_as_float(o[i + 2]) * inv, __uint_as_float(o[i + 3]) * inv), i, packed);
+#pragma unroll
+          for (int i = 0; i < 4; ++i) {
+            *reinterpret_cast<uint4*>(orow + c + 8 * i) = make_uint4(packed[4 * i], packed[4 * i + 1], packed[4 * i + 2], packed[4 * i + 3]);
+            if (HILO) *reinterpret_cast<uint4*>(lrow + c + 8 * i) = make_uint4(packed[16 + 4 * i], packed[17 + 4 * i], packed[18 + 4 * i], packed[19 + 4 * i]);
+          }
+        }
+        // a with p = (rho(x) a)^n: rho(-m_run) (l m^n)^(-1/n)
+        if (!partial && live && p.stat != nullptr)
+          p.stat[int64_t(head) * p.seqs.tokens + row] = l > 0.f ? (m_run != 0.f ? rho_any(-m_run) : 1.0f) * sc.inv_m * inv_root_rt(l, p.log2n) : 0.f;
+      }
+      work_done(k);
+    }
+  }
+
+  tc_fence_before();
+  __syncthreads();
+  if (ctl->abort_flag != 0) {
+    if (threadIdx.x == 0) {
+      if (p.status != nullptr) atomicExch(p.status, ALG_DEV_TIMEOUT);
+      const uint64_t t0 = global_timer_ns();            // let issued loads land before shared memory is released
+      while (global_timer_ns() - t0 < 200000ull) { }
+    }
+    __syncthreads();
+  }
+  if (warp == 1) {
+    __syncwarp();
+    tc_fence_after();
+    tmem_dealloc(tmem_base, TMEM_COLS);
+  }
+}
+
+// Adds up the parts of the items that were cut along the keys.  A CTA takes 32 of the 256 rows of an (item, head), a warp four of
+// them, a lane D / 32 columns; parts meet in their order, at the largest of their references.
+template <int D>
+__global__ void __launch_bounds__(256) ragged_combine_kernel(const RaggedParams p, const ScoreScale sc) {
+  griddep_wait();
+  constexpr int CPL = D / 32;
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  const int units = p.plan.header->combos * p.Hkv * 8;
+  for (int u = blockIdx.x; u < units; u += gridDim.x) {
+    const RaggedCombo it = p.plan.combos[u / (p.Hkv * 8)];
+    const int h = (u >> 3) % p.Hkv;
+    const bool two = it.Lq - it.t0 > p.tile_tokens;
+    for (int rr = 0; rr < 4; ++rr) {
+      const int in_item = (u & 7) * 32 + warp * 4 + rr, t = in_item >> 7, r = in_item & 127;
+      if (t == 0 && !two) continue;
+      const int tok_r = r / p.G, g = r - tok_r * p.G, tok = it.t0 + (t == 1 && two ? p.tile_tokens : 0) + tok_r;
+      if (tok_r >= p.tile_tokens || tok >= it.Lq) continue;
+      const float* row = p.plan.slots + ((int64_t(it.slot) * p.Hkv + h) * 256 + in_item) * (D + 4);
+      const int64_t step = int64_t(p.Hkv) * 256 * (D + 4);          // to the next part
+      float2 lm = lane < it.parts ? __ldcg(reinterpret_cast<const float2*>(row + lane * step + D)) : make_float2(0.f, 0.f);
+      float2 lm2 = lane + 32 < it.parts ? __ldcg(reinterpret_cast<const float2*>(row + (lane + 32) * step + D)) : make_float2(0.f, 0.f);
+      // a part that weighed nothing has no say in the reference
+      const bool nan = __any_sync(0xffffffffu, lm.x != lm.x || lm2.x != lm2.x);
+      float top = fmaxf(lm.x > 0.f ? lm.y : -INFINITY, lm2.x > 0.f ? lm2.y : -INFINITY);
+      top = warp_max(top);
+      const float ns = rho_any(-top);
+      const float f1 = lm.x > 0.f ? (lm.y == top ? 1.0f : pow2n_rt(rho_any(lm.y) * ns, p.log2n)) : 0.f;
+      const float f2 = lm2.x > 0.f ? (lm2.y == top ? 1.0f : pow2n_rt(rho_any(lm2.y) * ns, p.log2n)) : 0.f;
+      const float l = warp_sum(f1 * lm.x + f2 * lm2.x);
+      float acc[CPL];
+#pragma unroll
+      for (int c = 0; c < CPL; ++c) acc[c] = 0.f;
+      for (int pt = 0; pt < it.parts; ++pt) {
+        const float f = __shfl_sync(0xffffffffu, pt < 32 ? f1 : f2, pt & 31);
+        if (f == 0.f) continue;                         // warp-uniform; its accumulator may never have been written
+        const float* src = row + pt * step + lane * CPL;
+        if (CPL == 4) {
+          const float4 v = __ldcg(reinterpret_cast<const float4*>(src));
+          acc[0] = fmaf(f, v.x, acc[0]); acc[1] = fmaf(f, v.y, acc[1]); acc[CPL - 2] = fmaf(f, v.z, acc[CPL - 2]); acc[CPL - 1] = fmaf(f, v.w, acc[CPL - 1]);
+        } else {
+          const float2 v = __ldcg(reinterpret_cast<const float2*>(src));
+          acc[0] = fmaf(f, v.x, acc[0]); acc[1] = fmaf(f, v.y, acc[1]);
+        }
+      }
+      const float inv = nan ? __int_as_float(0x7fc00000) : l > 0.f ? 1.0f / l : 0.f;
+      const int64_t at = int64_t(it.row0) + tok;
+      const int head = h * p.G + g;
+      __nv_bfloat16* orow = static_cast<__nv_bfloat16*>(p.o) + at * p.os.t + head * p.os.h + lane * CPL;
+      __nv_bfloat16* lrow = p.o_lo != nullptr ? static_cast<__nv_bfloat16*>(p.o_lo) + (at * p.H + head) * D + lane * CPL : nullptr;
+#pragma unroll
+      for (int c = 0; c < CPL; c += 2) {
+        const float x = acc[c] * inv, y = acc[c + 1] * inv;
+        const uint32_t hi = pack_bf16(x, y);
+        *reinterpret_cast<uint32_t*>(orow + c) = hi;
+        if (lrow != nullptr) *reinterpret_cast<uint32_t*>(lrow + c) = pack_bf16(x - __uint_as_float(hi << 16), y - __uint_as_float(hi & 0xffff0000u));
+      }
+      if (p.stat != nullptr && lane == 0) {
+        const float a = l > 0.f ? ns * sc.inv_m * inv_root_rt(l, p.log2n) : 0.f;
+        p.stat[int64_t(head) * p.seqs.tokens + at] = nan ? __int_as_float(0x7fc00000) : a;
+      }
+    }
+  }
+}
+
+template <int D, int LOG2N, bool HILO, bool PAGED>
+int launch_kernel(const CUtensorMap& tq, const CUtensorMap& tk, const CUtensorMap& tv, const RaggedParams& p, const ScoreScale& sc, int grid,
+                  cudaStream_t stream) {
+  auto kern = ragged_attn_kernel<D, LOG2N, HILO, PAGED>;
+  static PerDeviceOnce configured;
+  if (int rc = configured.run([&] { return cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, int(smem_bytes<D>())); })) return rc;
+  ALG_CUDA_TRY(launch_dependent(kern, dim3(grid), dim3(NTHREADS), smem_bytes<D>(), stream, tq, tk, tv, p, sc));
+  count_launch();
+  return ALG_OK;
+}
+
+template <int D>
+int launch_d(const RaggedParams& p, cudaStream_t stream) {
+  CUtensorMap tq, tk, tv;
+  const uint64_t tokens = uint64_t(p.seqs.tokens);
+  {
+    const uint64_t dims[4] = {64, uint64_t(p.H), tokens, uint64_t(D / 64)};
+    const uint64_t strides[3] = {uint64_t(p.qs.h), uint64_t(p.qs.t), 64};
+    const uint32_t box[4] = {64, uint32_t(p.G), uint32_t(p.tile_tokens), 1};
+    if (int rc = make_tmap_bf16(&tq, p.q, 4, dims, strides, box, true)) return rc;
+  }
+  for (int i = 0; i < 2; ++i) {
+    const Strides2& s = i == 0 ? p.ks : p.vs;
+    const void* base = i == 0 ? p.k : p.v;
+    CUtensorMap* tm = i == 0 ? &tk : &tv;
+    if (p.table != nullptr) {
+      const uint64_t dims[5] = {64, uint64_t(p.page), uint64_t(D / 64), uint64_t(p.Hkv), uint64_t(p.pages)};
+      const uint64_t strides[4] = {uint64_t(s.t), 64, uint64_t(s.h), uint64_t(i == 0 ? p.k_page : p.v_page)};
+      const uint32_t box[5] = {64, uint32_t(std::min(p.page, BKEY)), 1, 1, 1};
+      if (int rc = make_tmap_bf16(tm, base, 5, dims, strides, box, true)) return rc;
+    } else {
+      const uint64_t dims[4] = {64, tokens, uint64_t(D / 64), uint64_t(p.Hkv)};
+      const uint64_t strides[3] = {uint64_t(s.t), 64, uint64_t(s.h)};
+      const uint32_t box[4] = {64, uint32_t(BKEY), uint32_t(D / 64), 1};
+      if (int rc = make_tmap_bf16(tm, base, 4, dims, strides, box, true)) return rc;
+    }
+  }
+  ScoreScale sc;
+  const int n = 1 << p.log2n;
+  {
+    int ex = 0;
+    const double f = frexp(double(p.scale), &ex);         // scale = f 2^ex = 2^(ex - 1) m, 1 <= m < 2
+    const double m = 2.0 * f;
+    sc.pow2 = float(ldexp(1.0, ex - 1));
+    sc.m = float(m); sc.inv_m = float(1.0 / m); sc.kappa = float(1.0 / (m * m));
+    const double rho = pow(2.0, 64.0 / n);                // rho(x_fast)^n = 2^64
+    sc.y_fast = float(std::min(8.0, 0.5 * (rho - 1.0 / rho)) / m);
+  }
+  const int64_t most = int64_t(p.plan.max_items) * p.Hkv;
+  const int grid = int(std::min<int64_t>(most, p.plan.sms));
+  const bool hilo = p.o_lo != nullptr, paged = p.table != nullptr;
+  int rc;
+  if (p.log2n == 4) {
+    if (paged) rc = launch_kernel<D, 4, false, true>(tq, tk, tv, p, sc, grid, stream);
+    else if (hilo) rc = launch_kernel<D, 4, true, false>(tq, tk, tv, p, sc, grid, stream);
+    else rc = launch_kernel<D, 4, false, false>(tq, tk, tv, p, sc, grid, stream);
+  } else {
+    if (paged) rc = launch_kernel<D, 0, false, true>(tq, tk, tv, p, sc, grid, stream);
+    else if (hilo) rc = launch_kernel<D, 0, true, false>(tq, tk, tv, p, sc, grid, stream);
+    else rc = launch_kernel<D, 0, false, false>(tq, tk, tv, p, sc, grid, stream);
+  }
+  if (rc) return rc;
+  if (p.plan.max_slots > 0) {
+    const int blocks = int(std::min<int64_t>(int64_t(p.plan.max_combos) * p.Hkv * 8, int64_t(p.plan.sms) * 4));
+    ALG_CUDA_TRY(launch_dependent(ragged_combine_kernel<D>, dim3(std::max(blocks, 1)), dim3(256), 0, stream, p, sc));
+    count_launch();
+  }
+  return ALG_OK;
+}
+
+}  // namespace
+
+int launch_ragged_attention(const RaggedParams& p, cudaStream_t stream) {
+  if (int rc = launch_ragged_plan(p.seqs, p.plan, p.G, stream)) return rc;
+  return p.D == 64 ? launch_d<64>(p, stream) : launch_d<128>(p, stream);
+}
+
+}  // namespace alg

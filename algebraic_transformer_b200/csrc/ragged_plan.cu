@@ -1,0 +1,214 @@
+// The plan of a ragged attention call: one CTA reads the lengths and writes the work items, longest first.
+//
+// An item is two query tiles (2 * 128 / G tokens) of one sequence; heads are not listed, the attention kernel takes every entry
+// once per key head.  Entries are placed by a counting sort over 1024 classes of their length in key tiles, so a
+// longest-first deal from a counter leaves the CTAs level to about one short item.  Where the longest items would outlast
+// an even share of the work (few long sequences), items are cut along the keys into parts whose accumulators a second
+// kernel adds up.  Order within a class varies from run to run; results do not depend on it.
+#include "common.cuh"
+#include "ragged.cuh"
+
+namespace alg {
+namespace {
+
+constexpr int NT = 1024, CLASSES = 1024;
+// A part is at least this many key tiles long: a part writes its accumulator and the combine kernel reads it back, which
+// is the traffic of about four key tiles.
+constexpr int MIN_PART = 8, MAX_PARTS = 64;
+
+__device__ __forceinline__ int block_scan(int v, int* warp_sums, int* total) {   // exclusive; all NT threads
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  int inc = v;
+#pragma unroll
+  for (int o = 1; o < 32; o <<= 1) {
+    const int u = __shfl_up_sync(0xffffffffu, inc, o);
+    if (lane >= o) inc += u;
+  }
+  __syncthreads();                                     // warp_sums of the call before are read
+  if (lane == 31) warp_sums[warp] = inc;
+  __syncthreads();
+  if (warp == 0) {
+    int w = warp_sums[lane], s = w;
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+      const int u = __shfl_up_sync(0xffffffffu, s, o);
+      if (lane >= o) s += u;
+    }
+    warp_sums[lane] = s - w;
+    if (lane == 31) warp_sums[32] = s;
+  }
+  __syncthreads();
+  *total = warp_sums[32];
+  return warp_sums[warp] + inc - v;
+}
+
+// prefix[s] = blocks of the sequences before s; returns their sum.  Saturates far above any list's size.
+__device__ int sequence_blocks(const RaggedSeqs& q, int block_tokens, int* prefix, int* warp_sums) {
+  int base = 0;
+  for (int s0 = 0; s0 < q.S; s0 += NT) {
+    const int s = s0 + int(threadIdx.x);
+    int n = 0;
+    if (s < q.S) {
+      int row0, Lq, Lk;
+      ragged_lengths(q, s, row0, Lq, Lk);
+      n = (Lq + block_tokens - 1) / block_tokens;
+    }
+    int total;
+    const int at = block_scan(n, warp_sums, &total);
+    if (s < q.S) prefix[s] = min(base + at, 1 << 29);
+    base = min(base + min(total, 1 << 29), 1 << 29);
+  }
+  if (threadIdx.x == 0) prefix[q.S] = base;
+  __syncthreads();
+  return base;
+}
+
+// the sequence of block i: the last s with prefix[s] <= i that has blocks
+__device__ __forceinline__ int sequence_of(const int* prefix, int S, int i) {
+  int lo = 0, hi = S;                                  // prefix[lo] <= i < prefix[hi]
+  while (hi - lo > 1) {
+    const int mid = (lo + hi) >> 1;
+    if (prefix[mid] <= i) lo = mid; else hi = mid;
+  }
+  return lo;
+}
+
+__global__ void __launch_bounds__(NT) ragged_plan_kernel(const RaggedSeqs q, const RaggedPlan plan) {
+  __shared__ int warp_sums[33], hist[CLASSES], s_max, s_target, s_slots, s_combos, s_parts;
+  __shared__ unsigned long long s_cost;
+  griddep_wait();                                      // the workspace may be another call's until here
+  hist[threadIdx.x] = 0;
+  if (threadIdx.x == 0) { s_max = 1; s_cost = 0; s_slots = 0; s_combos = 0; }
+  const int n = min(sequence_blocks(q, plan.block_tokens, plan.prefix, warp_sums), plan.max_items);
+
+  struct Block { int row0, Lq, Lk, seq, t0, n1, cost; };
+  auto block_at = [&](int i) {
+    Block b;
+    b.seq = sequence_of(plan.prefix, q.S, i);
+    ragged_lengths(q, b.seq, b.row0, b.Lq, b.Lk);
+    b.t0 = (i - plan.prefix[b.seq]) * plan.block_tokens;
+    b.n1 = ragged_tiles(b.Lq, b.Lk, b.t0 + plan.block_tokens);
+    b.cost = b.n1 + (b.Lq - b.t0 > plan.block_tokens / 2 ? ragged_tiles(b.Lq, b.Lk, b.t0 + plan.block_tokens / 2) : 0);
+    return b;
+  };
+
+  Block mine;                                          // a thread's first block; the others are worked out anew in every pass
+  {
+    unsigned long long cost = 0;
+    int longest = 1;
+    for (int i = threadIdx.x; i < n; i += NT) {
+      const Block b = block_at(i);
+      if (i < NT) mine = b;
+      cost += b.cost;
+      longest = max(longest, b.n1);
+    }
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) cost += __shfl_xor_sync(0xffffffffu, cost, o);
+    longest = __reduce_max_sync(0xffffffffu, longest);
+    if ((threadIdx.x & 31) == 0) { atomicAdd(&s_cost, cost); atomicMax(&s_max, longest); }
+  }
+  __syncthreads();
+  const int longest = s_max;
+
+  // parts: an item above an even share of the work is cut into parts of about half a share, of MIN_PART tiles at
+  // least, if the slots hold all the parts (else the parts grow)
+  int target = 1 << 30;                                // key tiles of a part
+  if (plan.max_slots > 0) {
+    const unsigned long long share = s_cost * plan.heads / plan.sms + 1;        // score tiles a CTA would have
+    if ((unsigned long long)longest * 2 > share) {
+      target = max(MIN_PART, int(min(share / 4 + 1, 1ull << 28)));
+      for (;;) {
+        __syncthreads();
+        if (threadIdx.x == 0) s_parts = 0;
+        __syncthreads();
+        int parts = 0;
+        for (int i = threadIdx.x; i < n; i += NT) {
+          const int n1 = i < NT ? mine.n1 : block_at(i).n1;
+          const int p = min((n1 + target - 1) / target, MAX_PARTS);
+          if (p > 1) parts += p;
+        }
+        parts = __reduce_add_sync(0xffffffffu, parts);
+        if ((threadIdx.x & 31) == 0 && parts) atomicAdd(&s_parts, parts);
+        __syncthreads();
+        if (s_parts <= plan.max_slots || target >= (1 << 28)) break;
+        target *= 2;
+      }
+    }
+  }
+  auto parts_of = [&](int n1) { return min((n1 + target - 1) / target, MAX_PARTS); };
+  auto class_of = [&](int nk) { return CLASSES - 1 - int(int64_t(nk) * (CLASSES - 1) / longest); };
+  for (int i = threadIdx.x; i < n; i += NT) {
+    const int n1 = i < NT ? mine.n1 : block_at(i).n1, parts = parts_of(n1);
+    atomicAdd(&hist[class_of((n1 + parts - 1) / parts)], parts);
+  }
+  __syncthreads();
+  int total;
+  const int start = block_scan(hist[threadIdx.x], warp_sums, &total);
+  __syncthreads();
+  hist[threadIdx.x] = start;                           // from now on: the next place of the class
+  __syncthreads();
+  for (int i = threadIdx.x; i < n; i += NT) {
+    const Block b = i < NT ? mine : block_at(i);
+    const int parts = parts_of(b.n1);
+    int at = atomicAdd(&hist[class_of((b.n1 + parts - 1) / parts)], parts);
+    int slot = -1;
+    if (parts > 1) {
+      slot = atomicAdd(&s_slots, parts);
+      const int c = atomicAdd(&s_combos, 1);
+      if (c < plan.max_combos) plan.combos[c] = RaggedCombo{b.row0, b.Lq, b.Lk, b.t0, slot, parts, 0, 0};
+    }
+    for (int pt = 0; pt < parts; ++pt, ++at) {
+      const int k0 = int(int64_t(b.n1) * pt / parts), k1 = int(int64_t(b.n1) * (pt + 1) / parts);
+      if (at < plan.max_items) plan.items[at] = RaggedItem{b.row0, b.Lq, b.Lk, b.seq, b.t0, k0, k1 - k0, parts > 1 ? slot + pt : -1};
+    }
+  }
+  __syncthreads();
+  if (threadIdx.x == 0) *plan.header = RaggedHeader{min(total, plan.max_items), min(s_combos, plan.max_combos), 0, 0};
+}
+
+constexpr size_t align256(size_t x) { return (x + 255) & ~size_t(255); }
+
+struct Sizes { int items, slots, combos; };
+Sizes plan_sizes(int S, int tokens, int G, int Hkv, bool may_split) {
+  const int block = 2 * (128 / G);
+  Sizes z{};
+  // parts of at least MIN_PART tiles and half a share of one of the CTAs: two or three times the CTAs, per head
+  z.slots = may_split ? (3 * sm_count() + Hkv - 1) / Hkv : 0;
+  z.combos = z.slots / 2;
+  z.items = tokens / block + (S < tokens ? S : tokens) + z.slots + 1;
+  return z;
+}
+
+}  // namespace
+
+size_t ragged_plan_bytes(int S, int tokens, int Hkv, int G, int D, bool may_split) {
+  const Sizes z = plan_sizes(S, tokens, G, Hkv, may_split);
+  return 256 + align256(size_t(z.items) * sizeof(RaggedItem)) + align256(size_t(z.combos) * sizeof(RaggedCombo)) +
+         align256((size_t(S) + 1) * sizeof(int)) + size_t(z.slots) * Hkv * 256 * (D + 4) * sizeof(float);
+}
+
+void ragged_plan_carve(RaggedPlan* plan, void* workspace, int S, int tokens, int Hkv, int G, int D, bool may_split) {
+  const Sizes z = plan_sizes(S, tokens, G, Hkv, may_split);
+  unsigned char* at = static_cast<unsigned char*>(workspace);
+  plan->header = reinterpret_cast<RaggedHeader*>(at);
+  at += 256;
+  plan->items = reinterpret_cast<RaggedItem*>(at);
+  at += align256(size_t(z.items) * sizeof(RaggedItem));
+  plan->combos = reinterpret_cast<RaggedCombo*>(at);
+  at += align256(size_t(z.combos) * sizeof(RaggedCombo));
+  plan->prefix = reinterpret_cast<int*>(at);
+  at += align256((size_t(S) + 1) * sizeof(int));
+  plan->slots = reinterpret_cast<float*>(at);
+  plan->max_items = z.items; plan->max_combos = z.combos; plan->max_slots = z.slots;
+  plan->block_tokens = 2 * (128 / G);
+  plan->heads = Hkv;
+  plan->sms = sm_count();
+}
+
+int launch_ragged_plan(const RaggedSeqs& seqs, const RaggedPlan& plan, int G, cudaStream_t stream) {
+  ALG_CUDA_TRY(launch_dependent(ragged_plan_kernel, dim3(1), dim3(NT), 0, stream, seqs, plan));
+  count_launch();
+  return ALG_OK;
+}
+
+}  // namespace alg

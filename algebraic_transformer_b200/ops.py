@@ -593,6 +593,137 @@ def decode_attention(q, k, v, sink_logit=None, *, n: int = 16, c: float = 8.0, o
     return o
 
 
+# -------------------------------------------------------- packed sequences, paged cache
+
+def _strides2(t: torch.Tensor):
+    if t.stride(-1) != 1:
+        raise ValueError("the last (head_dim) axis must be contiguous")
+    return L.I64x2(t.stride(0), t.stride(1))
+
+
+def _check_lengths(name: str, t: torch.Tensor, count: Optional[int]):
+    if t.dtype != torch.int32 or t.ndim != 1 or not t.is_contiguous() or (t.numel() < 1 if count is None else t.numel() != count):
+        raise ValueError(f"{name} must be a contiguous int32 vector" + ("" if count is None else f" of {count}"))
+
+
+def _check_link(n: int, c: float):
+    if n < 2 or n & (n - 1):
+        raise ValueError("asinh kernel needs n to be a power of two")
+    if not math.isfinite(c) or c <= 0:
+        raise ValueError("asinh scale c must be positive and finite")
+
+
+def _check_packed(q, k, v):
+    if q.ndim != 3 or k.ndim != 3 or k.shape != v.shape or k.shape[0] != q.shape[0] or k.shape[2] != q.shape[2]:
+        raise ValueError("q must be (tokens, H, D) and k, v (tokens, Hkv, D)")
+    if any(t.dtype != torch.bfloat16 for t in (q, k, v)):
+        raise ValueError("attention over packed sequences takes bfloat16 tensors")
+    if k.shape[1] < 1 or q.shape[1] < 1 or q.shape[1] % k.shape[1]:
+        raise ValueError("query heads must be a multiple of the key heads")
+
+
+def _output_like(q, out):
+    if out is None:
+        return torch.empty(q.shape, dtype=q.dtype, device=q.device)
+    if out.shape != q.shape or out.dtype != q.dtype:
+        raise ValueError("out must have the shape and type of q")
+    return out
+
+
+@_on_tensor_device
+def packed_attention(q, k, v, cu_seqlens, sink_logit=None, *, n: int = 16, c: float = 8.0, return_stat: bool = False, out=None):
+    """Causal asinh-power attention of sequences of different lengths that lie one behind the other: q (tokens, H, D), k and v
+    (tokens, Hkv, D) bf16, D = 64 or 128 contiguous, H a multiple of Hkv (query heads share key heads in groups of H / Hkv,
+    up to 128).  `cu_seqlens`: int32 (sequences + 1) on the device; sequence s is rows cu_seqlens[s] to cu_seqlens[s + 1] and may
+    be empty.  `sink_logit` broadcastable to (H,).  The weights are those of `flash_attention(kind="asinh")`, for any
+    scores (no range guard is needed).  Rows of no sequence: zeros, or, where `out` is given, left as they are.
+
+    The lengths are read on the device only, so a captured call can be replayed with others; rows beyond the
+    tensors are never touched whatever they say.  A NaN or infinite key or value stays within its sequence, where it may also reach
+    earlier queries of the same 128-row tile.
+
+    `return_stat=True` (training) returns `(o, stat, rest)` for `packed_attention_backward`: stat (H, tokens) float32, a with
+    p = (rho(x) a)^n, and rest, what the rounding to o left over, in bf16."""
+    _require_cuda(q, k, v, cu_seqlens)
+    _check_packed(q, k, v)
+    _check_link(n, c)
+    _check_lengths("cu_seqlens", cu_seqlens, None)
+    T, H, D = q.shape
+    sink = None
+    if sink_logit is not None:
+        sink = _sink_vector(sink_logit, H, q.device)
+        if sink.numel() != H:
+            raise ValueError("sink_logit must broadcast to (H,)")
+    o = _output_like(q, out)
+    stat = torch.empty((H, T), dtype=torch.float32, device=q.device) if return_stat else None
+    rest = torch.empty((T, H, D), dtype=q.dtype, device=q.device) if return_stat else None
+    a = L.PackedAttnArgs(q=q.data_ptr(), k=k.data_ptr(), v=v.data_ptr(), o=o.data_ptr(), cu_seqlens=cu_seqlens.data_ptr(),
+                         sink=_ptr(sink), stat=_ptr(stat), o_rest=_ptr(rest), sequences=cu_seqlens.numel() - 1, tokens=T, H=H,
+                         Hkv=k.shape[1], D=D, n=int(n), c=float(c), zero_tail=int(out is None), q_stride=_strides2(q),
+                         k_stride=_strides2(k), v_stride=_strides2(v), o_stride=_strides2(o))
+    if T:
+        lib = L.load()
+        ws = _workspace(q.device, lib.alg_packed_attn_workspace_bytes(a), "packed")
+        a.workspace, a.workspace_bytes = ws.data_ptr(), ws.numel()
+        L.check(lib.alg_packed_attn_fwd(a, _stream()))
+    return (o, stat, rest) if return_stat else o
+
+
+def _check_pages(q, k_pages, v_pages, block_table, kv_lens, cu_seqlens):
+    if q.ndim != 3 or k_pages.ndim != 4 or k_pages.shape != v_pages.shape or k_pages.shape[3] != q.shape[2]:
+        raise ValueError("q must be (tokens, H, D) and k_pages, v_pages (pages, page_size, Hkv, D)")
+    if any(t.dtype != torch.bfloat16 for t in (q, k_pages, v_pages)):
+        raise ValueError("attention over a paged cache takes bfloat16 tensors")
+    if k_pages.shape[2] < 1 or q.shape[1] < 1 or q.shape[1] % k_pages.shape[2]:
+        raise ValueError("query heads must be a multiple of the key heads")
+    if block_table.dtype != torch.int32 or block_table.ndim != 2 or block_table.stride(1) != 1:
+        raise ValueError("block_table must be int32 (sequences, pages of a sequence) with contiguous rows")
+    S = block_table.shape[0]
+    _check_lengths("kv_lens", kv_lens, S)
+    if cu_seqlens is not None:
+        _check_lengths("cu_seqlens", cu_seqlens, S + 1)
+    elif q.shape[0] != S:
+        raise ValueError("without cu_seqlens every sequence has one new token")
+    return S
+
+
+@_on_tensor_device
+def paged_attention(q, k_pages, v_pages, block_table, kv_lens, cu_seqlens=None, sink_logit=None, *, n: int = 16, c: float = 8.0,
+                    out=None):
+    """Causal asinh-power attention of the newest tokens of many sequences against a cache in pages.  q (tokens, H, D) bf16;
+    k_pages, v_pages (pages, page_size, Hkv, D) bf16, page_size a power of two from 16 on; `block_table` int32 (sequences, width): key
+    j of sequence s lies in page block_table[s, j // page_size]; `kv_lens` int32 (sequences): the keys of each, the new tokens'
+    own among them (`paged_append` writes them).  `cu_seqlens` int32 (sequences + 1): the rows of q of each sequence, a chunk of any
+    length; None: one token a sequence, the form for generation.  Token i of a chunk of m sees keys 0 to kv_len - m + i; one
+    that sees none, as of a sequence of length 0, has the output zero.
+
+    Lengths and table are read on the device only (a captured call can be replayed with others).  Lengths are clamped to the
+    table's width, a page number outside the pool reads as zeros, entries behind a length and rows behind a sequence's end are
+    not looked at.  Rows of no sequence: zeros, or, where `out` is given, left as they are."""
+    _require_cuda(q, k_pages, v_pages, block_table, kv_lens, cu_seqlens)
+    S = _check_pages(q, k_pages, v_pages, block_table, kv_lens, cu_seqlens)
+    _check_link(n, c)
+    T, H, D = q.shape
+    sink = None
+    if sink_logit is not None:
+        sink = _sink_vector(sink_logit, H, q.device)
+        if sink.numel() != H:
+            raise ValueError("sink_logit must broadcast to (H,)")
+    o = _output_like(q, out)
+    a = L.PagedAttnArgs(q=q.data_ptr(), k_pages=k_pages.data_ptr(), v_pages=v_pages.data_ptr(), o=o.data_ptr(),
+                        block_table=block_table.data_ptr(), kv_lens=kv_lens.data_ptr(), cu_seqlens=_ptr(cu_seqlens), sink=_ptr(sink),
+                        sequences=S, tokens=T, H=H, Hkv=k_pages.shape[2], D=D, pages=k_pages.shape[0], page_size=k_pages.shape[1],
+                        table_width=block_table.shape[1], n=int(n), c=float(c), zero_tail=int(out is None),
+                        table_stride=block_table.stride(0), q_stride=_strides2(q), k_stride=_strides3(k_pages),
+                        v_stride=_strides3(v_pages), o_stride=_strides2(o))
+    if T:
+        lib = L.load()
+        ws = _workspace(q.device, lib.alg_paged_attn_workspace_bytes(a), "paged")
+        a.workspace, a.workspace_bytes = ws.data_ptr(), ws.numel()
+        L.check(lib.alg_paged_attn_fwd(a, _stream()))
+    return o
+
+
 # ----------------------------------------------------------------------------- head
 
 @_on_tensor_device

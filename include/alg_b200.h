@@ -253,6 +253,73 @@ ALG_API int alg_attn_decode(const alg_decode_args* args, void* stream);
 ALG_API int alg_attn_decode_status(const alg_decode_args* args, int* status, void* stream);
 
 /* ------------------------------------------------------------------------------------
+ * Causal asinh-power attention over packed sequences of different lengths, grouped heads (no counterpart in
+ * the reference, whose batches have one length; the weights are asinh_power_weights,
+ * src/algebraic/algebraic.py:186-204).
+ * q, o: (tokens, H, D), k, v: (tokens, Hkv, D) bf16, D contiguous, 64 or 128; strides: elements of (token, head),
+ * multiples of 8.  H a multiple of Hkv; query heads [g H/Hkv, (g + 1) H/Hkv) share key head g.  cu_seqlens:
+ * (sequences + 1) device ints; sequence s is rows [cu[s], cu[s+1]) and may be empty.  The host does not read them:
+ * values outside the tensors are clamped to them, rows of no sequence are left as they are (zero_tail: rows before
+ * the first and behind the last sequence are written as zeros).  Any scores: tiles whose scores leave the range of the
+ * unshifted weights take the max-shifted form by themselves.  sink: (H) fp32 or NULL.
+ * stat, o_rest: both or neither; what alg_packed_attn_bwd takes.  stat: (H, tokens) fp32, the a with p = (rho(x) a)^n;
+ * o_rest: (tokens, H, D) dense bf16, what the rounding to o left over (the products then carry 16 bits of the weights).
+ * A key or value that is NaN or infinite reaches the queries of its own sequence only; among these it may
+ * reach earlier ones of the same 128-row tile.
+ * ---------------------------------------------------------------------------------- */
+typedef struct {
+  const void* q;
+  const void* k;
+  const void* v;
+  void* o;
+  const int* cu_seqlens;
+  const float* sink;
+  float* stat;
+  void* o_rest;
+  int sequences, tokens, H, Hkv, D;
+  int n;
+  float c;
+  int zero_tail;
+  int64_t q_stride[2], k_stride[2], v_stride[2], o_stride[2];
+  void* workspace;
+  size_t workspace_bytes;
+  int* status;             /* device int, may be NULL */
+} alg_packed_attn_args;
+ALG_API size_t alg_packed_attn_workspace_bytes(const alg_packed_attn_args* args);
+ALG_API int alg_packed_attn_fwd(const alg_packed_attn_args* args, void* stream);
+
+/* The same over a cache in pages: queries are the last tokens of their sequences, the keys of all of a sequence's tokens (the new
+ * ones too) lie in the pool's pages.
+ * k_pages, v_pages: (pages, page_size, Hkv, D) bf16, strides of (page, token, head); page_size a power of two from 16
+ * on.  block_table: (sequences, table_width) device ints, row stride table_stride: key j of sequence s is in page
+ * block_table[s][j / page_size].  A page number outside the pool reads as zeros.  kv_lens: (sequences) device ints, clamped to
+ * table_width page_size; entries of the table behind them are not read.  cu_seqlens: (sequences + 1) device ints, the
+ * new tokens' rows of q and o, or NULL: one token a sequence (tokens == sequences).  Token i of Lq sees keys [0, kv_len - Lq + i]; a
+ * token that sees none has the output zero. */
+typedef struct {
+  const void* q;
+  const void* k_pages;
+  const void* v_pages;
+  void* o;
+  const int* block_table;
+  const int* kv_lens;
+  const int* cu_seqlens;
+  const float* sink;
+  int sequences, tokens, H, Hkv, D;
+  int pages, page_size, table_width;
+  int n;
+  float c;
+  int zero_tail;
+  int64_t table_stride;
+  int64_t q_stride[2], k_stride[3], v_stride[3], o_stride[2];
+  void* workspace;
+  size_t workspace_bytes;
+  int* status;             /* device int, may be NULL */
+} alg_paged_attn_args;
+ALG_API size_t alg_paged_attn_workspace_bytes(const alg_paged_attn_args* args);
+ALG_API int alg_paged_attn_fwd(const alg_paged_attn_args* args, void* stream);
+
+/* ------------------------------------------------------------------------------------
  * Fused Alg-CE head, forward, over one vocabulary shard.
  * Replaces: fused_head(h, embed, targets, kind="alg_ce", n, c)
  *                                               src/algebraic/kernels/fused_head.py:260-275

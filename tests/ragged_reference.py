@@ -1,0 +1,87 @@
+"""Attention over packed sequences and paged caches from its definition, in 64 bits on the CPU, one (sequence, head) at a time, and
+what the kernels' roundings can add to it."""
+
+import torch
+
+BF16 = 2.0 ** -8          # half a step of bfloat16, relative
+
+
+def rho(x):
+    root = torch.sqrt(1.0 + x * x)
+    return torch.where(x >= 0, x + root, 1.0 / (root - x))
+
+
+def lengths_to_cu(lens, start=0):
+    cu = [start]
+    for n in lens:
+        cu.append(cu[-1] + n)
+    return torch.tensor(cu, dtype=torch.int32)
+
+
+def attend(q, k, v, sink, first, n, c):
+    """q (Lq, D), k, v (Lk, D) float64, token i at position first + i.  Returns (o, spread): spread is
+    sum_j p_ij |v_j|, what a relative error of the weights is multiplied by."""
+    Lq, D = q.shape
+    x = (q @ k.t()) / (D ** 0.5 * c)
+    a = n * torch.asinh(x)                                        # rho = exp(asinh)
+    a = a.masked_fill(torch.arange(k.shape[0])[None] > first + torch.arange(Lq)[:, None], -float("inf"))
+    b = torch.full((Lq, 1), -float("inf"), dtype=torch.float64) if sink is None else (n * torch.asinh(sink.double() / c)).expand(Lq, 1)
+    top = torch.cat([a, b], dim=1).amax(dim=1, keepdim=True)
+    empty = top == -float("inf")
+    top = torch.where(empty, torch.zeros_like(top), top)
+    w, ws = torch.exp(a - top), torch.exp(b - top)
+    p = torch.where(empty, torch.zeros_like(w), w / (w.sum(1, keepdim=True) + ws))
+    seen = (p != 0).any(dim=0)                                    # a key that no token sees may hold anything
+    v = torch.where(seen[:, None], v, torch.zeros_like(v))
+    return p @ v, p @ v.abs()
+
+
+def weight_error(q, k, n, c):
+    """Relative error of a weight formed in 32 bits: n times that of rho(x), x from a dot product of D terms."""
+    D = q.shape[-1]
+    size = q.norm(dim=-1).max() * k.norm(dim=-1).max() if k.numel() and q.numel() else torch.zeros(())
+    return float(n * (D * 2.0 ** -24 * size / (D ** 0.5 * c) + 2.0 ** -20))
+
+
+def packed(q, k, v, cu, sink, n, c):
+    """(o, spread, weight error), (T, H, D) and a number; rows of no sequence are zero."""
+    q, k, v = (t.double().cpu() for t in (q, k, v))
+    H, Hkv = q.shape[1], k.shape[1]
+    o, spread, err = torch.zeros_like(q), torch.zeros_like(q), 0.0
+    for a, b in zip(cu[:-1].tolist(), cu[1:].tolist()):
+        for h in range(H):
+            if b > a:
+                g = h // (H // Hkv)
+                o[a:b, h], spread[a:b, h] = attend(q[a:b, h], k[a:b, g], v[a:b, g], None if sink is None else sink[h].cpu(), 0, n, c)
+                err = max(err, weight_error(q[a:b, h], k[a:b, g], n, c))
+    return o, spread, err
+
+
+def paged(q, k_pages, v_pages, table, lens, cu, sink, n, c):
+    q, k_pages, v_pages, table = q.double().cpu(), k_pages.double().cpu(), v_pages.double().cpu(), table.cpu()
+    H, (pages, page, Hkv, D) = q.shape[1], k_pages.shape
+    o, spread, err = torch.zeros_like(q), torch.zeros_like(q), 0.0
+    for s, length in enumerate(lens):
+        a, b = (s, s + 1) if cu is None else (int(cu[s]), int(cu[s + 1]))
+        at = table[s, : -(-length // page)].long()
+        inside = (at >= 0) & (at < pages)
+        for g in range(Hkv):
+            k, v = (torch.where(inside[:, None, None], t[at.clamp(0, pages - 1), :, g], torch.zeros((), dtype=torch.float64))
+                    .reshape(-1, D)[:length] for t in (k_pages, v_pages))
+            for h in range(g * H // Hkv, (g + 1) * H // Hkv):
+                if b > a:
+                    o[a:b, h], spread[a:b, h] = attend(q[a:b, h], k, v, None if sink is None else sink[h].cpu(), length - (b - a), n, c)
+                    err = max(err, weight_error(q[a:b, h], k, n, c))
+    return o, spread, err
+
+
+def assert_close(got, o, spread, err, weights=BF16, result=BF16):
+    """|got - o| within: the weights' rounding (`weights`) and 32-bit error (`err`) times sum p |v|, the result's own rounding."""
+    got = got.detach().double().cpu()
+    if got.numel() == 0:
+        return
+    bound = (weights + 2 * err) * 1.01 * spread + result * 1.01 * (o.abs() + (weights + 2 * err) * spread) + 1e-30
+    off = (got - o).abs()
+    assert torch.isfinite(got).all(), f"{int((~torch.isfinite(got)).sum())} values are not finite"
+    worst = float((off / bound).max())
+    assert worst <= 1.0, f"{worst} times the bound, at {torch.nonzero(off / bound == (off / bound).max())[0].tolist()}"
