@@ -116,6 +116,15 @@ class PagedAttnArgs(C.Structure):
                 ("status", C.c_void_p)]
 
 
+class PagedAppendArgs(C.Structure):
+    _fields_ = [(name, C.c_void_p) for name in ("q", "k", "v", "q_out", "k_pages", "v_pages", "block_table", "kv_lens", "cu_seqlens",
+                                                "q_gain", "k_gain", "cos", "sin")] + \
+               [(name, C.c_int) for name in ("sequences", "tokens", "H", "Hkv", "D", "pages", "page_size", "table_width", "table_rows",
+                                             "table_dtype")] + \
+               [("eps", C.c_float), ("zero_tail", C.c_int), ("table_stride", C.c_int64), ("q_stride", I64x2), ("k_stride", I64x2),
+                ("v_stride", I64x2), ("o_stride", I64x2), ("kp_stride", I64x3), ("vp_stride", I64x3)]
+
+
 class HeadArgs(C.Structure):
     _fields_ = [("h", C.c_void_p), ("e", C.c_void_p), ("targets", C.c_void_p), ("l_out", C.c_void_p),
                 ("zt_out", C.c_void_p), ("N", C.c_int), ("d", C.c_int), ("V_local", C.c_int),
@@ -157,6 +166,7 @@ SYMBOLS = {
     "alg_packed_attn_fwd": (C.c_int, [C.POINTER(PackedAttnArgs), C.c_void_p]),
     "alg_paged_attn_workspace_bytes": (C.c_size_t, [C.POINTER(PagedAttnArgs)]),
     "alg_paged_attn_fwd": (C.c_int, [C.POINTER(PagedAttnArgs), C.c_void_p]),
+    "alg_paged_append": (C.c_int, [C.POINTER(PagedAppendArgs), C.c_void_p]),
     "alg_head_workspace_bytes": (C.c_size_t, [C.POINTER(HeadArgs)]),
     "alg_head_fwd": (C.c_int, [C.POINTER(HeadArgs), C.c_void_p]),
     "alg_head_fwd_static": (C.c_int, [C.POINTER(HeadArgs), C.c_void_p]),

@@ -102,6 +102,30 @@ struct RaggedParams {
   int* status;
 };
 
+struct AppendParams {
+  RaggedSeqs seqs;
+  const __nv_bfloat16* q;
+  const __nv_bfloat16* k;
+  const __nv_bfloat16* v;
+  __nv_bfloat16* q_out;
+  __nv_bfloat16* k_pages;
+  __nv_bfloat16* v_pages;
+  const float* q_gain;      // (D) or nullptr
+  const float* k_gain;
+  const void* cos;          // (>= capacity, D / 2)
+  const void* sin;
+  Strides2 qs, ks, vs, os, kps, vps;
+  int64_t k_page, v_page;
+  const int* table;
+  int64_t table_stride;
+  int page, log2_page, pages;
+  int H, Hkv, D;
+  int table_dtype;          // of cos and sin: ALG_BF16 or ALG_F32
+  float eps;
+  int zero_tail;
+};
+int launch_paged_append(const AppendParams& p, cudaStream_t stream);
+
 size_t ragged_plan_bytes(int S, int tokens, int Hkv, int G, int D, bool may_split);
 void ragged_plan_carve(RaggedPlan* plan, void* workspace, int S, int tokens, int Hkv, int G, int D, bool may_split);
 int launch_ragged_plan(const RaggedSeqs& seqs, const RaggedPlan& plan, int G, cudaStream_t stream);

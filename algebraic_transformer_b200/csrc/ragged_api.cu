@@ -86,7 +86,9 @@ int alg_packed_attn_fwd(const alg_packed_attn_args* a, void* stream_) {
   return launch_ragged_attention(p, stream);
 }
 
-static int paged_checks(const alg_paged_attn_args* a, const char* what) {
+}  // extern "C"
+
+template <class Args> static int paged_checks(const Args* a, const char* what) {
   if (a->tokens < 0 || a->sequences < 0 || a->pages < 1 || a->table_width < 0) { set_error("%s: bad extents", what); return ALG_ERR_INVALID; }
   if (a->page_size < 16 || a->page_size > 32768 || ilog2_exact(a->page_size) < 0) {
     set_error("%s: pages of a power of two of tokens, at least 16, got %d", what, a->page_size);
@@ -97,6 +99,8 @@ static int paged_checks(const alg_paged_attn_args* a, const char* what) {
   if (a->cu_seqlens == nullptr && a->tokens != a->sequences) { set_error("%s: without cu_seqlens every sequence has one token", what); return ALG_ERR_INVALID; }
   return ALG_OK;
 }
+
+extern "C" {
 
 size_t alg_paged_attn_workspace_bytes(const alg_paged_attn_args* a) {
   if (a == nullptr || a->H < 1 || a->Hkv < 1 || a->H % a->Hkv != 0 || a->H / a->Hkv > 128 || a->tokens < 0 || a->sequences < 0) return 0;
@@ -144,6 +148,47 @@ int alg_paged_attn_fwd(const alg_paged_attn_args* a, void* stream_) {
   p.zero_tail = a->zero_tail != 0 && a->cu_seqlens != nullptr;
   p.status = a->status;
   return launch_ragged_attention(p, stream);
+}
+
+int alg_paged_append(const alg_paged_append_args* a, void* stream_) {
+  if (a == nullptr || a->q == nullptr || a->k == nullptr || a->v == nullptr || a->q_out == nullptr || a->k_pages == nullptr ||
+      a->v_pages == nullptr || a->kv_lens == nullptr || a->block_table == nullptr || a->cos == nullptr || a->sin == nullptr) {
+    set_error("paged append: null tensor argument");
+    return ALG_ERR_INVALID;
+  }
+  if (a->D != 64 && a->D != 128) { set_error("paged append: head_dim must be 64 or 128, got %d", a->D); return ALG_ERR_UNSUPPORTED; }
+  if (a->H < 1 || a->Hkv < 1 || a->H > (1 << 20) || a->Hkv > (1 << 20)) { set_error("paged append: bad extents"); return ALG_ERR_INVALID; }
+  if (int rc = paged_checks(a, "paged append")) return rc;
+  if (!(a->eps > 0.0f)) { set_error("paged append: epsilon must be positive"); return ALG_ERR_INVALID; }
+  if (a->table_dtype != ALG_BF16 && a->table_dtype != ALG_F32) { set_error("paged append: rotation tables are bf16 or fp32"); return ALG_ERR_INVALID; }
+  const int64_t keys = int64_t(a->table_width) * a->page_size;
+  if (a->table_rows < keys) {
+    set_error("paged append: the rotation tables must cover the %lld positions of a sequence's pages, got %d rows", (long long)keys, a->table_rows);
+    return ALG_ERR_INVALID;
+  }
+  AppendParams p{};
+  p.k_page = a->kp_stride[0]; p.v_page = a->vp_stride[0];
+  const int64_t page_elems = int64_t(a->page_size) * a->Hkv * a->D;
+  if (!strides_ok(&p.qs, a->q_stride, a->tokens, a->H, a->D) || !strides_ok(&p.ks, a->k_stride, a->tokens, a->Hkv, a->D) ||
+      !strides_ok(&p.vs, a->v_stride, a->tokens, a->Hkv, a->D) || !strides_ok(&p.os, a->o_stride, a->tokens, a->H, a->D) ||
+      !strides_ok(&p.kps, a->kp_stride + 1, a->page_size, a->Hkv, a->D) || !strides_ok(&p.vps, a->vp_stride + 1, a->page_size, a->Hkv, a->D) ||
+      !stride_ok(&p.k_page, a->pages, page_elems) || !stride_ok(&p.v_page, a->pages, page_elems) || !aligned16(a->q) || !aligned16(a->k) ||
+      !aligned16(a->v) || !aligned16(a->q_out) || !aligned16(a->k_pages) || !aligned16(a->v_pages) || !aligned16(a->cos) || !aligned16(a->sin) ||
+      !aligned16(a->q_gain) || !aligned16(a->k_gain)) {
+    set_error("paged append: rows, gains and tables must start on 16-byte boundaries, rows lie apart");
+    return ALG_ERR_INVALID;
+  }
+  if (a->tokens == 0) return ALG_OK;
+  p.seqs = {a->cu_seqlens, a->kv_lens, a->sequences, a->tokens, int(keys)};
+  p.q = static_cast<const __nv_bfloat16*>(a->q); p.k = static_cast<const __nv_bfloat16*>(a->k); p.v = static_cast<const __nv_bfloat16*>(a->v);
+  p.q_out = static_cast<__nv_bfloat16*>(a->q_out);
+  p.k_pages = static_cast<__nv_bfloat16*>(a->k_pages); p.v_pages = static_cast<__nv_bfloat16*>(a->v_pages);
+  p.q_gain = a->q_gain; p.k_gain = a->k_gain; p.cos = a->cos; p.sin = a->sin;
+  p.table = a->block_table; p.table_stride = a->table_stride;
+  p.page = a->page_size; p.log2_page = ilog2_exact(a->page_size); p.pages = a->pages;
+  p.H = a->H; p.Hkv = a->Hkv; p.D = a->D; p.table_dtype = a->table_dtype; p.eps = a->eps;
+  p.zero_tail = a->zero_tail != 0;
+  return launch_paged_append(p, static_cast<cudaStream_t>(stream_));
 }
 
 }  // extern "C"

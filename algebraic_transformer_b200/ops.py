@@ -724,6 +724,48 @@ def paged_attention(q, k_pages, v_pages, block_table, kv_lens, cu_seqlens=None, 
     return o
 
 
+@_on_tensor_device
+def paged_append(q, k, v, k_pages, v_pages, block_table, kv_lens, cos, sin, cu_seqlens=None, *, q_gain: Optional[torch.Tensor] = None,
+                 k_gain: Optional[torch.Tensor] = None, eps: float = 1e-5, out=None) -> torch.Tensor:
+    """Writes new tokens into a paged cache and returns their queries: RMS-normalises q and k with their gains (as `qk_rms_norm`),
+    rotates them by each token's own position, writes k and v to the tokens' places in the pages, and returns q for
+    `paged_attention` with the same `block_table`, `kv_lens` and `cu_seqlens` (or, where a sequence's tokens are all new, for
+    `packed_attention` beside the pages).  q (tokens, H, D), k, v (tokens, Hkv, D) bf16 as a projection leaves them, D contiguous;
+    `kv_lens` count the new tokens: token j of m stands at position kv_len - m + j.  cos, sin (rows, D / 2) float32 or bf16, a
+    row for every position of the table's pages.  fp32 arithmetic, one rounding.  `out` may be q.
+
+    A token of no sequence or with a negative position writes nothing to the cache; its row of q is zero, or, where `out` is given,
+    left as it is.  A page number outside the pool drops the token's key and value.  Pages that are written belong to one
+    sequence: two tokens with one place leave either's key there."""
+    _require_cuda(q, k, v, k_pages, v_pages, block_table, kv_lens, cos, sin, cu_seqlens, q_gain, k_gain)
+    if q.ndim != 3 or k.ndim != 3 or k.shape != v.shape or k.shape[0] != q.shape[0] or k.shape[2] != q.shape[2] or \
+            any(t.dtype != torch.bfloat16 for t in (k, v)):
+        raise ValueError("q must be (tokens, H, D) and k, v (tokens, Hkv, D), all bfloat16")
+    S = _check_pages(q, k_pages, v_pages, block_table, kv_lens, cu_seqlens)
+    T, H, D = q.shape
+    if k.shape[1] != k_pages.shape[2]:
+        raise ValueError("k and the pages must have the same key heads")
+    for t in (cos, sin):
+        if t.dtype not in _DTYPES or t.dtype != cos.dtype or t.shape != cos.shape or t.ndim != 2 or t.shape[1] != D // 2 or not t.is_contiguous():
+            raise ValueError("rotation tables must be contiguous (rows, D/2), both float32 or both bfloat16")
+    for t in (q_gain, k_gain):
+        if t is not None and (t.dtype != torch.float32 or t.shape != (D,) or not t.is_contiguous()):
+            raise ValueError("q_gain / k_gain must be float32 of shape (D,)")
+    if eps <= 0:
+        raise ValueError("QK RMS epsilon must be positive")
+    o = _output_like(q, out)
+    a = L.PagedAppendArgs(q=q.data_ptr(), k=k.data_ptr(), v=v.data_ptr(), q_out=o.data_ptr(), k_pages=k_pages.data_ptr(),
+                          v_pages=v_pages.data_ptr(), block_table=block_table.data_ptr(), kv_lens=kv_lens.data_ptr(),
+                          cu_seqlens=_ptr(cu_seqlens), q_gain=_ptr(q_gain), k_gain=_ptr(k_gain), cos=cos.data_ptr(), sin=sin.data_ptr(),
+                          sequences=S, tokens=T, H=H, Hkv=k.shape[1], D=D, pages=k_pages.shape[0], page_size=k_pages.shape[1],
+                          table_width=block_table.shape[1], table_rows=cos.shape[0], table_dtype=_DTYPES[cos.dtype], eps=float(eps),
+                          zero_tail=int(out is None), table_stride=block_table.stride(0), q_stride=_strides2(q), k_stride=_strides2(k),
+                          v_stride=_strides2(v), o_stride=_strides2(o), kp_stride=_strides3(k_pages), vp_stride=_strides3(v_pages))
+    if T:
+        L.check(L.load().alg_paged_append(a, _stream()))
+    return o
+
+
 # ----------------------------------------------------------------------------- head
 
 @_on_tensor_device

@@ -319,6 +319,37 @@ typedef struct {
 ALG_API size_t alg_paged_attn_workspace_bytes(const alg_paged_attn_args* args);
 ALG_API int alg_paged_attn_fwd(const alg_paged_attn_args* args, void* stream);
 
+/* New tokens into such a cache: the QK RMS-norm and the Cayley rotation of alg_qk_rms_fwd, by each token's own position, and the
+ * write of keys and values (rms_norm and apply_rotary, src/algebraic/algebraic.py:76-83, 172-179, in fp32 with one rounding).
+ * q, q_out: (tokens, H, D), k, v: (tokens, Hkv, D) bf16, q_out may be q.  Lengths, table and pages as in alg_paged_attn_args; kv_lens
+ * count the new tokens.  Token j of the m of a sequence stands at position kv_len - m + j.  cos, sin: (table_rows, D / 2) of
+ * table_dtype, dense, table_rows >= table_width page_size.  q_gain, k_gain: (D) fp32 or NULL.  A token of no sequence, or whose
+ * position is negative, writes nothing (zero_tail: zeros to its row of q_out); a page number outside the pool drops the
+ * token's key and value.  Two tokens with one place (a page in two rows of the table) leave either's key there. */
+typedef struct {
+  const void* q;
+  const void* k;
+  const void* v;
+  void* q_out;
+  void* k_pages;
+  void* v_pages;
+  const int* block_table;
+  const int* kv_lens;
+  const int* cu_seqlens;
+  const float* q_gain;
+  const float* k_gain;
+  const void* cos;
+  const void* sin;
+  int sequences, tokens, H, Hkv, D;
+  int pages, page_size, table_width;
+  int table_rows, table_dtype;
+  float eps;
+  int zero_tail;
+  int64_t table_stride;
+  int64_t q_stride[2], k_stride[2], v_stride[2], o_stride[2], kp_stride[3], vp_stride[3];
+} alg_paged_append_args;
+ALG_API int alg_paged_append(const alg_paged_append_args* args, void* stream);
+
 /* ------------------------------------------------------------------------------------
  * Fused Alg-CE head, forward, over one vocabulary shard.
  * Replaces: fused_head(h, embed, targets, kind="alg_ce", n, c)
