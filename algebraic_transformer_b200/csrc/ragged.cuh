@@ -102,6 +102,23 @@ struct RaggedParams {
   int* status;
 };
 
+// One token a sequence (paged_token.cu).
+struct TokenPlan {
+  int groups, heads, grid;  // row groups of a key head; key heads times groups; CTAs
+  float* slots;             // two states a CTA: of the head its stretch begins in, of the one it ends in
+  unsigned long long* arrivals;   // a word per (sequence, head)
+  unsigned long long call;
+};
+size_t paged_token_workspace_bytes(int S, int Hkv, int G, int D, int64_t keys);
+int launch_paged_token(const RaggedParams& p, void* workspace, cudaStream_t stream);
+
+// rho(x) without cancellation, also where x^2 leaves the range
+__device__ __forceinline__ float rho_any(float x) {
+  const float rad = fmaf(x, x, 1.0f);
+  const float T = rad < 3.0e38f ? fmaf(rad, rsqrt_approx(rad), fabsf(x)) : 2.0f * fabsf(x);
+  return x >= 0.0f ? T : __fdividef(1.0f, T);
+}
+
 struct AppendParams {
   RaggedSeqs seqs;
   const __nv_bfloat16* q;

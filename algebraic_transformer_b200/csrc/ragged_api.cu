@@ -104,6 +104,8 @@ extern "C" {
 
 size_t alg_paged_attn_workspace_bytes(const alg_paged_attn_args* a) {
   if (a == nullptr || a->H < 1 || a->Hkv < 1 || a->H % a->Hkv != 0 || a->H / a->Hkv > 128 || a->tokens < 0 || a->sequences < 0) return 0;
+  if (a->cu_seqlens == nullptr)
+    return paged_token_workspace_bytes(a->sequences, a->Hkv, a->H / a->Hkv, a->D, int64_t(a->table_width) * a->page_size);
   return ragged_plan_bytes(a->sequences, a->tokens, a->Hkv, a->H / a->Hkv, a->D,
                            may_split(int64_t(a->table_width) * a->page_size, a->tokens, a->H, a->Hkv));
 }
@@ -135,7 +137,6 @@ int alg_paged_attn_fwd(const alg_paged_attn_args* a, void* stream_) {
   if (a->tokens == 0) return ALG_OK;
   const int64_t keys = int64_t(a->table_width) * a->page_size;
   p.G = a->H / a->Hkv;
-  ragged_plan_carve(&p.plan, a->workspace, a->sequences, a->tokens, a->Hkv, p.G, a->D, may_split(keys, a->tokens, a->H, a->Hkv));
   p.seqs = {a->cu_seqlens, a->kv_lens, a->sequences, a->tokens, int(keys)};
   p.q = a->q; p.k = a->k_pages; p.v = a->v_pages; p.o = a->o; p.sink = a->sink;
   p.k_page = kp; p.v_page = vp;
@@ -145,8 +146,10 @@ int alg_paged_attn_fwd(const alg_paged_attn_args* a, void* stream_) {
   p.tile_tokens = 128 / p.G;
   p.scale = float(1.0 / (sqrt(double(a->D)) * double(a->c)));
   p.inv_c = 1.0f / a->c;
-  p.zero_tail = a->zero_tail != 0 && a->cu_seqlens != nullptr;
   p.status = a->status;
+  if (a->cu_seqlens == nullptr) return launch_paged_token(p, a->workspace, stream);
+  ragged_plan_carve(&p.plan, a->workspace, a->sequences, a->tokens, a->Hkv, p.G, a->D, may_split(keys, a->tokens, a->H, a->Hkv));
+  p.zero_tail = a->zero_tail != 0;
   return launch_ragged_attention(p, stream);
 }
 

@@ -152,13 +152,6 @@ __device__ __forceinline__ void weigh_shifted(const uint32_t* s, float m, float 
     pack4<HILO>(t0, t1, i, packed);
   }
 }
-// the same rho for a single value, whose square may leave the range too
-__device__ __forceinline__ float rho_any(float x) {
-  const float rad = fmaf(x, x, 1.0f);
-  const float T = rad < 3.0e38f ? fmaf(rad, rsqrt_approx(rad), fabsf(x)) : 2.0f * fabsf(x);
-  return x >= 0.0f ? T : __fdividef(1.0f, T);
-}
-
 __device__ __forceinline__ void signal_weights(uint64_t* bar) {
   tmem_st_wait();
   tc_fence_before();
