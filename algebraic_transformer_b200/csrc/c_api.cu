@@ -562,16 +562,6 @@ static unsigned long long call_numbers_from() {
   for (int i = 0; i < 3; ++i) { x ^= x >> 31; x *= 0x9e3779b97f4a7c15ull; }
   return x ^ (x >> 29);
 }
-}  // extern "C"
-
-// The workspace comes uninitialised: what lies there must not read as arrivals of this call.  Counted from one, the
-// numbers would meet small integers and old words; counted from a place of the process's own they meet nothing likely.
-unsigned long long alg::next_call_number() {
-  static std::atomic<unsigned long long> calls{call_numbers_from()};
-  return calls.fetch_add(1) & ((1ull << 47) - 1);
-}
-
-extern "C" {
 
 static int decode_call(const alg_decode_args* a, int* status, unsigned long long wait_ns, int max_loads, void* stream) {
   if (a == nullptr || a->q == nullptr || a->k == nullptr || a->v == nullptr || a->o == nullptr) {
@@ -606,7 +596,10 @@ static int decode_call(const alg_decode_args* a, int* status, unsigned long long
   if (!aligned16(a->workspace)) { set_error("decode: workspace must be 16-byte aligned"); return ALG_ERR_INVALID; }
   p.arrivals = reinterpret_cast<unsigned long long*>(static_cast<unsigned char*>(a->workspace) +
                                                      align256(size_t(a->B) * a->H * p.splits * (a->D + 2) * sizeof(float)));
-  p.call = next_call_number();
+  // The workspace comes uninitialised: what lies there must not read as arrivals of this call.  Counted from one, the
+  // numbers would meet small integers and old words; counted from a place of the process's own they meet nothing likely.
+  static std::atomic<unsigned long long> calls{call_numbers_from()};
+  p.call = calls.fetch_add(1) & ((1ull << 47) - 1);
   return launch_decode(p, static_cast<cudaStream_t>(stream));
 }
 

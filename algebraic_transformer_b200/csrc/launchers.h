@@ -62,9 +62,6 @@ int launch_prep_batch(const PrepBatch& batch, int dtype, cudaStream_t stream);
 int launch_cast(const float* src, void* dst, size_t count, cudaStream_t stream);
 int launch_scale_bf16(const void* src, const float* scale, void* dst, int dst_dtype, size_t count, cudaStream_t stream);
 
-// A number for this call, unlike any other's in this process's workspaces (arrival words that nobody zeroes carry it); 47 bits.
-unsigned long long next_call_number();
-
 // ---- attention ----------------------------------------------------------------------
 struct AttnParams {
   int announce;            // tcgen05 kernel: items leave SMs free, let the next kernel's CTAs in early

@@ -4,8 +4,8 @@
 // every key head, is one long line, sequence by sequence; each CTA takes an equal stretch of it, whatever the lengths, so no
 // schedule has to be made: a CTA adds up the lengths (S loads over its threads) and finds where its stretch begins.  A stretch
 // covers the end of one (sequence, head), whole ones, and the start of another; states of heads that are not whole go
-// to the workspace, and the CTA that arrives last for such a head merges them (arrival words as in decode.cu: they carry the
-// call's number, so nothing has to be zeroed).
+// to the workspace and a second kernel merges them, launched ahead so that it only has to wait.  (Merged by the CTA that arrives
+// last, a head of 19 parts of 8 rows of 128 took 8 us: one SM's reads and code that it meets for the first time.)
 //
 // Inside a CTA a producer warp streams 32-key K and V tiles, page by page through the block table, into a shared-memory ring that
 // runs on over the heads; consumer warps take the tiles in turn, each with a state of its own (maximum m, normaliser l,
@@ -16,11 +16,13 @@
 //            query heads to a key head go as several groups of 16, which read the keys again, from L2.
 // Rows behind a sequence's end (the rest of its last page) may hold anything: scores there are masked, V is zeroed in registers.
 #include "common.cuh"
-#include "launchers.h"
 #include "ragged.cuh"
 #include "sm100_ptx.cuh"
 
+#include <math.h>
+
 #include <algorithm>
+#include <type_traits>
 
 namespace alg {
 namespace {
@@ -37,18 +39,21 @@ constexpr int MAX_STAGES = 12, MAX_CWARPS = 6;
 template <int D, int RB> struct Cfg {
   static constexpr int CTAS = D == 64 ? 2 : 1;                 // of an SM
   static constexpr int PANELS = D / 64, TILE_BYTES = PANELS * PANEL;
-  static constexpr int STAGES = 24 / PANELS / CTAS;            // 192 KB of K and V tiles per SM
+  // 192 KB of K and V tiles per SM; with sixteen rows less, for the sake of the scratch (96 KB in flight still cover 2 us at this
+  // SM's share of HBM)
+  static constexpr int STAGES = RB == 8 ? 24 / PANELS / CTAS : D == 64 ? 8 : 6;
   static constexpr int CWARPS = D == 64 ? 4 : 6, CONSUMERS = CWARPS * 32, NTHREADS = CONSUMERS + 32;
-  static constexpr int SCRATCH = CWARPS * RB * 32 * 4;         // 32 columns of the warps' accumulators
+  static constexpr int ROW = D + 8;                            // floats from row to row of the scratch: no bank conflicts
+  static constexpr int SCRATCH = CWARPS * RB * ROW * 4;        // the warps' accumulators
   static_assert(STAGES % CWARPS == 0 && STAGES <= MAX_STAGES && CWARPS <= MAX_CWARPS, "a slot belongs to one warp");
 };
 
 template <int RB> struct __align__(16) Control {
   uint64_t full[MAX_STAGES], empty[MAX_STAGES];
-  int abort_flag, tile_ok, last, start_seq;
-  int64_t start_base, total;                    // units ahead of the first sequence; of all sequences (one head)
+  int abort_flag, start_seq, start_len;
+  int64_t start_base;                           // units ahead of the first sequence
   int64_t warp_units[MAX_CWARPS + 1];
-  float m[MAX_CWARPS][RB], l[MAX_CWARPS][RB], f[MAX_CWARPS][RB], row_l[RB], row_m[RB];
+  float m[MAX_CWARPS][RB], l[MAX_CWARPS][RB];
 };
 template <int D, int RB> constexpr size_t smem_bytes() {
   return size_t(Cfg<D, RB>::STAGES) * 2 * Cfg<D, RB>::TILE_BYTES + Cfg<D, RB>::SCRATCH + sizeof(Control<RB>) + 1024;
@@ -74,19 +79,21 @@ __device__ __forceinline__ int units_of(int len) { return len > 0 ? (len + UNIT 
 struct Walk {
   int64_t at, end;          // units of the line; a sequence's heads lie one behind the other
   int64_t base;             // units before sequence s
-  int s, len, units;        // the sequence, its keys, its units (of one head)
+  int s, len, next_len;     // the sequence, its keys, those of the next one (fetched ahead)
+  int units;                // of one head of it
   int hh, u0, u1;           // head (and row group), units of the current segment
 };
-__device__ __forceinline__ void walk_sequence(const RaggedParams& p, Walk& w) {
-  w.len = min(max(__ldg(p.seqs.kv_lens + w.s), 0), p.seqs.kv_capacity);
-  w.units = units_of(w.len);
+__device__ __forceinline__ int length_of(const RaggedParams& p, int s) {
+  return s < p.seqs.S ? min(max(__ldg(p.seqs.kv_lens + s), 0), p.seqs.kv_capacity) : 0;
 }
 __device__ __forceinline__ bool walk_next(const RaggedParams& p, int heads, Walk& w) {
   if (w.at >= w.end) return false;
-  while (w.at >= w.base + int64_t(w.units) * heads) {          // every sequence has a unit: at most one step, but for the first
+  if (w.at >= w.base + int64_t(w.units) * heads) {             // every sequence has a unit: one step is enough
     w.base += int64_t(w.units) * heads;
+    w.len = w.next_len;
+    w.units = units_of(w.len);
     ++w.s;
-    walk_sequence(p, w);
+    w.next_len = length_of(p, w.s + 1);
   }
   const int64_t in = w.at - w.base;
   w.hh = int(in / w.units);
@@ -96,7 +103,45 @@ __device__ __forceinline__ bool walk_next(const RaggedParams& p, int heads, Walk
   return true;
 }
 
-template <int D, int RB>
+// (rho(x) sigma)^n.  Out of line: it runs where references differ and, per score, in the max-shifted form; the paths that run always
+// stay short for it, and code that is met for the first time costs its fetches.
+__device__ __noinline__ float rescale(float x, float sigma, int log2n) { return pow2n_rt(rho_any(x) * sigma, log2n); }
+
+// Four columns of a row's state while states with other references join it: a = sum f v, l = sum f l, f = (rho(m_i) rho(-m))^n.
+struct State {
+  float m, l, ns;           // reference, normaliser, rho(-m)
+  float4 a;
+  __device__ __forceinline__ void start(const RaggedParams& p, bool with_sink, int head) {
+    const bool sunk = with_sink && p.sink != nullptr;
+    m = sunk ? p.sink[head] * p.inv_c : -1e30f;
+    l = sunk ? 1.0f : 0.f;                                     // the sink's weight at its own reference
+    ns = rho_any(-m);
+    a = make_float4(0.f, 0.f, 0.f, 0.f);
+  }
+  __device__ __forceinline__ void raise(float most, int log2n) {                 // the reference of the states to come
+    if (!(most > m)) return;
+    ns = rho_any(-most);
+    const float f = m > -1e29f ? rescale(m, ns, log2n) : 0.f;
+    m = most;
+    l *= f; a.x *= f; a.y *= f; a.z *= f; a.w *= f;
+  }
+  __device__ __forceinline__ float factor(float mi, int log2n) const {
+    return mi == m ? 1.0f : mi > -1e29f ? rescale(mi, ns, log2n) : 0.f;
+  }
+  __device__ __forceinline__ void add(float mi, float li, const float4& v, int log2n) {
+    const float f = mi > -1e29f ? factor(mi, log2n) : 0.f;
+    if (li != li) l = li;                                      // a wait that ran out, or a NaN score
+    if (f == 0.f) return;                                      // nothing was weighed there, or nothing that counts
+    l = fmaf(f, li, l);
+    a.x = fmaf(f, v.x, a.x); a.y = fmaf(f, v.y, a.y); a.z = fmaf(f, v.z, a.z); a.w = fmaf(f, v.w, a.w);
+  }
+  __device__ __forceinline__ void write(__nv_bfloat16* to) const {
+    const float inv = l == 0.f ? 0.f : 1.0f / l;               // a sequence without keys: zero
+    *reinterpret_cast<uint2*>(to) = make_uint2(pack_bf16(a.x * inv, a.y * inv), pack_bf16(a.z * inv, a.w * inv));
+  }
+};
+
+template <int D, int RB, int LOG2N>
 __global__ void __launch_bounds__(Cfg<D, RB>::NTHREADS, Cfg<D, RB>::CTAS)
 paged_token_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_constant__ CUtensorMap tm_v, const __grid_constant__ RaggedParams p,
                    const TokenPlan plan) {
@@ -116,11 +161,17 @@ paged_token_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_consta
   }
   if (threadIdx.x == C::CONSUMERS) { tma_prefetch_desc(&tm_k); tma_prefetch_desc(&tm_v); }
   griddep_wait();
+  griddep_launch();                              // the merging kernel's CTAs move in beside these and wait
   // ---- the line: units of all sequences, and the sequence in which this CTA's stretch begins
   const int S = p.seqs.S, per_thread = (S + C::NTHREADS - 1) / C::NTHREADS;
   const int s_first = min(int(threadIdx.x) * per_thread, S), s_last = min(s_first + per_thread, S);
   int64_t mine = 0;
-  for (int s = s_first; s < s_last; ++s) mine += units_of(min(max(__ldg(p.seqs.kv_lens + s), 0), p.seqs.kv_capacity));
+  int len0 = 0;
+  for (int s = s_first; s < s_last; ++s) {
+    const int len = length_of(p, s);
+    if (s == s_first) len0 = len;
+    mine += units_of(len);
+  }
   int64_t incl = mine;
 #pragma unroll
   for (int o = 1; o < 32; o <<= 1) {
@@ -140,22 +191,28 @@ paged_token_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_consta
   const int64_t begin = per * blockIdx.x;
   if (begin < total && begin >= before * heads && begin < (before + mine) * heads) {
     int64_t base = before * heads;
-    int s = s_first;
-    for (;; ++s) {
-      const int64_t n = int64_t(units_of(min(max(__ldg(p.seqs.kv_lens + s), 0), p.seqs.kv_capacity))) * heads;
+    int s = s_first, len = len0;
+    for (;;) {
+      const int64_t n = int64_t(units_of(len)) * heads;
       if (begin < base + n) break;
       base += n;
+      len = length_of(p, ++s);
     }
     ctl->start_seq = s;
+    ctl->start_len = len;
     ctl->start_base = base;
   }
   __syncthreads();
-  if (begin >= total) return;
+  if (begin >= total) {
+    if (threadIdx.x == 0) plan.heads_open[blockIdx.x] = TokenHead{0, 0, 0, 0};
+    return;
+  }
   const BoundedWait bw{&ctl->abort_flag, 1000000000ull};
   Walk w;
   w.at = begin; w.end = min(begin + per, total);
-  w.s = ctl->start_seq; w.base = ctl->start_base;
-  walk_sequence(p, w);
+  w.s = ctl->start_seq; w.len = ctl->start_len; w.base = ctl->start_base;
+  w.units = units_of(w.len);
+  w.next_len = length_of(p, w.s + 1);
   int tiles = 0;                                 // of the heads before the current one
 
   if (warp == CWARPS) {                          // producer: the whole warp walks, lane 0 issues, lanes hold page numbers
@@ -196,7 +253,9 @@ paged_token_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_consta
     const uint32_t v_row = uint32_t(((lane >> 3) & 1) * 8 + (lane & 7)) * 128, v_chunk = uint32_t(lane >> 4);   // + 16 keys, + 2
     const uint32_t swz = uint32_t(lane & 7);
     constexpr int NR = RB / 8;                   // rows of this lane: r, and r + 8 where RB = 16
-    bool ok = true;
+    const float2 scale2 = make_float2(p.scale, p.scale), one2 = make_float2(1.f, 1.f);
+    bool ok = true, first_segment = true;
+    TokenHead open = {0, 0, 0, 0};               // the head that begins in this stretch and goes on behind it
     while (walk_next(p, heads, w)) {
       const int k0 = w.u0 * UNIT, k1 = min(w.len, w.u1 * UNIT), n = k1 > k0 ? (k1 - k0 + TILE - 1) / TILE : 0;
       const int h = w.hh / plan.groups, row0 = (w.hh % plan.groups) * RB, live_rows = min(RB, p.G - row0);
@@ -217,9 +276,13 @@ paged_token_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_consta
       float acc[D / 8][4];                       // RB = 8: rows r of the weights' leading and of their trailing halves
 #pragma unroll
       for (int c = 0; c < D / 8; ++c) acc[c][0] = acc[c][1] = acc[c][2] = acc[c][3] = 0.f;
-      float m_ref[NR], shift[NR], l_part[NR];
+      // weights are (rho(x) rho(-m_ref))^n: unshifted (m_ref = 0) until a score of the warp's rows leaves the range in which that is safe
+      // (|x| <= x_fast keeps them within 2^+-64 and the cancellation of x + sqrt(1 + x^2) below 2e-4), max-shifted from then on
+      float m_ref[NR];
+      float2 l_part[NR];
 #pragma unroll
-      for (int e = 0; e < NR; ++e) { m_ref[e] = -1e30f; shift[e] = 0.f; l_part[e] = 0.f; }
+      for (int e = 0; e < NR; ++e) { m_ref[e] = 0.f; l_part[e] = make_float2(0.f, 0.f); }
+      bool shifted = false, begun = false;
       for (int t = (warp + CWARPS - tiles % CWARPS) % CWARPS; t < n && ok; t += CWARPS) {
         const int number = tiles + t, stage = number % STAGES;
         if (!__all_sync(0xffffffffu, bw.wait(&ctl->full[stage], uint32_t(number / STAGES) & 1u))) { ok = false; break; }
@@ -238,43 +301,76 @@ paged_token_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_consta
           }
         }
         const int live = k1 - k0 - t * TILE;     // keys of the tile; columns 8 b + 2 i, + 1 are this lane's
-        float wgt[NR][8];
+        const bool tail = live < TILE;
+        auto seen = [&](int b, int j) { return 8 * b + 2 * i + j < live; };
+        float2 wgt[NR][4];
+        float most = 0.f;                        // largest |x| that counts; NaN if there is one
 #pragma unroll
-        for (int e = 0; e < NR; ++e) {
-          float top = -1e30f;
+        for (int e = 0; e < NR; ++e)
 #pragma unroll
-          for (int b = 0; b < 4; ++b)
-#pragma unroll
-            for (int j = 0; j < 2; ++j) {
-              const float x = sc[b][2 * e + j] * p.scale;
-              wgt[e][2 * b + j] = x;
-              top = (8 * b + 2 * i + j < live) ? fmaxf(top, x) : top;
+          for (int b = 0; b < 4; ++b) {
+            wgt[e][b] = __fmul2_rn(make_float2(sc[b][2 * e], sc[b][2 * e + 1]), scale2);
+            if (tail) {
+              if (!seen(b, 0)) wgt[e][b].x = 0.f;
+              if (!seen(b, 1)) wgt[e][b].y = 0.f;
             }
-          top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 1));
-          top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 2));
-          if (__any_sync(0xffffffffu, top > m_ref[e])) {
-            const float m_new = fmaxf(top, m_ref[e]);
-            const float ns = rho_any(-m_new);
-            const float alpha = m_new == m_ref[e] ? 1.0f : m_ref[e] > -1e29f ? pow2n_rt(rho_any(m_ref[e]) * ns, p.log2n) : 0.f;
-            l_part[e] *= alpha;
+            most = max3_abs_nan(most, wgt[e][b].x, wgt[e][b].y);
+          }
+        if (!shifted) shifted = __any_sync(0xffffffffu, !(most <= plan.x_fast));
+        if (!shifted) {
 #pragma unroll
-            for (int c = 0; c < D / 8; ++c) {
-              acc[c][2 * e] *= alpha; acc[c][2 * e + 1] *= alpha;
-              if (RB == 8) { acc[c][2] *= alpha; acc[c][3] *= alpha; }
+          for (int e = 0; e < NR; ++e)
+#pragma unroll
+            for (int b = 0; b < 4; ++b) {
+              const float2 x = wgt[e][b], rad = __ffma2_rn(x, x, one2);
+              float2 y = __ffma2_rn(rad, make_float2(rsqrt_approx(rad.x), rsqrt_approx(rad.y)), x);
+              if (LOG2N > 0) {
+#pragma unroll
+                for (int it = 0; it < LOG2N; ++it) y = __fmul2_rn(y, y);
+              } else {
+                for (int it = 0; it < p.log2n; ++it) y = __fmul2_rn(y, y);
+              }
+              if (tail) {
+                if (!seen(b, 0)) y.x = 0.f;
+                if (!seen(b, 1)) y.y = 0.f;
+              }
+              wgt[e][b] = y;
+              l_part[e] = __fadd2_rn(l_part[e], y);
+            }
+        } else {
+#pragma unroll
+          for (int e = 0; e < NR; ++e) {
+            float top = -INFINITY;
+#pragma unroll
+            for (int b = 0; b < 4; ++b) {
+              top = seen(b, 0) ? fmaxf(top, wgt[e][b].x) : top;
+              top = seen(b, 1) ? fmaxf(top, wgt[e][b].y) : top;
+            }
+            top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 1));
+            top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 2));
+            // the first tile's largest score, then the largest so far
+            const float m_new = !(top > -INFINITY) ? m_ref[e] : begun ? fmaxf(m_ref[e], top) : top;
+            const float ns = rho_any(-m_new), alpha = m_new == m_ref[e] ? 1.0f : rescale(m_ref[e], ns, p.log2n);
+            if (begun && __any_sync(0xffffffffu, alpha != 1.0f)) {
+              l_part[e].x *= alpha; l_part[e].y *= alpha;
+#pragma unroll
+              for (int c = 0; c < D / 8; ++c) {
+                acc[c][2 * e] *= alpha; acc[c][2 * e + 1] *= alpha;
+                if (RB == 8) { acc[c][2] *= alpha; acc[c][3] *= alpha; }
+              }
             }
             m_ref[e] = m_new;
-            shift[e] = m_new > -1e29f ? ns : 0.f;
-          }
 #pragma unroll
-          for (int b = 0; b < 4; ++b)
-#pragma unroll
-            for (int j = 0; j < 2; ++j) {
-              const float x = wgt[e][2 * b + j];
-              const float y = (8 * b + 2 * i + j < live) ? pow2n_rt(rho_any(x) * shift[e], p.log2n) : 0.f;
-              wgt[e][2 * b + j] = y;
-              l_part[e] += y;
+            for (int b = 0; b < 4; ++b) {
+              const float2 x = wgt[e][b];
+              const float2 y = make_float2(seen(b, 0) ? rescale(x.x, ns, p.log2n) : 0.f,
+                                           seen(b, 1) ? rescale(x.y, ns, p.log2n) : 0.f);
+              wgt[e][b] = y;
+              l_part[e] = __fadd2_rn(l_part[e], y);
             }
+          }
         }
+        begun = true;
 #pragma unroll
         for (int ks = 0; ks < 2; ++ks) {         // sixteen keys
           uint32_t hi[4], lo[4];                 // A fragments: rows r, r + 8 of keys 2 i, 2 i + 1, then of those 8 further
@@ -282,163 +378,89 @@ paged_token_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_consta
           for (int g = 0; g < 2; ++g)
 #pragma unroll
             for (int e = 0; e < NR; ++e) {
-              const float a = wgt[e][4 * ks + 2 * g], b = wgt[e][4 * ks + 2 * g + 1];
-              const uint32_t lead = pack_bf16(a, b), rest = pack_bf16(a - __uint_as_float(lead << 16), b - __uint_as_float(lead & 0xffff0000u));
+              const float2 y = wgt[e][2 * ks + g];
+              const uint32_t lead = pack_bf16(y.x, y.y), rest = pack_bf16(y.x - __uint_as_float(lead << 16), y.y - __uint_as_float(lead & 0xffff0000u));
               hi[2 * g + e] = lead;
               if (RB == 8) hi[2 * g + 1] = rest;
               else lo[2 * g + e] = rest;
             }
-          const int first = ks * 16 + 2 * i;
-          const uint32_t keep0 = (first < live ? 0xffffu : 0u) | (first + 1 < live ? 0xffff0000u : 0u);
-          const uint32_t keep1 = (first + 8 < live ? 0xffffu : 0u) | (first + 9 < live ? 0xffff0000u : 0u);
+          auto product = [&](auto tailed) {
+            const int first = ks * 16 + 2 * i;
+            const uint32_t keep0 = (first < live ? 0xffffu : 0u) | (first + 1 < live ? 0xffff0000u : 0u);
+            const uint32_t keep1 = (first + 8 < live ? 0xffffu : 0u) | (first + 9 < live ? 0xffff0000u : 0u);
 #pragma unroll
-          for (int c = 0; c < D / 8; c += 2) {   // sixteen columns of V a load
-            uint32_t vb[4];
-            ldsm4_trans(sv + (c >> 3) * PANEL + ks * 2048 + v_row + (((uint32_t(c & 7) + v_chunk) ^ swz) << 4), vb);
-            if (live < TILE) { vb[0] &= keep0; vb[1] &= keep1; vb[2] &= keep0; vb[3] &= keep1; }
-            mma(acc[c], hi, vb[0], vb[1]);
-            mma(acc[c + 1], hi, vb[2], vb[3]);
-            if (RB == 16) {
-              mma(acc[c], lo, vb[0], vb[1]);
-              mma(acc[c + 1], lo, vb[2], vb[3]);
+            for (int c = 0; c < D / 8; c += 2) { // sixteen columns of V a load
+              uint32_t vb[4];
+              ldsm4_trans(sv + (c >> 3) * PANEL + ks * 2048 + v_row + (((uint32_t(c & 7) + v_chunk) ^ swz) << 4), vb);
+              if (decltype(tailed)::value) { vb[0] &= keep0; vb[1] &= keep1; vb[2] &= keep0; vb[3] &= keep1; }
+              mma(acc[c], hi, vb[0], vb[1]);
+              mma(acc[c + 1], hi, vb[2], vb[3]);
+              if (RB == 16) {
+                mma(acc[c], lo, vb[0], vb[1]);
+                mma(acc[c + 1], lo, vb[2], vb[3]);
+              }
             }
-          }
+          };
+          if (tail) product(std::true_type{});
+          else product(std::false_type{});
         }
         __syncwarp();
         if (lane == 0) mbar_arrive(&ctl->empty[stage]);
       }
       tiles += n;
-      // ---- the warps' states together
+      // ---- the warps' states together: each leaves its own in shared memory, every thread adds up its columns of a row
+      if (!first_segment) consumer_sync<C::CONSUMERS>();        // the scratch has been read
+      first_segment = false;
 #pragma unroll
       for (int e = 0; e < NR; ++e) {
-        l_part[e] += __shfl_xor_sync(0xffffffffu, l_part[e], 1);
-        l_part[e] += __shfl_xor_sync(0xffffffffu, l_part[e], 2);
-        if (i == 0) { ctl->m[warp][r + 8 * e] = m_ref[e]; ctl->l[warp][r + 8 * e] = ok ? l_part[e] : __int_as_float(0x7fc00000); }
+        float l = l_part[e].x + l_part[e].y;
+        l += __shfl_xor_sync(0xffffffffu, l, 1);
+        l += __shfl_xor_sync(0xffffffffu, l, 2);
+        if (i == 0) { ctl->m[warp][r + 8 * e] = begun ? m_ref[e] : -1e30f; ctl->l[warp][r + 8 * e] = ok ? l : __int_as_float(0x7fc00000); }
+      }
+      if (begun) {
+#pragma unroll
+        for (int c = 0; c < D / 8; ++c) {
+          float* to = scratch + (warp * RB + r) * C::ROW + c * 8 + 2 * i;
+          if (RB == 8) {                         // an infinite V meets a zero trailing half as NaN: the leading half has the answer then
+            const float a = isinf(acc[c][0]) ? acc[c][0] : acc[c][0] + acc[c][2], b = isinf(acc[c][1]) ? acc[c][1] : acc[c][1] + acc[c][3];
+            *reinterpret_cast<float2*>(to) = make_float2(a, b);
+          } else {
+            *reinterpret_cast<float2*>(to) = make_float2(acc[c][0], acc[c][1]);
+            *reinterpret_cast<float2*>(to + 8 * C::ROW) = make_float2(acc[c][2], acc[c][3]);
+          }
+        }
       }
       consumer_sync<C::CONSUMERS>();
       const bool whole = w.u0 == 0 && w.u1 == w.units;
-      if (int(threadIdx.x) < RB) {
-        const int row = threadIdx.x;
-        const bool sunk = whole && p.sink != nullptr && row < live_rows;
-        const float bs = sunk ? p.sink[h * p.G + row0 + row] * p.inv_c : -1e30f;
-        float mm = bs;
+      const int kind = w.u0 > 0 ? 0 : 1;
+      float* slot = plan.slots + (int64_t(blockIdx.x) * 2 + kind) * (RB * (D + 2));
+      for (int x = threadIdx.x; x < live_rows * (D / 4); x += C::CONSUMERS) {
+        const int row = x / (D / 4), col = x % (D / 4) * 4;
+        State st;
+        st.start(p, whole, h * p.G + row0 + row);
+        float most = ctl->m[0][row];
 #pragma unroll
-        for (int wv = 0; wv < CWARPS; ++wv) mm = fmaxf(mm, ctl->m[wv][row]);
-        const float ns = rho_any(-mm);
-        float l = sunk ? pow2n_rt(rho_any(bs) * ns, p.log2n) : 0.f;
+        for (int wv = 1; wv < CWARPS; ++wv) most = fmaxf(most, ctl->m[wv][row]);
+        st.raise(most, p.log2n);
 #pragma unroll
-        for (int wv = 0; wv < CWARPS; ++wv) {
-          const float mw = ctl->m[wv][row], lw = ctl->l[wv][row];
-          const float f = mw == mm ? 1.0f : mw > -1e29f ? pow2n_rt(rho_any(mw) * ns, p.log2n) : 0.f;
-          ctl->f[wv][row] = f;
-          l += f == 0.f && lw == 0.f ? 0.f : f * lw;
-          if (lw != lw) l = lw;                  // a wait that ran out, or a NaN score
+        for (int wv = 0; wv < CWARPS; ++wv)
+          if (ctl->m[wv][row] > -1e29f)
+            st.add(ctl->m[wv][row], ctl->l[wv][row], *reinterpret_cast<const float4*>(scratch + (wv * RB + row) * C::ROW + col), p.log2n);
+          else if (!ok || ctl->l[wv][row] != 0.f) st.l = __int_as_float(0x7fc00000);       // a wait ran out
+        if (whole) {
+          st.write(static_cast<__nv_bfloat16*>(p.o) + w.s * p.os.t + int64_t(h * p.G + row0 + row) * p.os.h + col);
+        } else {
+          *reinterpret_cast<float4*>(slot + row * D + col) = st.a;
+          if (col == 0) *reinterpret_cast<float2*>(slot + RB * D + row * 2) = make_float2(st.m, st.l);
         }
-        ctl->row_l[row] = l;
-        ctl->row_m[row] = mm;
       }
-      const int64_t pair = int64_t(w.s) * heads + w.hh;
-      float* slot = plan.slots + (int64_t(blockIdx.x) * 2 + (w.u0 > 0 ? 0 : 1)) * (RB * (D + 2));
-      for (int c0 = 0; c0 < D; c0 += 32) {
-#pragma unroll
-        for (int c = 0; c < D / 8; ++c) {
-          if (c * 8 >= c0 && c * 8 < c0 + 32) {
-            float* to = scratch + (warp * RB + r) * 32 + c * 8 - c0 + 2 * i;
-            if (RB == 8) {                       // an infinite V meets a zero trailing half as NaN: the leading half has the answer then
-              const float a = isinf(acc[c][0]) ? acc[c][0] : acc[c][0] + acc[c][2], b = isinf(acc[c][1]) ? acc[c][1] : acc[c][1] + acc[c][3];
-              *reinterpret_cast<float2*>(to) = make_float2(a, b);
-            } else {
-              *reinterpret_cast<float2*>(to) = make_float2(acc[c][0], acc[c][1]);
-              *reinterpret_cast<float2*>(to + 8 * 32) = make_float2(acc[c][2], acc[c][3]);
-            }
-          }
-        }
-        consumer_sync<C::CONSUMERS>();
-        for (int x = threadIdx.x; x < RB * 32; x += C::CONSUMERS) {
-          const int row = x >> 5, col = x & 31;
-          float a = 0.f;
-#pragma unroll
-          for (int wv = 0; wv < CWARPS; ++wv) {
-            const float f = ctl->f[wv][row];
-            if (f != 0.f) a = fmaf(f, scratch[(wv * RB + row) * 32 + col], a);
-          }
-          if (whole) {
-            const float l = ctl->row_l[row];
-            if (row < live_rows)
-              static_cast<__nv_bfloat16*>(p.o)[w.s * p.os.t + int64_t(h * p.G + row0 + row) * p.os.h + c0 + col] = __float2bfloat16_rn(l == 0.f ? 0.f : a / l);
-          } else {
-            slot[row * D + c0 + col] = a;
-          }
-        }
-        consumer_sync<C::CONSUMERS>();
-      }
-      if (whole) continue;
-      if (int(threadIdx.x) < RB) {
-        slot[RB * D + threadIdx.x * 2] = ctl->row_m[threadIdx.x];
-        slot[RB * D + threadIdx.x * 2 + 1] = ctl->row_l[threadIdx.x];
-      }
-      __threadfence();                           // the state is visible before this CTA counts as arrived
-      consumer_sync<C::CONSUMERS>();
-      const int64_t pair_begin = w.base + int64_t(w.hh) * w.units;
-      const int c_first = int(pair_begin / per), c_last = int((pair_begin + w.units - 1) / per), parts = c_last - c_first + 1;
-      if (threadIdx.x == 0) {
-        unsigned long long* word = plan.arrivals + pair;
-        unsigned long long seen = *reinterpret_cast<volatile unsigned long long*>(word), next;
-        for (;;) {                               // at most `parts` contenders
-          next = ((seen >> 16) == plan.call) ? seen + 1 : ((plan.call << 16) | 1ull);
-          const unsigned long long prev = atomicCAS(word, seen, next);
-          if (prev == seen) break;
-          seen = prev;
-        }
-        const bool last = int(next & 0xffffull) == parts;
-        ctl->last = last;
-        if (last) *reinterpret_cast<volatile unsigned long long*>(word) = 0ull;     // for a replay with the same number
-        __threadfence();
-      }
-      consumer_sync<C::CONSUMERS>();
-      if (!ctl->last) continue;
-      // ---- the last to arrive merges the parts, in their order
-      auto part = [&](int c) { return plan.slots + (int64_t(c_first + c) * 2 + (c > 0 ? 0 : 1)) * (RB * (D + 2)); };
-      for (int row = warp; row < live_rows; row += CWARPS) {                         // a warp a row: reference and normaliser
-        const bool sunk = p.sink != nullptr;
-        const float bs = sunk ? p.sink[h * p.G + row0 + row] * p.inv_c : -1e30f;
-        float mm = bs;
-        for (int c = lane; c < parts; c += 32) mm = fmaxf(mm, __ldcg(part(c) + RB * D + row * 2));
-        mm = warp_max(mm);
-        const float ns = rho_any(-mm);
-        float l = 0.f;
-        bool nan = false;
-        for (int c = lane; c < parts; c += 32) {
-          const float mc = __ldcg(part(c) + RB * D + row * 2), lc = __ldcg(part(c) + RB * D + row * 2 + 1);
-          const float f = mc == mm ? 1.0f : mc > -1e29f ? pow2n_rt(rho_any(mc) * ns, p.log2n) : 0.f;
-          nan |= lc != lc;
-          if (f != 0.f) l += f * lc;
-        }
-        l = warp_sum(l) + (sunk ? pow2n_rt(rho_any(bs) * ns, p.log2n) : 0.f);
-        if (__any_sync(0xffffffffu, nan)) l = __int_as_float(0x7fc00000);
-        float a[D / 32];
-#pragma unroll
-        for (int e = 0; e < D / 32; ++e) a[e] = 0.f;
-        for (int c = 0; c < parts; c += 4) {     // four parts' loads in flight
-          float v[4][D / 32], f[4];
-#pragma unroll
-          for (int u = 0; u < 4; ++u) {
-            const float* src = part(min(c + u, parts - 1));
-            const float mc = __ldcg(src + RB * D + row * 2);
-            f[u] = c + u >= parts ? 0.f : mc == mm ? 1.0f : mc > -1e29f ? pow2n_rt(rho_any(mc) * ns, p.log2n) : 0.f;
-#pragma unroll
-            for (int e = 0; e < D / 32; ++e) v[u][e] = __ldcg(src + row * D + e * 32 + lane);
-          }
-#pragma unroll
-          for (int u = 0; u < 4; ++u)
-#pragma unroll
-            for (int e = 0; e < D / 32; ++e) a[e] = f[u] != 0.f ? fmaf(f[u], v[u][e], a[e]) : a[e];
-        }
-        __nv_bfloat16* out = static_cast<__nv_bfloat16*>(p.o) + w.s * p.os.t + int64_t(h * p.G + row0 + row) * p.os.h;
-#pragma unroll
-        for (int e = 0; e < D / 32; ++e) out[e * 32 + lane] = __float2bfloat16_rn(l == 0.f ? 0.f : a[e] / l);
+      if (!whole) {
+        const int64_t head_end = w.base + int64_t(w.hh + 1) * w.units;
+        if (kind == 1) open = TokenHead{w.s, h, row0, int((head_end - 1) / per) - int(blockIdx.x) + 1};
       }
     }
+    if (threadIdx.x == 0) plan.heads_open[blockIdx.x] = open;
   }
   __syncthreads();
   if (ctl->abort_flag != 0 && threadIdx.x == 0) {
@@ -448,8 +470,73 @@ paged_token_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_consta
   }
 }
 
+// Merges the parts of a head that goes on behind the stretch it began in: CTA c takes the head that CTA c of the kernel ahead left
+// open, a warp a row, a lane D / 32 columns.  References and normalisers come one a lane, 32 parts at a time.
 template <int D, int RB>
-int launch(const RaggedParams& p, const TokenPlan& plan, cudaStream_t stream) {
+__global__ void __launch_bounds__(256) paged_token_merge_kernel(const __grid_constant__ RaggedParams p, const TokenPlan plan) {
+  constexpr int CPL = D / 32, SLOT = RB * (D + 2), BATCH = 16;
+  griddep_wait();
+  const TokenHead head = plan.heads_open[blockIdx.x];
+  if (head.parts == 0) return;
+  const int lane = threadIdx.x & 31;
+  auto slot_of = [&](int part) { return plan.slots + (int64_t(blockIdx.x + part) * 2 + (part > 0 ? 0 : 1)) * SLOT; };
+  for (int row = threadIdx.x >> 5; row < min(RB, p.G - head.row0); row += 8) {
+    const int h = head.h * p.G + head.row0 + row;
+    float m = p.sink != nullptr ? p.sink[h] * p.inv_c : -1e30f, l = p.sink != nullptr ? 1.0f : 0.f;
+    float a[CPL];
+#pragma unroll
+    for (int c = 0; c < CPL; ++c) a[c] = 0.f;
+    for (int p0 = 0; p0 < head.parts; p0 += 32) {
+      const int n = min(32, head.parts - p0);
+      const float2 ml = lane < n ? __ldcg(reinterpret_cast<const float2*>(slot_of(p0 + lane) + RB * D + row * 2)) : make_float2(-1e30f, 0.f);
+      for (int b0 = 0; b0 < n; b0 += BATCH) {
+        float v[BATCH][CPL];
+#pragma unroll
+        for (int j = 0; j < BATCH; ++j) {
+          const float* src = slot_of(p0 + min(b0 + j, n - 1)) + row * D + lane * CPL;
+          if (CPL == 4) {
+            const float4 x = __ldcg(reinterpret_cast<const float4*>(src));
+            v[j][0] = x.x; v[j][1] = x.y; v[j][CPL - 2] = x.z; v[j][CPL - 1] = x.w;
+          } else {
+            const float2 x = __ldcg(reinterpret_cast<const float2*>(src));
+            v[j][0] = x.x; v[j][1] = x.y;
+          }
+        }
+        if (b0 == 0) {                                 // these parts' reference, and what was added up under the old one
+          const float top = fmaxf(m, warp_max(ml.x));
+          if (top != m) {
+            const float f = m > -1e29f ? rescale(m, rho_any(-top), p.log2n) : 0.f;
+            l *= f;
+#pragma unroll
+            for (int c = 0; c < CPL; ++c) a[c] *= f;
+            m = top;
+          }
+        }
+        const float f = ml.x == m ? 1.0f : ml.x > -1e29f ? rescale(ml.x, rho_any(-m), p.log2n) : 0.f;
+        if (b0 == 0) {
+          const bool nan = __any_sync(0xffffffffu, ml.y != ml.y);        // a wait that ran out, or a NaN score
+          l += warp_sum(f != 0.f ? f * ml.y : 0.f);
+          if (nan) l = __int_as_float(0x7fc00000);
+        }
+#pragma unroll
+        for (int j = 0; j < BATCH; ++j) {
+          const float fj = __shfl_sync(0xffffffffu, f, (b0 + j) & 31);
+          if (b0 + j < n && fj != 0.f) {
+#pragma unroll
+            for (int c = 0; c < CPL; ++c) a[c] = fmaf(fj, v[j][c], a[c]);
+          }
+        }
+      }
+    }
+    const float inv = l == 0.f ? 0.f : 1.0f / l;
+    __nv_bfloat16* out = static_cast<__nv_bfloat16*>(p.o) + head.s * p.os.t + int64_t(h) * p.os.h + lane * CPL;
+#pragma unroll
+    for (int c = 0; c < CPL; c += 2) *reinterpret_cast<uint32_t*>(out + c) = pack_bf16(a[c] * inv, a[c + 1] * inv);
+  }
+}
+
+template <int D, int RB, int LOG2N>
+int launch_n(const RaggedParams& p, const TokenPlan& plan, cudaStream_t stream) {
   using C = Cfg<D, RB>;
   static_assert(C::CTAS * (smem_bytes<D, RB>() + 1024) <= 233472, "shared memory of an SM");
   CUtensorMap tm[2];
@@ -458,14 +545,20 @@ int launch(const RaggedParams& p, const TokenPlan& plan, cudaStream_t stream) {
     const uint64_t dims[5] = {64, uint64_t(p.page), uint64_t(D / 64), uint64_t(p.Hkv), uint64_t(p.pages)};
     const uint64_t strides[4] = {uint64_t(s.t), 64, uint64_t(s.h), uint64_t(i == 0 ? p.k_page : p.v_page)};
     const uint32_t box[5] = {64, uint32_t(std::min(p.page, TILE)), 1, 1, 1};
-    if (int rc = make_tmap_bf16(&tm[i], i == 0 ? p.k : p.v, 5, dims, strides, box, true)) return rc;
+    if (int rc = make_tmap_bf16(&tm[i], i == 0 ? p.k : p.v, 5, dims, strides, box, true, D == 64 ? CU_TENSOR_MAP_L2_PROMOTION_L2_128B : CU_TENSOR_MAP_L2_PROMOTION_L2_256B)) return rc;
   }
-  auto kern = paged_token_kernel<D, RB>;
+  auto kern = paged_token_kernel<D, RB, LOG2N>;
   static PerDeviceOnce configured;
   if (int rc = configured.run([&] { return cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, int(smem_bytes<D, RB>())); })) return rc;
   ALG_CUDA_TRY(launch_dependent(kern, dim3(plan.grid), dim3(C::NTHREADS), smem_bytes<D, RB>(), stream, tm[0], tm[1], p, plan));
-  count_launch();
+  ALG_CUDA_TRY(launch_dependent(paged_token_merge_kernel<D, RB>, dim3(plan.grid), dim3(256), 0, stream, p, plan));
+  count_launch(2);
   return ALG_OK;
+}
+
+template <int D, int RB>
+int launch(const RaggedParams& p, const TokenPlan& plan, cudaStream_t stream) {
+  return p.log2n == 4 ? launch_n<D, RB, 4>(p, plan, stream) : launch_n<D, RB, 0>(p, plan, stream);
 }
 
 constexpr size_t align256(size_t x) { return (x + 255) & ~size_t(255); }
@@ -481,8 +574,8 @@ int token_grid(int S, int Hkv, int G, int D, int64_t keys) {
 }  // namespace
 
 size_t paged_token_workspace_bytes(int S, int Hkv, int G, int D, int64_t keys) {
-  const int rb = row_block(G), groups = (G + rb - 1) / rb;
-  return align256(size_t(token_grid(S, Hkv, G, D, keys)) * 2 * rb * (D + 2) * sizeof(float)) + size_t(S) * Hkv * groups * 8;
+  const size_t grid = size_t(token_grid(S, Hkv, G, D, keys));
+  return align256(grid * sizeof(TokenHead)) + grid * 2 * row_block(G) * (D + 2) * sizeof(float);
 }
 
 int launch_paged_token(const RaggedParams& p, void* workspace, cudaStream_t stream) {
@@ -491,10 +584,9 @@ int launch_paged_token(const RaggedParams& p, void* workspace, cudaStream_t stre
   plan.groups = (p.G + rb - 1) / rb;
   plan.heads = p.Hkv * plan.groups;
   plan.grid = token_grid(p.seqs.S, p.Hkv, p.G, p.D, p.seqs.kv_capacity);
-  plan.slots = static_cast<float*>(workspace);
-  plan.arrivals = reinterpret_cast<unsigned long long*>(static_cast<unsigned char*>(workspace) +
-                                                        align256(size_t(plan.grid) * 2 * rb * (p.D + 2) * sizeof(float)));
-  plan.call = next_call_number();
+  plan.heads_open = static_cast<TokenHead*>(workspace);
+  plan.slots = reinterpret_cast<float*>(static_cast<unsigned char*>(workspace) + align256(plan.grid * sizeof(TokenHead)));
+  plan.x_fast = ragged_fast_range(1 << p.log2n);
   if (p.D == 64) return rb == 8 ? launch<64, 8>(p, plan, stream) : launch<64, 16>(p, plan, stream);
   return rb == 8 ? launch<128, 8>(p, plan, stream) : launch<128, 16>(p, plan, stream);
 }

@@ -10,6 +10,8 @@
 // clamped to the tensors' extents, so that no value in them leads outside.
 #pragma once
 
+#include <math.h>
+
 #include "common.cuh"
 
 namespace alg {
@@ -103,11 +105,12 @@ struct RaggedParams {
 };
 
 // One token a sequence (paged_token.cu).
+struct __align__(16) TokenHead { int s, h, row0, parts; };   // a head that goes on behind the stretch it began in; parts 0: none
 struct TokenPlan {
   int groups, heads, grid;  // row groups of a key head; key heads times groups; CTAs
   float* slots;             // two states a CTA: of the head its stretch begins in, of the one it ends in
-  unsigned long long* arrivals;   // a word per (sequence, head)
-  unsigned long long call;
+  TokenHead* heads_open;    // per CTA
+  float x_fast;
 };
 size_t paged_token_workspace_bytes(int S, int Hkv, int G, int D, int64_t keys);
 int launch_paged_token(const RaggedParams& p, void* workspace, cudaStream_t stream);
@@ -117,6 +120,19 @@ __device__ __forceinline__ float rho_any(float x) {
   const float rad = fmaf(x, x, 1.0f);
   const float T = rad < 3.0e38f ? fmaf(rad, rsqrt_approx(rad), fabsf(x)) : 2.0f * fabsf(x);
   return x >= 0.0f ? T : __fdividef(1.0f, T);
+}
+
+// |x| up to which weights may go unshifted: rho(x)^n <= 2^64, and x + sqrt(1 + x^2) loses no more than n x^2 2^-23 < 2e-4 of a
+// weight to cancellation
+inline float ragged_fast_range(int n) {
+  const double rho = pow(2.0, 64.0 / n), x = 0.5 * (rho - 1.0 / rho);
+  return float(x < 8.0 ? x : 8.0);
+}
+
+__device__ __forceinline__ float max3_abs_nan(float a, float b, float c) {      // NaN if one of them is
+  float r;
+  asm("max.NaN.abs.f32 %0, %1, %2, %3;" : "=f"(r) : "f"(a), "f"(b), "f"(c));
+  return r;
 }
 
 struct AppendParams {

@@ -183,11 +183,6 @@ __device__ __forceinline__ void weigh_tile(uint32_t s_taddr, uint64_t* p_half, u
   signal_weights(p_full);
 }
 
-__device__ __forceinline__ float max3_abs_nan(float a, float b, float c) {      // NaN if one of them is
-  float r;
-  asm("max.NaN.abs.f32 %0, %1, %2, %3;" : "=f"(r) : "f"(a), "f"(b), "f"(c));
-  return r;
-}
 // Largest |y| of the row's visible scores, NaN if one is NaN.  Only what the row sees counts: which form its weights take, and
 // with it their rounding, must not depend on a neighbouring sequence.
 template <bool MASK>
@@ -752,15 +747,13 @@ int launch_d(const RaggedParams& p, cudaStream_t stream) {
     }
   }
   ScoreScale sc;
-  const int n = 1 << p.log2n;
   {
     int ex = 0;
     const double f = frexp(double(p.scale), &ex);         // scale = f 2^ex = 2^(ex - 1) m, 1 <= m < 2
     const double m = 2.0 * f;
     sc.pow2 = float(ldexp(1.0, ex - 1));
     sc.m = float(m); sc.inv_m = float(1.0 / m); sc.kappa = float(1.0 / (m * m));
-    const double rho = pow(2.0, 64.0 / n);                // rho(x_fast)^n = 2^64
-    sc.y_fast = float(std::min(8.0, 0.5 * (rho - 1.0 / rho)) / m);
+    sc.y_fast = float(ragged_fast_range(1 << p.log2n) / m);
   }
   const int64_t most = int64_t(p.plan.max_items) * p.Hkv;
   const int grid = int(std::min<int64_t>(most, p.plan.sms));

@@ -369,6 +369,6 @@ EncodeTiledFn get_encode_tiled();
 
 // bf16 tensor of `rank` dims (dims[0] innermost, contiguous); strides in ELEMENTS for dims 1..rank-1.
 int make_tmap_bf16(CUtensorMap* out, const void* base, int rank, const uint64_t* dims, const uint64_t* strides_elems,
-                   const uint32_t* box, bool swizzle128);
+                   const uint32_t* box, bool swizzle128, CUtensorMapL2promotion fetch = CU_TENSOR_MAP_L2_PROMOTION_L2_256B);
 
 }  // namespace alg

@@ -21,7 +21,7 @@ EncodeTiledFn get_encode_tiled() {
 }
 
 int make_tmap_bf16(CUtensorMap* out, const void* base, int rank, const uint64_t* dims, const uint64_t* strides_elems,
-                   const uint32_t* box, bool swizzle128) {
+                   const uint32_t* box, bool swizzle128, CUtensorMapL2promotion fetch) {
   EncodeTiledFn enc = get_encode_tiled();
   if (enc == nullptr) {
     set_error("cuTensorMapEncodeTiled is not available from this driver");
@@ -50,7 +50,7 @@ int make_tmap_bf16(CUtensorMap* out, const void* base, int rank, const uint64_t*
     return enc(out, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, cuuint32_t(rank), const_cast<void*>(base), gdim, gstride,
                bdim, estride, CU_TENSOR_MAP_INTERLEAVE_NONE,
                swizzle128 ? CU_TENSOR_MAP_SWIZZLE_128B : CU_TENSOR_MAP_SWIZZLE_NONE,
-               CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+               fetch, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
   };
   CUresult r = encode();
   if (r == CUDA_ERROR_INVALID_CONTEXT) {
