@@ -232,16 +232,13 @@ paged_token_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_consta
         unsigned char* dst = smem + size_t(stage) * 2 * TILE_BYTES;
         const int live = min(pieces, chunks - c0);
         if (lane == 0) mbar_arrive_expect_tx(&ctl->full[stage], uint32_t(live * rows) * (D * 2) * 2);
-        for (int i = 0; i < live; ++i) {
-          const int page = __shfl_sync(0xffffffffu, number, c0 + i - held);
-          if (lane == 0) {
-            const int row = (k0 + ((c0 + i) << log2_rows)) & (p.page - 1);
-#pragma unroll
-            for (int pn = 0; pn < C::PANELS; ++pn) {
-              tma_load_5d(dst + pn * PANEL + i * rows * 128, &tm_k, &ctl->full[stage], 0, row, pn, h, page);
-              tma_load_5d(dst + TILE_BYTES + pn * PANEL + i * rows * 128, &tm_v, &ctl->full[stage], 0, row, pn, h, page);
-            }
-          }
+        __syncwarp();
+        // a lane a copy: of K or V, a panel, a piece of a page
+        const int piece = lane / (2 * C::PANELS), pn = (lane >> 1) % C::PANELS, v = lane & 1;
+        const int page = __shfl_sync(0xffffffffu, number, (c0 + piece - held) & 31);
+        if (piece < live) {
+          const int row = (k0 + ((c0 + piece) << log2_rows)) & (p.page - 1);
+          tma_load_5d(dst + v * TILE_BYTES + pn * PANEL + piece * rows * 128, v ? &tm_v : &tm_k, &ctl->full[stage], 0, row, pn, h, page);
         }
         __syncwarp();
       }
