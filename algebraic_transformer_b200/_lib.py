@@ -108,6 +108,13 @@ class PackedAttnArgs(C.Structure):
                 ("o_stride", I64x2), ("workspace", C.c_void_p), ("workspace_bytes", C.c_size_t), ("status", C.c_void_p)]
 
 
+class PackedAttnBwdArgs(C.Structure):
+    _fields_ = [(name, C.c_void_p) for name in ("q", "k", "v", "o", "o_rest", "d_o", "stat", "cu_seqlens", "sink", "dq", "dk", "dv", "dsink")] + \
+               [(name, C.c_int) for name in ("sequences", "tokens", "H", "Hkv", "D", "n")] + [("c", C.c_float)] + \
+               [(name + "_stride", I64x2) for name in ("q", "k", "v", "o", "do", "dq", "dk", "dv")] + \
+               [("workspace", C.c_void_p), ("workspace_bytes", C.c_size_t), ("status", C.c_void_p)]
+
+
 class PagedAttnArgs(C.Structure):
     _fields_ = [(name, C.c_void_p) for name in ("q", "k_pages", "v_pages", "o", "block_table", "kv_lens", "cu_seqlens", "sink")] + \
                [(name, C.c_int) for name in ("sequences", "tokens", "H", "Hkv", "D", "pages", "page_size", "table_width", "n")] + \
@@ -164,6 +171,8 @@ SYMBOLS = {
     "alg_attn_decode_status": (C.c_int, [C.POINTER(DecodeArgs), C.c_void_p, C.c_void_p]),
     "alg_packed_attn_workspace_bytes": (C.c_size_t, [C.POINTER(PackedAttnArgs)]),
     "alg_packed_attn_fwd": (C.c_int, [C.POINTER(PackedAttnArgs), C.c_void_p]),
+    "alg_packed_attn_bwd_workspace_bytes": (C.c_size_t, [C.POINTER(PackedAttnBwdArgs)]),
+    "alg_packed_attn_bwd": (C.c_int, [C.POINTER(PackedAttnBwdArgs), C.c_void_p]),
     "alg_paged_attn_workspace_bytes": (C.c_size_t, [C.POINTER(PagedAttnArgs)]),
     "alg_paged_attn_fwd": (C.c_int, [C.POINTER(PagedAttnArgs), C.c_void_p]),
     "alg_paged_append": (C.c_int, [C.POINTER(PagedAppendArgs), C.c_void_p]),

@@ -3,6 +3,7 @@ reference's custom VJP, so that `.backward()` flows through the three fused oper
 `jax.grad` flows through the reference's:
 
     attention(q, k, v, sink, ...)      src/algebraic/kernels/flash.py:333-857   (dq, dk, dv, dsink)
+    packed_attention(q, k, v, cu, sink) the same over packed sequences of different lengths, with grouped heads
     head_loss(h, embed, targets, ...)  src/algebraic/kernels/fused_head.py:232-254 (dh, dembed)
     qk_norm(x, gain, eps)              src/algebraic/kernels/qk_norm.py:29-56   (dx, dgain)
 
@@ -51,6 +52,32 @@ def attention(q, k, v, sink_logit: Optional[torch.Tensor] = None, *, n: int = 16
     if sink_logit is not None and (sink_logit.dtype != torch.float32 or sink_logit.shape != (q.shape[1],)):
         raise ValueError("sink_logit must be a float32 tensor of shape (H,)")
     return _Attention.apply(q, k, v, sink_logit, int(n), float(c), bool(causal), bool(range_guard))
+
+
+class _PackedAttention(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, q, k, v, cu_seqlens, sink, n, c):
+        o, stat, rest = ops.packed_attention(q, k, v, cu_seqlens, sink, n=n, c=c, return_stat=True)
+        ctx.save_for_backward(q, k, v, o, stat, rest, cu_seqlens, sink if sink is not None else stat.new_empty(0))
+        ctx.has_sink, ctx.n, ctx.c = sink is not None, n, c
+        return o
+
+    @staticmethod
+    def backward(ctx, d_o):
+        q, k, v, o, stat, rest, cu_seqlens, sink = ctx.saved_tensors
+        dq, dk, dv, dsink = ops.packed_attention_backward(q, k, v, o, d_o.to(o.dtype), stat, rest, cu_seqlens, sink if ctx.has_sink else None,
+                                                          n=ctx.n, c=ctx.c)
+        return dq, dk, dv, None, dsink, None, None
+
+
+def packed_attention(q, k, v, cu_seqlens, sink_logit: Optional[torch.Tensor] = None, *, n: int = 16, c: float = 8.0):
+    """Differentiable attention over packed sequences of different lengths with grouped heads: `ops.packed_attention` and
+    `ops.packed_attention_backward`.  q (tokens, H, D), k, v (tokens, Hkv, D) bf16, `cu_seqlens` int32 (sequences + 1) on the device,
+    which has to keep its values until the backward pass; `sink_logit` is a float32 (H,) tensor or None.  Rows of no sequence have
+    output and gradients zero."""
+    if sink_logit is not None and (sink_logit.dtype != torch.float32 or sink_logit.shape != (q.shape[1],)):
+        raise ValueError("sink_logit must be a float32 tensor of shape (H,)")
+    return _PackedAttention.apply(q, k, v, cu_seqlens, sink_logit, int(n), float(c))
 
 
 def _scaled(x, g, dtype):

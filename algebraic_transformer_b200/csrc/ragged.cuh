@@ -159,6 +159,34 @@ struct AppendParams {
 };
 int launch_paged_append(const AppendParams& p, cudaStream_t stream);
 
+struct RaggedBwdParams {
+  const __nv_bfloat16* q;
+  const __nv_bfloat16* k;
+  const __nv_bfloat16* v;
+  const __nv_bfloat16* o;
+  const __nv_bfloat16* rest;
+  const __nv_bfloat16* d_o;
+  const float* stat;        // (H, tokens)
+  const float* sink;
+  const int* cu;
+  __nv_bfloat16* dq;
+  __nv_bfloat16* dk;
+  __nv_bfloat16* dv;
+  float* dsink;
+  float* delta;             // (H, tokens)
+  float* sink_parts;        // (chunks, H)
+  RaggedBlocks blocks;
+  Strides2 qs, ks, vs, os, gs, dqs, dks, dvs;
+  int S, tokens, H, Hkv, G, D, log2n, chunks;
+  float scale, inv_c, n_f, y_fast;
+  int* status;
+};
+size_t ragged_bwd_workspace_bytes(int S, int tokens, int H);
+int launch_ragged_backward(const RaggedBwdParams& p, void* workspace, cudaStream_t stream);
+size_t ragged_blocks_bytes(int S, int tokens);
+void ragged_blocks_carve(RaggedBlocks* blocks, void* workspace, int S, int tokens);
+int launch_ragged_blocks(const RaggedSeqs& seqs, const RaggedBlocks& blocks, cudaStream_t stream);
+
 size_t ragged_plan_bytes(int S, int tokens, int Hkv, int G, int D, bool may_split);
 void ragged_plan_carve(RaggedPlan* plan, void* workspace, int S, int tokens, int Hkv, int G, int D, bool may_split);
 int launch_ragged_plan(const RaggedSeqs& seqs, const RaggedPlan& plan, int G, cudaStream_t stream);

@@ -86,6 +86,54 @@ int alg_packed_attn_fwd(const alg_packed_attn_args* a, void* stream_) {
   return launch_ragged_attention(p, stream);
 }
 
+size_t alg_packed_attn_bwd_workspace_bytes(const alg_packed_attn_bwd_args* a) {
+  if (a == nullptr || a->tokens < 0 || a->sequences < 0 || a->H < 1) return 0;
+  return ragged_bwd_workspace_bytes(a->sequences, a->tokens, a->H);
+}
+
+int alg_packed_attn_bwd(const alg_packed_attn_bwd_args* a, void* stream) {
+  if (a == nullptr || a->q == nullptr || a->k == nullptr || a->v == nullptr || a->o == nullptr || a->o_rest == nullptr || a->d_o == nullptr ||
+      a->stat == nullptr || a->cu_seqlens == nullptr || a->dq == nullptr || a->dk == nullptr || a->dv == nullptr) {
+    set_error("packed attention backward: null tensor argument");
+    return ALG_ERR_INVALID;
+  }
+  if (int rc = check_link("packed attention backward", a->H, a->Hkv, a->D, a->n, a->c)) return rc;
+  if (a->tokens < 0 || a->sequences < 0) { set_error("packed attention backward: negative extent"); return ALG_ERR_INVALID; }
+  if ((a->sink == nullptr) != (a->dsink == nullptr)) { set_error("packed attention backward: sink and dsink come as a pair"); return ALG_ERR_INVALID; }
+  RaggedBwdParams p{};
+  if (!strides_ok(&p.qs, a->q_stride, a->tokens, a->H, a->D) || !strides_ok(&p.ks, a->k_stride, a->tokens, a->Hkv, a->D) ||
+      !strides_ok(&p.vs, a->v_stride, a->tokens, a->Hkv, a->D) || !strides_ok(&p.os, a->o_stride, a->tokens, a->H, a->D) ||
+      !strides_ok(&p.gs, a->do_stride, a->tokens, a->H, a->D) || !strides_ok(&p.dqs, a->dq_stride, a->tokens, a->H, a->D) ||
+      !strides_ok(&p.dks, a->dk_stride, a->tokens, a->Hkv, a->D) || !strides_ok(&p.dvs, a->dv_stride, a->tokens, a->Hkv, a->D) ||
+      !aligned16(a->q) || !aligned16(a->k) || !aligned16(a->v) || !aligned16(a->o) || !aligned16(a->o_rest) || !aligned16(a->d_o) ||
+      !aligned16(a->dq) || !aligned16(a->dk) || !aligned16(a->dv)) {
+    set_error("packed attention backward: rows must start on 16-byte boundaries and lie apart");
+    return ALG_ERR_INVALID;
+  }
+  const size_t need = alg_packed_attn_bwd_workspace_bytes(a);
+  if (a->workspace == nullptr || a->workspace_bytes < need || !aligned16(a->workspace)) {
+    set_error("packed attention backward: workspace of %zu bytes (16-byte aligned) required, got %zu", need, a->workspace_bytes);
+    return ALG_ERR_WORKSPACE;
+  }
+  if (a->tokens == 0) {
+    if (a->dsink != nullptr) ALG_CUDA_TRY(cudaMemsetAsync(a->dsink, 0, size_t(a->H) * sizeof(float), static_cast<cudaStream_t>(stream)));
+    return ALG_OK;
+  }
+  p.q = static_cast<const __nv_bfloat16*>(a->q); p.k = static_cast<const __nv_bfloat16*>(a->k); p.v = static_cast<const __nv_bfloat16*>(a->v);
+  p.o = static_cast<const __nv_bfloat16*>(a->o); p.rest = static_cast<const __nv_bfloat16*>(a->o_rest);
+  p.d_o = static_cast<const __nv_bfloat16*>(a->d_o);
+  p.stat = a->stat; p.sink = a->sink; p.cu = a->cu_seqlens;
+  p.dq = static_cast<__nv_bfloat16*>(a->dq); p.dk = static_cast<__nv_bfloat16*>(a->dk); p.dv = static_cast<__nv_bfloat16*>(a->dv);
+  p.dsink = a->dsink;
+  p.S = a->sequences; p.tokens = a->tokens; p.H = a->H; p.Hkv = a->Hkv; p.G = a->H / a->Hkv; p.D = a->D;
+  p.log2n = ilog2_exact(a->n);
+  p.scale = float(1.0 / (sqrt(double(a->D)) * double(a->c)));
+  p.inv_c = 1.0f / a->c;
+  p.n_f = float(a->n);
+  p.status = a->status;
+  return launch_ragged_backward(p, a->workspace, static_cast<cudaStream_t>(stream));
+}
+
 }  // extern "C"
 
 template <class Args> static int paged_checks(const Args* a, const char* what) {

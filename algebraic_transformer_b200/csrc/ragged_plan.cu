@@ -74,7 +74,7 @@ __device__ __forceinline__ int sequence_of(const int* prefix, int S, int i) {
 }
 
 __global__ void __launch_bounds__(NT) ragged_plan_kernel(const RaggedSeqs q, const RaggedPlan plan) {
-  __shared__ int warp_sums[33], hist[CLASSES], s_max, s_target, s_slots, s_combos, s_parts;
+  __shared__ int warp_sums[33], hist[CLASSES], s_max, s_slots, s_combos, s_parts;
   __shared__ unsigned long long s_cost;
   griddep_wait();                                      // the workspace may be another call's until here
   hist[threadIdx.x] = 0;
@@ -166,6 +166,47 @@ __global__ void __launch_bounds__(NT) ragged_plan_kernel(const RaggedSeqs q, con
   if (threadIdx.x == 0) *plan.header = RaggedHeader{min(total, plan.max_items), min(s_combos, plan.max_combos), 0, 0};
 }
 
+// The backward's two lists of 128-row blocks: by the rows from the block to the sequence's end (key blocks, seen by these
+// queries), by the rows up to the block's end (query blocks, which see these keys).
+__global__ void __launch_bounds__(NT) ragged_blocks_kernel(const RaggedSeqs q, const RaggedBlocks blocks) {
+  __shared__ int warp_sums[33], hist[2][CLASSES], s_max;
+  griddep_wait();
+  hist[0][threadIdx.x] = hist[1][threadIdx.x] = 0;
+  if (threadIdx.x == 0) s_max = 1;
+  const int n = min(sequence_blocks(q, 128, blocks.prefix, warp_sums), blocks.max_items);
+  auto block_at = [&](int i) {
+    const int s = sequence_of(blocks.prefix, q.S, i);
+    int row0, Lq, Lk;
+    ragged_lengths(q, s, row0, Lq, Lk);
+    return make_int4(row0, Lq, (i - blocks.prefix[s]) * 128, s);
+  };
+  for (int i = threadIdx.x; i < n; i += NT) atomicMax(&s_max, (block_at(i).y + 127) >> 7);
+  __syncthreads();
+  const int longest = s_max;
+  auto class_of = [&](const int4& b, int list) {
+    const int cost = list == 0 ? (b.y - b.z + 127) >> 7 : (b.z >> 7) + 1;
+    return CLASSES - 1 - int(int64_t(cost) * (CLASSES - 1) / longest);
+  };
+  for (int i = threadIdx.x; i < n; i += NT) {
+    const int4 b = block_at(i);
+    atomicAdd(&hist[0][class_of(b, 0)], 1);
+    atomicAdd(&hist[1][class_of(b, 1)], 1);
+  }
+  __syncthreads();
+  for (int list = 0; list < 2; ++list) {
+    int total;
+    const int start = block_scan(hist[list][threadIdx.x], warp_sums, &total);
+    __syncthreads();
+    hist[list][threadIdx.x] = start;
+  }
+  __syncthreads();
+  for (int i = threadIdx.x; i < n; i += NT) {
+    const int4 b = block_at(i);
+    for (int list = 0; list < 2; ++list) blocks.list[list * n + atomicAdd(&hist[list][class_of(b, list)], 1)] = b;
+  }
+  if (threadIdx.x == 0) *blocks.header = RaggedHeader{n, 0, 0, 0};
+}
+
 constexpr size_t align256(size_t x) { return (x + 255) & ~size_t(255); }
 
 struct Sizes { int items, slots, combos; };
@@ -207,6 +248,28 @@ void ragged_plan_carve(RaggedPlan* plan, void* workspace, int S, int tokens, int
 
 int launch_ragged_plan(const RaggedSeqs& seqs, const RaggedPlan& plan, int G, cudaStream_t stream) {
   ALG_CUDA_TRY(launch_dependent(ragged_plan_kernel, dim3(1), dim3(NT), 0, stream, seqs, plan));
+  count_launch();
+  return ALG_OK;
+}
+
+static int max_blocks(int S, int tokens) { return tokens / 128 + (S < tokens ? S : tokens); }
+
+size_t ragged_blocks_bytes(int S, int tokens) {
+  return 256 + align256(2 * size_t(max_blocks(S, tokens)) * sizeof(int4)) + align256((size_t(S) + 1) * sizeof(int));
+}
+
+void ragged_blocks_carve(RaggedBlocks* blocks, void* workspace, int S, int tokens) {
+  unsigned char* at = static_cast<unsigned char*>(workspace);
+  blocks->max_items = max_blocks(S, tokens);
+  blocks->header = reinterpret_cast<RaggedHeader*>(at);
+  at += 256;
+  blocks->list = reinterpret_cast<int4*>(at);
+  at += align256(2 * size_t(blocks->max_items) * sizeof(int4));
+  blocks->prefix = reinterpret_cast<int*>(at);
+}
+
+int launch_ragged_blocks(const RaggedSeqs& seqs, const RaggedBlocks& blocks, cudaStream_t stream) {
+  ALG_CUDA_TRY(launch_dependent(ragged_blocks_kernel, dim3(1), dim3(NT), 0, stream, seqs, blocks));
   count_launch();
   return ALG_OK;
 }

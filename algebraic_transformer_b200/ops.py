@@ -669,6 +669,46 @@ def packed_attention(q, k, v, cu_seqlens, sink_logit=None, *, n: int = 16, c: fl
     return (o, stat, rest) if return_stat else o
 
 
+@_on_tensor_device
+def packed_attention_backward(q, k, v, o, d_o, stat, rest, cu_seqlens, sink_logit=None, *, n: int = 16, c: float = 8.0):
+    """Gradients of `packed_attention(return_stat=True)`: `(dq, dk, dv, dsink)` from the forward's inputs, its output `o` with `stat`
+    and `rest`, and the output gradient `d_o`.  dk and dv are summed over the query heads of a group; dsink (H,) float32 is None
+    without a sink.  Gradients of rows of no sequence are zeros.  Results repeat bit for bit."""
+    _require_cuda(q, k, v, o, d_o, stat, rest, cu_seqlens)
+    _check_packed(q, k, v)
+    _check_link(n, c)
+    _check_lengths("cu_seqlens", cu_seqlens, None)
+    T, H, D = q.shape
+    if any(t.shape != q.shape or t.dtype != torch.bfloat16 for t in (o, d_o, rest)) or not rest.is_contiguous():
+        raise ValueError("o, d_o and rest must be (tokens, H, D) bfloat16 like q, rest contiguous")
+    if stat.shape != (H, T) or stat.dtype != torch.float32 or not stat.is_contiguous():
+        raise ValueError("stat must be the contiguous float32 (H, tokens) statistic of the forward")
+    # the gradient is read in the layout it comes in where its rows are 16-byte aligned and apart; any other (an expanded one) is copied
+    gt, gh, gd = d_o.stride()
+    if gd != 1 or (T > 1 and (gt <= 0 or gt % 8)) or (H > 1 and (gh <= 0 or gh % 8)) or d_o.data_ptr() % 16:
+        d_o = torch.empty(d_o.shape, dtype=d_o.dtype, device=d_o.device).copy_(d_o)
+    sink = None
+    if sink_logit is not None:
+        sink = _sink_vector(sink_logit, H, q.device)
+        if sink.numel() != H:
+            raise ValueError("sink_logit must broadcast to (H,)")
+    dq, dk, dv = (torch.empty(t.shape, dtype=t.dtype, device=t.device) for t in (q, k, v))
+    dsink = torch.empty(H, dtype=torch.float32, device=q.device) if sink is not None else None
+    if T == 0:
+        return dq, dk, dv, (dsink.zero_() if dsink is not None else None)
+    a = L.PackedAttnBwdArgs(q=q.data_ptr(), k=k.data_ptr(), v=v.data_ptr(), o=o.data_ptr(), o_rest=rest.data_ptr(), d_o=d_o.data_ptr(),
+                            stat=stat.data_ptr(), cu_seqlens=cu_seqlens.data_ptr(), sink=_ptr(sink), dq=dq.data_ptr(), dk=dk.data_ptr(),
+                            dv=dv.data_ptr(), dsink=_ptr(dsink), sequences=cu_seqlens.numel() - 1, tokens=T, H=H, Hkv=k.shape[1], D=D,
+                            n=int(n), c=float(c), q_stride=_strides2(q), k_stride=_strides2(k), v_stride=_strides2(v),
+                            o_stride=_strides2(o), do_stride=_strides2(d_o), dq_stride=_strides2(dq), dk_stride=_strides2(dk),
+                            dv_stride=_strides2(dv))
+    lib = L.load()
+    ws = _workspace(q.device, lib.alg_packed_attn_bwd_workspace_bytes(a), "packed_bwd")
+    a.workspace, a.workspace_bytes = ws.data_ptr(), ws.numel()
+    L.check(lib.alg_packed_attn_bwd(a, _stream()))
+    return dq, dk, dv, dsink
+
+
 def _check_pages(q, k_pages, v_pages, block_table, kv_lens, cu_seqlens):
     if q.ndim != 3 or k_pages.ndim != 4 or k_pages.shape != v_pages.shape or k_pages.shape[3] != q.shape[2]:
         raise ValueError("q must be (tokens, H, D) and k_pages, v_pages (pages, page_size, Hkv, D)")

@@ -288,6 +288,35 @@ typedef struct {
 ALG_API size_t alg_packed_attn_workspace_bytes(const alg_packed_attn_args* args);
 ALG_API int alg_packed_attn_fwd(const alg_packed_attn_args* args, void* stream);
 
+/* Backward: dq, dk, dv and dsink from the forward's inputs, its output o with o_rest and stat, and the output gradient d_o (the formulas
+ * are those of alg_attn_bwd; dk and dv are summed over the query heads of a group).  Layouts as in the forward, d_o and the
+ * gradients with strides of their own; gradients of rows of no sequence are zeros.  sink, dsink: (H) fp32, or both NULL.  Every
+ * sum is formed in an order of its own, so that results repeat bit for bit. */
+typedef struct {
+  const void* q;
+  const void* k;
+  const void* v;
+  const void* o;
+  const void* o_rest;
+  const void* d_o;
+  const float* stat;
+  const int* cu_seqlens;
+  const float* sink;
+  void* dq;
+  void* dk;
+  void* dv;
+  float* dsink;
+  int sequences, tokens, H, Hkv, D;
+  int n;
+  float c;
+  int64_t q_stride[2], k_stride[2], v_stride[2], o_stride[2], do_stride[2], dq_stride[2], dk_stride[2], dv_stride[2];
+  void* workspace;
+  size_t workspace_bytes;
+  int* status;             /* device int, may be NULL */
+} alg_packed_attn_bwd_args;
+ALG_API size_t alg_packed_attn_bwd_workspace_bytes(const alg_packed_attn_bwd_args* args);
+ALG_API int alg_packed_attn_bwd(const alg_packed_attn_bwd_args* args, void* stream);
+
 /* The same over a cache in pages: queries are the last tokens of their sequences, the keys of all of a sequence's tokens (the new
  * ones too) lie in the pool's pages.
  * k_pages, v_pages: (pages, page_size, Hkv, D) bf16, strides of (page, token, head); page_size a power of two from 16

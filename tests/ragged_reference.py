@@ -85,3 +85,50 @@ def assert_close(got, o, spread, err, weights=BF16, result=BF16):
     assert torch.isfinite(got).all(), f"{int((~torch.isfinite(got)).sum())} values are not finite"
     worst = float((off / bound).max())
     assert worst <= 1.0, f"{worst} times the bound, at {torch.nonzero(off / bound == (off / bound).max())[0].tolist()}"
+
+
+def packed_gradients(q, k, v, d_o, cu, sink, n, c):
+    """The formulas of the gradients, one (sequence, head) at a time, with what the kernels' roundings can add to each:
+    ((dq, dk, dv, dsink), their bounds).  p and dS are rounded to bf16 ahead of the products, delta comes from an output of 16 bits,
+    the rest is 32-bit arithmetic."""
+    q, k, v, d_o = (t.double().cpu() for t in (q, k, v, d_o))
+    H, Hkv, D = q.shape[1], k.shape[1], q.shape[2]
+    out = [torch.zeros_like(t) for t in (q, k, v)] + [torch.zeros(H, dtype=torch.float64)]
+    bound = [torch.zeros_like(t) for t in out]
+    for a, b in zip(cu[:-1].tolist(), cu[1:].tolist()):
+        for h in range(H):
+            if b <= a:
+                continue
+            g = h // (H // Hkv)
+            Q, K, V, G = q[a:b, h], k[a:b, g], v[a:b, g], d_o[a:b, h]
+            scale = 1.0 / (D ** 0.5 * c)
+            x = (Q @ K.t()) * scale
+            hidden = torch.arange(b - a)[None] > torch.arange(b - a)[:, None]
+            logw = (n * torch.asinh(x)).masked_fill(hidden, -float("inf"))
+            z = torch.tensor(-float("inf"), dtype=torch.float64) if sink is None else sink[h].double().cpu() / c
+            logs = n * torch.asinh(z) if sink is not None else z
+            top = torch.maximum(logw.amax(1, keepdim=True), logs)
+            w, ws = torch.exp(logw - top), torch.exp(logs - top)
+            total = w.sum(1, keepdim=True) + ws
+            p, ps = w / total, ws / total
+            o, spread = p @ V, p @ V.abs()
+            dP, delta = G @ V.t(), (G * o).sum(1, keepdim=True)
+            f = n * scale / torch.sqrt(1 + x * x)
+            dS = f * p * (dP - delta)
+            out[0][a:b, h] += dS @ K
+            out[1][a:b, g] += dS.t() @ Q
+            out[2][a:b, g] += p.t() @ G
+            err = weight_error(Q, K, n, c)
+            e_delta = (G.abs() * (2.0 ** -15 + 4 * err) * spread).sum(1, keepdim=True) + D * 2.0 ** -23 * G.norm(dim=1, keepdim=True) * V.norm(dim=1).max()
+            eS = f * p * ((BF16 + 2 * err) * (dP - delta).abs() + 1.01 * e_delta)
+            bound[0][a:b, h] += eS @ K.abs()
+            bound[1][a:b, g] += eS.t() @ Q.abs()
+            bound[2][a:b, g] += (BF16 + 2 * err) * (p.t() @ G.abs())
+            if sink is not None:
+                slope = n / c / torch.sqrt(1 + z * z)
+                out[3][h] -= slope * (ps * delta).sum()
+                bound[3][h] += slope * (ps * (e_delta + 2 * err * delta.abs())).sum()
+    for i in range(3):
+        bound[i] = 1.05 * bound[i] + BF16 * (out[i].abs() + bound[i]) + 1e-30
+    bound[3] = 1.05 * bound[3] + 2.0 ** -20 * out[3].abs() + 1e-30
+    return out, bound
