@@ -595,30 +595,59 @@ def decode_attention(q, k, v, sink_logit=None, *, n: int = 16, c: float = 8.0, o
 
 # -------------------------------------------------------- packed sequences, paged cache
 
-def _strides2(t: torch.Tensor):
-    if t.stride(-1) != 1:
+def _rows(t: torch.Tensor):
+    """Strides of all axes but the last, which has to be contiguous."""
+    st = t.stride()
+    if st[-1] != 1:
         raise ValueError("the last (head_dim) axis must be contiguous")
-    return L.I64x2(t.stride(0), t.stride(1))
+    return st[:-1]
+
+
+def _sink_of(sink_logit, H, device):
+    if sink_logit is None:
+        return None, 0
+    sink = _sink_vector(sink_logit, H, device)
+    if sink.numel() != H:
+        raise ValueError("sink_logit must broadcast to (H,)")
+    return sink, sink.data_ptr()
+
+
+@functools.lru_cache(maxsize=256)
+def _packed_bytes(device: int, sequences: int, tokens: int, H: int, Hkv: int, D: int) -> int:
+    return L.load().alg_packed_attn_workspace_bytes(L.PackedAttnArgs(sequences=sequences, tokens=tokens, H=H, Hkv=Hkv, D=D))
+
+
+@functools.lru_cache(maxsize=256)
+def _packed_bwd_bytes(sequences: int, tokens: int, H: int) -> int:
+    return L.load().alg_packed_attn_bwd_workspace_bytes(L.PackedAttnBwdArgs(sequences=sequences, tokens=tokens, H=H))
+
+
+@functools.lru_cache(maxsize=256)
+def _paged_bytes(device: int, sequences: int, tokens: int, H: int, Hkv: int, D: int, page_size: int, width: int, chunks: bool) -> int:
+    return L.load().alg_paged_attn_workspace_bytes(L.PagedAttnArgs(sequences=sequences, tokens=tokens, H=H, Hkv=Hkv, D=D, page_size=page_size,
+                                                                   table_width=width, cu_seqlens=1 if chunks else None))
 
 
 def _check_lengths(name: str, t: torch.Tensor, count: Optional[int]):
-    if t.dtype != torch.int32 or t.ndim != 1 or not t.is_contiguous() or (t.numel() < 1 if count is None else t.numel() != count):
+    shape = t.shape
+    if t.dtype != torch.int32 or len(shape) != 1 or not t.is_contiguous() or (shape[0] < 1 if count is None else shape[0] != count):
         raise ValueError(f"{name} must be a contiguous int32 vector" + ("" if count is None else f" of {count}"))
 
 
 def _check_link(n: int, c: float):
-    if n < 2 or n & (n - 1):
-        raise ValueError("asinh kernel needs n to be a power of two")
+    if n < 2 or n & (n - 1) or n > 32:
+        raise ValueError("asinh kernel needs n to be a power of two in [2, 32]")
     if not math.isfinite(c) or c <= 0:
         raise ValueError("asinh scale c must be positive and finite")
 
 
 def _check_packed(q, k, v):
-    if q.ndim != 3 or k.ndim != 3 or k.shape != v.shape or k.shape[0] != q.shape[0] or k.shape[2] != q.shape[2]:
+    qs, ks = q.shape, k.shape
+    if len(qs) != 3 or len(ks) != 3 or ks != v.shape or ks[0] != qs[0] or ks[2] != qs[2]:
         raise ValueError("q must be (tokens, H, D) and k, v (tokens, Hkv, D)")
-    if any(t.dtype != torch.bfloat16 for t in (q, k, v)):
+    if q.dtype != torch.bfloat16 or k.dtype != torch.bfloat16 or v.dtype != torch.bfloat16:
         raise ValueError("attention over packed sequences takes bfloat16 tensors")
-    if k.shape[1] < 1 or q.shape[1] < 1 or q.shape[1] % k.shape[1]:
+    if ks[1] < 1 or qs[1] < 1 or qs[1] % ks[1]:
         raise ValueError("query heads must be a multiple of the key heads")
 
 
@@ -649,23 +678,19 @@ def packed_attention(q, k, v, cu_seqlens, sink_logit=None, *, n: int = 16, c: fl
     _check_link(n, c)
     _check_lengths("cu_seqlens", cu_seqlens, None)
     T, H, D = q.shape
-    sink = None
-    if sink_logit is not None:
-        sink = _sink_vector(sink_logit, H, q.device)
-        if sink.numel() != H:
-            raise ValueError("sink_logit must broadcast to (H,)")
+    S, Hkv = cu_seqlens.shape[0] - 1, k.shape[1]
+    sink, sink_ptr = _sink_of(sink_logit, H, q.device)
     o = _output_like(q, out)
-    stat = torch.empty((H, T), dtype=torch.float32, device=q.device) if return_stat else None
-    rest = torch.empty((T, H, D), dtype=q.dtype, device=q.device) if return_stat else None
-    a = L.PackedAttnArgs(q=q.data_ptr(), k=k.data_ptr(), v=v.data_ptr(), o=o.data_ptr(), cu_seqlens=cu_seqlens.data_ptr(),
-                         sink=_ptr(sink), stat=_ptr(stat), o_rest=_ptr(rest), sequences=cu_seqlens.numel() - 1, tokens=T, H=H,
-                         Hkv=k.shape[1], D=D, n=int(n), c=float(c), zero_tail=int(out is None), q_stride=_strides2(q),
-                         k_stride=_strides2(k), v_stride=_strides2(v), o_stride=_strides2(o))
+    stat = rest = None
+    if return_stat:
+        stat = torch.empty((H, T), dtype=torch.float32, device=q.device)
+        rest = torch.empty((T, H, D), dtype=q.dtype, device=q.device)
     if T:
-        lib = L.load()
-        ws = _workspace(q.device, lib.alg_packed_attn_workspace_bytes(a), "packed")
-        a.workspace, a.workspace_bytes = ws.data_ptr(), ws.numel()
-        L.check(lib.alg_packed_attn_fwd(a, _stream()))
+        ws = _workspace(q.device, _packed_bytes(q.device.index, S, T, H, Hkv, D), "packed")
+        a = L.PACKED_ATTN.pack(q.data_ptr(), k.data_ptr(), v.data_ptr(), o.data_ptr(), cu_seqlens.data_ptr(), sink_ptr,
+                               stat.data_ptr() if return_stat else 0, rest.data_ptr() if return_stat else 0, S, T, H, Hkv, D, int(n), c,
+                               out is None, *_rows(q), *_rows(k), *_rows(v), *_rows(o), ws.data_ptr(), ws.shape[0], 0)
+        L.check(L.load().alg_packed_attn_fwd(L.PackedAttnArgs.from_buffer_copy(a), _stream()))
     return (o, stat, rest) if return_stat else o
 
 
@@ -687,34 +712,28 @@ def packed_attention_backward(q, k, v, o, d_o, stat, rest, cu_seqlens, sink_logi
     gt, gh, gd = d_o.stride()
     if gd != 1 or (T > 1 and (gt <= 0 or gt % 8)) or (H > 1 and (gh <= 0 or gh % 8)) or d_o.data_ptr() % 16:
         d_o = torch.empty(d_o.shape, dtype=d_o.dtype, device=d_o.device).copy_(d_o)
-    sink = None
-    if sink_logit is not None:
-        sink = _sink_vector(sink_logit, H, q.device)
-        if sink.numel() != H:
-            raise ValueError("sink_logit must broadcast to (H,)")
+    sink, sink_ptr = _sink_of(sink_logit, H, q.device)
+    S, Hkv = cu_seqlens.shape[0] - 1, k.shape[1]
     dq, dk, dv = (torch.empty(t.shape, dtype=t.dtype, device=t.device) for t in (q, k, v))
     dsink = torch.empty(H, dtype=torch.float32, device=q.device) if sink is not None else None
     if T == 0:
         return dq, dk, dv, (dsink.zero_() if dsink is not None else None)
-    a = L.PackedAttnBwdArgs(q=q.data_ptr(), k=k.data_ptr(), v=v.data_ptr(), o=o.data_ptr(), o_rest=rest.data_ptr(), d_o=d_o.data_ptr(),
-                            stat=stat.data_ptr(), cu_seqlens=cu_seqlens.data_ptr(), sink=_ptr(sink), dq=dq.data_ptr(), dk=dk.data_ptr(),
-                            dv=dv.data_ptr(), dsink=_ptr(dsink), sequences=cu_seqlens.numel() - 1, tokens=T, H=H, Hkv=k.shape[1], D=D,
-                            n=int(n), c=float(c), q_stride=_strides2(q), k_stride=_strides2(k), v_stride=_strides2(v),
-                            o_stride=_strides2(o), do_stride=_strides2(d_o), dq_stride=_strides2(dq), dk_stride=_strides2(dk),
-                            dv_stride=_strides2(dv))
-    lib = L.load()
-    ws = _workspace(q.device, lib.alg_packed_attn_bwd_workspace_bytes(a), "packed_bwd")
-    a.workspace, a.workspace_bytes = ws.data_ptr(), ws.numel()
-    L.check(lib.alg_packed_attn_bwd(a, _stream()))
+    ws = _workspace(q.device, _packed_bwd_bytes(S, T, H), "packed_bwd")
+    a = L.PACKED_ATTN_BWD.pack(q.data_ptr(), k.data_ptr(), v.data_ptr(), o.data_ptr(), rest.data_ptr(), d_o.data_ptr(), stat.data_ptr(),
+                               cu_seqlens.data_ptr(), sink_ptr, dq.data_ptr(), dk.data_ptr(), dv.data_ptr(),
+                               0 if dsink is None else dsink.data_ptr(), S, T, H, Hkv, D, int(n), c, *_rows(q), *_rows(k), *_rows(v), *_rows(o),
+                               *_rows(d_o), H * D, D, Hkv * D, D, Hkv * D, D, ws.data_ptr(), ws.shape[0], 0)
+    L.check(L.load().alg_packed_attn_bwd(L.PackedAttnBwdArgs.from_buffer_copy(a), _stream()))
     return dq, dk, dv, dsink
 
 
 def _check_pages(q, k_pages, v_pages, block_table, kv_lens, cu_seqlens):
-    if q.ndim != 3 or k_pages.ndim != 4 or k_pages.shape != v_pages.shape or k_pages.shape[3] != q.shape[2]:
+    qs, ks = q.shape, k_pages.shape
+    if len(qs) != 3 or len(ks) != 4 or ks != v_pages.shape or ks[3] != qs[2]:
         raise ValueError("q must be (tokens, H, D) and k_pages, v_pages (pages, page_size, Hkv, D)")
-    if any(t.dtype != torch.bfloat16 for t in (q, k_pages, v_pages)):
+    if q.dtype != torch.bfloat16 or k_pages.dtype != torch.bfloat16 or v_pages.dtype != torch.bfloat16:
         raise ValueError("attention over a paged cache takes bfloat16 tensors")
-    if k_pages.shape[2] < 1 or q.shape[1] < 1 or q.shape[1] % k_pages.shape[2]:
+    if ks[2] < 1 or qs[1] < 1 or qs[1] % ks[2]:
         raise ValueError("query heads must be a multiple of the key heads")
     if block_table.dtype != torch.int32 or block_table.ndim != 2 or block_table.stride(1) != 1:
         raise ValueError("block_table must be int32 (sequences, pages of a sequence) with contiguous rows")
@@ -722,7 +741,7 @@ def _check_pages(q, k_pages, v_pages, block_table, kv_lens, cu_seqlens):
     _check_lengths("kv_lens", kv_lens, S)
     if cu_seqlens is not None:
         _check_lengths("cu_seqlens", cu_seqlens, S + 1)
-    elif q.shape[0] != S:
+    elif qs[0] != S:
         raise ValueError("without cu_seqlens every sequence has one new token")
     return S
 
@@ -744,23 +763,17 @@ def paged_attention(q, k_pages, v_pages, block_table, kv_lens, cu_seqlens=None, 
     S = _check_pages(q, k_pages, v_pages, block_table, kv_lens, cu_seqlens)
     _check_link(n, c)
     T, H, D = q.shape
-    sink = None
-    if sink_logit is not None:
-        sink = _sink_vector(sink_logit, H, q.device)
-        if sink.numel() != H:
-            raise ValueError("sink_logit must broadcast to (H,)")
+    (pages, page_size, Hkv, _), width = k_pages.shape, block_table.shape[1]
+    sink, sink_ptr = _sink_of(sink_logit, H, q.device)
     o = _output_like(q, out)
-    a = L.PagedAttnArgs(q=q.data_ptr(), k_pages=k_pages.data_ptr(), v_pages=v_pages.data_ptr(), o=o.data_ptr(),
-                        block_table=block_table.data_ptr(), kv_lens=kv_lens.data_ptr(), cu_seqlens=_ptr(cu_seqlens), sink=_ptr(sink),
-                        sequences=S, tokens=T, H=H, Hkv=k_pages.shape[2], D=D, pages=k_pages.shape[0], page_size=k_pages.shape[1],
-                        table_width=block_table.shape[1], n=int(n), c=float(c), zero_tail=int(out is None),
-                        table_stride=block_table.stride(0), q_stride=_strides2(q), k_stride=_strides3(k_pages),
-                        v_stride=_strides3(v_pages), o_stride=_strides2(o))
     if T:
-        lib = L.load()
-        ws = _workspace(q.device, lib.alg_paged_attn_workspace_bytes(a), "paged")
-        a.workspace, a.workspace_bytes = ws.data_ptr(), ws.numel()
-        L.check(lib.alg_paged_attn_fwd(a, _stream()))
+        chunks = cu_seqlens is not None
+        ws = _workspace(q.device, _paged_bytes(q.device.index, S, T, H, Hkv, D, page_size, width, chunks), "paged")
+        a = L.PAGED_ATTN.pack(q.data_ptr(), k_pages.data_ptr(), v_pages.data_ptr(), o.data_ptr(), block_table.data_ptr(), kv_lens.data_ptr(),
+                              cu_seqlens.data_ptr() if chunks else 0, sink_ptr, S, T, H, Hkv, D, pages, page_size, width, int(n), c,
+                              out is None, block_table.stride(0), *_rows(q), *_rows(k_pages), *_rows(v_pages), *_rows(o), ws.data_ptr(),
+                              ws.shape[0], 0)
+        L.check(L.load().alg_paged_attn_fwd(L.PagedAttnArgs.from_buffer_copy(a), _stream()))
     return o
 
 
@@ -778,9 +791,7 @@ def paged_append(q, k, v, k_pages, v_pages, block_table, kv_lens, cos, sin, cu_s
     left as it is.  A page number outside the pool drops the token's key and value.  Pages that are written belong to one
     sequence: two tokens with one place leave either's key there."""
     _require_cuda(q, k, v, k_pages, v_pages, block_table, kv_lens, cos, sin, cu_seqlens, q_gain, k_gain)
-    if q.ndim != 3 or k.ndim != 3 or k.shape != v.shape or k.shape[0] != q.shape[0] or k.shape[2] != q.shape[2] or \
-            any(t.dtype != torch.bfloat16 for t in (k, v)):
-        raise ValueError("q must be (tokens, H, D) and k, v (tokens, Hkv, D), all bfloat16")
+    _check_packed(q, k, v)
     S = _check_pages(q, k_pages, v_pages, block_table, kv_lens, cu_seqlens)
     T, H, D = q.shape
     if k.shape[1] != k_pages.shape[2]:
@@ -794,15 +805,15 @@ def paged_append(q, k, v, k_pages, v_pages, block_table, kv_lens, cos, sin, cu_s
     if eps <= 0:
         raise ValueError("QK RMS epsilon must be positive")
     o = _output_like(q, out)
-    a = L.PagedAppendArgs(q=q.data_ptr(), k=k.data_ptr(), v=v.data_ptr(), q_out=o.data_ptr(), k_pages=k_pages.data_ptr(),
-                          v_pages=v_pages.data_ptr(), block_table=block_table.data_ptr(), kv_lens=kv_lens.data_ptr(),
-                          cu_seqlens=_ptr(cu_seqlens), q_gain=_ptr(q_gain), k_gain=_ptr(k_gain), cos=cos.data_ptr(), sin=sin.data_ptr(),
-                          sequences=S, tokens=T, H=H, Hkv=k.shape[1], D=D, pages=k_pages.shape[0], page_size=k_pages.shape[1],
-                          table_width=block_table.shape[1], table_rows=cos.shape[0], table_dtype=_DTYPES[cos.dtype], eps=float(eps),
-                          zero_tail=int(out is None), table_stride=block_table.stride(0), q_stride=_strides2(q), k_stride=_strides2(k),
-                          v_stride=_strides2(v), o_stride=_strides2(o), kp_stride=_strides3(k_pages), vp_stride=_strides3(v_pages))
     if T:
-        L.check(L.load().alg_paged_append(a, _stream()))
+        (pages, page_size, Hkv, _), (rows, _) = k_pages.shape, cos.shape
+        a = L.PAGED_APPEND.pack(q.data_ptr(), k.data_ptr(), v.data_ptr(), o.data_ptr(), k_pages.data_ptr(), v_pages.data_ptr(),
+                                block_table.data_ptr(), kv_lens.data_ptr(), 0 if cu_seqlens is None else cu_seqlens.data_ptr(),
+                                0 if q_gain is None else q_gain.data_ptr(), 0 if k_gain is None else k_gain.data_ptr(), cos.data_ptr(),
+                                sin.data_ptr(), S, T, H, Hkv, D, pages, page_size, block_table.shape[1], rows, _DTYPES[cos.dtype], eps,
+                                out is None, block_table.stride(0), *_rows(q), *_rows(k), *_rows(v), *_rows(o), *_rows(k_pages),
+                                *_rows(v_pages))
+        L.check(L.load().alg_paged_append(L.PagedAppendArgs.from_buffer_copy(a), _stream()))
     return o
 
 
