@@ -48,7 +48,6 @@ template <int D> struct Cfg {
   static constexpr int NKV = (D == 128) ? 5 : 10;           // K/V ring depth (tiles)
   static constexpr int KV_OFF = 2 * TILE_BYTES;             // behind the two Q tiles
   static constexpr int CTL_OFF = KV_OFF + NKV * TILE_BYTES;
-  static constexpr uint32_t S_COL = 0, O_COL = 256;         // S_w at 128 w (P_w inside it), O_w at O_COL + D w
   static constexpr uint32_t IDESC_S = make_idesc_bf16(BQ, BKEY, 0, 0);
   static constexpr uint32_t IDESC_PV = make_idesc_bf16(BQ, D, 0, 1);   // V is [key][d]: MN-major B
 };
@@ -66,6 +65,7 @@ struct Work {
 struct __align__(16) Control {
   uint64_t q_full[2], q_ready[2], q_free[2], kv_full[MAX_NKV], kv_empty[MAX_NKV];
   uint64_t s_full[2], p_half[2], p_full[2], o_full[2], o_free[2];
+  uint64_t s_read[2], pv_done[2];   // EARLY: scores are in registers; the second product of a tile is done
   uint64_t v_here, v_clean, work_full[RING], work_empty[RING];
   Work work[RING];
   uint32_t tmem_base;
@@ -158,59 +158,89 @@ __device__ __forceinline__ void signal_weights(uint64_t* bar) {
   mbar_arrive(bar);
 }
 
-// A tile of this thread's row, 32 columns at a time, the next load in flight while a block is weighed; `block(regs, b)` leaves
-// the packed weights of block b.
-template <bool HILO, class Block>
-__device__ __forceinline__ void weigh_tile(uint32_t s_taddr, uint64_t* p_half, uint64_t* p_full, Block&& block) {
-  uint32_t a[32], b[32], packed[HILO ? 32 : 16];
-  tmem_ld_32x32(s_taddr, a);
-  tmem_ld_wait_for(a);
-  tmem_ld_32x32(s_taddr + 32, b);
-  block(a, 0, packed);
-  store_packed<HILO>(s_taddr, packed);
-  tmem_ld_wait_for(b);
-  tmem_ld_32x32(s_taddr + 64, a);
-  block(b, 32, packed);
-  store_packed<HILO>(s_taddr + 32, packed);
-  signal_weights(p_half);
-  tmem_ld_wait_for(a);
-  tmem_ld_32x32(s_taddr + 96, b);
-  block(a, 64, packed);
-  store_packed<HILO>(s_taddr + 64, packed);
-  tmem_ld_wait_for(b);
-  block(b, 96, packed);
-  store_packed<HILO>(s_taddr + 96, packed);
-  signal_weights(p_full);
-}
-
-// Largest |y| of the row's visible scores, NaN if one is NaN.  Only what the row sees counts: which form its weights take, and
-// with it their rounding, must not depend on a neighbouring sequence.
-template <bool MASK>
-__device__ __forceinline__ float tile_abs_max(uint32_t s_taddr, int lim) {
+// Sum of y^2 over the row's 128 scores, whatever the mask: where it is within the square of the range, so is every score.
+__device__ __forceinline__ float tile_square_sum(uint32_t s_taddr) {
   uint32_t a[32], b[32];
-  float m[4] = {0.f, 0.f, 0.f, 0.f};
-  auto scan = [&](const uint32_t* s, int c) {
+  float2 m0 = make_float2(0.f, 0.f), m1 = make_float2(0.f, 0.f);
+  auto add = [&](const uint32_t* s) {
 #pragma unroll
-    for (int i = 0; i < 32; i += 2) {
-      const float y0 = !MASK || c + i <= lim ? __uint_as_float(s[i]) : 0.f, y1 = !MASK || c + i + 1 <= lim ? __uint_as_float(s[i + 1]) : 0.f;
-      m[(i >> 1) & 3] = max3_abs_nan(m[(i >> 1) & 3], y0, y1);
+    for (int i = 0; i < 32; i += 4) {
+      const float2 y0 = make_float2(__uint_as_float(s[i]), __uint_as_float(s[i + 1])), y1 = make_float2(__uint_as_float(s[i + 2]), __uint_as_float(s[i + 3]));
+      m0 = __ffma2_rn(y0, y0, m0);
+      m1 = __ffma2_rn(y1, y1, m1);
     }
   };
   tmem_ld_32x32(s_taddr, a);
   tmem_ld_32x32(s_taddr + 32, b);
   tmem_ld_wait_for(a);
-  scan(a, 0);
   tmem_ld_wait_for(b);                                  // complete already: orders the reads of b
+  add(a);
   tmem_ld_32x32(s_taddr + 64, a);
-  scan(b, 32);
+  add(b);
   tmem_ld_32x32(s_taddr + 96, b);
   tmem_ld_wait_for(a);
-  scan(a, 64);
+  add(a);
   tmem_ld_wait_for(b);
-  scan(b, 96);
-  return max3_abs_nan(max3_abs_nan(m[0], m[1], m[2]), m[3], 0.f);
+  add(b);
+  return (m0.x + m0.y) + (m1.x + m1.y);
 }
-// largest visible x of the row (NaN ignored: its weight will be NaN whatever the reference); -inf if there is none
+// Largest |y| of the row's visible scores, NaN if one is NaN.  Only what the row sees counts: which form its weights take, and
+// with it their rounding, must not depend on a neighbouring sequence.
+__device__ __forceinline__ float tile_abs_max(uint32_t s_taddr, int lim) {
+  float most = 0.f;
+#pragma unroll 1
+  for (int c = 0; c < 128; c += 32) {
+    uint32_t a[32];
+    tmem_ld_32x32(s_taddr + c, a);
+    tmem_ld_wait_for(a);
+#pragma unroll
+    for (int i = 0; i < 32; i += 2)
+      most = max3_abs_nan(most, c + i <= lim ? __uint_as_float(a[i]) : 0.f, c + i + 1 <= lim ? __uint_as_float(a[i + 1]) : 0.f);
+  }
+  return most;
+}
+
+// The unshifted weights of a tile to tensor memory, 32 keys every STEP columns, the next 32 scores in flight while a block is weighed.
+// A loop of two times two blocks: the unrolled tile is more code than the SM's instruction caches hold for two warps that are not
+// at the same place.  `loaded()` is called when the last scores are in registers, `second()` ahead of the second half's first store.
+template <int LOG2N, bool HILO, int STEP, class Loaded, class Second>
+__device__ __forceinline__ bool weigh_tile(uint32_t s_taddr, uint32_t p_taddr, uint64_t* p_half, uint64_t* p_full, float kappa, int log2n, int lim,
+                                           bool masked, float2& la, float2& lb, const Loaded& loaded, const Second& second) {
+  uint32_t a[32], b[32], packed[HILO ? 32 : 16];
+  const int warp_lim = masked ? __reduce_max_sync(0xffffffffu, lim) : 128;
+  auto block = [&](const uint32_t* s, int c) {
+    if (!masked) {
+      weigh<LOG2N, false, HILO>(s, kappa, log2n, 0, la, lb, packed);
+    } else if (c <= warp_lim) {
+      weigh<LOG2N, true, HILO>(s, kappa, log2n, lim - c, la, lb, packed);
+    } else {                                            // the block lies beyond what any row of the warp sees
+#pragma unroll
+      for (int i = 0; i < (HILO ? 32 : 16); ++i) packed[i] = 0u;
+    }
+  };
+  tmem_ld_32x32(s_taddr, a);
+#pragma unroll 1
+  for (int half = 0; half < 2; ++half) {
+    tmem_ld_wait_for(a);
+    tmem_ld_32x32(s_taddr + 32, b);
+    block(a, 64 * half);
+    if (half == 1 && !second()) return false;
+    store_packed<HILO>(p_taddr, packed);
+    tmem_ld_wait_for(b);
+    if (half == 0) tmem_ld_32x32(s_taddr + 64, a);
+    else loaded();
+    block(b, 64 * half + 32);
+    store_packed<HILO>(p_taddr + STEP, packed);
+    signal_weights(half == 0 ? p_half : p_full);
+    s_taddr += 64;
+    p_taddr += 2 * STEP;
+  }
+  return true;
+}
+
+// The max-shifted form reads the scores again from tensor memory, block by block: it runs where the short form may not, and
+// its code stays small.
+// Largest visible x of the row (NaN ignored: its weight will be NaN whatever the reference); -inf if there is none.
 __device__ __forceinline__ float tile_row_max(uint32_t s_taddr, float m, int lim) {
   float top = -INFINITY;
 #pragma unroll 1
@@ -222,6 +252,20 @@ __device__ __forceinline__ float tile_row_max(uint32_t s_taddr, float m, int lim
     for (int i = 0; i < 32; ++i) top = (c + i <= lim) ? fmaxf(top, __uint_as_float(a[i]) * m) : top;
   }
   return top;
+}
+template <bool HILO, int STEP>
+__device__ __forceinline__ void weigh_tile_shifted(uint32_t s_taddr, uint32_t p_taddr, uint64_t* p_half, uint64_t* p_full, float m, float sigma,
+                                                   int log2n, int lim, float2& la, float2& lb) {
+#pragma unroll 1
+  for (int b = 0; b < 4; ++b) {
+    uint32_t a[32], packed[HILO ? 32 : 16];
+    tmem_ld_32x32(s_taddr + 32 * b, a);
+    tmem_ld_wait_for(a);
+    weigh_shifted<HILO>(a, m, sigma, log2n, lim - 32 * b, la, lb, packed);
+    store_packed<HILO>(p_taddr + STEP * b, packed);
+    if (b == 1) signal_weights(p_half);
+  }
+  signal_weights(p_full);
 }
 
 template <int NKV> struct RingCursor {
@@ -235,6 +279,11 @@ __global__ void __launch_bounds__(NTHREADS, 1)
 ragged_attn_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant__ CUtensorMap tm_k,
                    const __grid_constant__ CUtensorMap tm_v, const __grid_constant__ RaggedParams p, const ScoreScale sc) {
   using C = Cfg<D>;
+  // Head_dim 64 leaves tensor memory for weights in columns of their own; then the next scores are issued as soon as these are in
+  // registers, and the weight warps find them when they come back.
+  constexpr bool EARLY = D == 64 && !HILO;
+  constexpr uint32_t O_COL = EARLY ? 384u : 256u, P_COL = EARLY ? 256u : 0u;      // O_t at O_COL + D t
+  constexpr uint32_t P_STRIDE = EARLY ? 64u : 128u, P_STEP = EARLY ? 16u : 32u;   // P_t at P_COL + P_STRIDE t, 32 keys every P_STEP columns
   extern __shared__ unsigned char smem_raw[];
   unsigned char* smem = reinterpret_cast<unsigned char*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
   Control* ctl = reinterpret_cast<Control*>(smem + C::CTL_OFF);
@@ -245,6 +294,7 @@ ragged_attn_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_consta
       mbar_init(&ctl->q_full[w], 1); mbar_init(&ctl->q_ready[w], 1); mbar_init(&ctl->q_free[w], 1);
       mbar_init(&ctl->s_full[w], 1); mbar_init(&ctl->p_half[w], 128); mbar_init(&ctl->p_full[w], 128);
       mbar_init(&ctl->o_full[w], 1); mbar_init(&ctl->o_free[w], 128);
+      mbar_init(&ctl->s_read[w], 128); mbar_init(&ctl->pv_done[w], 1);
     }
     for (int i = 0; i < C::NKV; ++i) { mbar_init(&ctl->kv_full[i], 1); mbar_init(&ctl->kv_empty[i], 1); }
     for (int i = 0; i < RING; ++i) { mbar_init(&ctl->work_full[i], 1); mbar_init(&ctl->work_empty[i], ITEM_READERS); }
@@ -357,7 +407,7 @@ ragged_attn_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_consta
 #pragma unroll
       for (int ks = 0; ks < D / 16; ++ks) {
         const uint32_t off = ((ks >> 2) * PANEL_BYTES + (ks & 3) * 32) >> 4;
-        umma_f16_ss_parts(tmem_base + C::S_COL + t * 128, qa + off, SW128_DESC_HI, ka + off, SW128_DESC_HI, C::IDESC_S, ks != 0 ? 1u : 0u);
+        umma_f16_ss_parts(tmem_base + t * 128, qa + off, SW128_DESC_HI, ka + off, SW128_DESC_HI, C::IDESC_S, ks != 0 ? 1u : 0u);
       }
     };
     auto issue_pv = [&](int t, int slot, int h64, bool first) {   // O_t += P_t V for the first or second 64 keys
@@ -365,9 +415,9 @@ ragged_attn_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_consta
 #pragma unroll
       for (int part = 0; part < (HILO ? 2 : 1); ++part)
 #pragma unroll
-        for (int i = 0; i < 4; ++i) {                   // 16 keys = 8 packed columns of P a step; 32 columns hold 32 keys' hi | lo
+        for (int i = 0; i < 4; ++i) {                   // 16 keys = 8 packed columns of P a step
           const int ks = 4 * h64 + i;
-          umma_f16_ts_parts(tmem_base + C::O_COL + t * D, tmem_base + C::S_COL + t * 128 + (ks >> 1) * 32 + (ks & 1) * 8 + part * 16,
+          umma_f16_ts_parts(tmem_base + O_COL + t * D, tmem_base + P_COL + t * P_STRIDE + (ks >> 1) * P_STEP + (ks & 1) * 8 + part * 16,
                             va + ks * (2048 >> 4), SW128_DESC_HI, C::IDESC_PV, (first && ks == 0 && part == 0) ? 0u : 1u);
         }
     };
@@ -378,8 +428,23 @@ ragged_attn_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_consta
       tc_fence_after();
       if (elect_one()) issue_pv(t, v_slot, 0, j == 0);
       __syncwarp();
+      if (EARLY && j + 1 < nt) {
+        if (!wait_all(&ctl->s_read[t], uint32_t(before + j) & 1u)) return false;
+        tc_fence_after();
+        if (elect_one()) { issue_s(t, k_slot); umma_commit(&ctl->s_full[t]); }
+        __syncwarp();
+      }
       if (!wait_all(&ctl->p_full[t], uint32_t(before + j) & 1u)) return false;
       tc_fence_after();
+      if (EARLY) {
+        if (elect_one()) {
+          issue_pv(t, v_slot, 1, false);
+          umma_commit(&ctl->pv_done[t]);
+          if (j + 1 == nt) umma_commit(&ctl->o_full[t]);
+        }
+        __syncwarp();
+        return true;
+      }
       if (elect_one()) {
         issue_pv(t, v_slot, 1, false);
         if (j + 1 < nt) { issue_s(t, k_slot); umma_commit(&ctl->s_full[t]); }    // behind P V: may overwrite P
@@ -486,12 +551,13 @@ ragged_attn_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_consta
     const int quarter = warp & 3;
     const int r = quarter * 32 + lane;                  // row of the tile
     const uint32_t lane_sel = uint32_t(quarter * 32) << 16;
-    const uint32_t s_taddr = tmem_base + lane_sel + C::S_COL + t * 128;
-    const uint32_t o_taddr = tmem_base + lane_sel + C::O_COL + t * D;
+    const uint32_t s_taddr = tmem_base + lane_sel + t * 128;
+    const uint32_t p_taddr = tmem_base + lane_sel + P_COL + t * P_STRIDE, o_taddr = tmem_base + lane_sel + O_COL + t * D;
     const int tok_r = r / p.G, g_r = r - tok_r * p.G;   // token and head of this row
     // the "scores there" barriers of tile 1, served second in every step, tell that V of the step before and K of this one are read
     const bool releaser = quarter == 0 && lane == 0;
     RingCursor<C::NKV> rel;
+    int kslot = 0, vslot = 1 % C::NKV;                  // EARLY: K and V slots are released apart, every other one from 0 and from 1
     int tiles = 0, items = 0;                           // of this group, in earlier items
     Work w;
     bool ok = true;
@@ -517,30 +583,43 @@ ragged_attn_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_consta
         tc_fence_after();
         if (releaser) {
           if (t == 1) {
-            if (j > 0) { mbar_arrive(&ctl->kv_empty[rel.slot]); rel.next(); }    // V_{j-1}
-            mbar_arrive(&ctl->kv_empty[rel.slot]); rel.next();                   // K_j
+            if (EARLY) {                                                         // K_j; V_{j-1} follows at pv_done
+              mbar_arrive(&ctl->kv_empty[kslot]); kslot = (kslot + 2) % C::NKV;
+            } else {
+              if (j > 0) { mbar_arrive(&ctl->kv_empty[rel.slot]); rel.next(); }  // V_{j-1}
+              mbar_arrive(&ctl->kv_empty[rel.slot]); rel.next();                 // K_j
+            }
           }
           if (j == nk - 1) mbar_arrive(&ctl->q_free[t]);
         }
         const int lim = limit - j * BKEY;
         const bool masked = limit0 - j * BKEY < BKEY - 1;                        // uniform over the group
         if (!shifted) {
-          const float top = masked ? tile_abs_max<true>(s_taddr, lim) : tile_abs_max<false>(s_taddr, lim);
-          shifted = __any_sync(0xffffffffu, live && !(top <= sc.y_fast));
+          const float sum = tile_square_sum(s_taddr);   // by all lanes: the loads are the whole warp's
+          if (!__all_sync(0xffffffffu, !live || sum <= sc.y_fast * sc.y_fast)) {
+            const float top = tile_abs_max(s_taddr, lim);
+            shifted = __any_sync(0xffffffffu, live && !(top <= sc.y_fast));
+          }
         }
+        // EARLY: the product with the tile before has read its weights, and V, which goes back to the ring; nothing to wait for where
+        // the weights lie in the scores' place
+        auto product_done = [&]() -> bool {
+          if (EARLY && tiles + j > 0) {
+            if (!__all_sync(0xffffffffu, bw.wait(&ctl->pv_done[t], uint32_t(tiles + j - 1) & 1u))) return false;
+            tc_fence_after();
+            if (releaser && t == 1 && j > 0) { mbar_arrive(&ctl->kv_empty[vslot]); vslot = (vslot + 2) % C::NKV; }
+          }
+          return true;
+        };
+        auto scores_loaded = [&] {                      // EARLY: the next scores may come
+          if (EARLY) {
+            tc_fence_before();
+            mbar_arrive(&ctl->s_read[t]);
+          }
+        };
         if (!shifted) {
-          const int warp_lim = masked ? __reduce_max_sync(0xffffffffu, lim) : 0;
-          if (masked) weigh_tile<HILO>(s_taddr, &ctl->p_half[t], &ctl->p_full[t], [&](const uint32_t* s, int c, uint32_t* packed) {
-            if (c <= warp_lim) {
-              weigh<LOG2N, true, HILO>(s, sc.kappa, p.log2n, lim - c, la, lb, packed);
-            } else {                                    // the block lies beyond what any row of the warp sees
-#pragma unroll
-              for (int i = 0; i < (HILO ? 32 : 16); ++i) packed[i] = 0u;
-            }
-          });
-          else weigh_tile<HILO>(s_taddr, &ctl->p_half[t], &ctl->p_full[t], [&](const uint32_t* s, int c, uint32_t* packed) {
-            weigh<LOG2N, false, HILO>(s, sc.kappa, p.log2n, 0, la, lb, packed);
-          });
+          ok = weigh_tile<LOG2N, HILO, P_STEP>(s_taddr, p_taddr, &ctl->p_half[t], &ctl->p_full[t], sc.kappa, p.log2n, lim, masked, la, lb,
+                                               scores_loaded, product_done);
         } else {
           l += (la.x + la.y) + (lb.x + lb.y);
           la = make_float2(0.f, 0.f); lb = make_float2(0.f, 0.f);
@@ -549,7 +628,9 @@ ragged_attn_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_consta
           float m_new = m_run;
           if (lim >= 0 && top > -INFINITY) m_new = l > 0.f ? fmaxf(m_run, top) : top;
           const float alpha = m_new != m_run ? pow2n_rt(rho_any(m_run) * rho_any(-m_new), p.log2n) : 1.0f;
-          // O of the earlier tiles is at rest (these scores were issued behind their product): rescale it where a reference moved
+          // O of the earlier tiles is at rest (these scores were issued behind their product, or it is waited for): rescale it where
+          // a reference moved
+          if (!product_done()) { ok = false; break; }
           if (__any_sync(0xffffffffu, j > 0 && alpha != 1.0f)) {
             const float a_row = j > 0 ? alpha : 1.0f;
 #pragma unroll 1
@@ -565,10 +646,8 @@ ragged_attn_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_consta
           }
           if (l > 0.f) l *= alpha;
           m_run = m_new;
-          const float sigma = rho_any(-m_run) * sc.inv_m;
-          weigh_tile<HILO>(s_taddr, &ctl->p_half[t], &ctl->p_full[t], [&](const uint32_t* s, int c, uint32_t* packed) {
-            weigh_shifted<HILO>(s, sc.m, sigma, p.log2n, lim - c, la, lb, packed);
-          });
+          weigh_tile_shifted<HILO, P_STEP>(s_taddr, p_taddr, &ctl->p_half[t], &ctl->p_full[t], sc.m, rho_any(-m_run) * sc.inv_m, p.log2n, lim, la, lb);
+          scores_loaded();
         }
       }
       if (!ok) break;
@@ -583,7 +662,10 @@ ragged_attn_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_consta
       if (nk > 0) {
         if (!__all_sync(0xffffffffu, bw.wait(&ctl->o_full[t], uint32_t(items) & 1u))) { ok = false; break; }
         ++items;
-        if (releaser && t == 1) { mbar_arrive(&ctl->kv_empty[rel.slot]); rel.next(); }     // the item's last V tile
+        if (releaser && t == 1) {                       // the item's last V tile
+          if (EARLY) { mbar_arrive(&ctl->kv_empty[vslot]); vslot = (vslot + 2) % C::NKV; }
+          else { mbar_arrive(&ctl->kv_empty[rel.slot]); rel.next(); }
+        }
         tc_fence_after();
         const float inv = l != 0.f ? 1.0f / l : 0.f;    // a row that sees nothing: zero
         const int64_t row = int64_t(w.row0) + tok;
