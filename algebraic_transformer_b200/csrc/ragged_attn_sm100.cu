@@ -727,66 +727,81 @@ ragged_attn_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_consta
   }
 }
 
-// Adds up the parts of the items that were cut along the keys.  A CTA takes 32 of the 256 rows of an (item, head), a warp four of
-// them, a lane D / 32 columns; parts meet in their order, at the largest of their references.
+// Adds up the parts of the items that were cut along the keys: a warp a row, a lane D / 32 columns, references and normalisers one a
+// lane, the accumulators of sixteen parts in flight at once.  Parts meet in their order, at the largest of their references.
 template <int D>
-__global__ void __launch_bounds__(256) ragged_combine_kernel(const RaggedParams p, const ScoreScale sc) {
+__global__ void __launch_bounds__(256) ragged_combine_kernel(const __grid_constant__ RaggedParams p, const ScoreScale sc) {
   griddep_wait();
-  constexpr int CPL = D / 32;
+  constexpr int CPL = D / 32, BATCH = 16;
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-  const int units = p.plan.header->combos * p.Hkv * 8;
+  const int units = p.plan.header->combos * p.Hkv * 32;              // eight rows each
   for (int u = blockIdx.x; u < units; u += gridDim.x) {
-    const RaggedCombo it = p.plan.combos[u / (p.Hkv * 8)];
-    const int h = (u >> 3) % p.Hkv;
+    const RaggedCombo it = p.plan.combos[u / (p.Hkv * 32)];
+    const int h = (u >> 5) % p.Hkv, in_item = (u & 31) * 8 + warp, t = in_item >> 7, r = in_item & 127;
     const bool two = it.Lq - it.t0 > p.tile_tokens;
-    for (int rr = 0; rr < 4; ++rr) {
-      const int in_item = (u & 7) * 32 + warp * 4 + rr, t = in_item >> 7, r = in_item & 127;
-      if (t == 0 && !two) continue;
-      const int tok_r = r / p.G, g = r - tok_r * p.G, tok = it.t0 + (t == 1 && two ? p.tile_tokens : 0) + tok_r;
-      if (tok_r >= p.tile_tokens || tok >= it.Lq) continue;
-      const float* row = p.plan.slots + ((int64_t(it.slot) * p.Hkv + h) * 256 + in_item) * (D + 4);
-      const int64_t step = int64_t(p.Hkv) * 256 * (D + 4);          // to the next part
-      float2 lm = lane < it.parts ? __ldcg(reinterpret_cast<const float2*>(row + lane * step + D)) : make_float2(0.f, 0.f);
-      float2 lm2 = lane + 32 < it.parts ? __ldcg(reinterpret_cast<const float2*>(row + (lane + 32) * step + D)) : make_float2(0.f, 0.f);
-      // a part that weighed nothing has no say in the reference
-      const bool nan = __any_sync(0xffffffffu, lm.x != lm.x || lm2.x != lm2.x);
-      float top = fmaxf(lm.x > 0.f ? lm.y : -INFINITY, lm2.x > 0.f ? lm2.y : -INFINITY);
-      top = warp_max(top);
-      const float ns = rho_any(-top);
-      const float f1 = lm.x > 0.f ? (lm.y == top ? 1.0f : pow2n_rt(rho_any(lm.y) * ns, p.log2n)) : 0.f;
-      const float f2 = lm2.x > 0.f ? (lm2.y == top ? 1.0f : pow2n_rt(rho_any(lm2.y) * ns, p.log2n)) : 0.f;
-      const float l = warp_sum(f1 * lm.x + f2 * lm2.x);
-      float acc[CPL];
+    const int tok_r = r / p.G, g = r - tok_r * p.G, tok = it.t0 + (t == 1 && two ? p.tile_tokens : 0) + tok_r;
+    if ((t == 0 && !two) || tok_r >= p.tile_tokens || tok >= it.Lq) continue;
+    const float* row = p.plan.slots + ((int64_t(it.slot) * p.Hkv + h) * 256 + in_item) * (D + 4);
+    const int64_t step = int64_t(p.Hkv) * 256 * (D + 4);            // to the next part
+    float m = -INFINITY, l = 0.f, a[CPL];
 #pragma unroll
-      for (int c = 0; c < CPL; ++c) acc[c] = 0.f;
-      for (int pt = 0; pt < it.parts; ++pt) {
-        const float f = __shfl_sync(0xffffffffu, pt < 32 ? f1 : f2, pt & 31);
-        if (f == 0.f) continue;                         // warp-uniform; its accumulator may never have been written
-        const float* src = row + pt * step + lane * CPL;
-        if (CPL == 4) {
-          const float4 v = __ldcg(reinterpret_cast<const float4*>(src));
-          acc[0] = fmaf(f, v.x, acc[0]); acc[1] = fmaf(f, v.y, acc[1]); acc[CPL - 2] = fmaf(f, v.z, acc[CPL - 2]); acc[CPL - 1] = fmaf(f, v.w, acc[CPL - 1]);
-        } else {
-          const float2 v = __ldcg(reinterpret_cast<const float2*>(src));
-          acc[0] = fmaf(f, v.x, acc[0]); acc[1] = fmaf(f, v.y, acc[1]);
+    for (int c = 0; c < CPL; ++c) a[c] = 0.f;
+    bool nan = false;
+    for (int p0 = 0; p0 < it.parts; p0 += 32) {
+      const int n = min(32, it.parts - p0);
+      const float2 lm = lane < n ? __ldcg(reinterpret_cast<const float2*>(row + (p0 + lane) * step + D)) : make_float2(0.f, 0.f);
+      float f = 0.f;
+      for (int b0 = 0; b0 < n; b0 += BATCH) {
+        float v[BATCH][CPL];
+#pragma unroll
+        for (int j = 0; j < BATCH; ++j) {
+          const float* src = row + (p0 + min(b0 + j, n - 1)) * step + lane * CPL;
+          if (CPL == 4) {
+            const float4 x = __ldcg(reinterpret_cast<const float4*>(src));
+            v[j][0] = x.x; v[j][1] = x.y; v[j][CPL - 2] = x.z; v[j][CPL - 1] = x.w;
+          } else {
+            const float2 x = __ldcg(reinterpret_cast<const float2*>(src));
+            v[j][0] = x.x; v[j][1] = x.y;
+          }
+        }
+        if (b0 == 0) {                                 // a part that weighed nothing has no say in the reference
+          nan |= __any_sync(0xffffffffu, lm.x != lm.x) != 0;
+          const float top = fmaxf(m, warp_max(lm.x > 0.f ? lm.y : -INFINITY));
+          if (top > m) {
+            const float old = m > -INFINITY ? pow2n_rt(rho_any(m) * rho_any(-top), p.log2n) : 0.f;
+            l *= old;
+#pragma unroll
+            for (int c = 0; c < CPL; ++c) a[c] *= old;
+            m = top;
+          }
+          f = lm.x > 0.f ? (lm.y == m ? 1.0f : pow2n_rt(rho_any(lm.y) * rho_any(-m), p.log2n)) : 0.f;
+          l += warp_sum(f * lm.x);
+        }
+#pragma unroll
+        for (int j = 0; j < BATCH; ++j) {
+          const float fj = __shfl_sync(0xffffffffu, f, (b0 + j) & 31);
+          if (b0 + j < n && fj != 0.f) {               // else the accumulator may never have been written
+#pragma unroll
+            for (int c = 0; c < CPL; ++c) a[c] = fmaf(fj, v[j][c], a[c]);
+          }
         }
       }
-      const float inv = nan ? __int_as_float(0x7fc00000) : l > 0.f ? 1.0f / l : 0.f;
-      const int64_t at = int64_t(it.row0) + tok;
-      const int head = h * p.G + g;
-      __nv_bfloat16* orow = static_cast<__nv_bfloat16*>(p.o) + at * p.os.t + head * p.os.h + lane * CPL;
-      __nv_bfloat16* lrow = p.o_lo != nullptr ? static_cast<__nv_bfloat16*>(p.o_lo) + (at * p.H + head) * D + lane * CPL : nullptr;
+    }
+    const float inv = nan ? __int_as_float(0x7fc00000) : l > 0.f ? 1.0f / l : 0.f;
+    const int64_t at = int64_t(it.row0) + tok;
+    const int head = h * p.G + g;
+    __nv_bfloat16* orow = static_cast<__nv_bfloat16*>(p.o) + at * p.os.t + head * p.os.h + lane * CPL;
+    __nv_bfloat16* lrow = p.o_lo != nullptr ? static_cast<__nv_bfloat16*>(p.o_lo) + (at * p.H + head) * D + lane * CPL : nullptr;
 #pragma unroll
-      for (int c = 0; c < CPL; c += 2) {
-        const float x = acc[c] * inv, y = acc[c + 1] * inv;
-        const uint32_t hi = pack_bf16(x, y);
-        *reinterpret_cast<uint32_t*>(orow + c) = hi;
-        if (lrow != nullptr) *reinterpret_cast<uint32_t*>(lrow + c) = pack_bf16(x - __uint_as_float(hi << 16), y - __uint_as_float(hi & 0xffff0000u));
-      }
-      if (p.stat != nullptr && lane == 0) {
-        const float a = l > 0.f ? ns * sc.inv_m * inv_root_rt(l, p.log2n) : 0.f;
-        p.stat[int64_t(head) * p.seqs.tokens + at] = nan ? __int_as_float(0x7fc00000) : a;
-      }
+    for (int c = 0; c < CPL; c += 2) {
+      const float x = a[c] * inv, y = a[c + 1] * inv;
+      const uint32_t hi = pack_bf16(x, y);
+      *reinterpret_cast<uint32_t*>(orow + c) = hi;
+      if (lrow != nullptr) *reinterpret_cast<uint32_t*>(lrow + c) = pack_bf16(x - __uint_as_float(hi << 16), y - __uint_as_float(hi & 0xffff0000u));
+    }
+    if (p.stat != nullptr && lane == 0) {
+      const float stat = l > 0.f ? rho_any(-m) * sc.inv_m * inv_root_rt(l, p.log2n) : 0.f;
+      p.stat[int64_t(head) * p.seqs.tokens + at] = nan ? __int_as_float(0x7fc00000) : stat;
     }
   }
 }
@@ -852,7 +867,7 @@ int launch_d(const RaggedParams& p, cudaStream_t stream) {
   }
   if (rc) return rc;
   if (p.plan.max_slots > 0) {
-    const int blocks = int(std::min<int64_t>(int64_t(p.plan.max_combos) * p.Hkv * 8, int64_t(p.plan.sms) * 4));
+    const int blocks = int(std::min<int64_t>(int64_t(p.plan.max_combos) * p.Hkv * 32, int64_t(p.plan.sms) * 8));
     ALG_CUDA_TRY(launch_dependent(ragged_combine_kernel<D>, dim3(std::max(blocks, 1)), dim3(256), 0, stream, p, sc));
     count_launch();
   }

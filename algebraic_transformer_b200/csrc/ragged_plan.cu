@@ -14,7 +14,8 @@ namespace {
 constexpr int NT = 1024, CLASSES = 1024;
 // A part is at least this many key tiles long: a part writes its accumulator and the combine kernel reads it back, which
 // is the traffic of about four key tiles.
-constexpr int MIN_PART = 8, MAX_PARTS = 64;
+constexpr int MIN_PART = 16, MAX_PARTS = 64;
+constexpr int MAX_CUT = 16384;                         // lists longer than this are not cut
 
 __device__ __forceinline__ int block_scan(int v, int* warp_sums, int* total) {   // exclusive; all NT threads
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
@@ -74,7 +75,8 @@ __device__ __forceinline__ int sequence_of(const int* prefix, int S, int i) {
 }
 
 __global__ void __launch_bounds__(NT) ragged_plan_kernel(const RaggedSeqs q, const RaggedPlan plan) {
-  __shared__ int warp_sums[33], hist[CLASSES], s_max, s_slots, s_combos, s_parts;
+  __shared__ int warp_sums[33], hist[CLASSES], s_max, s_slots, s_combos, s_parts, s_class, s_quota;
+  __shared__ unsigned whole[MAX_CUT / 32];
   __shared__ unsigned long long s_cost;
   griddep_wait();                                      // the workspace may be another call's until here
   hist[threadIdx.x] = 0;
@@ -109,36 +111,61 @@ __global__ void __launch_bounds__(NT) ragged_plan_kernel(const RaggedSeqs q, con
   }
   __syncthreads();
   const int longest = s_max;
+  auto class_of = [&](int nk) { return CLASSES - 1 - int(int64_t(nk) * (CLASSES - 1) / longest); };
 
-  // parts: an item above an even share of the work is cut into parts of about half a share, of MIN_PART tiles at
-  // least, if the slots hold all the parts (else the parts grow)
+  // Parts.  Where the longest items are more than half of an even share of the work, the CTAs cannot be level: 168 items of 470
+  // score tiles over 148 CTAs take as long as 296 would (847 us).  As many of the longest as fill whole rounds stay whole, the
+  // others are cut to fill what the share has left over; where the longest is above the share, all are cut, into quarters of a share.
+  // Parts are MIN_PART tiles at least, and grow until the slots hold them all.  Which items stay whole is decided by length and,
+  // among equals, by their order in the call, never by the order of arrival: a cut item's sums round differently.
   int target = 1 << 30;                                // key tiles of a part
-  if (plan.max_slots > 0) {
-    const unsigned long long share = s_cost * plan.heads / plan.sms + 1;        // score tiles a CTA would have
-    if ((unsigned long long)longest * 2 > share) {
-      target = max(MIN_PART, int(min(share / 4 + 1, 1ull << 28)));
+  if (plan.max_slots > 0 && n <= MAX_CUT) {
+    const unsigned long long share = s_cost * plan.heads / plan.sms + 1;        // score tiles a CTA would have, two to a key tile
+    if ((unsigned long long)longest * 4 > share) {
+      const unsigned long long rounds = share / (2ull * longest);
+      const int stay = int(min(rounds * plan.sms / plan.heads, (unsigned long long)n));
+      target = int(min(rounds > 0 ? max(share - rounds * 2 * longest, share / 16) / 2 : share / 8, 1ull << 28));
+      target = max(MIN_PART, target + 1);
+      auto length_of = [&](int i) { return i < NT ? mine.n1 : block_at(i).n1; };
+      for (int i = threadIdx.x; i < (n + 31) / 32; i += NT) whole[i] = 0u;
+      if (stay > 0) {                                  // the `stay` longest: all of the classes ahead of one, the first of that one
+        for (int i = threadIdx.x; i < n; i += NT) atomicAdd(&hist[class_of(length_of(i))], 1);
+        __syncthreads();
+        int total;
+        const int at = block_scan(hist[threadIdx.x], warp_sums, &total);
+        if (at < stay && at + hist[threadIdx.x] >= stay) { s_class = threadIdx.x; s_quota = stay - at; }
+        __syncthreads();
+        hist[threadIdx.x] = 0;
+        int seen = 0;
+        for (int i0 = 0; i0 < n; i0 += NT) {
+          const int i = i0 + int(threadIdx.x), c = i < n ? class_of(length_of(i)) : CLASSES;
+          int of_class;
+          const int rank = seen + block_scan(c == s_class ? 1 : 0, warp_sums, &of_class);
+          seen += of_class;
+          if (c < s_class || (c == s_class && rank < s_quota)) atomicOr(&whole[i >> 5], 1u << (i & 31));
+        }
+      }
       for (;;) {
         __syncthreads();
         if (threadIdx.x == 0) s_parts = 0;
         __syncthreads();
         int parts = 0;
         for (int i = threadIdx.x; i < n; i += NT) {
-          const int n1 = i < NT ? mine.n1 : block_at(i).n1;
-          const int p = min((n1 + target - 1) / target, MAX_PARTS);
+          const int p = (whole[i >> 5] >> (i & 31)) & 1u ? 1 : min((length_of(i) + target - 1) / target, MAX_PARTS);
           if (p > 1) parts += p;
         }
         parts = __reduce_add_sync(0xffffffffu, parts);
         if ((threadIdx.x & 31) == 0 && parts) atomicAdd(&s_parts, parts);
         __syncthreads();
         if (s_parts <= plan.max_slots || target >= (1 << 28)) break;
-        target *= 2;
+        target += target / 4 + 1;
       }
     }
   }
-  auto parts_of = [&](int n1) { return min((n1 + target - 1) / target, MAX_PARTS); };
-  auto class_of = [&](int nk) { return CLASSES - 1 - int(int64_t(nk) * (CLASSES - 1) / longest); };
+  const bool cut = target < (1 << 30);
+  auto parts_of = [&](int i, int n1) { return !cut || ((whole[i >> 5] >> (i & 31)) & 1u) ? 1 : min((n1 + target - 1) / target, MAX_PARTS); };
   for (int i = threadIdx.x; i < n; i += NT) {
-    const int n1 = i < NT ? mine.n1 : block_at(i).n1, parts = parts_of(n1);
+    const int n1 = i < NT ? mine.n1 : block_at(i).n1, parts = parts_of(i, n1);
     atomicAdd(&hist[class_of((n1 + parts - 1) / parts)], parts);
   }
   __syncthreads();
@@ -149,7 +176,7 @@ __global__ void __launch_bounds__(NT) ragged_plan_kernel(const RaggedSeqs q, con
   __syncthreads();
   for (int i = threadIdx.x; i < n; i += NT) {
     const Block b = i < NT ? mine : block_at(i);
-    const int parts = parts_of(b.n1);
+    const int parts = parts_of(i, b.n1);
     int at = atomicAdd(&hist[class_of((b.n1 + parts - 1) / parts)], parts);
     int slot = -1;
     if (parts > 1) {
@@ -213,8 +240,8 @@ struct Sizes { int items, slots, combos; };
 Sizes plan_sizes(int S, int tokens, int G, int Hkv, bool may_split) {
   const int block = 2 * (128 / G);
   Sizes z{};
-  // parts of at least MIN_PART tiles and half a share of one of the CTAs: two or three times the CTAs, per head
-  z.slots = may_split ? (3 * sm_count() + Hkv - 1) / Hkv : 0;
+  // parts of a quarter of a CTA's share: four or five times the CTAs, over all heads
+  z.slots = may_split ? (5 * sm_count() + Hkv - 1) / Hkv : 0;
   z.combos = z.slots / 2;
   z.items = tokens / block + (S < tokens ? S : tokens) + z.slots + 1;
   return z;
