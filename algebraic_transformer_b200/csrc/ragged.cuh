@@ -65,6 +65,8 @@ struct RaggedPlan {
   RaggedCombo* combos;
   int* prefix;              // (S + 1)
   float* slots;             // parts' accumulators, (slot, head, 256 rows, D + 4)
+  float* norms;             // per CTA of the plan kernel but the first: largest squared row norm of the keys it saw; nullptr: not taken
+  int norm_ctas;
   int max_items, max_combos, max_slots;   // slots: of one head
   int block_tokens;         // tokens of an item: two tiles of 128 / G
   int heads;                // Hkv
@@ -187,9 +189,10 @@ size_t ragged_blocks_bytes(int S, int tokens);
 void ragged_blocks_carve(RaggedBlocks* blocks, void* workspace, int S, int tokens);
 int launch_ragged_blocks(const RaggedSeqs& seqs, const RaggedBlocks& blocks, cudaStream_t stream);
 
+bool ragged_takes_norms(int tokens, int Hkv);
 size_t ragged_plan_bytes(int S, int tokens, int Hkv, int G, int D, bool may_split);
-void ragged_plan_carve(RaggedPlan* plan, void* workspace, int S, int tokens, int Hkv, int G, int D, bool may_split);
-int launch_ragged_plan(const RaggedSeqs& seqs, const RaggedPlan& plan, int G, cudaStream_t stream);
+void ragged_plan_carve(RaggedPlan* plan, void* workspace, int S, int tokens, int Hkv, int G, int D, bool may_split, bool norms);
+int launch_ragged_plan(const RaggedParams& p, cudaStream_t stream);
 int launch_ragged_attention(const RaggedParams& p, cudaStream_t stream);
 
 }  // namespace alg

@@ -74,7 +74,8 @@ int alg_packed_attn_fwd(const alg_packed_attn_args* a, void* stream_) {
   }
   if (a->tokens == 0) return ALG_OK;
   p.G = a->H / a->Hkv;
-  ragged_plan_carve(&p.plan, a->workspace, a->sequences, a->tokens, a->Hkv, p.G, a->D, may_split(a->tokens, a->tokens, a->H, a->Hkv));
+  ragged_plan_carve(&p.plan, a->workspace, a->sequences, a->tokens, a->Hkv, p.G, a->D, may_split(a->tokens, a->tokens, a->H, a->Hkv),
+                    ragged_takes_norms(a->tokens, a->Hkv));
   p.seqs = {a->cu_seqlens, nullptr, a->sequences, a->tokens, a->tokens};
   p.q = a->q; p.k = a->k; p.v = a->v; p.o = a->o; p.o_lo = a->o_rest; p.stat = a->stat; p.sink = a->sink;
   p.H = a->H; p.Hkv = a->Hkv; p.D = a->D; p.log2n = ilog2_exact(a->n);
@@ -196,7 +197,7 @@ int alg_paged_attn_fwd(const alg_paged_attn_args* a, void* stream_) {
   p.inv_c = 1.0f / a->c;
   p.status = a->status;
   if (a->cu_seqlens == nullptr) return launch_paged_token(p, a->workspace, stream);
-  ragged_plan_carve(&p.plan, a->workspace, a->sequences, a->tokens, a->Hkv, p.G, a->D, may_split(keys, a->tokens, a->H, a->Hkv));
+  ragged_plan_carve(&p.plan, a->workspace, a->sequences, a->tokens, a->Hkv, p.G, a->D, may_split(keys, a->tokens, a->H, a->Hkv), false);
   p.zero_tail = a->zero_tail != 0;
   return launch_ragged_attention(p, stream);
 }

@@ -11,11 +11,12 @@
 //   - K and V tiles come from packed rows (a tile reads on into the next sequence) or page by page through the block table.
 //     Keys past the sequence's end are masked by the causal limit, but 0 times the NaN or infinity that a
 //     foreign V row may hold is NaN: one warp zeroes those rows of a sequence's last V tile in shared memory;
-//   - any scores: a warp whose 32 rows have all |x| <= x_fast in a tile takes the tile unshifted (x_fast keeps the weights within
-//     2^+-64 and the cancellation of y + sqrt(kappa + y^2) below 2e-4); a larger score, or a NaN, sends the warp to the max-shifted
-//     form with the cancellation-free rho for the rest of the item.  So no pass over q and k decides beforehand.
+//   - any scores: a warp takes a tile unshifted where all its |x| <= x_fast (which keeps the weights within 2^+-64 and the
+//     cancellation of y + sqrt(kappa + y^2) below 2e-4).  For packed keys the largest row norms of the call's keys (ragged_plan.cu) and
+//     of the item's queries settle that as a rule; else the scores are looked at ahead of their weights: a sum of squares, then the largest.  A
+//     score out of range, or a NaN, sends the warp to the max-shifted form with the cancellation-free rho for the rest of the item.
 //
-// Roles: warp 0 takes the work and runs the TMA loads, warp 1 issues the MMAs, warp 2 scales Q in shared memory, warp 3 clears the
+// Roles: warp 0 takes the work and runs the TMA loads, warp 1 issues the MMAs, warp 2 scales Q in shared memory and takes its row norms, warp 3 clears the
 // foreign V rows, warps 4..7 and 8..11 weigh query tile 0 and 1, a thread a row.  An item of one tile runs as tile 1.
 // HILO (training): the weights go to the second product as two bf16 halves and the output is stored as two, since the
 // gradient of the sinks is a float32 sum of what the output's rounding would leave of its digits.
@@ -66,8 +67,9 @@ struct __align__(16) Control {
   uint64_t q_full[2], q_ready[2], q_free[2], kv_full[MAX_NKV], kv_empty[MAX_NKV];
   uint64_t s_full[2], p_half[2], p_full[2], o_full[2], o_free[2];
   uint64_t s_read[2], pv_done[2];   // EARLY: scores are in registers; the second product of a tile is done
-  uint64_t v_here, v_clean, work_full[RING], work_empty[RING];
+  uint64_t q_norm_full[2], v_here, v_clean, work_full[RING], work_empty[RING];
   Work work[RING];
+  float q_norm[2][2];             // largest squared row norm of a query tile, of this item and the next one
   uint32_t tmem_base;
   int abort_flag;
 };
@@ -82,16 +84,6 @@ struct ScoreScale {
   float inv_m;     // every weight is (rho(x) / m)^n
   float y_fast;    // x_fast / m
 };
-
-template <int LOG2N> __device__ __forceinline__ float2 power2(float2 t, int log2n) {
-  if (LOG2N > 0) {
-#pragma unroll
-    for (int k = 0; k < LOG2N; ++k) t = __fmul2_rn(t, t);
-  } else {
-    for (int k = 0; k < log2n; ++k) t = __fmul2_rn(t, t);
-  }
-  return t;
-}
 
 // 32 weights of this thread's row into bf16 pairs, hi and (HILO) what the rounding left over
 template <bool HILO>
@@ -109,25 +101,47 @@ template <bool HILO> __device__ __forceinline__ void store_packed(uint32_t taddr
   else tmem_st_32x16(taddr, packed);
 }
 
-// Unshifted: 32 scores y -> (y + sqrt(kappa + y^2))^n.  `lim`: the last visible column of this row, counted from column 0 of the 32.
+// Unshifted: 32 scores y -> (y + sqrt(kappa + y^2))^n.  `lim`: the last visible column of this row, counted from column 0 of the 32.  Formed
+// in passes over PAIRS pairs, so that every pass has independent operations: with two warps on a scheduler nothing else hides their latency.
 template <int LOG2N, bool MASK, bool HILO>
 __device__ __forceinline__ void weigh(const uint32_t* s, float kappa, int log2n, int lim, float2& la, float2& lb, uint32_t* packed) {
+  constexpr int PAIRS = 8;
   const float2 kp = make_float2(kappa, kappa);
 #pragma unroll
-  for (int i = 0; i < 32; i += 4) {
-    const float2 y0 = make_float2(__uint_as_float(s[i]), __uint_as_float(s[i + 1]));
-    const float2 y1 = make_float2(__uint_as_float(s[i + 2]), __uint_as_float(s[i + 3]));
-    const float2 rad0 = __ffma2_rn(y0, y0, kp), rad1 = __ffma2_rn(y1, y1, kp);
-    const float2 rs0 = make_float2(rsqrt_approx(rad0.x), rsqrt_approx(rad0.y));
-    const float2 rs1 = make_float2(rsqrt_approx(rad1.x), rsqrt_approx(rad1.y));
-    float2 t0 = power2<LOG2N>(__ffma2_rn(rad0, rs0, y0), log2n), t1 = power2<LOG2N>(__ffma2_rn(rad1, rs1, y1), log2n);
-    if (MASK) {
-      t0.x = (i <= lim) ? t0.x : 0.f;     t0.y = (i + 1 <= lim) ? t0.y : 0.f;
-      t1.x = (i + 2 <= lim) ? t1.x : 0.f; t1.y = (i + 3 <= lim) ? t1.y : 0.f;
+  for (int i0 = 0; i0 < 32; i0 += 2 * PAIRS) {
+    float2 t[PAIRS];
+    {
+      float2 rad[PAIRS];
+#pragma unroll
+      for (int i = 0; i < PAIRS; ++i) {
+        const float2 y = make_float2(__uint_as_float(s[i0 + 2 * i]), __uint_as_float(s[i0 + 2 * i + 1]));
+        rad[i] = __ffma2_rn(y, y, kp);
+      }
+#pragma unroll
+      for (int i = 0; i < PAIRS; ++i) t[i] = make_float2(rsqrt_approx(rad[i].x), rsqrt_approx(rad[i].y));
+#pragma unroll
+      for (int i = 0; i < PAIRS; ++i) t[i] = __ffma2_rn(rad[i], t[i], make_float2(__uint_as_float(s[i0 + 2 * i]), __uint_as_float(s[i0 + 2 * i + 1])));
     }
-    la = __fadd2_rn(la, t0);
-    lb = __fadd2_rn(lb, t1);
-    pack4<HILO>(t0, t1, i, packed);
+    if (LOG2N > 0) {
+#pragma unroll
+      for (int k = 0; k < LOG2N; ++k)
+#pragma unroll
+        for (int i = 0; i < PAIRS; ++i) t[i] = __fmul2_rn(t[i], t[i]);
+    } else {
+      for (int k = 0; k < log2n; ++k)
+#pragma unroll
+        for (int i = 0; i < PAIRS; ++i) t[i] = __fmul2_rn(t[i], t[i]);
+    }
+#pragma unroll
+    for (int i = 0; i < PAIRS; i += 2) {
+      if (MASK) {
+        t[i].x = (i0 + 2 * i <= lim) ? t[i].x : 0.f;             t[i].y = (i0 + 2 * i + 1 <= lim) ? t[i].y : 0.f;
+        t[i + 1].x = (i0 + 2 * i + 2 <= lim) ? t[i + 1].x : 0.f; t[i + 1].y = (i0 + 2 * i + 3 <= lim) ? t[i + 1].y : 0.f;
+      }
+      la = __fadd2_rn(la, t[i]);
+      lb = __fadd2_rn(lb, t[i + 1]);
+      pack4<HILO>(t[i], t[i + 1], i0 + 2 * i, packed);
+    }
   }
 }
 
@@ -152,10 +166,16 @@ __device__ __forceinline__ void weigh_shifted(const uint32_t* s, float m, float 
     pack4<HILO>(t0, t1, i, packed);
   }
 }
+// What this warp has done with tensor memory is done: one arrival a warp.  (An arrival a thread is 32 operations on one word of
+// shared memory, two or three times a tile.)
+__device__ __forceinline__ void warp_arrive(uint64_t* bar) {
+  tc_fence_before();
+  __syncwarp();
+  if ((threadIdx.x & 31) == 0) mbar_arrive(bar);
+}
 __device__ __forceinline__ void signal_weights(uint64_t* bar) {
   tmem_st_wait();
-  tc_fence_before();
-  mbar_arrive(bar);
+  warp_arrive(bar);
 }
 
 // Sum of y^2 over the row's 128 scores, whatever the mask: where it is within the square of the range, so is every score.
@@ -268,6 +288,34 @@ __device__ __forceinline__ void weigh_tile_shifted(uint32_t s_taddr, uint32_t p_
   signal_weights(p_full);
 }
 
+// Largest squared norm of a query tile's 128 rows, a little above the true one: squares are added up in bf16, D / 8 of them to a sum, each
+// sum off by a half step at most.  NaN or infinity where a row holds one.
+template <int D> __device__ __forceinline__ float largest_row_norm(const unsigned char* tile, int lane) {
+  float most = 0.f;
+#pragma unroll 1
+  for (int r = lane; r < 128; r += 32) {
+    __nv_bfloat162 sum[4];
+#pragma unroll
+    for (int e = 0; e < 4; ++e) sum[e] = __float2bfloat162_rn(0.f);
+#pragma unroll
+    for (int pn = 0; pn < D / 64; ++pn)
+#pragma unroll
+      for (int c = 0; c < 8; ++c) {                    // chunks in an order of the row's own: no two of eight lanes in one bank group
+        const uint4 v = *reinterpret_cast<const uint4*>(tile + pn * PANEL_BYTES + r * 128 + ((c ^ (r & 7)) << 4));
+        const __nv_bfloat162* h = reinterpret_cast<const __nv_bfloat162*>(&v);
+#pragma unroll
+        for (int e = 0; e < 4; ++e) sum[e] = __hfma2(h[e], h[e], sum[e]);
+      }
+    float n = 0.f;
+#pragma unroll
+    for (int e = 0; e < 4; ++e) { const float2 f = __bfloat1622float2(sum[e]); n += f.x + f.y; }
+    most = max3_abs_nan(most, n, 0.f);
+  }
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) most = max3_abs_nan(most, __shfl_xor_sync(0xffffffffu, most, o), 0.f);
+  return most * 1.07f;                                 // (1 - 2^-9)^-16 and the sum of the eight
+}
+
 template <int NKV> struct RingCursor {
   int slot = 0;
   uint32_t phase = 0;
@@ -281,7 +329,7 @@ ragged_attn_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_consta
   using C = Cfg<D>;
   // Head_dim 64 leaves tensor memory for weights in columns of their own; then the next scores are issued as soon as these are in
   // registers, and the weight warps find them when they come back.
-  constexpr bool EARLY = D == 64 && !HILO;
+  constexpr bool EARLY = D == 64 && !HILO, NORMS = !PAGED;
   constexpr uint32_t O_COL = EARLY ? 384u : 256u, P_COL = EARLY ? 256u : 0u;      // O_t at O_COL + D t
   constexpr uint32_t P_STRIDE = EARLY ? 64u : 128u, P_STEP = EARLY ? 16u : 32u;   // P_t at P_COL + P_STRIDE t, 32 keys every P_STEP columns
   extern __shared__ unsigned char smem_raw[];
@@ -291,10 +339,10 @@ ragged_attn_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_consta
 
   if (threadIdx.x == 0) {
     for (int w = 0; w < 2; ++w) {
-      mbar_init(&ctl->q_full[w], 1); mbar_init(&ctl->q_ready[w], 1); mbar_init(&ctl->q_free[w], 1);
-      mbar_init(&ctl->s_full[w], 1); mbar_init(&ctl->p_half[w], 128); mbar_init(&ctl->p_full[w], 128);
-      mbar_init(&ctl->o_full[w], 1); mbar_init(&ctl->o_free[w], 128);
-      mbar_init(&ctl->s_read[w], 128); mbar_init(&ctl->pv_done[w], 1);
+      mbar_init(&ctl->q_full[w], 1); mbar_init(&ctl->q_ready[w], 1); mbar_init(&ctl->q_free[w], NORMS ? 2 : 1);
+      mbar_init(&ctl->s_full[w], 1); mbar_init(&ctl->p_half[w], 4); mbar_init(&ctl->p_full[w], 4);
+      mbar_init(&ctl->o_full[w], 1); mbar_init(&ctl->o_free[w], 4);
+      mbar_init(&ctl->s_read[w], 4); mbar_init(&ctl->pv_done[w], 1); mbar_init(&ctl->q_norm_full[w], 1);
     }
     for (int i = 0; i < C::NKV; ++i) { mbar_init(&ctl->kv_full[i], 1); mbar_init(&ctl->kv_empty[i], 1); }
     for (int i = 0; i < RING; ++i) { mbar_init(&ctl->work_full[i], 1); mbar_init(&ctl->work_empty[i], ITEM_READERS); }
@@ -511,6 +559,17 @@ ragged_attn_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_consta
         __syncwarp();
         if (lane == 0) mbar_arrive(&ctl->q_ready[t]);
       }
+      if (NORMS) {                                      // beside the first products
+        for (int t = 0; t < 2 && ok; ++t) {
+          if (t == 0 && w.n0 == 0) continue;
+          const float norm = largest_row_norm<D>(smem + t * C::TILE_BYTES, lane);
+          if (lane == 0) {
+            ctl->q_norm[t][(t == 0 ? items0 : k) & 1] = norm;
+            mbar_arrive(&ctl->q_norm_full[t]);
+            mbar_arrive(&ctl->q_free[t]);               // with the weight warps' word that the last scores are there
+          }
+        }
+      }
       if (w.n0 > 0) ++items0;
     }
   } else if (warp == 3) {
@@ -559,6 +618,14 @@ ragged_attn_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_consta
     RingCursor<C::NKV> rel;
     int kslot = 0, vslot = 1 % C::NKV;                  // EARLY: K and V slots are released apart, every other one from 0 and from 1
     int tiles = 0, items = 0;                           // of this group, in earlier items
+    float q_limit = -1.f;                               // queries of smaller squared norm keep every score in the unshifted range
+    if (NORMS && p.plan.norms != nullptr) {
+      float nk = 0.f;
+      for (int i = lane; i < p.plan.norm_ctas; i += 32) nk = max3_abs_nan(nk, p.plan.norms[i], 0.f);
+#pragma unroll
+      for (int o = 16; o > 0; o >>= 1) nk = max3_abs_nan(nk, __shfl_xor_sync(0xffffffffu, nk, o), 0.f);
+      q_limit = sc.y_fast * sc.y_fast / (1.001f * nk);  // NaN: never smaller
+    }
     Work w;
     bool ok = true;
     for (int k = 0; ok && work_at(k, w); ++k) {
@@ -570,7 +637,7 @@ ragged_attn_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_consta
       const int head = w.head * p.G + g_r;
       float l = 0.f, m_run = 0.f;                       // weights are (rho(x) rho(-m_run) / m)^n: unshifted at first
       const bool whole_sink = live && p.sink != nullptr && w.k0 == 0;
-      bool shifted = false;                             // the warp's form
+      bool shifted = false, trusted = false;            // the warp's form; its scores need not be looked at
       if (whole_sink) {
         const float b = p.sink[head] * p.inv_c;
         if (!(fabsf(b) <= sc.y_fast * sc.m)) m_run = b;
@@ -594,7 +661,11 @@ ragged_attn_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_consta
         }
         const int lim = limit - j * BKEY;
         const bool masked = limit0 - j * BKEY < BKEY - 1;                        // uniform over the group
-        if (!shifted) {
+        if (NORMS && j == 0) {
+          if (!__all_sync(0xffffffffu, bw.wait(&ctl->q_norm_full[t], uint32_t(items) & 1u))) { ok = false; break; }
+          trusted = ctl->q_norm[t][items & 1] <= q_limit;
+        }
+        if (!shifted && !trusted) {
           const float sum = tile_square_sum(s_taddr);   // by all lanes: the loads are the whole warp's
           if (!__all_sync(0xffffffffu, !live || sum <= sc.y_fast * sc.y_fast)) {
             const float top = tile_abs_max(s_taddr, lim);
@@ -612,10 +683,7 @@ ragged_attn_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_consta
           return true;
         };
         auto scores_loaded = [&] {                      // EARLY: the next scores may come
-          if (EARLY) {
-            tc_fence_before();
-            mbar_arrive(&ctl->s_read[t]);
-          }
+          if (EARLY) warp_arrive(&ctl->s_read[t]);
         };
         if (!shifted) {
           ok = weigh_tile<LOG2N, HILO, P_STEP>(s_taddr, p_taddr, &ctl->p_half[t], &ctl->p_full[t], sc.kappa, p.log2n, lim, masked, la, lb,
@@ -677,8 +745,7 @@ ragged_attn_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_consta
           tmem_ld_32x32(o_taddr + c, o);
           tmem_ld_wait_for(o);
           if (c == D - 32) {                            // O is in registers: the next item may overwrite it
-            tc_fence_before();
-            mbar_arrive(&ctl->o_free[t]);
+            warp_arrive(&ctl->o_free[t]);
           }
           if (partial) {
 #pragma unroll
@@ -877,7 +944,7 @@ int launch_d(const RaggedParams& p, cudaStream_t stream) {
 }  // namespace
 
 int launch_ragged_attention(const RaggedParams& p, cudaStream_t stream) {
-  if (int rc = launch_ragged_plan(p.seqs, p.plan, p.G, stream)) return rc;
+  if (int rc = launch_ragged_plan(p, stream)) return rc;
   return p.D == 64 ? launch_d<64>(p, stream) : launch_d<128>(p, stream);
 }
 
