@@ -66,7 +66,6 @@ struct Work {
 struct __align__(16) Control {
   uint64_t q_full[2], q_ready[2], q_free[2], kv_full[MAX_NKV], kv_empty[MAX_NKV];
   uint64_t s_full[2], p_half[2], p_full[2], o_full[2], o_free[2];
-  uint64_t s_read[2], pv_done[2];   // EARLY: scores are in registers; the second product of a tile is done
   uint64_t q_norm_full[2], v_here, v_clean, work_full[RING], work_empty[RING];
   Work work[RING];
   float q_norm[2][2];             // largest squared row norm of a query tile, of this item and the next one
@@ -220,12 +219,13 @@ __device__ __forceinline__ float tile_abs_max(uint32_t s_taddr, int lim) {
   return most;
 }
 
-// The unshifted weights of a tile to tensor memory, 32 keys every STEP columns, the next 32 scores in flight while a block is weighed.
-// A loop of two times two blocks: the unrolled tile is more code than the SM's instruction caches hold for two warps that are not
-// at the same place.  `loaded()` is called when the last scores are in registers, `second()` ahead of the second half's first store.
-template <int LOG2N, bool HILO, int STEP, class Loaded, class Second>
-__device__ __forceinline__ bool weigh_tile(uint32_t s_taddr, uint32_t p_taddr, uint64_t* p_half, uint64_t* p_full, float kappa, int log2n, int lim,
-                                           bool masked, float2& la, float2& lb, const Loaded& loaded, const Second& second) {
+// The unshifted weights of a tile, written over the scores, the next 32 scores in flight while a block is weighed.  A loop of two times
+// two blocks: unrolled, the tile is more code than two warps that are not at the same place in it find in the SM's instruction caches
+// (97 against 94 us for 24 prompts, 16 heads on 4 of 64).  Weights in columns of their own, so that the next scores could be issued
+// as soon as these are read, were no faster (94 against 92), nor were all 128 scores in registers.
+template <int LOG2N, bool HILO>
+__device__ __forceinline__ void weigh_tile(uint32_t s_taddr, uint64_t* p_half, uint64_t* p_full, float kappa, int log2n, int lim, bool masked,
+                                           float2& la, float2& lb) {
   uint32_t a[32], b[32], packed[HILO ? 32 : 16];
   const int warp_lim = masked ? __reduce_max_sync(0xffffffffu, lim) : 128;
   auto block = [&](const uint32_t* s, int c) {
@@ -244,18 +244,14 @@ __device__ __forceinline__ bool weigh_tile(uint32_t s_taddr, uint32_t p_taddr, u
     tmem_ld_wait_for(a);
     tmem_ld_32x32(s_taddr + 32, b);
     block(a, 64 * half);
-    if (half == 1 && !second()) return false;
-    store_packed<HILO>(p_taddr, packed);
+    store_packed<HILO>(s_taddr, packed);
     tmem_ld_wait_for(b);
     if (half == 0) tmem_ld_32x32(s_taddr + 64, a);
-    else loaded();
     block(b, 64 * half + 32);
-    store_packed<HILO>(p_taddr + STEP, packed);
+    store_packed<HILO>(s_taddr + 32, packed);
     signal_weights(half == 0 ? p_half : p_full);
     s_taddr += 64;
-    p_taddr += 2 * STEP;
   }
-  return true;
 }
 
 // The max-shifted form reads the scores again from tensor memory, block by block: it runs where the short form may not, and
@@ -273,8 +269,8 @@ __device__ __forceinline__ float tile_row_max(uint32_t s_taddr, float m, int lim
   }
   return top;
 }
-template <bool HILO, int STEP>
-__device__ __forceinline__ void weigh_tile_shifted(uint32_t s_taddr, uint32_t p_taddr, uint64_t* p_half, uint64_t* p_full, float m, float sigma,
+template <bool HILO>
+__device__ __forceinline__ void weigh_tile_shifted(uint32_t s_taddr, uint64_t* p_half, uint64_t* p_full, float m, float sigma,
                                                    int log2n, int lim, float2& la, float2& lb) {
 #pragma unroll 1
   for (int b = 0; b < 4; ++b) {
@@ -282,7 +278,7 @@ __device__ __forceinline__ void weigh_tile_shifted(uint32_t s_taddr, uint32_t p_
     tmem_ld_32x32(s_taddr + 32 * b, a);
     tmem_ld_wait_for(a);
     weigh_shifted<HILO>(a, m, sigma, log2n, lim - 32 * b, la, lb, packed);
-    store_packed<HILO>(p_taddr + STEP * b, packed);
+    store_packed<HILO>(s_taddr + 32 * b, packed);
     if (b == 1) signal_weights(p_half);
   }
   signal_weights(p_full);
@@ -327,11 +323,8 @@ __global__ void __launch_bounds__(NTHREADS, 1)
 ragged_attn_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant__ CUtensorMap tm_k,
                    const __grid_constant__ CUtensorMap tm_v, const __grid_constant__ RaggedParams p, const ScoreScale sc) {
   using C = Cfg<D>;
-  // Head_dim 64 leaves tensor memory for weights in columns of their own; then the next scores are issued as soon as these are in
-  // registers, and the weight warps find them when they come back.
-  constexpr bool EARLY = D == 64 && !HILO, NORMS = !PAGED;
-  constexpr uint32_t O_COL = EARLY ? 384u : 256u, P_COL = EARLY ? 256u : 0u;      // O_t at O_COL + D t
-  constexpr uint32_t P_STRIDE = EARLY ? 64u : 128u, P_STEP = EARLY ? 16u : 32u;   // P_t at P_COL + P_STRIDE t, 32 keys every P_STEP columns
+  constexpr bool NORMS = !PAGED;
+  constexpr uint32_t O_COL = 256;                       // tensor memory: S_t at 128 t with P_t inside it, O_t at O_COL + D t
   extern __shared__ unsigned char smem_raw[];
   unsigned char* smem = reinterpret_cast<unsigned char*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
   Control* ctl = reinterpret_cast<Control*>(smem + C::CTL_OFF);
@@ -342,7 +335,7 @@ ragged_attn_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_consta
       mbar_init(&ctl->q_full[w], 1); mbar_init(&ctl->q_ready[w], 1); mbar_init(&ctl->q_free[w], NORMS ? 2 : 1);
       mbar_init(&ctl->s_full[w], 1); mbar_init(&ctl->p_half[w], 4); mbar_init(&ctl->p_full[w], 4);
       mbar_init(&ctl->o_full[w], 1); mbar_init(&ctl->o_free[w], 4);
-      mbar_init(&ctl->s_read[w], 4); mbar_init(&ctl->pv_done[w], 1); mbar_init(&ctl->q_norm_full[w], 1);
+      mbar_init(&ctl->q_norm_full[w], 1);
     }
     for (int i = 0; i < C::NKV; ++i) { mbar_init(&ctl->kv_full[i], 1); mbar_init(&ctl->kv_empty[i], 1); }
     for (int i = 0; i < RING; ++i) { mbar_init(&ctl->work_full[i], 1); mbar_init(&ctl->work_empty[i], ITEM_READERS); }
@@ -465,7 +458,7 @@ ragged_attn_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_consta
 #pragma unroll
         for (int i = 0; i < 4; ++i) {                   // 16 keys = 8 packed columns of P a step
           const int ks = 4 * h64 + i;
-          umma_f16_ts_parts(tmem_base + O_COL + t * D, tmem_base + P_COL + t * P_STRIDE + (ks >> 1) * P_STEP + (ks & 1) * 8 + part * 16,
+          umma_f16_ts_parts(tmem_base + O_COL + t * D, tmem_base + t * 128 + (ks >> 1) * 32 + (ks & 1) * 8 + part * 16,
                             va + ks * (2048 >> 4), SW128_DESC_HI, C::IDESC_PV, (first && ks == 0 && part == 0) ? 0u : 1u);
         }
     };
@@ -476,23 +469,8 @@ ragged_attn_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_consta
       tc_fence_after();
       if (elect_one()) issue_pv(t, v_slot, 0, j == 0);
       __syncwarp();
-      if (EARLY && j + 1 < nt) {
-        if (!wait_all(&ctl->s_read[t], uint32_t(before + j) & 1u)) return false;
-        tc_fence_after();
-        if (elect_one()) { issue_s(t, k_slot); umma_commit(&ctl->s_full[t]); }
-        __syncwarp();
-      }
       if (!wait_all(&ctl->p_full[t], uint32_t(before + j) & 1u)) return false;
       tc_fence_after();
-      if (EARLY) {
-        if (elect_one()) {
-          issue_pv(t, v_slot, 1, false);
-          umma_commit(&ctl->pv_done[t]);
-          if (j + 1 == nt) umma_commit(&ctl->o_full[t]);
-        }
-        __syncwarp();
-        return true;
-      }
       if (elect_one()) {
         issue_pv(t, v_slot, 1, false);
         if (j + 1 < nt) { issue_s(t, k_slot); umma_commit(&ctl->s_full[t]); }    // behind P V: may overwrite P
@@ -611,12 +589,11 @@ ragged_attn_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_consta
     const int r = quarter * 32 + lane;                  // row of the tile
     const uint32_t lane_sel = uint32_t(quarter * 32) << 16;
     const uint32_t s_taddr = tmem_base + lane_sel + t * 128;
-    const uint32_t p_taddr = tmem_base + lane_sel + P_COL + t * P_STRIDE, o_taddr = tmem_base + lane_sel + O_COL + t * D;
+    const uint32_t o_taddr = tmem_base + lane_sel + O_COL + t * D;
     const int tok_r = r / p.G, g_r = r - tok_r * p.G;   // token and head of this row
     // the "scores there" barriers of tile 1, served second in every step, tell that V of the step before and K of this one are read
     const bool releaser = quarter == 0 && lane == 0;
     RingCursor<C::NKV> rel;
-    int kslot = 0, vslot = 1 % C::NKV;                  // EARLY: K and V slots are released apart, every other one from 0 and from 1
     int tiles = 0, items = 0;                           // of this group, in earlier items
     float q_limit = -1.f;                               // queries of smaller squared norm keep every score in the unshifted range
     if (NORMS && p.plan.norms != nullptr) {
@@ -650,12 +627,8 @@ ragged_attn_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_consta
         tc_fence_after();
         if (releaser) {
           if (t == 1) {
-            if (EARLY) {                                                         // K_j; V_{j-1} follows at pv_done
-              mbar_arrive(&ctl->kv_empty[kslot]); kslot = (kslot + 2) % C::NKV;
-            } else {
-              if (j > 0) { mbar_arrive(&ctl->kv_empty[rel.slot]); rel.next(); }  // V_{j-1}
-              mbar_arrive(&ctl->kv_empty[rel.slot]); rel.next();                 // K_j
-            }
+            if (j > 0) { mbar_arrive(&ctl->kv_empty[rel.slot]); rel.next(); }    // V_{j-1}
+            mbar_arrive(&ctl->kv_empty[rel.slot]); rel.next();                   // K_j
           }
           if (j == nk - 1) mbar_arrive(&ctl->q_free[t]);
         }
@@ -672,22 +645,8 @@ ragged_attn_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_consta
             shifted = __any_sync(0xffffffffu, live && !(top <= sc.y_fast));
           }
         }
-        // EARLY: the product with the tile before has read its weights, and V, which goes back to the ring; nothing to wait for where
-        // the weights lie in the scores' place
-        auto product_done = [&]() -> bool {
-          if (EARLY && tiles + j > 0) {
-            if (!__all_sync(0xffffffffu, bw.wait(&ctl->pv_done[t], uint32_t(tiles + j - 1) & 1u))) return false;
-            tc_fence_after();
-            if (releaser && t == 1 && j > 0) { mbar_arrive(&ctl->kv_empty[vslot]); vslot = (vslot + 2) % C::NKV; }
-          }
-          return true;
-        };
-        auto scores_loaded = [&] {                      // EARLY: the next scores may come
-          if (EARLY) warp_arrive(&ctl->s_read[t]);
-        };
         if (!shifted) {
-          ok = weigh_tile<LOG2N, HILO, P_STEP>(s_taddr, p_taddr, &ctl->p_half[t], &ctl->p_full[t], sc.kappa, p.log2n, lim, masked, la, lb,
-                                               scores_loaded, product_done);
+          weigh_tile<LOG2N, HILO>(s_taddr, &ctl->p_half[t], &ctl->p_full[t], sc.kappa, p.log2n, lim, masked, la, lb);
         } else {
           l += (la.x + la.y) + (lb.x + lb.y);
           la = make_float2(0.f, 0.f); lb = make_float2(0.f, 0.f);
@@ -696,9 +655,7 @@ ragged_attn_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_consta
           float m_new = m_run;
           if (lim >= 0 && top > -INFINITY) m_new = l > 0.f ? fmaxf(m_run, top) : top;
           const float alpha = m_new != m_run ? pow2n_rt(rho_any(m_run) * rho_any(-m_new), p.log2n) : 1.0f;
-          // O of the earlier tiles is at rest (these scores were issued behind their product, or it is waited for): rescale it where
-          // a reference moved
-          if (!product_done()) { ok = false; break; }
+          // O of the earlier tiles is at rest (these scores were issued behind their product): rescale it where a reference moved
           if (__any_sync(0xffffffffu, j > 0 && alpha != 1.0f)) {
             const float a_row = j > 0 ? alpha : 1.0f;
 #pragma unroll 1
@@ -714,8 +671,7 @@ ragged_attn_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_consta
           }
           if (l > 0.f) l *= alpha;
           m_run = m_new;
-          weigh_tile_shifted<HILO, P_STEP>(s_taddr, p_taddr, &ctl->p_half[t], &ctl->p_full[t], sc.m, rho_any(-m_run) * sc.inv_m, p.log2n, lim, la, lb);
-          scores_loaded();
+          weigh_tile_shifted<HILO>(s_taddr, &ctl->p_half[t], &ctl->p_full[t], sc.m, rho_any(-m_run) * sc.inv_m, p.log2n, lim, la, lb);
         }
       }
       if (!ok) break;
@@ -730,10 +686,7 @@ ragged_attn_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_consta
       if (nk > 0) {
         if (!__all_sync(0xffffffffu, bw.wait(&ctl->o_full[t], uint32_t(items) & 1u))) { ok = false; break; }
         ++items;
-        if (releaser && t == 1) {                       // the item's last V tile
-          if (EARLY) { mbar_arrive(&ctl->kv_empty[vslot]); vslot = (vslot + 2) % C::NKV; }
-          else { mbar_arrive(&ctl->kv_empty[rel.slot]); rel.next(); }
-        }
+        if (releaser && t == 1) { mbar_arrive(&ctl->kv_empty[rel.slot]); rel.next(); }     // the item's last V tile
         tc_fence_after();
         const float inv = l != 0.f ? 1.0f / l : 0.f;    // a row that sees nothing: zero
         const int64_t row = int64_t(w.row0) + tok;

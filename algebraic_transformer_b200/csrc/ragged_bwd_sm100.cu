@@ -514,7 +514,7 @@ ragged_bwd_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constan
 
 // delta_i = dO_i . (o_i + rest_i), a CTA per head and CHUNK tokens, a row per LPR lanes; the chunk's share of the sink's gradient; zeros to
 // the gradients of rows of no sequence.
-constexpr int CHUNK = 128;
+constexpr int CHUNK = 64;
 template <int D>
 __global__ void __launch_bounds__(256) ragged_delta_kernel(const __grid_constant__ RaggedBwdParams p) {
   constexpr int LPR = D / 8, RPW = 32 / LPR, ROWS = CHUNK / 8 / RPW;
@@ -532,6 +532,9 @@ __global__ void __launch_bounds__(256) ragged_delta_kernel(const __grid_constant
     r[u] = __ldg(reinterpret_cast<const uint4*>(p.rest + (t * p.H + h) * D + lir * 8));
   }
   const bool sunk = p.sink != nullptr;
+  float stat[ROWS];                                      // with the rows, not behind their sums
+#pragma unroll
+  for (int u = 0; u < ROWS; ++u) stat[u] = sunk && lir == 0 ? __ldg(p.stat + int64_t(h) * p.tokens + min(t0 + u * RPW, p.tokens - 1)) : 0.f;
   const float bs = sunk ? p.sink[h] * p.inv_c : 0.f, rho_b = rho_any(bs);
   const float slope = -p.n_f * p.inv_c * rsqrtf(fmaf(bs, bs, 1.0f));
   float sum = 0.f;
@@ -560,7 +563,7 @@ __global__ void __launch_bounds__(256) ragged_delta_kernel(const __grid_constant
     } else if (lir == 0) {
       const int64_t at = int64_t(h) * p.tokens + t;
       p.delta[at] = d;
-      if (sunk) sum = fmaf(d, pow2n_rt(rho_b * __ldg(p.stat + at), p.log2n), sum);
+      if (sunk) sum = fmaf(d, pow2n_rt(rho_b * stat[u], p.log2n), sum);
     }
   }
   if (!sunk) return;
