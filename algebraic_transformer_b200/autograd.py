@@ -16,6 +16,7 @@ log-likelihood for `alg_ce`, of the mean cross-entropy for `ce`), not the deriva
 from typing import Optional
 
 import torch
+from torch.autograd.function import once_differentiable
 
 from . import ops
 
@@ -63,6 +64,7 @@ class _PackedAttention(torch.autograd.Function):
         return o
 
     @staticmethod
+    @once_differentiable
     def backward(ctx, d_o):
         q, k, v, o, stat, rest, cu_seqlens, sink = ctx.saved_tensors
         dq, dk, dv, dsink = ops.packed_attention_backward(q, k, v, o, d_o.to(o.dtype), stat, rest, cu_seqlens, sink if ctx.has_sink else None,
@@ -74,7 +76,8 @@ def packed_attention(q, k, v, cu_seqlens, sink_logit: Optional[torch.Tensor] = N
     """Differentiable attention over packed sequences of different lengths with grouped heads: `ops.packed_attention` and
     `ops.packed_attention_backward`.  q (tokens, H, D), k, v (tokens, Hkv, D) bf16, `cu_seqlens` int32 (sequences + 1) on the device,
     which has to keep its values until the backward pass; `sink_logit` is a float32 (H,) tensor or None.  Rows of no sequence have
-    output and gradients zero."""
+    output and gradients zero.  First derivatives only.  A backward pass is captured into a CUDA graph while no eager graph of the
+    same leaves is alive, as torch requires of every operator."""
     if sink_logit is not None and (sink_logit.dtype != torch.float32 or sink_logit.shape != (q.shape[1],)):
         raise ValueError("sink_logit must be a float32 tensor of shape (H,)")
     return _PackedAttention.apply(q, k, v, cu_seqlens, sink_logit, int(n), float(c))

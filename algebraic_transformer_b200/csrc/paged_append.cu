@@ -57,9 +57,9 @@ __global__ void __launch_bounds__(WARPS * 32) paged_append_kernel(const __grid_c
   if (s >= 0) {
     int first, Lq, Lk;
     ragged_lengths(p.seqs, s, first, Lq, Lk);
-    position = Lk - Lq + token - first;
+    position = max(__ldg(p.seqs.kv_lens + s), 0) - Lq + token - first;      // by the length as it is given: one past the table is no place
   }
-  if (position < 0) {                                  // no place in the cache: the row of q is no query either
+  if (position < 0 || position >= p.seqs.kv_capacity) {                                  // no place in the cache: the row of q is no query either
     if (p.zero_tail) {
 #pragma unroll
       for (int u = 0; u < STEPS; ++u) {

@@ -113,7 +113,7 @@ struct State {
   float4 a;
   __device__ __forceinline__ void start(const RaggedParams& p, bool with_sink, int head) {
     const bool sunk = with_sink && p.sink != nullptr;
-    m = sunk ? p.sink[head] * p.inv_c : -1e30f;
+    m = sunk ? ragged_sink(p.sink, head, p.inv_c) : -1e30f;
     l = sunk ? 1.0f : 0.f;                                     // the sink's weight at its own reference
     ns = rho_any(-m);
     a = make_float4(0.f, 0.f, 0.f, 0.f);
@@ -479,7 +479,8 @@ __global__ void __launch_bounds__(256) paged_token_merge_kernel(const __grid_con
   auto slot_of = [&](int part) { return plan.slots + (int64_t(blockIdx.x + part) * 2 + (part > 0 ? 0 : 1)) * SLOT; };
   for (int row = threadIdx.x >> 5; row < min(RB, p.G - head.row0); row += 8) {
     const int h = head.h * p.G + head.row0 + row;
-    float m = p.sink != nullptr ? p.sink[h] * p.inv_c : -1e30f, l = p.sink != nullptr ? 1.0f : 0.f;
+    const float sunk = p.sink != nullptr ? ragged_sink(p.sink, h, p.inv_c) : -1e30f;
+    float m = sunk, l = p.sink != nullptr ? 1.0f : 0.f;
     float a[CPL];
 #pragma unroll
     for (int c = 0; c < CPL; ++c) a[c] = 0.f;
@@ -525,7 +526,7 @@ __global__ void __launch_bounds__(256) paged_token_merge_kernel(const __grid_con
         }
       }
     }
-    const float inv = l == 0.f ? 0.f : 1.0f / l;
+    const float inv = sunk != sunk ? sunk : l == 0.f ? 0.f : 1.0f / l;
     __nv_bfloat16* out = static_cast<__nv_bfloat16*>(p.o) + head.s * p.os.t + int64_t(h) * p.os.h + lane * CPL;
 #pragma unroll
     for (int c = 0; c < CPL; c += 2) *reinterpret_cast<uint32_t*>(out + c) = pack_bf16(a[c] * inv, a[c + 1] * inv);

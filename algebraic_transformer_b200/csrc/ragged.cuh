@@ -124,6 +124,13 @@ __device__ __forceinline__ float rho_any(float x) {
   return x >= 0.0f ? T : __fdividef(1.0f, T);
 }
 
+// b / c of a sink.  Past 1e30 either way it takes all of the weight or none, as it does there; an infinite one would meet its own
+// reference as infinity times zero.  NaN stays.
+__device__ __forceinline__ float ragged_sink(const float* sink, int head, float inv_c) {
+  const float b = sink[head] * inv_c;
+  return b > 1e30f ? 1e30f : b < -1e30f ? -1e30f : b;
+}
+
 // |x| up to which weights may go unshifted: rho(x)^n <= 2^64, and x + sqrt(1 + x^2) loses no more than n x^2 2^-23 < 2e-4 of a
 // weight to cancellation
 inline float ragged_fast_range(int n) {

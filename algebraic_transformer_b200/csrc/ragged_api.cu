@@ -25,7 +25,8 @@ bool strides_ok(Strides2* s, const int64_t given[2], int64_t rows, int64_t heads
 int check_link(const char* what, int H, int Hkv, int D, int n, float c) {
   if (D != 64 && D != 128) { set_error("%s: head_dim must be 64 or 128, got %d", what, D); return ALG_ERR_UNSUPPORTED; }
   if (n < 2 || n > 32 || ilog2_exact(n) < 0) { set_error("%s: n must be a power of two in [2, 32], got %d", what, n); return ALG_ERR_INVALID; }
-  if (!(c > 0.0f) || !isfinite(c)) { set_error("%s: scale c must be positive and finite", what); return ALG_ERR_INVALID; }
+  // c^2 D and its reciprocal, times scores within the unshifted range, stay far inside fp32
+  if (!(c >= 0x1p-40f && c <= 0x1p40f)) { set_error("%s: scale c must be positive and finite, within 2^-40 and 2^40", what); return ALG_ERR_INVALID; }
   if (H < 1 || Hkv < 1 || H % Hkv != 0 || H / Hkv > 128) {
     set_error("%s: query heads must be a multiple of the key heads, up to 128 times as many (got %d and %d)", what, H, Hkv);
     return ALG_ERR_INVALID;

@@ -601,7 +601,9 @@ ragged_attn_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_consta
       for (int i = lane; i < p.plan.norm_ctas; i += 32) nk = max3_abs_nan(nk, p.plan.norms[i], 0.f);
 #pragma unroll
       for (int o = 16; o > 0; o >>= 1) nk = max3_abs_nan(nk, __shfl_xor_sync(0xffffffffu, nk, o), 0.f);
-      q_limit = sc.y_fast * sc.y_fast / (1.001f * nk);  // NaN: never smaller
+      // NaN: nothing is below it.  Squares may underflow on one side and overflow on the other: the small term keeps the limit finite, so
+      // that an infinite norm is never below it, and no norm is below a limit of zero
+      q_limit = sc.y_fast * sc.y_fast / (1.001f * nk + 1e-36f);
     }
     Work w;
     bool ok = true;
@@ -616,7 +618,7 @@ ragged_attn_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_consta
       const bool whole_sink = live && p.sink != nullptr && w.k0 == 0;
       bool shifted = false, trusted = false;            // the warp's form; its scores need not be looked at
       if (whole_sink) {
-        const float b = p.sink[head] * p.inv_c;
+        const float b = ragged_sink(p.sink, head, p.inv_c);
         if (!(fabsf(b) <= sc.y_fast * sc.m)) m_run = b;
         l = pow2n_rt(rho_any(b) * (m_run != 0.f ? rho_any(-m_run) : 1.0f) * sc.inv_m, p.log2n);
       }
@@ -636,7 +638,7 @@ ragged_attn_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_consta
         const bool masked = limit0 - j * BKEY < BKEY - 1;                        // uniform over the group
         if (NORMS && j == 0) {
           if (!__all_sync(0xffffffffu, bw.wait(&ctl->q_norm_full[t], uint32_t(items) & 1u))) { ok = false; break; }
-          trusted = ctl->q_norm[t][items & 1] <= q_limit;
+          trusted = ctl->q_norm[t][items & 1] < q_limit;
         }
         if (!shifted && !trusted) {
           const float sum = tile_square_sum(s_taddr);   // by all lanes: the loads are the whole warp's

@@ -535,7 +535,7 @@ __global__ void __launch_bounds__(256) ragged_delta_kernel(const __grid_constant
   float stat[ROWS];                                      // with the rows, not behind their sums
 #pragma unroll
   for (int u = 0; u < ROWS; ++u) stat[u] = sunk && lir == 0 ? __ldg(p.stat + int64_t(h) * p.tokens + min(t0 + u * RPW, p.tokens - 1)) : 0.f;
-  const float bs = sunk ? p.sink[h] * p.inv_c : 0.f, rho_b = rho_any(bs);
+  const float bs = sunk ? ragged_sink(p.sink, h, p.inv_c) : 0.f, rho_b = rho_any(bs);
   const float slope = -p.n_f * p.inv_c * rsqrtf(fmaf(bs, bs, 1.0f));
   float sum = 0.f;
 #pragma unroll

@@ -637,8 +637,8 @@ def _check_lengths(name: str, t: torch.Tensor, count: Optional[int]):
 def _check_link(n: int, c: float):
     if n < 2 or n & (n - 1) or n > 32:
         raise ValueError("asinh kernel needs n to be a power of two in [2, 32]")
-    if not math.isfinite(c) or c <= 0:
-        raise ValueError("asinh scale c must be positive and finite")
+    if not 2.0 ** -40 <= c <= 2.0 ** 40:
+        raise ValueError("asinh scale c must be positive and finite, within 2^-40 and 2^40")
 
 
 def _check_packed(q, k, v):
@@ -654,8 +654,8 @@ def _check_packed(q, k, v):
 def _output_like(q, out):
     if out is None:
         return torch.empty(q.shape, dtype=q.dtype, device=q.device)
-    if out.shape != q.shape or out.dtype != q.dtype:
-        raise ValueError("out must have the shape and type of q")
+    if out.shape != q.shape or out.dtype != q.dtype or out.device != q.device:
+        raise ValueError("out must have the shape, type and device of q")
     return out
 
 
@@ -665,7 +665,8 @@ def packed_attention(q, k, v, cu_seqlens, sink_logit=None, *, n: int = 16, c: fl
     (tokens, Hkv, D) bf16, D = 64 or 128 contiguous, H a multiple of Hkv (query heads share key heads in groups of H / Hkv,
     up to 128).  `cu_seqlens`: int32 (sequences + 1) on the device; sequence s is rows cu_seqlens[s] to cu_seqlens[s + 1] and may
     be empty.  `sink_logit` broadcastable to (H,).  The weights are those of `flash_attention(kind="asinh")`, for any
-    scores (no range guard is needed).  Rows of no sequence: zeros, or, where `out` is given, left as they are.
+    scores (no range guard is needed).  Rows of no sequence: zeros, or, where `out` is given, left as they are;
+    `out` shares no memory with the inputs.
 
     The lengths are read on the device only, so a captured call can be replayed with others; rows beyond the
     tensors are never touched whatever they say.  A NaN or infinite key or value stays within its sequence, where it may also reach
@@ -750,7 +751,7 @@ def _check_pages(q, k_pages, v_pages, block_table, kv_lens, cu_seqlens):
 def paged_attention(q, k_pages, v_pages, block_table, kv_lens, cu_seqlens=None, sink_logit=None, *, n: int = 16, c: float = 8.0,
                     out=None):
     """Causal asinh-power attention of the newest tokens of many sequences against a cache in pages.  q (tokens, H, D) bf16;
-    k_pages, v_pages (pages, page_size, Hkv, D) bf16, page_size a power of two from 16 on; `block_table` int32 (sequences, width): key
+    k_pages, v_pages (pages, page_size, Hkv, D) bf16, page_size a power of two from 16 to 32768; `block_table` int32 (sequences, width): key
     j of sequence s lies in page block_table[s, j // page_size]; `kv_lens` int32 (sequences): the keys of each, the new tokens'
     own among them (`paged_append` writes them).  `cu_seqlens` int32 (sequences + 1): the rows of q of each sequence, a chunk of any
     length; None: one token a sequence, the form for generation.  Token i of a chunk of m sees keys 0 to kv_len - m + i; one
@@ -758,7 +759,7 @@ def paged_attention(q, k_pages, v_pages, block_table, kv_lens, cu_seqlens=None, 
 
     Lengths and table are read on the device only (a captured call can be replayed with others).  Lengths are clamped to the
     table's width, a page number outside the pool reads as zeros, entries behind a length and rows behind a sequence's end are
-    not looked at.  Rows of no sequence: zeros, or, where `out` is given, left as they are."""
+    not looked at.  Rows of no sequence: zeros, or, where `out` is given, left as they are; `out` shares no memory with the inputs."""
     _require_cuda(q, k_pages, v_pages, block_table, kv_lens, cu_seqlens)
     S = _check_pages(q, k_pages, v_pages, block_table, kv_lens, cu_seqlens)
     _check_link(n, c)
@@ -787,9 +788,9 @@ def paged_append(q, k, v, k_pages, v_pages, block_table, kv_lens, cos, sin, cu_s
     `kv_lens` count the new tokens: token j of m stands at position kv_len - m + j.  cos, sin (rows, D / 2) float32 or bf16, a
     row for every position of the table's pages.  fp32 arithmetic, one rounding.  `out` may be q.
 
-    A token of no sequence or with a negative position writes nothing to the cache; its row of q is zero, or, where `out` is given,
-    left as it is.  A page number outside the pool drops the token's key and value.  Pages that are written belong to one
-    sequence: two tokens with one place leave either's key there."""
+    A token of no sequence, with a negative position or with one behind the table's pages writes nothing to the cache; its row of q
+    is zero, or, where `out` is given, left as it is.  A page number outside the pool drops the token's key and value.  Places that
+    are written belong to one token each: where tables give one to two tokens, what is left there is of either."""
     _require_cuda(q, k, v, k_pages, v_pages, block_table, kv_lens, cos, sin, cu_seqlens, q_gain, k_gain)
     _check_packed(q, k, v)
     S = _check_pages(q, k_pages, v_pages, block_table, kv_lens, cu_seqlens)

@@ -261,7 +261,8 @@ ALG_API int alg_attn_decode_status(const alg_decode_args* args, int* status, voi
  * (sequences + 1) device ints; sequence s is rows [cu[s], cu[s+1]) and may be empty.  The host does not read them:
  * values outside the tensors are clamped to them, rows of no sequence are left as they are (zero_tail: rows before
  * the first and behind the last sequence are written as zeros).  Any scores: tiles whose scores leave the range of the
- * unshifted weights take the max-shifted form by themselves.  sink: (H) fp32 or NULL.
+ * unshifted weights take the max-shifted form by themselves.  sink: (H) fp32 or NULL; -inf takes no weight, +inf all.
+ * n: a power of two in [2, 32]; c within 2^-40 and 2^40.  o shares no memory with the inputs.
  * stat, o_rest: both or neither; what alg_packed_attn_bwd takes.  stat: (H, tokens) fp32, the a with p = (rho(x) a)^n;
  * o_rest: (tokens, H, D) dense bf16, what the rounding to o left over (the products then carry 16 bits of the weights).
  * A key or value that is NaN or infinite reaches the queries of its own sequence only; among these it may
@@ -320,7 +321,7 @@ ALG_API int alg_packed_attn_bwd(const alg_packed_attn_bwd_args* args, void* stre
 /* The same over a cache in pages: queries are the last tokens of their sequences, the keys of all of a sequence's tokens (the new
  * ones too) lie in the pool's pages.
  * k_pages, v_pages: (pages, page_size, Hkv, D) bf16, strides of (page, token, head); page_size a power of two from 16
- * on.  block_table: (sequences, table_width) device ints, row stride table_stride: key j of sequence s is in page
+ * to 32768.  block_table: (sequences, table_width) device ints, row stride table_stride: key j of sequence s is in page
  * block_table[s][j / page_size].  A page number outside the pool reads as zeros.  kv_lens: (sequences) device ints, clamped to
  * table_width page_size; entries of the table behind them are not read.  cu_seqlens: (sequences + 1) device ints, the
  * new tokens' rows of q and o, or NULL: one token a sequence (tokens == sequences).  Token i of Lq sees keys [0, kv_len - Lq + i]; a
@@ -353,8 +354,8 @@ ALG_API int alg_paged_attn_fwd(const alg_paged_attn_args* args, void* stream);
  * q, q_out: (tokens, H, D), k, v: (tokens, Hkv, D) bf16, q_out may be q.  Lengths, table and pages as in alg_paged_attn_args; kv_lens
  * count the new tokens.  Token j of the m of a sequence stands at position kv_len - m + j.  cos, sin: (table_rows, D / 2) of
  * table_dtype, dense, table_rows >= table_width page_size.  q_gain, k_gain: (D) fp32 or NULL.  A token of no sequence, or whose
- * position is negative, writes nothing (zero_tail: zeros to its row of q_out); a page number outside the pool drops the
- * token's key and value.  Two tokens with one place (a page in two rows of the table) leave either's key there. */
+ * position is negative or behind the table's pages, writes nothing (zero_tail: zeros to its row of q_out); a page number outside
+ * the pool drops the token's key and value.  A place that tables give to two tokens holds either's key afterwards. */
 typedef struct {
   const void* q;
   const void* k;
