@@ -183,7 +183,7 @@ struct RaggedBwdParams {
   __nv_bfloat16* dv;
   float* dsink;
   float* delta;             // (H, tokens)
-  float* sink_parts;        // (chunks, H)
+  float* sink_parts;        // (blocks, H)
   RaggedBlocks blocks;
   Strides2 qs, ks, vs, os, gs, dqs, dks, dvs;
   int S, tokens, H, Hkv, G, D, log2n, chunks;
@@ -192,6 +192,7 @@ struct RaggedBwdParams {
 };
 size_t ragged_bwd_workspace_bytes(int S, int tokens, int H);
 int launch_ragged_backward(const RaggedBwdParams& p, void* workspace, cudaStream_t stream);
+int ragged_max_blocks(int S, int tokens);
 size_t ragged_blocks_bytes(int S, int tokens);
 void ragged_blocks_carve(RaggedBlocks* blocks, void* workspace, int S, int tokens);
 int launch_ragged_blocks(const RaggedSeqs& seqs, const RaggedBlocks& blocks, cudaStream_t stream);

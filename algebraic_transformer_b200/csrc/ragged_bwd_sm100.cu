@@ -14,8 +14,10 @@
 //     the producer warp zeroes the foreign rows of a streamed tile before the tensor core reads it;
 //   - any scores: 16 columns at a time go the short way, y + sqrt(kappa + y^2), where all their |x| of the warp's rows are within
 //     the range of the forward's unshifted weights, else the cancellation-free one;
-//   - dsink is a float32 sum over all tokens, for which delta from a bf16 output is too coarse: delta takes the forward's output as two
-//     bf16 halves, and partial sums are added in a fixed order.
+//   - delta takes the forward's output as two bf16 halves.  dsink is a float32 sum over all tokens, for which the 16 bits of these, and of
+//     the weights that made them, are still too coarse (2 to 3e-6 of it): the query blocks add up delta_i = sum_j p_ij dP_ij
+//     and l_i = p_sink,i + sum_j p_ij from the weights in fp32, a row's share is p_sink delta / l^2 (l is 1 but for the statistic's last bits),
+//     and blocks' shares are added in a fixed order by the block that arrives last.
 // Measured: see the launcher.
 #include "common.cuh"
 #include "ragged.cuh"
@@ -73,7 +75,8 @@ template <class C> constexpr size_t smem_bytes() { return size_t(C::CTL_OFF) + s
 // multiplies (dP - delta) by, x = scale y, kappa = 1 / scale^2.  `a2`: scale times the statistic, by row (MODE 0: a2[0]) or by
 // column (MODE 1: a2[0..7]).
 //   short:  scale (y + sqrt(kappa + y^2)) = rho(x),  rsqrt(kappa + y^2) = scale / sqrt(1 + x^2)
-template <bool BY_COLUMN, int LOG2N, bool MASK>
+// `pw`: the weights, as bf16 pairs (MODE 1) or, where the sinks' gradients need them, in fp32 (MODE 0).
+template <bool BY_COLUMN, bool SINK, int LOG2N, bool MASK>
 __device__ __forceinline__ void weights16(const uint32_t* s, float2* slope, uint32_t* pw, const float2* a2, float scale, float kappa,
                                           float y_fast, int log2n, int row, int col0, bool live) {
   const float2 kp = make_float2(kappa, kappa);
@@ -120,13 +123,18 @@ __device__ __forceinline__ void weights16(const uint32_t* s, float2* slope, uint
 #pragma unroll
   for (int i = 0; i < 8; ++i) {
     slope[i] = __fmul2_rn(slope[i], t[i]);
-    if (BY_COLUMN) pw[i] = pack_bf16(t[i].x, t[i].y);
+    if (BY_COLUMN) {
+      pw[i] = pack_bf16(t[i].x, t[i].y);
+    } else if (SINK) {
+      pw[2 * i] = __float_as_uint(t[i].x);
+      pw[2 * i + 1] = __float_as_uint(t[i].y);
+    }
   }
 }
 
 // Phase 1 on this thread's 32 scores at tensor-memory address s_t; `vec`: the columns' statistics in shared memory
-// (MODE 1).  MODE 1 leaves the packed weights over the columns read.
-template <int MODE, int LOG2N, bool MASK>
+// (MODE 1).  MODE 1 leaves the packed weights over the columns read, SINK the weights in fp32 over the scores.
+template <int MODE, bool SINK, int LOG2N, bool MASK>
 __device__ __forceinline__ void phase1(uint32_t s_t, float2* slope, const float* vec, float2 a_row, float scale, float kappa, float y_fast,
                                        int log2n, int row, int col0, bool live) {
   uint32_t s0[16], s1[16];
@@ -135,7 +143,7 @@ __device__ __forceinline__ void phase1(uint32_t s_t, float2* slope, const float*
   tmem_ld_32x16(s_t + 16, s1);
 #pragma unroll
   for (int c = 0; c < 2; ++c) {
-    uint32_t pw[8];
+    uint32_t pw[16];
     float2 a2[8];
     if (MODE == 1) {
 #pragma unroll
@@ -148,8 +156,9 @@ __device__ __forceinline__ void phase1(uint32_t s_t, float2* slope, const float*
       a2[0] = a_row;
     }
     if (c == 1) tmem_ld_wait_for16(s1);
-    weights16<MODE == 1, LOG2N, MASK>(c == 0 ? s0 : s1, slope + 8 * c, pw, a2, scale, kappa, y_fast, log2n, row, col0 + c * 16, live);
+    weights16<MODE == 1, SINK, LOG2N, MASK>(c == 0 ? s0 : s1, slope + 8 * c, pw, a2, scale, kappa, y_fast, log2n, row, col0 + c * 16, live);
     if (MODE == 1) tmem_st_32x8(s_t + c * 8, pw);
+    if (SINK) tmem_st_32x16(s_t + c * 16, pw);
   }
 }
 
@@ -343,8 +352,11 @@ __device__ __forceinline__ void bwd_block(unsigned char* smem, Control* ctl, con
       delta_row = make_float2(d, d);
     }
     const uint32_t dp_t = tmem_base + lane_sel + C::DP_COL + group * 32;
-    auto steps = [&](auto power) -> bool {
+    float row_delta = 0.f, row_sum = 0.f;                     // of this thread's columns
+    auto steps = [&](auto power, auto sunk) -> bool {
       constexpr int LOG2N = decltype(power)::value;
+      constexpr bool SINK = MODE == 0 && decltype(sunk)::value;
+      static_assert(!SINK || DB, "the weights stay where the scores were until phase 2 has read them");
       int slot = 0;
       uint32_t ring = 0;                                      // ring position and phase
       for (int j = 0; j < nsteps; ++j) {
@@ -360,9 +372,9 @@ __device__ __forceinline__ void bwd_block(unsigned char* smem, Control* ctl, con
         // the causal mask removes none, some or all of a 32 x 32 block (warp-uniform)
         const int ahead = (MODE == 0) ? col0 - wrow0 : wrow0 - col0;      // > -32: some, >= 32: all
         if (ahead <= -32) {
-          phase1<MODE, LOG2N, false>(s_t, slope, vec, a_row, p.scale, kappa, p.y_fast, p.log2n, row, col0, live);
+          phase1<MODE, SINK, LOG2N, false>(s_t, slope, vec, a_row, p.scale, kappa, p.y_fast, p.log2n, row, col0, live);
         } else if (ahead < 32) {
-          phase1<MODE, LOG2N, true>(s_t, slope, vec, a_row, p.scale, kappa, p.y_fast, p.log2n, row, col0, live);
+          phase1<MODE, SINK, LOG2N, true>(s_t, slope, vec, a_row, p.scale, kappa, p.y_fast, p.log2n, row, col0, live);
         } else {
           uint32_t zero[16];
 #pragma unroll
@@ -376,9 +388,29 @@ __device__ __forceinline__ void bwd_block(unsigned char* smem, Control* ctl, con
         // ---- phase 2: dP -> dS = slope (dP - delta)
         if (!bw.wait(&ctl->dp_full, j & 1u)) return false;
         tc_fence_after();
-        uint32_t d0[16], d1[16];
+        uint32_t d0[16], d1[16], w[16];
+        // sums of sixteen columns at a time: a long row's sum is one of short sums
+        auto add_row = [&](const uint32_t* dp) {
+          float2 ds2 = make_float2(0.f, 0.f), l2 = ds2;
+#pragma unroll
+          for (int i = 0; i < 8; ++i) {
+            const float2 wv = make_float2(__uint_as_float(w[2 * i]), __uint_as_float(w[2 * i + 1]));
+            ds2 = __ffma2_rn(wv, make_float2(__uint_as_float(dp[2 * i]), __uint_as_float(dp[2 * i + 1])), ds2);
+            l2 = __fadd2_rn(l2, wv);
+          }
+          row_delta += ds2.x + ds2.y;
+          row_sum += l2.x + l2.y;
+        };
         tmem_ld_32x16(dp_t, d0);
-        tmem_ld_wait_for16(d0);
+        if (SINK && ahead < 32) {
+          tmem_st_wait();                                     // phase 1's
+          tmem_ld_32x16(s_t, w);
+          tmem_ld_wait_for16(w);
+          tmem_ld_wait_for16(d0);
+          add_row(d0);
+        } else {
+          tmem_ld_wait_for16(d0);
+        }
         tmem_ld_32x16(dp_t + 16, d1);
 #pragma unroll
         for (int c = 0; c < 2; ++c) {
@@ -391,7 +423,14 @@ __device__ __forceinline__ void bwd_block(unsigned char* smem, Control* ctl, con
               nd[2 * i + 1] = make_float2(v.z, v.w);
             }
           }
-          if (c == 1) tmem_ld_wait_for16(d1);
+          if (c == 1) {
+            if (SINK && ahead < 32) {
+              tmem_ld_32x16(s_t + 16, w);
+              tmem_ld_wait_for16(w);
+            }
+            tmem_ld_wait_for16(d1);
+            if (SINK && ahead < 32) add_row(d1);
+          }
           const uint32_t* dp = c == 0 ? d0 : d1;
           uint32_t ds[8];
 #pragma unroll
@@ -410,9 +449,13 @@ __device__ __forceinline__ void bwd_block(unsigned char* smem, Control* ctl, con
       return true;
     };
     using std::integral_constant;
-    const bool ok = p.log2n == 4 ? steps(integral_constant<int, 4>{}) : steps(integral_constant<int, 0>{});
+    const bool sunk = MODE == 0 && p.dsink != nullptr;
+    const bool ok = p.log2n == 4 ? (sunk ? steps(integral_constant<int, 4>{}, std::true_type{}) : steps(integral_constant<int, 4>{}, std::false_type{}))
+                                 : (sunk ? steps(integral_constant<int, 0>{}, std::true_type{}) : steps(integral_constant<int, 0>{}, std::false_type{}));
     if (ok && bw.wait(&ctl->acc_full, 0)) {
       tc_fence_after();
+      if (sunk)                                                // the ring has been read to its end
+        reinterpret_cast<float2*>(smem + C::RING_OFF)[group * BT + r] = live ? make_float2(row_delta, row_sum) : make_float2(0.f, 0.f);
       constexpr int CPT = D / C::NG;                           // accumulator columns per thread
       const int64_t at = int64_t(base) + row;
       __nv_bfloat16* out0 = ((MODE == 0) ? p.dq + at * p.dqs.t + h * p.dqs.h : p.dv + at * p.dvs.t + h * p.dvs.h) + group * CPT;
@@ -443,6 +486,55 @@ __device__ __forceinline__ void bwd_block(unsigned char* smem, Control* ctl, con
   }
 }
 
+// A query block's share of dsink, from the rows' sums that its threads left in shared memory; the block that arrives last adds up all
+// shares, in the order of the blocks in the call.  The power of the sink's weight is taken in 64 bits, of the statistic as the weights had it.
+template <class C>
+__device__ void sink_share(unsigned char* smem, const Control* ctl, const RaggedBwdParams& p, const int4& block, int h, int n) {
+  float* scratch = reinterpret_cast<float*>(smem);             // the resident tiles have been read
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  if (threadIdx.x < BT) {
+    float share = 0.f;
+    if (block.z + int(threadIdx.x) < block.y) {
+      float delta = 0.f, l = 0.f;
+#pragma unroll
+      for (int g = 0; g < C::NG; ++g) {
+        const float2 v = reinterpret_cast<const float2*>(smem + C::RING_OFF)[g * BT + threadIdx.x];
+        delta += v.x;
+        l += v.y;
+      }
+      const double b = ragged_sink(p.sink, h, p.inv_c), root = fabs(b) + sqrt(1.0 + b * b);
+      const float a = p.stat[int64_t(h) * p.tokens + block.x + block.z + threadIdx.x] * p.scale;
+      double w = (b >= 0.0 ? root : 1.0 / root) * (double(a) / double(p.scale));
+      for (int i = 0; i < p.log2n; ++i) w *= w;
+      const float ps = float(w);
+      l += ps;
+      share = l == 0.f ? 0.f : ps * delta / (l * l);
+    }
+    share = warp_sum(share);
+    if (lane == 0) scratch[warp] = share;
+  }
+  __syncthreads();
+  if (threadIdx.x == 0) {
+    const double b = ragged_sink(p.sink, h, p.inv_c);
+    const float all = (scratch[0] + scratch[1]) + (scratch[2] + scratch[3]);
+    p.sink_parts[int64_t(p.blocks.prefix[block.w] + (block.z >> 7)) * p.H + h] =
+        ctl->abort_flag != 0 ? __int_as_float(0x7fc00000) : float(-double(p.n_f) * double(p.inv_c) / sqrt(1.0 + b * b) * double(all));
+    __threadfence();
+    const int64_t last = int64_t(n) * p.H - 1;
+    scratch[4] = atomicAdd(&p.blocks.header->counter, 1) == last ? 1.f : 0.f;
+  }
+  __syncthreads();
+  if (scratch[4] == 0.f) return;
+  __threadfence();
+  for (int head = warp; head < p.H; head += int(blockDim.x >> 5)) {
+    double sum = 0.0;
+    for (int c = lane; c < n; c += 32) sum += double(__ldcg(p.sink_parts + int64_t(c) * p.H + head));
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
+    if (lane == 0) p.dsink[head] = float(sum);
+  }
+}
+
 template <int D, int BS, int CTAS>
 __global__ void __launch_bounds__(Cfg<D, BS, CTAS>::NTHREADS, CTAS)
 ragged_bwd_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant__ CUtensorMap tm_k,
@@ -454,19 +546,12 @@ ragged_bwd_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constan
   Control* ctl = reinterpret_cast<Control*>(smem + C::CTL_OFF);
   const int warp = threadIdx.x >> 5;
   // The lists are in place when the delta kernel has finished; a CTA behind their end has nothing to set up for.  dK/dV blocks, the
-  // dearer kind, come first; the last CTA adds up the sinks' gradients.
+  // dearer kind, come first; the last CTA writes the sinks' gradients where there are no blocks.
   griddep_wait();
   const int n = p.blocks.header->items, kv_ctas = p.blocks.max_items * p.Hkv;
   if (blockIdx.x + 1 == gridDim.x) {
-    if (p.dsink == nullptr) return;
-    const int lane = threadIdx.x & 31, warps = blockDim.x >> 5;
-    for (int h = warp; h < p.H; h += warps) {                  // a warp a head, in an order that does not change
-      double sum = 0.0;
-      for (int c = lane; c < p.chunks; c += 32) sum += double(p.sink_parts[int64_t(c) * p.H + h]);
-#pragma unroll
-      for (int o = 16; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
-      if (lane == 0) p.dsink[h] = float(sum);
-    }
+    if (p.dsink != nullptr && n == 0)
+      for (int h = threadIdx.x; h < p.H; h += blockDim.x) p.dsink[h] = 0.f;
     return;
   }
   const bool keys = int(blockIdx.x) < kv_ctas;
@@ -510,15 +595,14 @@ ragged_bwd_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constan
     tc_fence_after();
     tmem_dealloc(ctl->tmem_base, C::TMEM_COLS);
   }
+  if (!keys && p.dsink != nullptr) sink_share<C>(smem, ctl, p, block, idx % heads, n);
 }
 
-// delta_i = dO_i . (o_i + rest_i), a CTA per head and CHUNK tokens, a row per LPR lanes; the chunk's share of the sink's gradient; zeros to
-// the gradients of rows of no sequence.
+// delta_i = dO_i . (o_i + rest_i), a CTA per head and CHUNK tokens, a row per LPR lanes; zeros to the gradients of rows of no sequence.
 constexpr int CHUNK = 64;
 template <int D>
 __global__ void __launch_bounds__(256) ragged_delta_kernel(const __grid_constant__ RaggedBwdParams p) {
   constexpr int LPR = D / 8, RPW = 32 / LPR, ROWS = CHUNK / 8 / RPW;
-  __shared__ float parts[8];
   griddep_wait();
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, lir = lane % LPR, sub = lane / LPR, h = blockIdx.y;
   const int t0 = blockIdx.x * CHUNK + warp * (CHUNK / 8) + sub;
@@ -531,13 +615,6 @@ __global__ void __launch_bounds__(256) ragged_delta_kernel(const __grid_constant
     o[u] = __ldg(reinterpret_cast<const uint4*>(p.o + t * p.os.t + h * p.os.h + lir * 8));
     r[u] = __ldg(reinterpret_cast<const uint4*>(p.rest + (t * p.H + h) * D + lir * 8));
   }
-  const bool sunk = p.sink != nullptr;
-  float stat[ROWS];                                      // with the rows, not behind their sums
-#pragma unroll
-  for (int u = 0; u < ROWS; ++u) stat[u] = sunk && lir == 0 ? __ldg(p.stat + int64_t(h) * p.tokens + min(t0 + u * RPW, p.tokens - 1)) : 0.f;
-  const float bs = sunk ? ragged_sink(p.sink, h, p.inv_c) : 0.f, rho_b = rho_any(bs);
-  const float slope = -p.n_f * p.inv_c * rsqrtf(fmaf(bs, bs, 1.0f));
-  float sum = 0.f;
 #pragma unroll
   for (int u = 0; u < ROWS; ++u) {
     const __nv_bfloat162 *g2 = reinterpret_cast<const __nv_bfloat162*>(&g[u]), *o2 = reinterpret_cast<const __nv_bfloat162*>(&o[u]),
@@ -561,20 +638,8 @@ __global__ void __launch_bounds__(256) ragged_delta_kernel(const __grid_constant
         *reinterpret_cast<uint4*>(p.dv + t * p.dvs.t + h * p.dvs.h + lir * 8) = zero;
       }
     } else if (lir == 0) {
-      const int64_t at = int64_t(h) * p.tokens + t;
-      p.delta[at] = d;
-      if (sunk) sum = fmaf(d, pow2n_rt(rho_b * stat[u], p.log2n), sum);
+      p.delta[int64_t(h) * p.tokens + t] = d;
     }
-  }
-  if (!sunk) return;
-  sum = warp_sum(sum);
-  if (lane == 0) parts[warp] = sum;
-  __syncthreads();
-  if (threadIdx.x == 0) {
-    float all = 0.f;
-#pragma unroll
-    for (int i = 0; i < 8; ++i) all += parts[i];
-    p.sink_parts[int64_t(blockIdx.x) * p.H + h] = all * slope;
   }
 }
 
@@ -613,8 +678,7 @@ constexpr size_t align256(size_t x) { return (x + 255) & ~size_t(255); }
 
 // delta | sink's partial sums | header | lists | prefix
 size_t ragged_bwd_workspace_bytes(int S, int tokens, int H) {
-  const size_t chunks = (size_t(tokens) + CHUNK - 1) / CHUNK;
-  return align256(size_t(tokens) * H * sizeof(float)) + align256(chunks * H * sizeof(float)) + ragged_blocks_bytes(S, tokens);
+  return align256(size_t(tokens) * H * sizeof(float)) + align256(size_t(ragged_max_blocks(S, tokens)) * H * sizeof(float)) + ragged_blocks_bytes(S, tokens);
 }
 
 int launch_ragged_backward(const RaggedBwdParams& params, void* workspace, cudaStream_t stream) {
@@ -624,7 +688,7 @@ int launch_ragged_backward(const RaggedBwdParams& params, void* workspace, cudaS
   p.delta = reinterpret_cast<float*>(at);
   at += align256(size_t(p.tokens) * p.H * sizeof(float));
   p.sink_parts = reinterpret_cast<float*>(at);
-  at += align256(size_t(p.chunks) * p.H * sizeof(float));
+  at += align256(size_t(ragged_max_blocks(p.S, p.tokens)) * p.H * sizeof(float));
   ragged_blocks_carve(&p.blocks, at, p.S, p.tokens);
   p.y_fast = ragged_fast_range(1 << p.log2n) / p.scale;
   if (int rc = launch_ragged_blocks({p.cu, nullptr, p.S, p.tokens, p.tokens}, p.blocks, stream)) return rc;

@@ -340,15 +340,15 @@ int launch_ragged_plan(const RaggedParams& p, cudaStream_t stream) {
   return ALG_OK;
 }
 
-static int max_blocks(int S, int tokens) { return tokens / 128 + (S < tokens ? S : tokens); }
+int ragged_max_blocks(int S, int tokens) { return tokens / 128 + (S < tokens ? S : tokens); }
 
 size_t ragged_blocks_bytes(int S, int tokens) {
-  return 256 + align256(2 * size_t(max_blocks(S, tokens)) * sizeof(int4)) + align256((size_t(S) + 1) * sizeof(int));
+  return 256 + align256(2 * size_t(ragged_max_blocks(S, tokens)) * sizeof(int4)) + align256((size_t(S) + 1) * sizeof(int));
 }
 
 void ragged_blocks_carve(RaggedBlocks* blocks, void* workspace, int S, int tokens) {
   unsigned char* at = static_cast<unsigned char*>(workspace);
-  blocks->max_items = max_blocks(S, tokens);
+  blocks->max_items = ragged_max_blocks(S, tokens);
   blocks->header = reinterpret_cast<RaggedHeader*>(at);
   at += 256;
   blocks->list = reinterpret_cast<int4*>(at);
