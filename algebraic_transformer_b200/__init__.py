@@ -5,7 +5,7 @@ the entry points and `include/alg_b200.h` for the C ABI underneath."""
 from .ops import (cast_embedding, cayley_powers, cayley_table_geometric, decode_attention,  # noqa: F401
                   flash_attention, flash_attention_backward, flash_clamp, fused_head, fused_head_backward,
                   glu_projection, head_finalize, head_statistic, interleave_gate_up, packed_attention, packed_attention_backward,
-                  paged_append, paged_attention,                  qk_rms_norm,                  qk_rms_norm_backward, qkv_projection, resid_projection, row_sumsq)
+                  paged_append, paged_attention, qk_rms_norm, qk_rms_norm_backward, qkv_projection, resid_projection, row_sumsq)
 from .dist import unit_shard, vocab_shard  # noqa: F401
 
 __all__ = ["flash_attention", "fused_head", "qk_rms_norm", "decode_attention", "cayley_table_geometric",

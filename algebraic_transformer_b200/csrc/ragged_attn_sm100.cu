@@ -21,6 +21,11 @@
 // HILO (training): the weights go to the second product as two bf16 halves and the output is stored as two, since the
 // gradient of the sinks is a float32 sum of what the output's rounding would leave of its digits.
 //
+// Measured, with the plan ahead: 24 prompts of 17 to 2001 tokens, 16 heads on 4 of 64: 92 us; two of 5000 and 8192, 16 on 2 of 128: 427 us,
+// 948 TFLOP/s; 2048 new tokens on two caches of 20000 and 30001 keys, 16 on 4 of 128: 676 us, 903 TFLOP/s.  No pipe is full (MUFU 37 %,
+// FMA 34 %, tensor 20 % in the first): the chain scores -> weights -> P V -> next scores through tensor memory and barriers is what it
+// waits for; with the weights' arithmetic left out it still takes 72 of 92 us, 356 of 427.
+//
 // Every mbarrier wait is bounded; a wait that runs out reports ALG_DEV_TIMEOUT.
 #include "common.cuh"
 #include "launchers.h"

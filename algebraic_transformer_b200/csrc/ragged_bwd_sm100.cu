@@ -18,7 +18,10 @@
 //     the weights that made them, are still too coarse (2 to 3e-6 of it): the query blocks add up delta_i = sum_j p_ij dP_ij
 //     and l_i = p_sink,i + sum_j p_ij from the weights in fp32, a row's share is p_sink delta / l^2 (l is 1 but for the statistic's last bits),
 //     and blocks' shares are added in a fixed order by the block that arrives last.
-// Measured: see the launcher.
+// Bound as the batched backward is: the element-wise phases, a tensor-memory load and an mbarrier between every two products.  Measured
+// with the forward (three sequences of 901 to 4096, 16 heads of 128): 838 us, 510 TFLOP/s of 3.5 times the forward's products, the
+// forward's second half of the weights not counted; of it 5 % are the sinks' sums.  20 sequences of 60 to 1024, 12 heads on 4 of 64: the GPU's
+// part is 140 us, the call's 181 (autograd's host side).
 #include "common.cuh"
 #include "ragged.cuh"
 #include "sm100_ptx.cuh"
