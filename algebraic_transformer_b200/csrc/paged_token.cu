@@ -1,7 +1,7 @@
 // One new token of each sequence against its pages: the generation step's attention.
 //
 // HBM bound: every K and V row is read once for all the G query heads that share it.  The work, all sequences' 64-key units for
-// every key head, is one long line, sequence by sequence; each CTA takes an equal stretch of it, whatever the lengths, so no
+// every key head and one more for what a head's end costs, is one long line, sequence by sequence; each CTA takes an equal stretch of it, whatever the lengths, so no
 // schedule has to be made: a CTA adds up the lengths (S loads over its threads) and finds where its stretch begins.  A stretch
 // covers the end of one (sequence, head), whole ones, and the start of another; states of heads that are not whole go
 // to the workspace and a second kernel merges them, launched ahead so that it only has to wait.  (Merged by the CTA that arrives
@@ -15,8 +15,9 @@
 //            ldmatrix.trans.  Up to 8 rows: both halves in one product, rows 0-7 and 8-15; up to 16: two products.  More
 //            query heads to a key head go as several groups of 16, which read the keys again, from L2.
 // Measured: four sequences of 20000 to 60001 keys, 16 heads on 2 of 128 (170 MB): 37 us, 4.6 TB/s; 64 sequences of 70 to 4001, 24 heads
-// on 8 of 64 (108 MB): 40 us, 2.7 TB/s (38 on another run).  The stream itself goes at 6.1 to 6.3 TB/s; some 8 to 10 us are launch,
-// line, first tile and merge, and at head_dim 64 the 32-key tiles' arithmetic does not quite keep up with the ring.
+// on 8 of 64 (108 MB): 31.4 us, 3.4 TB/s.  The stream itself goes at 5.3 (head_dim 64) to 6.3 TB/s; some 8 us are launch, line, first tile
+// and merge.  A head alone takes 1.7 us in its CTA, the latency of a tile and of the warps' meeting: 1024 sequences of 64 keys, 55 us, are bound
+// by that (asking for the next head's q and page numbers ahead of the meeting did not help).
 // Rows behind a sequence's end (the rest of its last page) may hold anything: scores there are masked, V is zeroed in registers.
 #include "common.cuh"
 #include "ragged.cuh"
@@ -57,6 +58,7 @@ template <int RB> struct __align__(16) Control {
   int64_t start_base;                           // units ahead of the first sequence
   int64_t warp_units[MAX_CWARPS + 1];
   float m[MAX_CWARPS][RB], l[MAX_CWARPS][RB];
+  float sink[RB];                               // the sinks' weights at the unshifted reference, negative: out of its range
 };
 template <int D, int RB> constexpr size_t smem_bytes() {
   return size_t(Cfg<D, RB>::STAGES) * 2 * Cfg<D, RB>::TILE_BYTES + Cfg<D, RB>::SCRATCH + sizeof(Control<RB>) + 1024;
@@ -77,6 +79,9 @@ __device__ __forceinline__ void mma(float* c, const uint32_t* a, uint32_t b0, ui
 }
 
 __device__ __forceinline__ int units_of(int len) { return len > 0 ? (len + UNIT - 1) / UNIT : 1; }
+// A head's place on the line: its units and one for its end, where the warps' states meet.  (Without, the stretches of short sequences
+// were the last to finish: 33.9 against 29.5 us for 64 sequences of 70 to 4001 keys, 24 heads on 8 of 64, no sinks.)
+__device__ __forceinline__ int line_of(int len) { return units_of(len) + 1; }
 
 // A CTA's stretch, head by head.
 struct Walk {
@@ -90,19 +95,23 @@ __device__ __forceinline__ int length_of(const RaggedParams& p, int s) {
   return s < p.seqs.S ? min(max(__ldg(p.seqs.kv_lens + s), 0), p.seqs.kv_capacity) : 0;
 }
 __device__ __forceinline__ bool walk_next(const RaggedParams& p, int heads, Walk& w) {
-  if (w.at >= w.end) return false;
-  if (w.at >= w.base + int64_t(w.units) * heads) {             // every sequence has a unit: one step is enough
-    w.base += int64_t(w.units) * heads;
-    w.len = w.next_len;
-    w.units = units_of(w.len);
-    ++w.s;
-    w.next_len = length_of(p, w.s + 1);
+  for (;;) {
+    if (w.at >= w.end) return false;
+    if (w.at >= w.base + int64_t(w.units + 1) * heads) {       // every sequence has a place: one step is enough
+      w.base += int64_t(w.units + 1) * heads;
+      w.len = w.next_len;
+      w.units = units_of(w.len);
+      ++w.s;
+      w.next_len = length_of(p, w.s + 1);
+    }
+    const int64_t in = w.at - w.base;
+    w.hh = int(in / (w.units + 1));
+    w.u0 = int(in - int64_t(w.hh) * (w.units + 1));
+    if (w.u0 < w.units) break;
+    ++w.at;                                                    // a stretch that begins at a head's end
   }
-  const int64_t in = w.at - w.base;
-  w.hh = int(in / w.units);
-  w.u0 = int(in - int64_t(w.hh) * w.units);
   w.u1 = int(min(int64_t(w.units), w.u0 + (w.end - w.at)));
-  w.at += w.u1 - w.u0;
+  w.at += w.u1 - w.u0 + (w.u1 == w.units ? 1 : 0);
   return true;
 }
 
@@ -173,7 +182,7 @@ paged_token_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_consta
   for (int s = s_first; s < s_last; ++s) {
     const int len = length_of(p, s);
     if (s == s_first) len0 = len;
-    mine += units_of(len);
+    mine += line_of(len);
   }
   int64_t incl = mine;
 #pragma unroll
@@ -196,7 +205,7 @@ paged_token_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_consta
     int64_t base = before * heads;
     int s = s_first, len = len0;
     for (;;) {
-      const int64_t n = int64_t(units_of(len)) * heads;
+      const int64_t n = int64_t(line_of(len)) * heads;
       if (begin < base + n) break;
       base += n;
       len = length_of(p, ++s);
@@ -272,6 +281,11 @@ paged_token_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_consta
             qa[ks][2 + e] = there ? __ldg(src + ks * 8 + 4 + i) : 0u;
           }
         }
+      }
+      float sink = 0.f;                          // of row `lane`, by warp 0: ready when the tiles are
+      if (warp == 0 && p.sink != nullptr && lane < live_rows) {
+        const float b = ragged_sink(p.sink, h * p.G + row0 + lane, p.inv_c);
+        sink = fabsf(b) <= plan.x_fast ? rescale(b, 1.0f, p.log2n) : -1.0f;
       }
       float acc[D / 8][4];                       // RB = 8: rows r of the weights' leading and of their trailing halves
 #pragma unroll
@@ -418,6 +432,7 @@ paged_token_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_consta
         l += __shfl_xor_sync(0xffffffffu, l, 2);
         if (i == 0) { ctl->m[warp][r + 8 * e] = begun ? m_ref[e] : -1e30f; ctl->l[warp][r + 8 * e] = ok ? l : __int_as_float(0x7fc00000); }
       }
+      if (warp == 0 && lane < RB) ctl->sink[lane] = sink;
       if (begun) {
 #pragma unroll
         for (int c = 0; c < D / 8; ++c) {
@@ -438,11 +453,20 @@ paged_token_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_consta
       for (int x = threadIdx.x; x < live_rows * (D / 4); x += C::CONSUMERS) {
         const int row = x / (D / 4), col = x % (D / 4) * 4;
         State st;
-        st.start(p, whole, h * p.G + row0 + row);
-        float most = ctl->m[0][row];
+        bool plain = !whole || ctl->sink[row] >= 0.f;          // everything at the unshifted reference, as a rule: sums
 #pragma unroll
-        for (int wv = 1; wv < CWARPS; ++wv) most = fmaxf(most, ctl->m[wv][row]);
-        st.raise(most, p.log2n);
+        for (int wv = 0; wv < CWARPS; ++wv) plain = plain && (ctl->m[wv][row] == 0.f || !(ctl->m[wv][row] > -1e29f));
+        if (plain) {
+          st.m = 0.f;
+          st.l = whole ? ctl->sink[row] : 0.f;
+          st.a = make_float4(0.f, 0.f, 0.f, 0.f);
+        } else {
+          st.start(p, whole, h * p.G + row0 + row);
+          float most = ctl->m[0][row];
+#pragma unroll
+          for (int wv = 1; wv < CWARPS; ++wv) most = fmaxf(most, ctl->m[wv][row]);
+          st.raise(most, p.log2n);
+        }
 #pragma unroll
         for (int wv = 0; wv < CWARPS; ++wv)
           if (ctl->m[wv][row] > -1e29f)
@@ -456,7 +480,7 @@ paged_token_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_consta
         }
       }
       if (!whole) {
-        const int64_t head_end = w.base + int64_t(w.hh + 1) * w.units;
+        const int64_t head_end = w.base + int64_t(w.hh) * (w.units + 1) + w.units;
         if (kind == 1) open = TokenHead{w.s, h, row0, int((head_end - 1) / per) - int(blockIdx.x) + 1};
       }
     }
@@ -567,7 +591,7 @@ constexpr size_t align256(size_t x) { return (x + 255) & ~size_t(255); }
 int row_block(int G) { return G <= 8 ? 8 : 16; }
 // CTAs: every SM's, but no more than there can be stretches of MIN_UNITS
 int token_grid(int S, int Hkv, int G, int D, int64_t keys) {
-  const int64_t groups = (G + row_block(G) - 1) / row_block(G), units = std::max<int64_t>(1, (keys + UNIT - 1) / UNIT);
+  const int64_t groups = (G + row_block(G) - 1) / row_block(G), units = std::max<int64_t>(1, (keys + UNIT - 1) / UNIT) + 1;
   const int64_t stretches = (int64_t(S) * Hkv * groups * units + MIN_UNITS - 1) / MIN_UNITS;
   return int(std::max<int64_t>(1, std::min<int64_t>(stretches, int64_t(sm_count()) * (D == 64 ? 2 : 1))));
 }
