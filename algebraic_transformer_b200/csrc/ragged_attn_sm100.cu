@@ -337,7 +337,7 @@ ragged_attn_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_consta
 
   if (threadIdx.x == 0) {
     for (int w = 0; w < 2; ++w) {
-      mbar_init(&ctl->q_full[w], 1); mbar_init(&ctl->q_ready[w], 1); mbar_init(&ctl->q_free[w], NORMS ? 2 : 1);
+      mbar_init(&ctl->q_full[w], 1); mbar_init(&ctl->q_ready[w], 1); mbar_init(&ctl->q_free[w], NORMS ? 5 : 1);
       mbar_init(&ctl->s_full[w], 1); mbar_init(&ctl->p_half[w], 4); mbar_init(&ctl->p_full[w], 4);
       mbar_init(&ctl->o_full[w], 1); mbar_init(&ctl->o_free[w], 4);
       mbar_init(&ctl->q_norm_full[w], 1);
@@ -549,7 +549,7 @@ ragged_attn_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_consta
           if (lane == 0) {
             ctl->q_norm[t][(t == 0 ? items0 : k) & 1] = norm;
             mbar_arrive(&ctl->q_norm_full[t]);
-            mbar_arrive(&ctl->q_free[t]);               // with the weight warps' word that the last scores are there
+            mbar_arrive(&ctl->q_free[t]);               // with the weight warps' words that the last scores are there
           }
         }
       }
@@ -637,7 +637,7 @@ ragged_attn_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_consta
             if (j > 0) { mbar_arrive(&ctl->kv_empty[rel.slot]); rel.next(); }    // V_{j-1}
             mbar_arrive(&ctl->kv_empty[rel.slot]); rel.next();                   // K_j
           }
-          if (j == nk - 1) mbar_arrive(&ctl->q_free[t]);
+          if (!NORMS && j == nk - 1) mbar_arrive(&ctl->q_free[t]);
         }
         const int lim = limit - j * BKEY;
         const bool masked = limit0 - j * BKEY < BKEY - 1;                        // uniform over the group
@@ -645,6 +645,9 @@ ragged_attn_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_consta
           if (!__all_sync(0xffffffffu, bw.wait(&ctl->q_norm_full[t], uint32_t(items) & 1u))) { ok = false; break; }
           trusted = ctl->q_norm[t][items & 1] < q_limit;
         }
+        // Every warp's word that the last scores are there and that it has read the norm: with one warp's word alone the next norm, and the one
+        // after, could come while another warp still waits for this one, in an item of one key tile
+        if (NORMS && j == nk - 1 && lane == 0) mbar_arrive(&ctl->q_free[t]);
         if (!shifted && !trusted) {
           const float sum = tile_square_sum(s_taddr);   // by all lanes: the loads are the whole warp's
           if (!__all_sync(0xffffffffu, !live || sum <= sc.y_fast * sc.y_fast)) {
