@@ -42,3 +42,17 @@ def test_many_items_of_one_key_tile(H, Hkv, D):
             first = o
         assert torch.equal(o, first)
     assert torch.equal(A.packed_attention(q, k, v, cu, sink), first)
+
+
+@pytest.mark.parametrize("D", [64, 128])
+def test_what_the_call_before_left_in_rows_that_no_load_writes(D):
+    """Three heads to a key head fill 126 of a tile's 128 rows; the call before filled all of them, with NaN."""
+    q, k, v, sink, cu = make([700, 300], 6, 2, D, seed=3)
+    ref, spread, err = R.packed(q, k, v, cu, sink, 16, 8.0)
+    before = make([256 * 80], 8, 2, D, seed=4)
+    outs = []
+    for value in (0.0, float("nan"), float("inf"), 3e38):
+        A.packed_attention(before[0].fill_(value), *before[1:3], before[4])
+        outs.append(A.packed_attention(q, k, v, cu, sink))
+    R.assert_close(outs[0], ref, spread, err)
+    assert all(torch.equal(o, outs[0]) for o in outs)
