@@ -23,11 +23,20 @@ struct RaggedSeqs {
   int kv_capacity;          // no sequence has more keys than this
 };
 
-// first row and number of the sequence's packed rows, number of its keys
+// the rows that sequences may have, [first, end): from the first offset to the last
+__device__ __forceinline__ void ragged_extent(const int* cu, int S, int tokens, int& first, int& end) {
+  first = min(max(__ldg(cu), 0), tokens);
+  end = min(max(__ldg(cu + S), first), tokens);
+}
+
+// First row and number of the sequence's packed rows, number of its keys.  Offsets that decrease do not lead out of the extent
+// either: its rows' keys are those whose norms are taken, and rows outside it are written by the zero tail.
 __device__ __forceinline__ void ragged_lengths(const RaggedSeqs& q, int s, int& row0, int& Lq, int& Lk) {
   if (q.cu != nullptr) {
-    row0 = min(max(__ldg(q.cu + s), 0), q.tokens);
-    Lq = min(max(__ldg(q.cu + s + 1), row0), q.tokens) - row0;
+    int first, end;
+    ragged_extent(q.cu, q.S, q.tokens, first, end);
+    row0 = min(max(__ldg(q.cu + s), first), end);
+    Lq = min(max(__ldg(q.cu + s + 1), row0), end) - row0;
   } else {
     row0 = s;
     Lq = 1;

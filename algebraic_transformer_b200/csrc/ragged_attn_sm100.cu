@@ -589,8 +589,8 @@ ragged_attn_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_consta
       slot = (slot + 2 * w.n1) % C::NKV;
     }
     if (p.zero_tail) {                                  // rows of no sequence: before the first, behind the last
-      const int S = p.seqs.S;
-      const int first = min(max(__ldg(p.seqs.cu), 0), p.seqs.tokens), end = min(max(__ldg(p.seqs.cu + S), first), p.seqs.tokens);
+      int first, end;
+      ragged_extent(p.seqs.cu, p.seqs.S, p.seqs.tokens, first, end);
       const int none = first + p.seqs.tokens - end;
       for (int64_t i = blockIdx.x; i < int64_t(none) * p.H; i += gridDim.x) {
         const int at = int(i / p.H), h = int(i % p.H), row = at < first ? at : end + at - first;

@@ -609,7 +609,8 @@ __global__ void __launch_bounds__(256) ragged_delta_kernel(const __grid_constant
   griddep_wait();
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, lir = lane % LPR, sub = lane / LPR, h = blockIdx.y;
   const int t0 = blockIdx.x * CHUNK + warp * (CHUNK / 8) + sub;
-  const int first = min(max(__ldg(p.cu), 0), p.tokens), last = min(max(__ldg(p.cu + p.S), first), p.tokens);
+  int first, last;
+  ragged_extent(p.cu, p.S, p.tokens, first, last);
   uint4 g[ROWS], o[ROWS], r[ROWS];
 #pragma unroll
   for (int u = 0; u < ROWS; ++u) {

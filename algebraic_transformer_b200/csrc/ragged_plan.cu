@@ -93,7 +93,9 @@ __device__ __forceinline__ float row_square(const uint4& v) {
 __device__ void take_norms(const RaggedParams& p, float* shared) {
   const RaggedSeqs& q = p.seqs;
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, lpr = p.D / 8, lir = lane & (lpr - 1), sub = lane / lpr, rpw = 32 / lpr;
-  const int first = min(max(__ldg(q.cu), 0), q.tokens), tokens = min(max(__ldg(q.cu + q.S), first), q.tokens) - first;
+  int first, end;
+  ragged_extent(q.cu, q.S, q.tokens, first, end);
+  const int tokens = end - first;
   const __nv_bfloat16* K = static_cast<const __nv_bfloat16*>(p.k) + first * p.ks.t + lir * 8;
   const unsigned rows = unsigned(tokens) * unsigned(p.Hkv), heads = unsigned(p.Hkv);        // below 2^31: ragged_takes_norms
   float most = 0.f;

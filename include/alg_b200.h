@@ -259,8 +259,9 @@ ALG_API int alg_attn_decode_status(const alg_decode_args* args, int* status, voi
  * q, o: (tokens, H, D), k, v: (tokens, Hkv, D) bf16, D contiguous, 64 or 128; strides: elements of (token, head),
  * multiples of 8.  H a multiple of Hkv; query heads [g H/Hkv, (g + 1) H/Hkv) share key head g.  cu_seqlens:
  * (sequences + 1) device ints; sequence s is rows [cu[s], cu[s+1]) and may be empty.  The host does not read them:
- * values outside the tensors are clamped to them, rows of no sequence are left as they are (zero_tail: rows before
- * the first and behind the last sequence are written as zeros).  Any scores: tiles whose scores leave the range of the
+ * values outside the tensors are clamped to them, and to [cu[0], cu[sequences]); where they decrease all the same, a sequence that would
+ * end ahead of its first row is empty, and a row given to two sequences is either's (their shares of dsink are both added).  Rows of
+ * no sequence are left as they are (zero_tail: rows before cu[0] and from cu[sequences] on are written as zeros).  Any scores: tiles whose scores leave the range of the
  * unshifted weights take the max-shifted form by themselves.  sink: (H) fp32 or NULL; -inf takes no weight, +inf all.
  * n: a power of two in [2, 32]; c within 2^-40 and 2^40.  o shares no memory with the inputs.
  * stat, o_rest: both or neither; what alg_packed_attn_bwd takes.  stat: (H, tokens) fp32, the a with p = (rho(x) a)^n;
