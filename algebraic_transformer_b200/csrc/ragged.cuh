@@ -67,12 +67,13 @@ struct __align__(16) RaggedHeader {
   int pad;
 };
 
-// Workspace of a forward call: header | items | combos | prefix of the sequences' blocks | slots.
+// Workspace of a forward call: header | norms | items | combos | prefix of the sequences' blocks | again | slots.
 struct RaggedPlan {
   RaggedHeader* header;
   RaggedItem* items;
   RaggedCombo* combos;
   int* prefix;              // (S + 1)
+  int* again;               // (items, heads): after an (item, head) that a CTA weighs again, the one it found before
   float* slots;             // parts' accumulators, (slot, head, 256 rows, D + 4)
   float* norms;             // per CTA of the plan kernel but the first: largest squared row norm of the keys it saw; nullptr: not taken
   int norm_ctas;

@@ -14,7 +14,10 @@
 //   - any scores: a warp takes a tile unshifted where all its |x| <= x_fast (which keeps the weights within 2^+-64 and the
 //     cancellation of y + sqrt(kappa + y^2) below 2e-4).  For packed keys the largest row norms of the call's keys (ragged_plan.cu) and
 //     of the item's queries settle that as a rule; else the scores are looked at ahead of their weights: a sum of squares, then the largest.  A
-//     score out of range, or a NaN, sends the warp to the max-shifted form with the cancellation-free rho for the rest of the item.
+//     score out of range, or a NaN, sends the warp to the max-shifted form with the cancellation-free rho for the rest of the item;
+//   - values of any size: unshifted weights go up to 2^64 and may take the sum of finite values out of range.  A row that comes out
+//     infinite or NaN with finite weights has its item noted; when the list is done the CTA takes its noted items once more,
+//     max-shifted from the first tile on (weights of 1 at most), and writes the rows again that had come out so.
 //
 // Roles: warp 0 takes the work and runs the TMA loads, warp 1 issues the MMAs, warp 2 scales Q in shared memory and takes its row norms, warp 3 clears the
 // foreign V rows, warps 4..7 and 8..11 weigh query tile 0 and 1, a thread a row.  An item of one tile runs as tile 1.
@@ -35,6 +38,7 @@
 #include <math.h>
 
 #include <algorithm>
+#include <type_traits>
 
 namespace alg {
 namespace {
@@ -67,6 +71,7 @@ struct Work {
   int k0, n0, n1;                 // first key tile; key tiles of query tile 0 (0: it has none in this item) and 1 (< 0: no more work)
   int has0;                       // query tile 0 has tokens
   int slot;                       // < 0: whole
+  int index;                      // its place in the list, times Hkv, plus the head
 };
 
 struct __align__(16) Control {
@@ -75,6 +80,9 @@ struct __align__(16) Control {
   uint64_t q_norm_full[2], v_here, v_clean, work_full[RING], work_empty[RING];
   Work work[RING];
   float q_norm[2][2];             // largest squared row norm of a query tile, of this item and the next one
+  int overflowed[RING];           // a row of the item came out infinite or NaN
+  int taken, noted;               // items that this CTA has taken; those of them that it has looked at for the word above
+  int again;                      // the last item to be weighed again; -1: none
   uint32_t tmem_base;
   int abort_flag;
 };
@@ -318,6 +326,27 @@ template <int D> __device__ __forceinline__ float largest_row_norm(const unsigne
   return most * 1.07f;                                 // (1 - 2^-9)^-16 and the sum of the eight
 }
 
+constexpr float FLT_LARGEST = 0x1.fffffep127f, BF16_INFINITE = 0x1.ffp127f;     // the latter and what is larger round to infinity
+// Is one of the row's D numbers infinite or NaN?
+template <int D> __device__ __forceinline__ bool any_not_finite(const float* row) {
+  float most = 0.f;
+#pragma unroll 1
+  for (int i = 0; i < D; i += 4) {
+    const float4 v = *reinterpret_cast<const float4*>(row + i);
+    most = max3_abs_nan(max3_abs_nan(most, v.x, v.y), v.z, v.w);
+  }
+  return !(most <= FLT_LARGEST);
+}
+template <int D> __device__ __forceinline__ bool any_not_finite(const __nv_bfloat16* row) {
+  bool any = false;
+#pragma unroll 1
+  for (int i = 0; i < D; i += 2) {
+    const uint32_t w = *reinterpret_cast<const uint32_t*>(row + i);
+    any |= (w & 0x7f80u) == 0x7f80u || (w & 0x7f800000u) == 0x7f800000u;
+  }
+  return any;
+}
+
 template <int NKV> struct RingCursor {
   int slot = 0;
   uint32_t phase = 0;
@@ -336,18 +365,23 @@ ragged_attn_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_consta
   Control* ctl = reinterpret_cast<Control*>(smem + C::CTL_OFF);
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
 
-  if (threadIdx.x == 0) {
+  auto init_barriers = [&] {
     for (int w = 0; w < 2; ++w) {
       mbar_init(&ctl->q_full[w], 1); mbar_init(&ctl->q_ready[w], 1); mbar_init(&ctl->q_free[w], NORMS ? 5 : 1);
       mbar_init(&ctl->s_full[w], 1); mbar_init(&ctl->p_half[w], 4); mbar_init(&ctl->p_full[w], 4);
       mbar_init(&ctl->o_full[w], 1); mbar_init(&ctl->o_free[w], 4);
       mbar_init(&ctl->q_norm_full[w], 1);
     }
-    for (int i = 0; i < C::NKV; ++i) { mbar_init(&ctl->kv_full[i], 1); mbar_init(&ctl->kv_empty[i], 1); }
+    for (int i = 0; i < MAX_NKV; ++i) { mbar_init(&ctl->kv_full[i], 1); mbar_init(&ctl->kv_empty[i], 1); }
     for (int i = 0; i < RING; ++i) { mbar_init(&ctl->work_full[i], 1); mbar_init(&ctl->work_empty[i], ITEM_READERS); }
     mbar_init(&ctl->v_here, 1); mbar_init(&ctl->v_clean, 1);
-    ctl->abort_flag = 0;
     fence_barrier_init();
+  };
+  if (threadIdx.x == 0) {
+    init_barriers();
+    ctl->abort_flag = 0;
+    ctl->taken = ctl->noted = 0;
+    ctl->again = -1;
     tma_prefetch_desc(&tm_q); tma_prefetch_desc(&tm_k); tma_prefetch_desc(&tm_v);
   }
   if (warp == 1) {
@@ -381,377 +415,413 @@ ragged_attn_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_consta
     __syncwarp();
     if (lane == 0) mbar_arrive(&ctl->work_empty[k % RING]);
   };
+  // the oldest item that has not been looked at; all roles are done with it
+  auto note = [&] {
+    const int k = ctl->noted++ % RING;
+    if (ctl->overflowed[k] == 0) return;
+    p.plan.again[ctl->work[k].index] = ctl->again;
+    ctl->again = ctl->work[k].index;
+  };
 
-  if (warp == 0) {
-    if (lane == 0) {
-      const int total = p.plan.header->items * p.Hkv;
-      // the next item: the CTA's own number first, then from the counter; shown to the other roles.  It is asked for when the loads of
-      // the item before have been issued, which is as late as can be without a pause, so that longest-first holds to the end
-      auto fetch = [&](int k, Work& w) -> bool {
-        if (k >= RING && !bw.wait(&ctl->work_empty[k % RING], uint32_t(k / RING - 1) & 1u)) return false;
-        const int next = k == 0 ? int(blockIdx.x) : int(gridDim.x) + atomicAdd(&p.plan.header->counter, 1);
-        w.n1 = -1;
-        if (next < total) {
-          const RaggedItem it = p.plan.items[next / p.Hkv];
-          w.head = next % p.Hkv;
-          w.row0 = it.row0; w.Lq = it.Lq; w.Lk = it.Lk; w.seq = it.seq; w.k0 = it.k0; w.slot = it.slot; w.n1 = it.nk;
-          const bool two = it.Lq - it.t0 > TT;
-          w.has0 = two ? 1 : 0;
-          w.tok0 = it.t0;
-          w.tok1 = two ? it.t0 + TT : it.t0;
-          w.n0 = two ? min(max(ragged_tiles(it.Lq, it.Lk, it.t0 + TT) - it.k0, 0), it.nk) : 0;
+  auto run = [&](auto again) {                          // the list; again: the noted items, in a copy of its own that costs the first nothing
+    constexpr bool SECOND = decltype(again)::value;
+    if (warp == 0) {
+      if (lane == 0) {
+        const int total = p.plan.header->items * p.Hkv;
+        // the next item: the CTA's own number first, then from the counter; shown to the other roles.  It is asked for when the loads of
+        // the item before have been issued, which is as late as can be without a pause, so that longest-first holds to the end
+        auto fetch = [&](int k, Work& w) -> bool {
+          if (k >= RING && !bw.wait(&ctl->work_empty[k % RING], uint32_t(k / RING - 1) & 1u)) return false;
+          int next;
+          if (!SECOND) {
+            if (k >= RING) note();
+            next = k == 0 ? int(blockIdx.x) : int(gridDim.x) + atomicAdd(&p.plan.header->counter, 1);
+          } else {
+            next = ctl->again < 0 ? total : ctl->again;
+            if (next < total) ctl->again = p.plan.again[next];
+          }
+          w.n1 = -1;
+          if (next < total) {
+            w.index = next;
+            ctl->overflowed[k % RING] = 0;
+            ++ctl->taken;
+            const RaggedItem it = p.plan.items[next / p.Hkv];
+            w.head = next % p.Hkv;
+            w.row0 = it.row0; w.Lq = it.Lq; w.Lk = it.Lk; w.seq = it.seq; w.k0 = it.k0; w.slot = it.slot; w.n1 = it.nk;
+            const bool two = it.Lq - it.t0 > TT;
+            w.has0 = two ? 1 : 0;
+            w.tok0 = it.t0;
+            w.tok1 = two ? it.t0 + TT : it.t0;
+            w.n0 = two ? min(max(ragged_tiles(it.Lq, it.Lk, it.t0 + TT) - it.k0, 0), it.nk) : 0;
+          }
+          ctl->work[k % RING] = w;
+          mbar_arrive(&ctl->work_full[k % RING]);
+          return w.n1 >= 0;
+        };
+        RingCursor<C::NKV> cur;
+        int items0 = 0;                                   // items in which query tile 0 took part
+        Work w;
+        bool ok = true;
+        for (int k = 0; ok && fetch(k, w); ++k) {
+          auto load_kv = [&](int idx) {                   // K_0, V_0, K_1, V_1, ... of this item
+            const int buf = cur.slot;
+            if (!bw.wait(&ctl->kv_empty[buf], cur.phase ^ 1u)) return false;
+            const CUtensorMap* tm = (idx & 1) ? &tm_v : &tm_k;
+            unsigned char* dst = smem + C::KV_OFF + buf * C::TILE_BYTES;
+            const int key0 = (w.k0 + (idx >> 1)) * BKEY;
+            if (PAGED) {
+              const int rows = min(p.page, BKEY), live = min(BKEY, w.Lk - key0);      // keys of the tile that the sequence has
+              const int loads = live > 0 ? (live + rows - 1) / rows : 0;
+              mbar_arrive_expect_tx(&ctl->kv_full[buf], uint32_t(loads * rows) * (D * 2));
+              const int* pages = p.table + w.seq * p.table_stride;
+              for (int i = 0; i < loads; ++i) {
+                const int key = key0 + i * rows;
+                const int number = __ldg(pages + (key >> p.log2_page));    // outside the pool: the copy fills zeros
+                for (int pn = 0; pn < C::PANELS; ++pn)
+                  tma_load_5d(dst + pn * PANEL_BYTES + i * rows * 128, tm, &ctl->kv_full[buf], 0, key & (p.page - 1), pn, w.head, number);
+              }
+            } else {
+              mbar_arrive_expect_tx(&ctl->kv_full[buf], C::TILE_BYTES);
+              tma_load_4d(dst, tm, &ctl->kv_full[buf], 0, w.row0 + key0, 0, w.head);
+            }
+            cur.next();
+            return true;
+          };
+          auto load_q = [&](int t) {                      // after the previous item's last S_t has read the tile
+            if (t == 0 && w.n0 == 0) return true;
+            const int before = t == 0 ? items0 : k;
+            if (before > 0 && !bw.wait(&ctl->q_free[t], uint32_t(before - 1) & 1u)) return false;
+            mbar_arrive_expect_tx(&ctl->q_full[t], uint32_t(p.G * TT) * (D * 2));
+            for (int pn = 0; pn < C::PANELS; ++pn)
+              tma_load_4d(smem + t * C::TILE_BYTES + pn * PANEL_BYTES, &tm_q, &ctl->q_full[t], 0, w.head * p.G,
+                          w.row0 + (t == 0 ? w.tok0 : w.tok1), pn);
+            return true;
+          };
+          if (k == 0) ok = load_q(0) && load_kv(0) && load_q(1) && load_kv(1);
+          else ok = load_kv(0) && load_q(0) && load_kv(1) && load_q(1);
+          for (int idx = 2; idx < 2 * w.n1 && ok; ++idx) ok = load_kv(idx);
+          if (w.n0 > 0) ++items0;
         }
-        ctl->work[k % RING] = w;
-        mbar_arrive(&ctl->work_full[k % RING]);
-        return w.n1 >= 0;
+      }
+    } else if (warp == 1) {
+      const uint32_t q_addr = smem_u32(smem), kv_addr = smem_u32(smem + C::KV_OFF);
+      using Cur = RingCursor<C::NKV>;
+      Cur cur;
+      int t0 = 0, t1 = 0, items0 = 0, cleans = 0;         // score tiles of query tile 0 / 1 in earlier items; items of tile 0
+      auto wait_all = [&](uint64_t* bar, uint32_t parity) { return __all_sync(0xffffffffu, bw.wait(bar, parity)) != 0; };
+      auto kv_wait = [&](const Cur& c) { return wait_all(&ctl->kv_full[c.slot], c.phase); };
+      const uint32_t q_lo0 = sw128_desc_lo(q_addr, 16), k_lo0 = sw128_desc_lo(kv_addr, 16), v_lo0 = sw128_desc_lo(kv_addr, PANEL_BYTES);
+      auto issue_s = [&](int t, int slot) {               // S_t = Q_t K^T
+        const uint32_t qa = q_lo0 + t * (C::TILE_BYTES >> 4), ka = k_lo0 + slot * (C::TILE_BYTES >> 4);
+#pragma unroll
+        for (int ks = 0; ks < D / 16; ++ks) {
+          const uint32_t off = ((ks >> 2) * PANEL_BYTES + (ks & 3) * 32) >> 4;
+          umma_f16_ss_parts(tmem_base + t * 128, qa + off, SW128_DESC_HI, ka + off, SW128_DESC_HI, C::IDESC_S, ks != 0 ? 1u : 0u);
+        }
       };
-      RingCursor<C::NKV> cur;
-      int items0 = 0;                                   // items in which query tile 0 took part
+      auto issue_pv = [&](int t, int slot, int h64, bool first) {   // O_t += P_t V for the first or second 64 keys
+        const uint32_t va = v_lo0 + slot * (C::TILE_BYTES >> 4);
+#pragma unroll
+        for (int part = 0; part < (HILO ? 2 : 1); ++part)
+#pragma unroll
+          for (int i = 0; i < 4; ++i) {                   // 16 keys = 8 packed columns of P a step
+            const int ks = 4 * h64 + i;
+            umma_f16_ts_parts(tmem_base + O_COL + t * D, tmem_base + t * 128 + (ks >> 1) * 32 + (ks & 1) * 8 + part * 16,
+                              va + ks * (2048 >> 4), SW128_DESC_HI, C::IDESC_PV, (first && ks == 0 && part == 0) ? 0u : 1u);
+          }
+      };
+      // P of query tile t, tile j of nt, then the next scores into its place
+      auto serve = [&](int t, int j, int nt, int before, int items, int v_slot, int k_slot) -> bool {
+        if (!wait_all(&ctl->p_half[t], uint32_t(before + j) & 1u)) return false;
+        if (j == 0 && items > 0 && !wait_all(&ctl->o_free[t], uint32_t(items - 1) & 1u)) return false;   // the last output has been read
+        tc_fence_after();
+        if (elect_one()) issue_pv(t, v_slot, 0, j == 0);
+        __syncwarp();
+        if (!wait_all(&ctl->p_full[t], uint32_t(before + j) & 1u)) return false;
+        tc_fence_after();
+        if (elect_one()) {
+          issue_pv(t, v_slot, 1, false);
+          if (j + 1 < nt) { issue_s(t, k_slot); umma_commit(&ctl->s_full[t]); }    // behind P V: may overwrite P
+          else umma_commit(&ctl->o_full[t]);
+        }
+        __syncwarp();
+        return true;
+      };
       Work w;
       bool ok = true;
-      for (int k = 0; ok && fetch(k, w); ++k) {
-        auto load_kv = [&](int idx) {                   // K_0, V_0, K_1, V_1, ... of this item
-          const int buf = cur.slot;
-          if (!bw.wait(&ctl->kv_empty[buf], cur.phase ^ 1u)) return false;
-          const CUtensorMap* tm = (idx & 1) ? &tm_v : &tm_k;
-          unsigned char* dst = smem + C::KV_OFF + buf * C::TILE_BYTES;
-          const int key0 = (w.k0 + (idx >> 1)) * BKEY;
-          if (PAGED) {
-            const int rows = min(p.page, BKEY), live = min(BKEY, w.Lk - key0);      // keys of the tile that the sequence has
-            const int loads = live > 0 ? (live + rows - 1) / rows : 0;
-            mbar_arrive_expect_tx(&ctl->kv_full[buf], uint32_t(loads * rows) * (D * 2));
-            const int* pages = p.table + w.seq * p.table_stride;
-            for (int i = 0; i < loads; ++i) {
-              const int key = key0 + i * rows;
-              const int number = __ldg(pages + (key >> p.log2_page));    // outside the pool: the copy fills zeros
-              for (int pn = 0; pn < C::PANELS; ++pn)
-                tma_load_5d(dst + pn * PANEL_BYTES + i * rows * 128, tm, &ctl->kv_full[buf], 0, key & (p.page - 1), pn, w.head, number);
-            }
-          } else {
-            mbar_arrive_expect_tx(&ctl->kv_full[buf], C::TILE_BYTES);
-            tma_load_4d(dst, tm, &ctl->kv_full[buf], 0, w.row0 + key0, 0, w.head);
-          }
-          cur.next();
-          return true;
-        };
-        auto load_q = [&](int t) {                      // after the previous item's last S_t has read the tile
-          if (t == 0 && w.n0 == 0) return true;
-          const int before = t == 0 ? items0 : k;
-          if (before > 0 && !bw.wait(&ctl->q_free[t], uint32_t(before - 1) & 1u)) return false;
-          mbar_arrive_expect_tx(&ctl->q_full[t], uint32_t(p.G * TT) * (D * 2));
-          for (int pn = 0; pn < C::PANELS; ++pn)
-            tma_load_4d(smem + t * C::TILE_BYTES + pn * PANEL_BYTES, &tm_q, &ctl->q_full[t], 0, w.head * p.G,
-                        w.row0 + (t == 0 ? w.tok0 : w.tok1), pn);
-          return true;
-        };
-        if (k == 0) ok = load_q(0) && load_kv(0) && load_q(1) && load_kv(1);
-        else ok = load_kv(0) && load_q(0) && load_kv(1) && load_q(1);
-        for (int idx = 2; idx < 2 * w.n1 && ok; ++idx) ok = load_kv(idx);
-        if (w.n0 > 0) ++items0;
-      }
-    }
-  } else if (warp == 1) {
-    const uint32_t q_addr = smem_u32(smem), kv_addr = smem_u32(smem + C::KV_OFF);
-    using Cur = RingCursor<C::NKV>;
-    Cur cur;
-    int t0 = 0, t1 = 0, items0 = 0, cleans = 0;         // score tiles of query tile 0 / 1 in earlier items; items of tile 0
-    auto wait_all = [&](uint64_t* bar, uint32_t parity) { return __all_sync(0xffffffffu, bw.wait(bar, parity)) != 0; };
-    auto kv_wait = [&](const Cur& c) { return wait_all(&ctl->kv_full[c.slot], c.phase); };
-    const uint32_t q_lo0 = sw128_desc_lo(q_addr, 16), k_lo0 = sw128_desc_lo(kv_addr, 16), v_lo0 = sw128_desc_lo(kv_addr, PANEL_BYTES);
-    auto issue_s = [&](int t, int slot) {               // S_t = Q_t K^T
-      const uint32_t qa = q_lo0 + t * (C::TILE_BYTES >> 4), ka = k_lo0 + slot * (C::TILE_BYTES >> 4);
-#pragma unroll
-      for (int ks = 0; ks < D / 16; ++ks) {
-        const uint32_t off = ((ks >> 2) * PANEL_BYTES + (ks & 3) * 32) >> 4;
-        umma_f16_ss_parts(tmem_base + t * 128, qa + off, SW128_DESC_HI, ka + off, SW128_DESC_HI, C::IDESC_S, ks != 0 ? 1u : 0u);
-      }
-    };
-    auto issue_pv = [&](int t, int slot, int h64, bool first) {   // O_t += P_t V for the first or second 64 keys
-      const uint32_t va = v_lo0 + slot * (C::TILE_BYTES >> 4);
-#pragma unroll
-      for (int part = 0; part < (HILO ? 2 : 1); ++part)
-#pragma unroll
-        for (int i = 0; i < 4; ++i) {                   // 16 keys = 8 packed columns of P a step
-          const int ks = 4 * h64 + i;
-          umma_f16_ts_parts(tmem_base + O_COL + t * D, tmem_base + t * 128 + (ks >> 1) * 32 + (ks & 1) * 8 + part * 16,
-                            va + ks * (2048 >> 4), SW128_DESC_HI, C::IDESC_PV, (first && ks == 0 && part == 0) ? 0u : 1u);
-        }
-    };
-    // P of query tile t, tile j of nt, then the next scores into its place
-    auto serve = [&](int t, int j, int nt, int before, int items, int v_slot, int k_slot) -> bool {
-      if (!wait_all(&ctl->p_half[t], uint32_t(before + j) & 1u)) return false;
-      if (j == 0 && items > 0 && !wait_all(&ctl->o_free[t], uint32_t(items - 1) & 1u)) return false;   // the last output has been read
-      tc_fence_after();
-      if (elect_one()) issue_pv(t, v_slot, 0, j == 0);
-      __syncwarp();
-      if (!wait_all(&ctl->p_full[t], uint32_t(before + j) & 1u)) return false;
-      tc_fence_after();
-      if (elect_one()) {
-        issue_pv(t, v_slot, 1, false);
-        if (j + 1 < nt) { issue_s(t, k_slot); umma_commit(&ctl->s_full[t]); }    // behind P V: may overwrite P
-        else umma_commit(&ctl->o_full[t]);
-      }
-      __syncwarp();
-      return true;
-    };
-    Work w;
-    bool ok = true;
-    int k = 0;
-    for (; ok && work_at(k, w); ++k) {
-      work_done(k);
-      const int n0 = w.n0, n1 = w.n1;
-      const bool foreign = (w.k0 + n1) * BKEY > w.Lk;   // the last V tile has rows of no key of this sequence
-      if ((n0 > 0 && !wait_all(&ctl->q_ready[0], uint32_t(items0) & 1u)) || !kv_wait(cur)) { ok = false; break; }
-      tc_fence_after();
-      if (n0 > 0 && elect_one()) { issue_s(0, cur.slot); umma_commit(&ctl->s_full[0]); }
-      __syncwarp();
-      if (!wait_all(&ctl->q_ready[1], uint32_t(k) & 1u)) { ok = false; break; }
-      tc_fence_after();
-      if (elect_one()) { issue_s(1, cur.slot); umma_commit(&ctl->s_full[1]); }
-      __syncwarp();
-      cur.next();
-      for (int j = 0; j < n1 && ok; ++j) {
-        const Cur vc = cur;                             // V_j
-        cur.next();
-        const Cur kc = cur;                             // K_{j+1}
-        if (j + 1 < n1) cur.next();
-        if (!kv_wait(vc) || (j + 1 < n1 && !kv_wait(kc))) { ok = false; break; }
-        if (foreign && j + 1 == n1) {                   // the weights of this step take longer than the clearing
-          if (lane == 0) mbar_arrive(&ctl->v_here);
-          if (!wait_all(&ctl->v_clean, uint32_t(cleans) & 1u)) { ok = false; break; }
-        }
-        if (j < n0 && !serve(0, j, n0, t0, items0, vc.slot, kc.slot)) { ok = false; break; }
-        if (!serve(1, j, n1, t1, k, vc.slot, kc.slot)) { ok = false; break; }
-      }
-      t0 += n0; t1 += n1;
-      if (n0 > 0) ++items0;
-      if (foreign) ++cleans;
-    }
-  } else if (warp == 2) {
-    // Q scaler: multiplies a landed Q tile by 2^e where it lies
-    const __nv_bfloat162 f2 = __float2bfloat162_rn(sc.pow2);
-    Work w;
-    int items0 = 0;
-    bool ok = true;
-    for (int k = 0; ok && work_at(k, w); ++k) {
-      work_done(k);
-      for (int t = 0; t < 2 && ok; ++t) {
-        if (t == 0 && w.n0 == 0) continue;
-        if (!__all_sync(0xffffffffu, bw.wait(&ctl->q_full[t], uint32_t(t == 0 ? items0 : k) & 1u))) { ok = false; break; }
-        if (sc.pow2 != 1.0f) {
-          uint4* tile = reinterpret_cast<uint4*>(smem + t * C::TILE_BYTES);
-#pragma unroll 8
-          for (int i = lane; i < C::TILE_BYTES / 16; i += 32) {
-            uint4 v = tile[i];
-            __nv_bfloat162* h = reinterpret_cast<__nv_bfloat162*>(&v);
-            h[0] = __hmul2(h[0], f2); h[1] = __hmul2(h[1], f2); h[2] = __hmul2(h[2], f2); h[3] = __hmul2(h[3], f2);
-            tile[i] = v;
-          }
-          fence_async_shared();
-        }
+      int k = 0;
+      for (; ok && work_at(k, w); ++k) {
+        work_done(k);
+        const int n0 = w.n0, n1 = w.n1;
+        const bool foreign = (w.k0 + n1) * BKEY > w.Lk;   // the last V tile has rows of no key of this sequence
+        if ((n0 > 0 && !wait_all(&ctl->q_ready[0], uint32_t(items0) & 1u)) || !kv_wait(cur)) { ok = false; break; }
+        tc_fence_after();
+        if (n0 > 0 && elect_one()) { issue_s(0, cur.slot); umma_commit(&ctl->s_full[0]); }
         __syncwarp();
-        if (lane == 0) mbar_arrive(&ctl->q_ready[t]);
+        if (!wait_all(&ctl->q_ready[1], uint32_t(k) & 1u)) { ok = false; break; }
+        tc_fence_after();
+        if (elect_one()) { issue_s(1, cur.slot); umma_commit(&ctl->s_full[1]); }
+        __syncwarp();
+        cur.next();
+        for (int j = 0; j < n1 && ok; ++j) {
+          const Cur vc = cur;                             // V_j
+          cur.next();
+          const Cur kc = cur;                             // K_{j+1}
+          if (j + 1 < n1) cur.next();
+          if (!kv_wait(vc) || (j + 1 < n1 && !kv_wait(kc))) { ok = false; break; }
+          if (foreign && j + 1 == n1) {                   // the weights of this step take longer than the clearing
+            if (lane == 0) mbar_arrive(&ctl->v_here);
+            if (!wait_all(&ctl->v_clean, uint32_t(cleans) & 1u)) { ok = false; break; }
+          }
+          if (j < n0 && !serve(0, j, n0, t0, items0, vc.slot, kc.slot)) { ok = false; break; }
+          if (!serve(1, j, n1, t1, k, vc.slot, kc.slot)) { ok = false; break; }
+        }
+        t0 += n0; t1 += n1;
+        if (n0 > 0) ++items0;
+        if (foreign) ++cleans;
       }
-      if (NORMS) {                                      // beside the first products
+    } else if (warp == 2) {
+      // Q scaler: multiplies a landed Q tile by 2^e where it lies
+      const __nv_bfloat162 f2 = __float2bfloat162_rn(sc.pow2);
+      Work w;
+      int items0 = 0;
+      bool ok = true;
+      for (int k = 0; ok && work_at(k, w); ++k) {
+        work_done(k);
         for (int t = 0; t < 2 && ok; ++t) {
           if (t == 0 && w.n0 == 0) continue;
-          const float norm = largest_row_norm<D>(smem + t * C::TILE_BYTES, lane);
-          if (lane == 0) {
-            ctl->q_norm[t][(t == 0 ? items0 : k) & 1] = norm;
-            mbar_arrive(&ctl->q_norm_full[t]);
-            mbar_arrive(&ctl->q_free[t]);               // with the weight warps' words that the last scores are there
-          }
-        }
-      }
-      if (w.n0 > 0) ++items0;
-    }
-  } else if (warp == 3) {
-    // zeroes the rows of a sequence's last V tile that hold none of its keys
-    Work w;
-    int slot = 0, cleans = 0;                           // ring slot of the item's first tile
-    bool ok = true;
-    for (int k = 0; ok && work_at(k, w); ++k) {
-      work_done(k);
-      const int live = max(w.Lk - (w.k0 + w.n1 - 1) * BKEY, 0);
-      if (live < BKEY) {
-        if (!__all_sync(0xffffffffu, bw.wait(&ctl->v_here, uint32_t(cleans) & 1u))) { ok = false; break; }
-        unsigned char* tile = smem + C::KV_OFF + (slot + 2 * w.n1 - 1) % C::NKV * C::TILE_BYTES;
-        const uint4 zero = make_uint4(0u, 0u, 0u, 0u);
-        for (int pn = 0; pn < C::PANELS; ++pn) {
-          uint4* panel = reinterpret_cast<uint4*>(tile + pn * PANEL_BYTES);
-          for (int i = live * 8 + lane; i < 1024; i += 32) panel[i] = zero;
-        }
-        fence_async_shared();
-        __syncwarp();
-        if (lane == 0) mbar_arrive(&ctl->v_clean);
-        ++cleans;
-      }
-      slot = (slot + 2 * w.n1) % C::NKV;
-    }
-    if (p.zero_tail) {                                  // rows of no sequence: before the first, behind the last
-      int first, end;
-      ragged_extent(p.seqs.cu, p.seqs.S, p.seqs.tokens, first, end);
-      const int none = first + p.seqs.tokens - end;
-      for (int64_t i = blockIdx.x; i < int64_t(none) * p.H; i += gridDim.x) {
-        const int at = int(i / p.H), h = int(i % p.H), row = at < first ? at : end + at - first;
-        if (lane < D / 8)
-          *reinterpret_cast<uint4*>(static_cast<__nv_bfloat16*>(p.o) + row * p.os.t + h * p.os.h + lane * 8) = make_uint4(0u, 0u, 0u, 0u);
-      }
-    }
-  } else {
-    const int t = (warp - FIRST_WEIGHT_WARP) >> 2;      // query tile
-    const int quarter = warp & 3;
-    const int r = quarter * 32 + lane;                  // row of the tile
-    const uint32_t lane_sel = uint32_t(quarter * 32) << 16;
-    const uint32_t s_taddr = tmem_base + lane_sel + t * 128;
-    const uint32_t o_taddr = tmem_base + lane_sel + O_COL + t * D;
-    const int tok_r = r / p.G, g_r = r - tok_r * p.G;   // token and head of this row
-    // the "scores there" barriers of tile 1, served second in every step, tell that V of the step before and K of this one are read
-    const bool releaser = quarter == 0 && lane == 0;
-    RingCursor<C::NKV> rel;
-    int tiles = 0, items = 0;                           // of this group, in earlier items
-    float q_limit = -1.f;                               // queries of smaller squared norm keep every score in the unshifted range
-    if (NORMS && p.plan.norms != nullptr) {
-      float nk = 0.f;
-      for (int i = lane; i < p.plan.norm_ctas; i += 32) nk = max3_abs_nan(nk, p.plan.norms[i], 0.f);
-#pragma unroll
-      for (int o = 16; o > 0; o >>= 1) nk = max3_abs_nan(nk, __shfl_xor_sync(0xffffffffu, nk, o), 0.f);
-      // NaN: nothing is below it.  Squares may underflow on one side and overflow on the other: the small term keeps the limit finite, so
-      // that an infinite norm is never below it, and no norm is below a limit of zero
-      q_limit = sc.y_fast * sc.y_fast / (1.001f * nk + 1e-36f);
-    }
-    Work w;
-    bool ok = true;
-    for (int k = 0; ok && work_at(k, w); ++k) {
-      const int nk = t == 0 ? w.n0 : w.n1;
-      const int tok = (t == 0 ? w.tok0 : w.tok1) + tok_r;
-      const bool live = tok_r < TT && tok < w.Lq && (t == 1 || w.has0 != 0);
-      const int limit = live ? w.Lk - w.Lq + tok - w.k0 * BKEY : -1;             // last visible key, from the item's first on
-      const int limit0 = w.Lk - w.Lq + (t == 0 ? w.tok0 : w.tok1) - w.k0 * BKEY; // of the tile's first row
-      const int head = w.head * p.G + g_r;
-      float l = 0.f, m_run = 0.f;                       // weights are (rho(x) rho(-m_run) / m)^n: unshifted at first
-      const bool whole_sink = live && p.sink != nullptr && w.k0 == 0;
-      bool shifted = false, trusted = false;            // the warp's form; its scores need not be looked at
-      if (whole_sink) {
-        const float b = ragged_sink(p.sink, head, p.inv_c);
-        if (!(fabsf(b) <= sc.y_fast * sc.m)) m_run = b;
-        l = pow2n_rt(rho_any(b) * (m_run != 0.f ? rho_any(-m_run) : 1.0f) * sc.inv_m, p.log2n);
-      }
-      shifted = __any_sync(0xffffffffu, m_run != 0.f);
-      float2 la = make_float2(0.f, 0.f), lb = make_float2(0.f, 0.f);
-      for (int j = 0; j < nk && ok; ++j) {
-        if (!__all_sync(0xffffffffu, bw.wait(&ctl->s_full[t], uint32_t(tiles + j) & 1u))) { ok = false; break; }
-        tc_fence_after();
-        if (releaser) {
-          if (t == 1) {
-            if (j > 0) { mbar_arrive(&ctl->kv_empty[rel.slot]); rel.next(); }    // V_{j-1}
-            mbar_arrive(&ctl->kv_empty[rel.slot]); rel.next();                   // K_j
-          }
-          if (!NORMS && j == nk - 1) mbar_arrive(&ctl->q_free[t]);
-        }
-        const int lim = limit - j * BKEY;
-        const bool masked = limit0 - j * BKEY < BKEY - 1;                        // uniform over the group
-        if (NORMS && j == 0) {
-          if (!__all_sync(0xffffffffu, bw.wait(&ctl->q_norm_full[t], uint32_t(items) & 1u))) { ok = false; break; }
-          trusted = ctl->q_norm[t][items & 1] < q_limit;
-        }
-        // Every warp's word that the last scores are there and that it has read the norm: with one warp's word alone the next norm, and the one
-        // after, could come while another warp still waits for this one, in an item of one key tile
-        if (NORMS && j == nk - 1 && lane == 0) mbar_arrive(&ctl->q_free[t]);
-        if (!shifted && !trusted) {
-          const float sum = tile_square_sum(s_taddr);   // by all lanes: the loads are the whole warp's
-          if (!__all_sync(0xffffffffu, !live || sum <= sc.y_fast * sc.y_fast)) {
-            const float top = tile_abs_max(s_taddr, lim);
-            shifted = __any_sync(0xffffffffu, live && !(top <= sc.y_fast));
-          }
-        }
-        if (!shifted) {
-          weigh_tile<LOG2N, HILO>(s_taddr, &ctl->p_half[t], &ctl->p_full[t], sc.kappa, p.log2n, lim, masked, la, lb);
-        } else {
-          l += (la.x + la.y) + (lb.x + lb.y);
-          la = make_float2(0.f, 0.f); lb = make_float2(0.f, 0.f);
-          // the reference moves to the row's largest score so far; with nothing weighed yet it may also fall
-          const float top = tile_row_max(s_taddr, sc.m, lim);
-          float m_new = m_run;
-          if (lim >= 0 && top > -INFINITY) m_new = l > 0.f ? fmaxf(m_run, top) : top;
-          const float alpha = m_new != m_run ? pow2n_rt(rho_any(m_run) * rho_any(-m_new), p.log2n) : 1.0f;
-          // O of the earlier tiles is at rest (these scores were issued behind their product): rescale it where a reference moved
-          if (__any_sync(0xffffffffu, j > 0 && alpha != 1.0f)) {
-            const float a_row = j > 0 ? alpha : 1.0f;
-#pragma unroll 1
-            for (int c = 0; c < D; c += 32) {
-              uint32_t o[32];
-              tmem_ld_32x32(o_taddr + c, o);
-              tmem_ld_wait_for(o);
-#pragma unroll
-              for (int i = 0; i < 32; ++i) o[i] = __float_as_uint(a_row == 0.f ? 0.f : __uint_as_float(o[i]) * a_row);
-              tmem_st_32x32(o_taddr + c, o);
+          if (!__all_sync(0xffffffffu, bw.wait(&ctl->q_full[t], uint32_t(t == 0 ? items0 : k) & 1u))) { ok = false; break; }
+          if (sc.pow2 != 1.0f) {
+            uint4* tile = reinterpret_cast<uint4*>(smem + t * C::TILE_BYTES);
+#pragma unroll 8
+            for (int i = lane; i < C::TILE_BYTES / 16; i += 32) {
+              uint4 v = tile[i];
+              __nv_bfloat162* h = reinterpret_cast<__nv_bfloat162*>(&v);
+              h[0] = __hmul2(h[0], f2); h[1] = __hmul2(h[1], f2); h[2] = __hmul2(h[2], f2); h[3] = __hmul2(h[3], f2);
+              tile[i] = v;
             }
-            tmem_st_wait();
+            fence_async_shared();
           }
-          if (l > 0.f) l *= alpha;
-          m_run = m_new;
-          weigh_tile_shifted<HILO>(s_taddr, &ctl->p_half[t], &ctl->p_full[t], sc.m, rho_any(-m_run) * sc.inv_m, p.log2n, lim, la, lb);
+          __syncwarp();
+          if (lane == 0) mbar_arrive(&ctl->q_ready[t]);
+        }
+        if (NORMS) {                                      // beside the first products
+          for (int t = 0; t < 2 && ok; ++t) {
+            if (t == 0 && w.n0 == 0) continue;
+            const float norm = largest_row_norm<D>(smem + t * C::TILE_BYTES, lane);
+            if (lane == 0) {
+              ctl->q_norm[t][(t == 0 ? items0 : k) & 1] = norm;
+              mbar_arrive(&ctl->q_norm_full[t]);
+              mbar_arrive(&ctl->q_free[t]);               // with the weight warps' words that the last scores are there
+            }
+          }
+        }
+        if (w.n0 > 0) ++items0;
+      }
+    } else if (warp == 3) {
+      // zeroes the rows of a sequence's last V tile that hold none of its keys
+      Work w;
+      int slot = 0, cleans = 0;                           // ring slot of the item's first tile
+      bool ok = true;
+      for (int k = 0; ok && work_at(k, w); ++k) {
+        work_done(k);
+        const int live = max(w.Lk - (w.k0 + w.n1 - 1) * BKEY, 0);
+        if (live < BKEY) {
+          if (!__all_sync(0xffffffffu, bw.wait(&ctl->v_here, uint32_t(cleans) & 1u))) { ok = false; break; }
+          unsigned char* tile = smem + C::KV_OFF + (slot + 2 * w.n1 - 1) % C::NKV * C::TILE_BYTES;
+          const uint4 zero = make_uint4(0u, 0u, 0u, 0u);
+          for (int pn = 0; pn < C::PANELS; ++pn) {
+            uint4* panel = reinterpret_cast<uint4*>(tile + pn * PANEL_BYTES);
+            for (int i = live * 8 + lane; i < 1024; i += 32) panel[i] = zero;
+          }
+          fence_async_shared();
+          __syncwarp();
+          if (lane == 0) mbar_arrive(&ctl->v_clean);
+          ++cleans;
+        }
+        slot = (slot + 2 * w.n1) % C::NKV;
+      }
+      if (!SECOND && p.zero_tail) {                       // rows of no sequence: before the first, behind the last
+        int first, end;
+        ragged_extent(p.seqs.cu, p.seqs.S, p.seqs.tokens, first, end);
+        const int none = first + p.seqs.tokens - end;
+        for (int64_t i = blockIdx.x; i < int64_t(none) * p.H; i += gridDim.x) {
+          const int at = int(i / p.H), h = int(i % p.H), row = at < first ? at : end + at - first;
+          if (lane < D / 8)
+            *reinterpret_cast<uint4*>(static_cast<__nv_bfloat16*>(p.o) + row * p.os.t + h * p.os.h + lane * 8) = make_uint4(0u, 0u, 0u, 0u);
         }
       }
-      if (!ok) break;
-      tiles += nk;
-      l += (la.x + la.y) + (lb.x + lb.y);
-      const bool partial = w.slot >= 0;
-      float* dst = nullptr;
-      if (partial && (t == 1 || w.has0)) {
-        dst = p.plan.slots + ((int64_t(w.slot) * p.Hkv + w.head) * 256 + t * BQ + r) * (D + 4);
-        *reinterpret_cast<float4*>(dst + D) = make_float4(nk > 0 && live ? l : 0.f, m_run, 0.f, 0.f);
+    } else {
+      const int t = (warp - FIRST_WEIGHT_WARP) >> 2;      // query tile
+      const int quarter = warp & 3;
+      const int r = quarter * 32 + lane;                  // row of the tile
+      const uint32_t lane_sel = uint32_t(quarter * 32) << 16;
+      const uint32_t s_taddr = tmem_base + lane_sel + t * 128;
+      const uint32_t o_taddr = tmem_base + lane_sel + O_COL + t * D;
+      const int tok_r = r / p.G, g_r = r - tok_r * p.G;   // token and head of this row
+      // the "scores there" barriers of tile 1, served second in every step, tell that V of the step before and K of this one are read
+      const bool releaser = quarter == 0 && lane == 0;
+      RingCursor<C::NKV> rel;
+      int tiles = 0, items = 0;                           // of this group, in earlier items
+      float q_limit = -1.f;                               // queries of smaller squared norm keep every score in the unshifted range
+      if (NORMS && p.plan.norms != nullptr) {
+        float nk = 0.f;
+        for (int i = lane; i < p.plan.norm_ctas; i += 32) nk = max3_abs_nan(nk, p.plan.norms[i], 0.f);
+#pragma unroll
+        for (int o = 16; o > 0; o >>= 1) nk = max3_abs_nan(nk, __shfl_xor_sync(0xffffffffu, nk, o), 0.f);
+        // NaN: nothing is below it.  Squares may underflow on one side and overflow on the other: the small term keeps the limit finite, so
+        // that an infinite norm is never below it, and no norm is below a limit of zero
+        q_limit = sc.y_fast * sc.y_fast / (1.001f * nk + 1e-36f);
       }
-      if (nk > 0) {
-        if (!__all_sync(0xffffffffu, bw.wait(&ctl->o_full[t], uint32_t(items) & 1u))) { ok = false; break; }
-        ++items;
-        if (releaser && t == 1) { mbar_arrive(&ctl->kv_empty[rel.slot]); rel.next(); }     // the item's last V tile
-        tc_fence_after();
-        const float inv = l != 0.f ? 1.0f / l : 0.f;    // a row that sees nothing: zero
+      Work w;
+      bool ok = true;
+      for (int k = 0; ok && work_at(k, w); ++k) {
+        const int nk = t == 0 ? w.n0 : w.n1;
+        const int tok = (t == 0 ? w.tok0 : w.tok1) + tok_r;
+        const bool live = tok_r < TT && tok < w.Lq && (t == 1 || w.has0 != 0);
+        const int limit = live ? w.Lk - w.Lq + tok - w.k0 * BKEY : -1;             // last visible key, from the item's first on
+        const int limit0 = w.Lk - w.Lq + (t == 0 ? w.tok0 : w.tok1) - w.k0 * BKEY; // of the tile's first row
+        const int head = w.head * p.G + g_r;
+        float l = 0.f, m_run = 0.f;                       // weights are (rho(x) rho(-m_run) / m)^n: unshifted at first
+        const bool whole_sink = live && p.sink != nullptr && w.k0 == 0;
+        bool shifted = false, trusted = false;            // the warp's form; its scores need not be looked at
+        if (whole_sink) {
+          const float b = ragged_sink(p.sink, head, p.inv_c);
+          if (!(fabsf(b) <= sc.y_fast * sc.m)) m_run = b;
+          l = pow2n_rt(rho_any(b) * (m_run != 0.f ? rho_any(-m_run) : 1.0f) * sc.inv_m, p.log2n);
+        }
+        shifted = SECOND || __any_sync(0xffffffffu, m_run != 0.f);
+        float2 la = make_float2(0.f, 0.f), lb = make_float2(0.f, 0.f);
+        for (int j = 0; j < nk && ok; ++j) {
+          if (!__all_sync(0xffffffffu, bw.wait(&ctl->s_full[t], uint32_t(tiles + j) & 1u))) { ok = false; break; }
+          tc_fence_after();
+          if (releaser) {
+            if (t == 1) {
+              if (j > 0) { mbar_arrive(&ctl->kv_empty[rel.slot]); rel.next(); }    // V_{j-1}
+              mbar_arrive(&ctl->kv_empty[rel.slot]); rel.next();                   // K_j
+            }
+            if (!NORMS && j == nk - 1) mbar_arrive(&ctl->q_free[t]);
+          }
+          const int lim = limit - j * BKEY;
+          const bool masked = limit0 - j * BKEY < BKEY - 1;                        // uniform over the group
+          if (NORMS && j == 0) {
+            if (!__all_sync(0xffffffffu, bw.wait(&ctl->q_norm_full[t], uint32_t(items) & 1u))) { ok = false; break; }
+            trusted = ctl->q_norm[t][items & 1] < q_limit;
+          }
+          // Every warp's word that the last scores are there and that it has read the norm: with one warp's word alone the next norm, and the one
+          // after, could come while another warp still waits for this one, in an item of one key tile
+          if (NORMS && j == nk - 1 && lane == 0) mbar_arrive(&ctl->q_free[t]);
+          if (!SECOND && !shifted && !trusted) {
+            const float sum = tile_square_sum(s_taddr);   // by all lanes: the loads are the whole warp's
+            if (!__all_sync(0xffffffffu, !live || sum <= sc.y_fast * sc.y_fast)) {
+              const float top = tile_abs_max(s_taddr, lim);
+              shifted = __any_sync(0xffffffffu, live && !(top <= sc.y_fast));
+            }
+          }
+          if (!SECOND && !shifted) {
+            weigh_tile<LOG2N, HILO>(s_taddr, &ctl->p_half[t], &ctl->p_full[t], sc.kappa, p.log2n, lim, masked, la, lb);
+          } else {
+            l += (la.x + la.y) + (lb.x + lb.y);
+            la = make_float2(0.f, 0.f); lb = make_float2(0.f, 0.f);
+            // the reference moves to the row's largest score so far; with nothing weighed yet it may also fall
+            const float top = tile_row_max(s_taddr, sc.m, lim);
+            float m_new = m_run;
+            if (lim >= 0 && top > -INFINITY) m_new = l > 0.f ? fmaxf(m_run, top) : top;
+            const float alpha = m_new != m_run ? pow2n_rt(rho_any(m_run) * rho_any(-m_new), p.log2n) : 1.0f;
+            // O of the earlier tiles is at rest (these scores were issued behind their product): rescale it where a reference moved
+            if (__any_sync(0xffffffffu, j > 0 && alpha != 1.0f)) {
+              const float a_row = j > 0 ? alpha : 1.0f;
+#pragma unroll 1
+              for (int c = 0; c < D; c += 32) {
+                uint32_t o[32];
+                tmem_ld_32x32(o_taddr + c, o);
+                tmem_ld_wait_for(o);
+#pragma unroll
+                for (int i = 0; i < 32; ++i) o[i] = __float_as_uint(a_row == 0.f ? 0.f : __uint_as_float(o[i]) * a_row);
+                tmem_st_32x32(o_taddr + c, o);
+              }
+              tmem_st_wait();
+            }
+            if (l > 0.f) l *= alpha;
+            m_run = m_new;
+            weigh_tile_shifted<HILO>(s_taddr, &ctl->p_half[t], &ctl->p_full[t], sc.m, rho_any(-m_run) * sc.inv_m, p.log2n, lim, la, lb);
+          }
+        }
+        if (!ok) break;
+        tiles += nk;
+        l += (la.x + la.y) + (lb.x + lb.y);
+        const bool partial = w.slot >= 0;
+        const float inv = l != 0.f ? 1.0f / l : 0.f;      // a row that sees nothing: zero
         const int64_t row = int64_t(w.row0) + tok;
         __nv_bfloat16* orow = static_cast<__nv_bfloat16*>(p.o) + row * p.os.t + head * p.os.h;
-        __nv_bfloat16* lrow = HILO ? static_cast<__nv_bfloat16*>(p.o_lo) + (row * p.H + head) * D : nullptr;
+        float* dst = nullptr;
+        if (partial && (t == 1 || w.has0)) dst = p.plan.slots + ((int64_t(w.slot) * p.Hkv + w.head) * 256 + t * BQ + r) * (D + 4);
+        bool write = true;                                // in the second pass: what the first one left infinite or NaN
+        if (SECOND) write = live && nk > 0 && (partial ? any_not_finite<D>(dst) : any_not_finite<D>(orow));
+        if (dst != nullptr && write) *reinterpret_cast<float4*>(dst + D) = make_float4(nk > 0 && live ? l : 0.f, m_run, 0.f, 0.f);
+        if (nk > 0) {
+          if (!__all_sync(0xffffffffu, bw.wait(&ctl->o_full[t], uint32_t(items) & 1u))) { ok = false; break; }
+          ++items;
+          if (releaser && t == 1) { mbar_arrive(&ctl->kv_empty[rel.slot]); rel.next(); }     // the item's last V tile
+          tc_fence_after();
+          __nv_bfloat16* lrow = HILO ? static_cast<__nv_bfloat16*>(p.o_lo) + (row * p.H + head) * D : nullptr;
+          float most = 0.f;                               // largest number of the row, as it is written
 #pragma unroll 1
-        for (int c = 0; c < D; c += 32) {
-          uint32_t o[32];
-          tmem_ld_32x32(o_taddr + c, o);
-          tmem_ld_wait_for(o);
-          if (c == D - 32) {                            // O is in registers: the next item may overwrite it
-            warp_arrive(&ctl->o_free[t]);
-          }
-          if (partial) {
+          for (int c = 0; c < D; c += 32) {
+            uint32_t o[32];
+            tmem_ld_32x32(o_taddr + c, o);
+            tmem_ld_wait_for(o);
+            if (c == D - 32) {                            // O is in registers: the next item may overwrite it
+              warp_arrive(&ctl->o_free[t]);
+            }
+            if (!partial) {
 #pragma unroll
-            for (int i = 0; i < 8; ++i)
-              *reinterpret_cast<uint4*>(dst + c + 4 * i) = make_uint4(o[4 * i], o[4 * i + 1], o[4 * i + 2], o[4 * i + 3]);
-            continue;
-          }
-          if (!live) continue;
-          if (l == 0.f) {
+              for (int i = 0; i < 32; ++i) o[i] = l == 0.f ? 0u : __float_as_uint(__uint_as_float(o[i]) * inv);
+            }
 #pragma unroll
-            for (int i = 0; i < 32; ++i) o[i] = 0u;
-          }
-          uint32_t packed[HILO ? 32 : 16];
+            for (int i = 0; i < 32; i += 2) most = max3_abs_nan(most, __uint_as_float(o[i]), __uint_as_float(o[i + 1]));
+            if (!write) continue;
+            if (partial) {
 #pragma unroll
-          for (int i = 0; i < 32; i += 4)
-            pack4<HILO>(make_float2(__uint_as_float(o[i]) * inv, __uint_as_float(o[i + 1]) * inv),
-                        make_float2(__uint_as_float(o[i + 2]) * inv, __uint_as_float(o[i + 3]) * inv), i, packed);
+              for (int i = 0; i < 8; ++i)
+                *reinterpret_cast<uint4*>(dst + c + 4 * i) = make_uint4(o[4 * i], o[4 * i + 1], o[4 * i + 2], o[4 * i + 3]);
+              continue;
+            }
+            if (!live) continue;
+            uint32_t packed[HILO ? 32 : 16];
 #pragma unroll
-          for (int i = 0; i < 4; ++i) {
-            *reinterpret_cast<uint4*>(orow + c + 8 * i) = make_uint4(packed[4 * i], packed[4 * i + 1], packed[4 * i + 2], packed[4 * i + 3]);
-            if (HILO) *reinterpret_cast<uint4*>(lrow + c + 8 * i) = make_uint4(packed[16 + 4 * i], packed[17 + 4 * i], packed[18 + 4 * i], packed[19 + 4 * i]);
+            for (int i = 0; i < 32; i += 4)
+              pack4<HILO>(make_float2(__uint_as_float(o[i]), __uint_as_float(o[i + 1])),
+                          make_float2(__uint_as_float(o[i + 2]), __uint_as_float(o[i + 3])), i, packed);
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+              *reinterpret_cast<uint4*>(orow + c + 8 * i) = make_uint4(packed[4 * i], packed[4 * i + 1], packed[4 * i + 2], packed[4 * i + 3]);
+              if (HILO) *reinterpret_cast<uint4*>(lrow + c + 8 * i) = make_uint4(packed[16 + 4 * i], packed[17 + 4 * i], packed[18 + 4 * i], packed[19 + 4 * i]);
+            }
           }
+          // out of range as it is written (a bf16 is infinite from half a step above its largest number on), and not for a NaN among its weights
+          if (!SECOND && live && l == l && !(partial ? most <= FLT_LARGEST : most < BF16_INFINITE)) ctl->overflowed[k % RING] = 1;
+          // a with p = (rho(x) a)^n: rho(-m_run) (l m^n)^(-1/n)
+          if (!partial && live && write && p.stat != nullptr)
+            p.stat[int64_t(head) * p.seqs.tokens + row] = l > 0.f ? (m_run != 0.f ? rho_any(-m_run) : 1.0f) * sc.inv_m * inv_root_rt(l, p.log2n) : 0.f;
         }
-        // a with p = (rho(x) a)^n: rho(-m_run) (l m^n)^(-1/n)
-        if (!partial && live && p.stat != nullptr)
-          p.stat[int64_t(head) * p.seqs.tokens + row] = l > 0.f ? (m_run != 0.f ? rho_any(-m_run) : 1.0f) * sc.inv_m * inv_root_rt(l, p.log2n) : 0.f;
+        work_done(k);
       }
-      work_done(k);
+    }
+    tc_fence_before();
+    __syncthreads();
+    tc_fence_after();
+  };
+  run(std::false_type{});
+  if (threadIdx.x == 0 && ctl->abort_flag == 0) {
+    while (ctl->noted < ctl->taken) note();
+    if (ctl->again >= 0) {                              // every load, product and arrival of the first pass has been waited for
+      for (uint64_t* bar = ctl->q_full; bar < ctl->work_empty + RING; ++bar) mbar_inval(bar);
+      init_barriers();
     }
   }
+  if (__syncthreads_or(threadIdx.x == 0 && ctl->abort_flag == 0 && ctl->again >= 0)) run(std::true_type{});
 
-  tc_fence_before();
-  __syncthreads();
   if (ctl->abort_flag != 0) {
     if (threadIdx.x == 0) {
       if (p.status != nullptr) atomicExch(p.status, ALG_DEV_TIMEOUT);
@@ -768,7 +838,8 @@ ragged_attn_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_consta
 }
 
 // Adds up the parts of the items that were cut along the keys: a warp a row, a lane D / 32 columns, references and normalisers one a
-// lane, the accumulators of sixteen parts in flight at once.  Parts meet in their order, at the largest of their references.
+// lane, the accumulators of sixteen parts in flight at once.  Parts meet in their order, at the largest of their references, and at 2^-7 of
+// their size: 64 finite ones may add up to more than fp32 holds.
 template <int D>
 __global__ void __launch_bounds__(256) ragged_combine_kernel(const __grid_constant__ RaggedParams p, const ScoreScale sc) {
   griddep_wait();
@@ -819,7 +890,7 @@ __global__ void __launch_bounds__(256) ragged_combine_kernel(const __grid_consta
         }
 #pragma unroll
         for (int j = 0; j < BATCH; ++j) {
-          const float fj = __shfl_sync(0xffffffffu, f, (b0 + j) & 31);
+          const float fj = __shfl_sync(0xffffffffu, f, (b0 + j) & 31) * 0x1p-7f;
           if (b0 + j < n && fj != 0.f) {               // else the accumulator may never have been written
 #pragma unroll
             for (int c = 0; c < CPL; ++c) a[c] = fmaf(fj, v[j][c], a[c]);
@@ -834,7 +905,7 @@ __global__ void __launch_bounds__(256) ragged_combine_kernel(const __grid_consta
     __nv_bfloat16* lrow = p.o_lo != nullptr ? static_cast<__nv_bfloat16*>(p.o_lo) + (at * p.H + head) * D + lane * CPL : nullptr;
 #pragma unroll
     for (int c = 0; c < CPL; c += 2) {
-      const float x = a[c] * inv, y = a[c + 1] * inv;
+      const float x = a[c] * inv * 0x1p7f, y = a[c + 1] * inv * 0x1p7f;
       const uint32_t hi = pack_bf16(x, y);
       *reinterpret_cast<uint32_t*>(orow + c) = hi;
       if (lrow != nullptr) *reinterpret_cast<uint32_t*>(lrow + c) = pack_bf16(x - __uint_as_float(hi << 16), y - __uint_as_float(hi & 0xffff0000u));

@@ -312,7 +312,8 @@ constexpr size_t kNormBytes = 256 * sizeof(float);
 size_t ragged_plan_bytes(int S, int tokens, int Hkv, int G, int D, bool may_split) {
   const Sizes z = plan_sizes(S, tokens, G, Hkv, may_split);
   return 256 + kNormBytes + align256(size_t(z.items) * sizeof(RaggedItem)) + align256(size_t(z.combos) * sizeof(RaggedCombo)) +
-         align256((size_t(S) + 1) * sizeof(int)) + size_t(z.slots) * Hkv * 256 * (D + 4) * sizeof(float);
+         align256((size_t(S) + 1) * sizeof(int)) + align256(size_t(z.items) * Hkv * sizeof(int)) +
+         size_t(z.slots) * Hkv * 256 * (D + 4) * sizeof(float);
 }
 
 void ragged_plan_carve(RaggedPlan* plan, void* workspace, int S, int tokens, int Hkv, int G, int D, bool may_split, bool norms) {
@@ -329,6 +330,8 @@ void ragged_plan_carve(RaggedPlan* plan, void* workspace, int S, int tokens, int
   at += align256(size_t(z.combos) * sizeof(RaggedCombo));
   plan->prefix = reinterpret_cast<int*>(at);
   at += align256((size_t(S) + 1) * sizeof(int));
+  plan->again = reinterpret_cast<int*>(at);
+  at += align256(size_t(z.items) * Hkv * sizeof(int));
   plan->slots = reinterpret_cast<float*>(at);
   plan->max_items = z.items; plan->max_combos = z.combos; plan->max_slots = z.slots;
   plan->block_tokens = 2 * (128 / G);

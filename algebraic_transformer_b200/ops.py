@@ -665,7 +665,7 @@ def packed_attention(q, k, v, cu_seqlens, sink_logit=None, *, n: int = 16, c: fl
     (tokens, Hkv, D) bf16, D = 64 or 128 contiguous, H a multiple of Hkv (query heads share key heads in groups of H / Hkv,
     up to 128).  `cu_seqlens`: int32 (sequences + 1) on the device; sequence s is rows cu_seqlens[s] to cu_seqlens[s + 1] and may
     be empty.  `sink_logit` broadcastable to (H,).  The weights are those of `flash_attention(kind="asinh")`, for any
-    scores (no range guard is needed).  Rows of no sequence: zeros, or, where `out` is given, left as they are;
+    scores and any values whose sum of |v| over a row's keys is a finite float32 (no range guard is needed).  Rows of no sequence: zeros, or, where `out` is given, left as they are;
     `out` shares no memory with the inputs.
 
     The lengths are read on the device only, so a captured call can be replayed with others; rows beyond the

@@ -262,7 +262,8 @@ ALG_API int alg_attn_decode_status(const alg_decode_args* args, int* status, voi
  * values outside the tensors are clamped to them, and to [cu[0], cu[sequences]); where they decrease all the same, a sequence that would
  * end ahead of its first row is empty, and a row given to two sequences is either's (their shares of dsink are both added).  Rows of
  * no sequence are left as they are (zero_tail: rows before cu[0] and from cu[sequences] on are written as zeros).  Any scores: tiles whose scores leave the range of the
- * unshifted weights take the max-shifted form by themselves.  sink: (H) fp32 or NULL; -inf takes no weight, +inf all.
+ * unshifted weights take the max-shifted form by themselves.  Any values: the result is finite as long as the sum of a row's
+ * visible |v| is.  sink: (H) fp32 or NULL; -inf takes no weight, +inf all.
  * n: a power of two in [2, 32]; c within 2^-40 and 2^40.  o shares no memory with the inputs.
  * stat, o_rest: both or neither; what alg_packed_attn_bwd takes.  stat: (H, tokens) fp32, the a with p = (rho(x) a)^n;
  * o_rest: (tokens, H, D) dense bf16, what the rounding to o left over (the products then carry 16 bits of the weights).
