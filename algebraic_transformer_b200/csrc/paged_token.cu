@@ -18,6 +18,9 @@
 // on 8 of 64 (108 MB): 31.4 us, 3.4 TB/s.  The stream itself goes at 5.3 (head_dim 64) to 6.3 TB/s; some 8 us are launch, line, first tile
 // and merge.  A head alone takes 1.7 us in its CTA, the latency of a tile and of the warps' meeting: 1024 sequences of 64 keys, 55 us, are bound
 // by that (asking for the next head's q and page numbers ahead of the meeting did not help).
+// Unshifted weights go up to 2^64, and with them the sum of finite values may leave the range.  Where a row of a CTA's stretch comes out infinite
+// or NaN although its weights are finite, the CTA goes over its stretch once more, max-shifted from the first tile on (weights of 1 at
+// most), and writes the rows again that had come out so.
 // Rows behind a sequence's end (the rest of its last page) may hold anything: scores there are masked, V is zeroed in registers.
 #include "common.cuh"
 #include "ragged.cuh"
@@ -54,7 +57,7 @@ template <int D, int RB> struct Cfg {
 
 template <int RB> struct __align__(16) Control {
   uint64_t full[MAX_STAGES], empty[MAX_STAGES];
-  int abort_flag, start_seq, start_len;
+  int abort_flag, overflowed, start_seq, start_len;
   int64_t start_base;                           // units ahead of the first sequence
   int64_t warp_units[MAX_CWARPS + 1];
   float m[MAX_CWARPS][RB], l[MAX_CWARPS][RB];
@@ -147,11 +150,12 @@ struct State {
     l = fmaf(f, li, l);
     a.x = fmaf(f, v.x, a.x); a.y = fmaf(f, v.y, a.y); a.z = fmaf(f, v.z, a.z); a.w = fmaf(f, v.w, a.w);
   }
-  __device__ __forceinline__ void write(__nv_bfloat16* to) const {
+  __device__ __forceinline__ float4 result() const {
     const float inv = l == 0.f ? 0.f : 1.0f / l;               // a sequence without keys: zero
-    *reinterpret_cast<uint2*>(to) = make_uint2(pack_bf16(a.x * inv, a.y * inv), pack_bf16(a.z * inv, a.w * inv));
+    return make_float4(a.x * inv, a.y * inv, a.z * inv, a.w * inv);
   }
 };
+__device__ __forceinline__ float largest(const float4& v) { return max3_abs_nan(max3_abs_nan(0.f, v.x, v.y), v.z, v.w); }   // NaN if one is
 
 template <int D, int RB, int LOG2N>
 __global__ void __launch_bounds__(Cfg<D, RB>::NTHREADS, Cfg<D, RB>::CTAS)
@@ -166,10 +170,13 @@ paged_token_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_consta
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int heads = plan.heads;                  // key heads times row groups
 
-  if (threadIdx.x == 0) {
+  auto init_barriers = [&] {
     for (int s = 0; s < STAGES; ++s) { mbar_init(&ctl->full[s], 1); mbar_init(&ctl->empty[s], 1); }
-    ctl->abort_flag = 0;
     fence_barrier_init();
+  };
+  if (threadIdx.x == 0) {
+    init_barriers();
+    ctl->abort_flag = ctl->overflowed = 0;
   }
   if (threadIdx.x == C::CONSUMERS) { tma_prefetch_desc(&tm_k); tma_prefetch_desc(&tm_v); }
   griddep_wait();
@@ -220,271 +227,298 @@ paged_token_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_consta
     return;
   }
   const BoundedWait bw{&ctl->abort_flag, 1000000000ull};
-  Walk w;
-  w.at = begin; w.end = min(begin + per, total);
-  w.s = ctl->start_seq; w.len = ctl->start_len; w.base = ctl->start_base;
-  w.units = units_of(w.len);
-  w.next_len = length_of(p, w.s + 1);
-  int tiles = 0;                                 // of the heads before the current one
+  auto run = [&](auto again) {                   // the stretch; again: the second time, in a copy of its own that costs the first nothing
+    constexpr bool SECOND = decltype(again)::value;
+    Walk w;
+    w.at = begin; w.end = min(begin + per, total);
+    w.s = ctl->start_seq; w.len = ctl->start_len; w.base = ctl->start_base;
+    w.units = units_of(w.len);
+    w.next_len = length_of(p, w.s + 1);
+    int tiles = 0;                                 // of the heads before the current one
 
-  if (warp == CWARPS) {                          // producer: the whole warp walks, lane 0 issues, lanes hold page numbers
-    const int rows = min(p.page, TILE), log2_rows = 31 - __clz(rows), pieces = TILE >> log2_rows;
-    bool ok = true;
-    while (ok && walk_next(p, heads, w)) {
-      const int k0 = w.u0 * UNIT, k1 = min(w.len, w.u1 * UNIT), h = w.hh / plan.groups;
-      const int n = k1 > k0 ? (k1 - k0 + TILE - 1) / TILE : 0, chunks = k1 > k0 ? (k1 - k0 + rows - 1) >> log2_rows : 0;
-      const int* pages = p.table + w.s * p.table_stride;
-      auto number_at = [&](int c) { return c < chunks ? __ldg(pages + ((k0 + (c << log2_rows)) >> p.log2_page)) : 0; };
-      int number = number_at(lane), ahead = number_at(32 + lane), held = 0;       // of chunks [held, held + 32) and the next 32
-      for (int t = 0; t < n; ++t, ++tiles) {
-        const int c0 = t * pieces;
-        if (c0 >= held + 32) { held += 32; number = ahead; ahead = number_at(held + 32 + lane); }
-        const int stage = tiles % STAGES;
-        if (!__all_sync(0xffffffffu, bw.wait(&ctl->empty[stage], (uint32_t(tiles / STAGES) & 1u) ^ 1u))) { ok = false; break; }
-        unsigned char* dst = smem + size_t(stage) * 2 * TILE_BYTES;
-        const int live = min(pieces, chunks - c0);
-        if (lane == 0) mbar_arrive_expect_tx(&ctl->full[stage], uint32_t(live * rows) * (D * 2) * 2);
-        __syncwarp();
-        // a lane a copy: of K or V, a panel, a piece of a page
-        const int piece = lane / (2 * C::PANELS), pn = (lane >> 1) % C::PANELS, v = lane & 1;
-        const int page = __shfl_sync(0xffffffffu, number, (c0 + piece - held) & 31);
-        if (piece < live) {
-          const int row = (k0 + ((c0 + piece) << log2_rows)) & (p.page - 1);
-          tma_load_5d(dst + v * TILE_BYTES + pn * PANEL + piece * rows * 128, v ? &tm_v : &tm_k, &ctl->full[stage], 0, row, pn, h, page);
-        }
-        __syncwarp();
-      }
-    }
-  } else {
-    const int r = lane >> 2, i = lane & 3;       // row and column pair of an mma result
-    const uint32_t ring = smem_u32(smem);
-    const uint32_t k_row = uint32_t(lane & 7) * 128, k_chunk = uint32_t(lane >> 3);              // + 8 keys, + 4 chunks
-    const uint32_t v_row = uint32_t(((lane >> 3) & 1) * 8 + (lane & 7)) * 128, v_chunk = uint32_t(lane >> 4);   // + 16 keys, + 2
-    const uint32_t swz = uint32_t(lane & 7);
-    constexpr int NR = RB / 8;                   // rows of this lane: r, and r + 8 where RB = 16
-    const float2 scale2 = make_float2(p.scale, p.scale), one2 = make_float2(1.f, 1.f);
-    bool ok = true, first_segment = true;
-    TokenHead open = {0, 0, 0, 0};               // the head that begins in this stretch and goes on behind it
-    while (walk_next(p, heads, w)) {
-      const int k0 = w.u0 * UNIT, k1 = min(w.len, w.u1 * UNIT), n = k1 > k0 ? (k1 - k0 + TILE - 1) / TILE : 0;
-      const int h = w.hh / plan.groups, row0 = (w.hh % plan.groups) * RB, live_rows = min(RB, p.G - row0);
-      uint32_t qa[D / 16][4];                    // A fragments of q: rows r, r + 8, columns 2 i, 2 i + 1 and 8 further of each 16
-      {
-        const __nv_bfloat16* q = static_cast<const __nv_bfloat16*>(p.q) + w.s * p.qs.t + int64_t(h * p.G + row0) * p.qs.h;
-#pragma unroll
-        for (int e = 0; e < 2; ++e) {
-          const bool there = e < NR && r + 8 * e < live_rows;
-          const uint32_t* src = reinterpret_cast<const uint32_t*>(q + int64_t(there ? r + 8 * e : 0) * p.qs.h);
-#pragma unroll
-          for (int ks = 0; ks < D / 16; ++ks) {
-            qa[ks][e] = there ? __ldg(src + ks * 8 + i) : 0u;
-            qa[ks][2 + e] = there ? __ldg(src + ks * 8 + 4 + i) : 0u;
+    if (warp == CWARPS) {                          // producer: the whole warp walks, lane 0 issues, lanes hold page numbers
+      const int rows = min(p.page, TILE), log2_rows = 31 - __clz(rows), pieces = TILE >> log2_rows;
+      bool ok = true;
+      while (ok && walk_next(p, heads, w)) {
+        const int k0 = w.u0 * UNIT, k1 = min(w.len, w.u1 * UNIT), h = w.hh / plan.groups;
+        const int n = k1 > k0 ? (k1 - k0 + TILE - 1) / TILE : 0, chunks = k1 > k0 ? (k1 - k0 + rows - 1) >> log2_rows : 0;
+        const int* pages = p.table + w.s * p.table_stride;
+        auto number_at = [&](int c) { return c < chunks ? __ldg(pages + ((k0 + (c << log2_rows)) >> p.log2_page)) : 0; };
+        int number = number_at(lane), ahead = number_at(32 + lane), held = 0;       // of chunks [held, held + 32) and the next 32
+        for (int t = 0; t < n; ++t, ++tiles) {
+          const int c0 = t * pieces;
+          if (c0 >= held + 32) { held += 32; number = ahead; ahead = number_at(held + 32 + lane); }
+          const int stage = tiles % STAGES;
+          if (!__all_sync(0xffffffffu, bw.wait(&ctl->empty[stage], (uint32_t(tiles / STAGES) & 1u) ^ 1u))) { ok = false; break; }
+          unsigned char* dst = smem + size_t(stage) * 2 * TILE_BYTES;
+          const int live = min(pieces, chunks - c0);
+          if (lane == 0) mbar_arrive_expect_tx(&ctl->full[stage], uint32_t(live * rows) * (D * 2) * 2);
+          __syncwarp();
+          // a lane a copy: of K or V, a panel, a piece of a page
+          const int piece = lane / (2 * C::PANELS), pn = (lane >> 1) % C::PANELS, v = lane & 1;
+          const int page = __shfl_sync(0xffffffffu, number, (c0 + piece - held) & 31);
+          if (piece < live) {
+            const int row = (k0 + ((c0 + piece) << log2_rows)) & (p.page - 1);
+            tma_load_5d(dst + v * TILE_BYTES + pn * PANEL + piece * rows * 128, v ? &tm_v : &tm_k, &ctl->full[stage], 0, row, pn, h, page);
           }
+          __syncwarp();
         }
       }
-      float sink = 0.f;                          // of row `lane`, by warp 0: ready when the tiles are
-      if (warp == 0 && p.sink != nullptr && lane < live_rows) {
-        const float b = ragged_sink(p.sink, h * p.G + row0 + lane, p.inv_c);
-        sink = fabsf(b) <= plan.x_fast ? rescale(b, 1.0f, p.log2n) : -1.0f;
-      }
-      float acc[D / 8][4];                       // RB = 8: rows r of the weights' leading and of their trailing halves
+    } else {
+      const int r = lane >> 2, i = lane & 3;       // row and column pair of an mma result
+      const uint32_t ring = smem_u32(smem);
+      const uint32_t k_row = uint32_t(lane & 7) * 128, k_chunk = uint32_t(lane >> 3);              // + 8 keys, + 4 chunks
+      const uint32_t v_row = uint32_t(((lane >> 3) & 1) * 8 + (lane & 7)) * 128, v_chunk = uint32_t(lane >> 4);   // + 16 keys, + 2
+      const uint32_t swz = uint32_t(lane & 7);
+      constexpr int NR = RB / 8;                   // rows of this lane: r, and r + 8 where RB = 16
+      const float2 scale2 = make_float2(p.scale, p.scale), one2 = make_float2(1.f, 1.f);
+      bool ok = true, first_segment = true;
+      TokenHead open = {0, 0, 0, 0};               // the head that begins in this stretch and goes on behind it
+      while (walk_next(p, heads, w)) {
+        const int k0 = w.u0 * UNIT, k1 = min(w.len, w.u1 * UNIT), n = k1 > k0 ? (k1 - k0 + TILE - 1) / TILE : 0;
+        const int h = w.hh / plan.groups, row0 = (w.hh % plan.groups) * RB, live_rows = min(RB, p.G - row0);
+        uint32_t qa[D / 16][4];                    // A fragments of q: rows r, r + 8, columns 2 i, 2 i + 1 and 8 further of each 16
+        {
+          const __nv_bfloat16* q = static_cast<const __nv_bfloat16*>(p.q) + w.s * p.qs.t + int64_t(h * p.G + row0) * p.qs.h;
 #pragma unroll
-      for (int c = 0; c < D / 8; ++c) acc[c][0] = acc[c][1] = acc[c][2] = acc[c][3] = 0.f;
-      // weights are (rho(x) rho(-m_ref))^n: unshifted (m_ref = 0) until a score of the warp's rows leaves the range in which that is safe
-      // (|x| <= x_fast keeps them within 2^+-64 and the cancellation of x + sqrt(1 + x^2) below 2e-4), max-shifted from then on
-      float m_ref[NR];
-      float2 l_part[NR];
+          for (int e = 0; e < 2; ++e) {
+            const bool there = e < NR && r + 8 * e < live_rows;
+            const uint32_t* src = reinterpret_cast<const uint32_t*>(q + int64_t(there ? r + 8 * e : 0) * p.qs.h);
 #pragma unroll
-      for (int e = 0; e < NR; ++e) { m_ref[e] = 0.f; l_part[e] = make_float2(0.f, 0.f); }
-      bool shifted = false, begun = false;
-      for (int t = (warp + CWARPS - tiles % CWARPS) % CWARPS; t < n && ok; t += CWARPS) {
-        const int number = tiles + t, stage = number % STAGES;
-        if (!__all_sync(0xffffffffu, bw.wait(&ctl->full[stage], uint32_t(number / STAGES) & 1u))) { ok = false; break; }
-        const uint32_t sk = ring + uint32_t(stage) * (2 * TILE_BYTES), sv = sk + TILE_BYTES;
-        float sc[4][4];
-#pragma unroll
-        for (int b = 0; b < 4; ++b) sc[b][0] = sc[b][1] = sc[b][2] = sc[b][3] = 0.f;
-#pragma unroll
-        for (int kq = 0; kq < D / 32; ++kq) {    // 32 columns of K a load
-#pragma unroll
-          for (int b = 0; b < 4; ++b) {          // eight keys
-            uint32_t kb[4];
-            ldsm4(sk + (kq >> 1) * PANEL + b * 1024 + k_row + (((uint32_t(kq & 1) * 4 + k_chunk) ^ swz) << 4), kb);
-            mma(sc[b], qa[2 * kq], kb[0], kb[1]);
-            mma(sc[b], qa[2 * kq + 1], kb[2], kb[3]);
-          }
-        }
-        const int live = k1 - k0 - t * TILE;     // keys of the tile; columns 8 b + 2 i, + 1 are this lane's
-        const bool tail = live < TILE;
-        auto seen = [&](int b, int j) { return 8 * b + 2 * i + j < live; };
-        float2 wgt[NR][4];
-        float most = 0.f;                        // largest |x| that counts; NaN if there is one
-#pragma unroll
-        for (int e = 0; e < NR; ++e)
-#pragma unroll
-          for (int b = 0; b < 4; ++b) {
-            wgt[e][b] = __fmul2_rn(make_float2(sc[b][2 * e], sc[b][2 * e + 1]), scale2);
-            if (tail) {
-              if (!seen(b, 0)) wgt[e][b].x = 0.f;
-              if (!seen(b, 1)) wgt[e][b].y = 0.f;
+            for (int ks = 0; ks < D / 16; ++ks) {
+              qa[ks][e] = there ? __ldg(src + ks * 8 + i) : 0u;
+              qa[ks][2 + e] = there ? __ldg(src + ks * 8 + 4 + i) : 0u;
             }
-            most = max3_abs_nan(most, wgt[e][b].x, wgt[e][b].y);
           }
-        if (!shifted) shifted = __any_sync(0xffffffffu, !(most <= plan.x_fast));
-        if (!shifted) {
+        }
+        float sink = 0.f;                          // of row `lane`, by warp 0: ready when the tiles are
+        if (warp == 0 && p.sink != nullptr && lane < live_rows) {
+          const float b = ragged_sink(p.sink, h * p.G + row0 + lane, p.inv_c);
+          sink = fabsf(b) <= plan.x_fast ? rescale(b, 1.0f, p.log2n) : -1.0f;
+        }
+        float acc[D / 8][4];                       // RB = 8: rows r of the weights' leading and of their trailing halves
+#pragma unroll
+        for (int c = 0; c < D / 8; ++c) acc[c][0] = acc[c][1] = acc[c][2] = acc[c][3] = 0.f;
+        // weights are (rho(x) rho(-m_ref))^n: unshifted (m_ref = 0) until a score of the warp's rows leaves the range in which that is safe
+        // (|x| <= x_fast keeps them within 2^+-64 and the cancellation of x + sqrt(1 + x^2) below 2e-4), max-shifted from then on
+        float m_ref[NR];
+        float2 l_part[NR];
+#pragma unroll
+        for (int e = 0; e < NR; ++e) { m_ref[e] = 0.f; l_part[e] = make_float2(0.f, 0.f); }
+        bool shifted = SECOND, begun = false;
+        for (int t = (warp + CWARPS - tiles % CWARPS) % CWARPS; t < n && ok; t += CWARPS) {
+          const int number = tiles + t, stage = number % STAGES;
+          if (!__all_sync(0xffffffffu, bw.wait(&ctl->full[stage], uint32_t(number / STAGES) & 1u))) { ok = false; break; }
+          const uint32_t sk = ring + uint32_t(stage) * (2 * TILE_BYTES), sv = sk + TILE_BYTES;
+          float sc[4][4];
+#pragma unroll
+          for (int b = 0; b < 4; ++b) sc[b][0] = sc[b][1] = sc[b][2] = sc[b][3] = 0.f;
+#pragma unroll
+          for (int kq = 0; kq < D / 32; ++kq) {    // 32 columns of K a load
+#pragma unroll
+            for (int b = 0; b < 4; ++b) {          // eight keys
+              uint32_t kb[4];
+              ldsm4(sk + (kq >> 1) * PANEL + b * 1024 + k_row + (((uint32_t(kq & 1) * 4 + k_chunk) ^ swz) << 4), kb);
+              mma(sc[b], qa[2 * kq], kb[0], kb[1]);
+              mma(sc[b], qa[2 * kq + 1], kb[2], kb[3]);
+            }
+          }
+          const int live = k1 - k0 - t * TILE;     // keys of the tile; columns 8 b + 2 i, + 1 are this lane's
+          const bool tail = live < TILE;
+          auto seen = [&](int b, int j) { return 8 * b + 2 * i + j < live; };
+          float2 wgt[NR][4];
+          float most = 0.f;                        // largest |x| that counts; NaN if there is one
 #pragma unroll
           for (int e = 0; e < NR; ++e)
 #pragma unroll
             for (int b = 0; b < 4; ++b) {
-              const float2 x = wgt[e][b], rad = __ffma2_rn(x, x, one2);
-              float2 y = __ffma2_rn(rad, make_float2(rsqrt_approx(rad.x), rsqrt_approx(rad.y)), x);
-              if (LOG2N > 0) {
-#pragma unroll
-                for (int it = 0; it < LOG2N; ++it) y = __fmul2_rn(y, y);
-              } else {
-                for (int it = 0; it < p.log2n; ++it) y = __fmul2_rn(y, y);
-              }
+              wgt[e][b] = __fmul2_rn(make_float2(sc[b][2 * e], sc[b][2 * e + 1]), scale2);
               if (tail) {
-                if (!seen(b, 0)) y.x = 0.f;
-                if (!seen(b, 1)) y.y = 0.f;
+                if (!seen(b, 0)) wgt[e][b].x = 0.f;
+                if (!seen(b, 1)) wgt[e][b].y = 0.f;
               }
-              wgt[e][b] = y;
-              l_part[e] = __fadd2_rn(l_part[e], y);
+              most = max3_abs_nan(most, wgt[e][b].x, wgt[e][b].y);
             }
-        } else {
+          if (!SECOND && !shifted) shifted = __any_sync(0xffffffffu, !(most <= plan.x_fast));
+          if (!SECOND && !shifted) {
 #pragma unroll
-          for (int e = 0; e < NR; ++e) {
-            float top = -INFINITY;
+            for (int e = 0; e < NR; ++e)
 #pragma unroll
-            for (int b = 0; b < 4; ++b) {
-              top = seen(b, 0) ? fmaxf(top, wgt[e][b].x) : top;
-              top = seen(b, 1) ? fmaxf(top, wgt[e][b].y) : top;
-            }
-            top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 1));
-            top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 2));
-            // the first tile's largest score, then the largest so far
-            const float m_new = !(top > -INFINITY) ? m_ref[e] : begun ? fmaxf(m_ref[e], top) : top;
-            const float ns = rho_any(-m_new), alpha = m_new == m_ref[e] ? 1.0f : rescale(m_ref[e], ns, p.log2n);
-            if (begun && __any_sync(0xffffffffu, alpha != 1.0f)) {
-              l_part[e].x *= alpha; l_part[e].y *= alpha;
+              for (int b = 0; b < 4; ++b) {
+                const float2 x = wgt[e][b], rad = __ffma2_rn(x, x, one2);
+                float2 y = __ffma2_rn(rad, make_float2(rsqrt_approx(rad.x), rsqrt_approx(rad.y)), x);
+                if (LOG2N > 0) {
 #pragma unroll
-              for (int c = 0; c < D / 8; ++c) {
-                acc[c][2 * e] *= alpha; acc[c][2 * e + 1] *= alpha;
-                if (RB == 8) { acc[c][2] *= alpha; acc[c][3] *= alpha; }
+                  for (int it = 0; it < LOG2N; ++it) y = __fmul2_rn(y, y);
+                } else {
+                  for (int it = 0; it < p.log2n; ++it) y = __fmul2_rn(y, y);
+                }
+                if (tail) {
+                  if (!seen(b, 0)) y.x = 0.f;
+                  if (!seen(b, 1)) y.y = 0.f;
+                }
+                wgt[e][b] = y;
+                l_part[e] = __fadd2_rn(l_part[e], y);
               }
-            }
-            m_ref[e] = m_new;
-#pragma unroll
-            for (int b = 0; b < 4; ++b) {
-              const float2 x = wgt[e][b];
-              const float2 y = make_float2(seen(b, 0) ? rescale(x.x, ns, p.log2n) : 0.f,
-                                           seen(b, 1) ? rescale(x.y, ns, p.log2n) : 0.f);
-              wgt[e][b] = y;
-              l_part[e] = __fadd2_rn(l_part[e], y);
-            }
-          }
-        }
-        begun = true;
-#pragma unroll
-        for (int ks = 0; ks < 2; ++ks) {         // sixteen keys
-          uint32_t hi[4], lo[4];                 // A fragments: rows r, r + 8 of keys 2 i, 2 i + 1, then of those 8 further
-#pragma unroll
-          for (int g = 0; g < 2; ++g)
+          } else {
 #pragma unroll
             for (int e = 0; e < NR; ++e) {
-              const float2 y = wgt[e][2 * ks + g];
-              const uint32_t lead = pack_bf16(y.x, y.y), rest = pack_bf16(y.x - __uint_as_float(lead << 16), y.y - __uint_as_float(lead & 0xffff0000u));
-              hi[2 * g + e] = lead;
-              if (RB == 8) hi[2 * g + 1] = rest;
-              else lo[2 * g + e] = rest;
-            }
-          auto product = [&](auto tailed) {
-            const int first = ks * 16 + 2 * i;
-            const uint32_t keep0 = (first < live ? 0xffffu : 0u) | (first + 1 < live ? 0xffff0000u : 0u);
-            const uint32_t keep1 = (first + 8 < live ? 0xffffu : 0u) | (first + 9 < live ? 0xffff0000u : 0u);
+              float top = -INFINITY;
 #pragma unroll
-            for (int c = 0; c < D / 8; c += 2) { // sixteen columns of V a load
-              uint32_t vb[4];
-              ldsm4_trans(sv + (c >> 3) * PANEL + ks * 2048 + v_row + (((uint32_t(c & 7) + v_chunk) ^ swz) << 4), vb);
-              if (decltype(tailed)::value) { vb[0] &= keep0; vb[1] &= keep1; vb[2] &= keep0; vb[3] &= keep1; }
-              mma(acc[c], hi, vb[0], vb[1]);
-              mma(acc[c + 1], hi, vb[2], vb[3]);
-              if (RB == 16) {
-                mma(acc[c], lo, vb[0], vb[1]);
-                mma(acc[c + 1], lo, vb[2], vb[3]);
+              for (int b = 0; b < 4; ++b) {
+                top = seen(b, 0) ? fmaxf(top, wgt[e][b].x) : top;
+                top = seen(b, 1) ? fmaxf(top, wgt[e][b].y) : top;
+              }
+              top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 1));
+              top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 2));
+              // the first tile's largest score, then the largest so far
+              const float m_new = !(top > -INFINITY) ? m_ref[e] : begun ? fmaxf(m_ref[e], top) : top;
+              const float ns = rho_any(-m_new), alpha = m_new == m_ref[e] ? 1.0f : rescale(m_ref[e], ns, p.log2n);
+              if (begun && __any_sync(0xffffffffu, alpha != 1.0f)) {
+                l_part[e].x *= alpha; l_part[e].y *= alpha;
+#pragma unroll
+                for (int c = 0; c < D / 8; ++c) {
+                  acc[c][2 * e] *= alpha; acc[c][2 * e + 1] *= alpha;
+                  if (RB == 8) { acc[c][2] *= alpha; acc[c][3] *= alpha; }
+                }
+              }
+              m_ref[e] = m_new;
+#pragma unroll
+              for (int b = 0; b < 4; ++b) {
+                const float2 x = wgt[e][b];
+                const float2 y = make_float2(seen(b, 0) ? rescale(x.x, ns, p.log2n) : 0.f,
+                                             seen(b, 1) ? rescale(x.y, ns, p.log2n) : 0.f);
+                wgt[e][b] = y;
+                l_part[e] = __fadd2_rn(l_part[e], y);
               }
             }
-          };
-          if (tail) product(std::true_type{});
-          else product(std::false_type{});
+          }
+          begun = true;
+#pragma unroll
+          for (int ks = 0; ks < 2; ++ks) {         // sixteen keys
+            uint32_t hi[4], lo[4];                 // A fragments: rows r, r + 8 of keys 2 i, 2 i + 1, then of those 8 further
+#pragma unroll
+            for (int g = 0; g < 2; ++g)
+#pragma unroll
+              for (int e = 0; e < NR; ++e) {
+                const float2 y = wgt[e][2 * ks + g];
+                const uint32_t lead = pack_bf16(y.x, y.y), rest = pack_bf16(y.x - __uint_as_float(lead << 16), y.y - __uint_as_float(lead & 0xffff0000u));
+                hi[2 * g + e] = lead;
+                if (RB == 8) hi[2 * g + 1] = rest;
+                else lo[2 * g + e] = rest;
+              }
+            auto product = [&](auto tailed) {
+              const int first = ks * 16 + 2 * i;
+              const uint32_t keep0 = (first < live ? 0xffffu : 0u) | (first + 1 < live ? 0xffff0000u : 0u);
+              const uint32_t keep1 = (first + 8 < live ? 0xffffu : 0u) | (first + 9 < live ? 0xffff0000u : 0u);
+#pragma unroll
+              for (int c = 0; c < D / 8; c += 2) { // sixteen columns of V a load
+                uint32_t vb[4];
+                ldsm4_trans(sv + (c >> 3) * PANEL + ks * 2048 + v_row + (((uint32_t(c & 7) + v_chunk) ^ swz) << 4), vb);
+                if (decltype(tailed)::value) { vb[0] &= keep0; vb[1] &= keep1; vb[2] &= keep0; vb[3] &= keep1; }
+                mma(acc[c], hi, vb[0], vb[1]);
+                mma(acc[c + 1], hi, vb[2], vb[3]);
+                if (RB == 16) {
+                  mma(acc[c], lo, vb[0], vb[1]);
+                  mma(acc[c + 1], lo, vb[2], vb[3]);
+                }
+              }
+            };
+            if (tail) product(std::true_type{});
+            else product(std::false_type{});
+          }
+          __syncwarp();
+          if (lane == 0) mbar_arrive(&ctl->empty[stage]);
         }
-        __syncwarp();
-        if (lane == 0) mbar_arrive(&ctl->empty[stage]);
-      }
-      tiles += n;
-      // ---- the warps' states together: each leaves its own in shared memory, every thread adds up its columns of a row
-      if (!first_segment) consumer_sync<C::CONSUMERS>();        // the scratch has been read
-      first_segment = false;
+        tiles += n;
+        // ---- the warps' states together: each leaves its own in shared memory, every thread adds up its columns of a row
+        if (!first_segment) consumer_sync<C::CONSUMERS>();        // the scratch has been read
+        first_segment = false;
 #pragma unroll
-      for (int e = 0; e < NR; ++e) {
-        float l = l_part[e].x + l_part[e].y;
-        l += __shfl_xor_sync(0xffffffffu, l, 1);
-        l += __shfl_xor_sync(0xffffffffu, l, 2);
-        if (i == 0) { ctl->m[warp][r + 8 * e] = begun ? m_ref[e] : -1e30f; ctl->l[warp][r + 8 * e] = ok ? l : __int_as_float(0x7fc00000); }
-      }
-      if (warp == 0 && lane < RB) ctl->sink[lane] = sink;
-      if (begun) {
+        for (int e = 0; e < NR; ++e) {
+          float l = l_part[e].x + l_part[e].y;
+          l += __shfl_xor_sync(0xffffffffu, l, 1);
+          l += __shfl_xor_sync(0xffffffffu, l, 2);
+          if (i == 0) { ctl->m[warp][r + 8 * e] = begun ? m_ref[e] : -1e30f; ctl->l[warp][r + 8 * e] = ok ? l : __int_as_float(0x7fc00000); }
+        }
+        if (warp == 0 && lane < RB) ctl->sink[lane] = sink;
+        if (begun) {
 #pragma unroll
-        for (int c = 0; c < D / 8; ++c) {
-          float* to = scratch + (warp * RB + r) * C::ROW + c * 8 + 2 * i;
-          if (RB == 8) {                         // an infinite V meets a zero trailing half as NaN: the leading half has the answer then
-            const float a = isinf(acc[c][0]) ? acc[c][0] : acc[c][0] + acc[c][2], b = isinf(acc[c][1]) ? acc[c][1] : acc[c][1] + acc[c][3];
-            *reinterpret_cast<float2*>(to) = make_float2(a, b);
-          } else {
-            *reinterpret_cast<float2*>(to) = make_float2(acc[c][0], acc[c][1]);
-            *reinterpret_cast<float2*>(to + 8 * C::ROW) = make_float2(acc[c][2], acc[c][3]);
+          for (int c = 0; c < D / 8; ++c) {
+            float* to = scratch + (warp * RB + r) * C::ROW + c * 8 + 2 * i;
+            if (RB == 8) {                         // an infinite V meets a zero trailing half as NaN: the leading half has the answer then
+              const float a = isinf(acc[c][0]) ? acc[c][0] : acc[c][0] + acc[c][2], b = isinf(acc[c][1]) ? acc[c][1] : acc[c][1] + acc[c][3];
+              *reinterpret_cast<float2*>(to) = make_float2(a, b);
+            } else {
+              *reinterpret_cast<float2*>(to) = make_float2(acc[c][0], acc[c][1]);
+              *reinterpret_cast<float2*>(to + 8 * C::ROW) = make_float2(acc[c][2], acc[c][3]);
+            }
           }
         }
-      }
-      consumer_sync<C::CONSUMERS>();
-      const bool whole = w.u0 == 0 && w.u1 == w.units;
-      const int kind = w.u0 > 0 ? 0 : 1;
-      float* slot = plan.slots + (int64_t(blockIdx.x) * 2 + kind) * (RB * (D + 2));
-      for (int x = threadIdx.x; x < live_rows * (D / 4); x += C::CONSUMERS) {
-        const int row = x / (D / 4), col = x % (D / 4) * 4;
-        State st;
-        bool plain = !whole || ctl->sink[row] >= 0.f;          // everything at the unshifted reference, as a rule: sums
+        consumer_sync<C::CONSUMERS>();
+        const bool whole = w.u0 == 0 && w.u1 == w.units;
+        const int kind = w.u0 > 0 ? 0 : 1;
+        float* slot = plan.slots + (int64_t(blockIdx.x) * 2 + kind) * (RB * (D + 2));
+        for (int x = threadIdx.x; x < live_rows * (D / 4); x += C::CONSUMERS) {
+          const int row = x / (D / 4), col = x % (D / 4) * 4;
+          State st;
+          bool plain = !whole || ctl->sink[row] >= 0.f;          // everything at the unshifted reference, as a rule: sums
 #pragma unroll
-        for (int wv = 0; wv < CWARPS; ++wv) plain = plain && (ctl->m[wv][row] == 0.f || !(ctl->m[wv][row] > -1e29f));
-        if (plain) {
-          st.m = 0.f;
-          st.l = whole ? ctl->sink[row] : 0.f;
-          st.a = make_float4(0.f, 0.f, 0.f, 0.f);
-        } else {
-          st.start(p, whole, h * p.G + row0 + row);
-          float most = ctl->m[0][row];
+          for (int wv = 0; wv < CWARPS; ++wv) plain = plain && (ctl->m[wv][row] == 0.f || !(ctl->m[wv][row] > -1e29f));
+          if (plain) {
+            st.m = 0.f;
+            st.l = whole ? ctl->sink[row] : 0.f;
+            st.a = make_float4(0.f, 0.f, 0.f, 0.f);
+          } else {
+            st.start(p, whole, h * p.G + row0 + row);
+            float most = ctl->m[0][row];
 #pragma unroll
-          for (int wv = 1; wv < CWARPS; ++wv) most = fmaxf(most, ctl->m[wv][row]);
-          st.raise(most, p.log2n);
+            for (int wv = 1; wv < CWARPS; ++wv) most = fmaxf(most, ctl->m[wv][row]);
+            st.raise(most, p.log2n);
+          }
+#pragma unroll
+          for (int wv = 0; wv < CWARPS; ++wv)
+            if (ctl->m[wv][row] > -1e29f)
+              st.add(ctl->m[wv][row], ctl->l[wv][row], *reinterpret_cast<const float4*>(scratch + (wv * RB + row) * C::ROW + col), p.log2n);
+            else if (!ok || ctl->l[wv][row] != 0.f) st.l = __int_as_float(0x7fc00000);       // a wait ran out
+          // Out of range as it is written (a bf16 is infinite from half a step above its largest number on), and not for a NaN among its weights?
+          // Then the stretch is gone over again, for the rows that hold such numbers.
+          const float4 res = whole ? st.result() : st.a;
+          __nv_bfloat16* to = static_cast<__nv_bfloat16*>(p.o) + w.s * p.os.t + int64_t(h * p.G + row0 + row) * p.os.h + col;
+          float4* part = reinterpret_cast<float4*>(slot + row * D + col);
+          if (!SECOND) {
+            if (st.l == st.l && !(whole ? largest(res) < 0x1.ffp127f : largest(res) <= 0x1.fffffep127f)) ctl->overflowed = 1;
+          } else {
+            const uint2 old = whole ? *reinterpret_cast<const uint2*>(to) : make_uint2(0u, 0u);
+            const float4 held = whole ? make_float4(__uint_as_float(old.x << 16), __uint_as_float(old.x & 0xffff0000u), __uint_as_float(old.y << 16),
+                                                    __uint_as_float(old.y & 0xffff0000u))
+                                      : *part;
+            const unsigned lanes = D == 128 ? 0xffffffffu : 0xffffu << (lane & 16);      // that have this row
+            if (!__any_sync(lanes, !(largest(held) <= 0x1.fffffep127f))) continue;
+          }
+          if (whole) {
+            *reinterpret_cast<uint2*>(to) = make_uint2(pack_bf16(res.x, res.y), pack_bf16(res.z, res.w));
+          } else {
+            *part = res;
+            if (col == 0) *reinterpret_cast<float2*>(slot + RB * D + row * 2) = make_float2(st.m, st.l);
+          }
         }
-#pragma unroll
-        for (int wv = 0; wv < CWARPS; ++wv)
-          if (ctl->m[wv][row] > -1e29f)
-            st.add(ctl->m[wv][row], ctl->l[wv][row], *reinterpret_cast<const float4*>(scratch + (wv * RB + row) * C::ROW + col), p.log2n);
-          else if (!ok || ctl->l[wv][row] != 0.f) st.l = __int_as_float(0x7fc00000);       // a wait ran out
-        if (whole) {
-          st.write(static_cast<__nv_bfloat16*>(p.o) + w.s * p.os.t + int64_t(h * p.G + row0 + row) * p.os.h + col);
-        } else {
-          *reinterpret_cast<float4*>(slot + row * D + col) = st.a;
-          if (col == 0) *reinterpret_cast<float2*>(slot + RB * D + row * 2) = make_float2(st.m, st.l);
+        if (!whole) {
+          const int64_t head_end = w.base + int64_t(w.hh) * (w.units + 1) + w.units;
+          if (kind == 1) open = TokenHead{w.s, h, row0, int((head_end - 1) / per) - int(blockIdx.x) + 1};
         }
       }
-      if (!whole) {
-        const int64_t head_end = w.base + int64_t(w.hh) * (w.units + 1) + w.units;
-        if (kind == 1) open = TokenHead{w.s, h, row0, int((head_end - 1) / per) - int(blockIdx.x) + 1};
-      }
+      if (threadIdx.x == 0) plan.heads_open[blockIdx.x] = open;
     }
-    if (threadIdx.x == 0) plan.heads_open[blockIdx.x] = open;
+  };
+  run(std::false_type{});
+  if (__syncthreads_or(threadIdx.x == 0 && ctl->abort_flag == 0 && ctl->overflowed != 0)) {
+    if (threadIdx.x == 0) {                      // every load and arrival of the first time has been waited for
+      for (int s = 0; s < STAGES; ++s) { mbar_inval(&ctl->full[s]); mbar_inval(&ctl->empty[s]); }
+      init_barriers();
+    }
+    __syncthreads();
+    run(std::true_type{});
   }
   __syncthreads();
   if (ctl->abort_flag != 0 && threadIdx.x == 0) {
@@ -495,7 +529,8 @@ paged_token_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_consta
 }
 
 // Merges the parts of a head that goes on behind the stretch it began in: CTA c takes the head that CTA c of the kernel ahead left
-// open, a warp a row, a lane D / 32 columns.  References and normalisers come one a lane, 32 parts at a time.
+// open, a warp a row, a lane D / 32 columns.  References and normalisers come one a lane, 32 parts at a time; accumulators meet at 2^-10 of
+// their size, since as many finite ones as there are CTAs may add up to more than fp32 holds.
 template <int D, int RB>
 __global__ void __launch_bounds__(256) paged_token_merge_kernel(const __grid_constant__ RaggedParams p, const TokenPlan plan) {
   constexpr int CPL = D / 32, SLOT = RB * (D + 2), BATCH = 16;
@@ -545,7 +580,7 @@ __global__ void __launch_bounds__(256) paged_token_merge_kernel(const __grid_con
         }
 #pragma unroll
         for (int j = 0; j < BATCH; ++j) {
-          const float fj = __shfl_sync(0xffffffffu, f, (b0 + j) & 31);
+          const float fj = __shfl_sync(0xffffffffu, f, (b0 + j) & 31) * 0x1p-10f;
           if (b0 + j < n && fj != 0.f) {
 #pragma unroll
             for (int c = 0; c < CPL; ++c) a[c] = fmaf(fj, v[j][c], a[c]);
@@ -556,7 +591,7 @@ __global__ void __launch_bounds__(256) paged_token_merge_kernel(const __grid_con
     const float inv = sunk != sunk ? sunk : l == 0.f ? 0.f : 1.0f / l;
     __nv_bfloat16* out = static_cast<__nv_bfloat16*>(p.o) + head.s * p.os.t + int64_t(h) * p.os.h + lane * CPL;
 #pragma unroll
-    for (int c = 0; c < CPL; c += 2) *reinterpret_cast<uint32_t*>(out + c) = pack_bf16(a[c] * inv, a[c + 1] * inv);
+    for (int c = 0; c < CPL; c += 2) *reinterpret_cast<uint32_t*>(out + c) = pack_bf16(a[c] * inv * 0x1p10f, a[c + 1] * inv * 0x1p10f);
   }
 }
 

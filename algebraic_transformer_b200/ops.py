@@ -755,7 +755,7 @@ def paged_attention(q, k_pages, v_pages, block_table, kv_lens, cu_seqlens=None, 
     j of sequence s lies in page block_table[s, j // page_size]; `kv_lens` int32 (sequences): the keys of each, the new tokens'
     own among them (`paged_append` writes them).  `cu_seqlens` int32 (sequences + 1): the rows of q of each sequence, a chunk of any
     length; None: one token a sequence, the form for generation.  Token i of a chunk of m sees keys 0 to kv_len - m + i; one
-    that sees none, as of a sequence of length 0, has the output zero.
+    that sees none, as of a sequence of length 0, has the output zero.  Scores and values as in `packed_attention`.
 
     Lengths and table are read on the device only (a captured call can be replayed with others).  Lengths are clamped to the
     table's width, a page number outside the pool reads as zeros, entries behind a length and rows behind a sequence's end are

@@ -327,7 +327,7 @@ ALG_API int alg_packed_attn_bwd(const alg_packed_attn_bwd_args* args, void* stre
  * block_table[s][j / page_size].  A page number outside the pool reads as zeros.  kv_lens: (sequences) device ints, clamped to
  * table_width page_size; entries of the table behind them are not read.  cu_seqlens: (sequences + 1) device ints, the
  * new tokens' rows of q and o, or NULL: one token a sequence (tokens == sequences).  Token i of Lq sees keys [0, kv_len - Lq + i]; a
- * token that sees none has the output zero. */
+ * token that sees none has the output zero.  Scores and values as in alg_packed_attn_args. */
 typedef struct {
   const void* q;
   const void* k_pages;

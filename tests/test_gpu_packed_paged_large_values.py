@@ -75,13 +75,17 @@ def test_packed_cut_along_the_keys(D, size):
 
 @pytest.mark.parametrize("size", SIZES)
 @pytest.mark.parametrize("n,rows", POWERS)
+@pytest.mark.parametrize("single", [False, True])
 @pytest.mark.parametrize("H,Hkv,D", [(4, 2, 64), (12, 1, 64), (3, 1, 128), (24, 1, 128)])
-def test_paged_chunks(H, Hkv, D, n, rows, size):
+def test_paged(H, Hkv, D, single, n, rows, size):
     lens = [700, 1, 60, 2500]
-    a = make_paged([40, 1, 9, 3], lens, H, Hkv, D, 32, seed=n, size=rows, garbage=False)
+    a = make_paged([1] * 4 if single else [40, 1, 9, 3], lens, H, Hkv, D, 32, seed=n, size=rows, garbage=False)
     a["q"], a["k_pages"] = a["q"].clone(), a["k_pages"].clone()
     towards(a["q"], a["k_pages"], D, n)
     a["v_pages"] = sized(a["v_pages"], size)
+    if single:
+        a["cu_seqlens"] = None
+        a["q"][3] = a["q"][0]
     for s in (a["sink_logit"], None):
         o = A.paged_attention(**dict(a, sink_logit=s), n=n)
         R.assert_close(o, *R.paged(a["q"], a["k_pages"], a["v_pages"], a["block_table"], lens, a["cu_seqlens"], s, n, 8.0))
@@ -96,6 +100,13 @@ def test_rows_beside_a_large_value_keep_their_bits(D):
     large[650, 1, 7] = 3e38                               # seen by the last 50 tokens of the first sequence, heads 2 and 3
     got = A.packed_attention(q, k, large, cu, sink)
     assert torch.equal(got[:650], want[:650]) and torch.equal(got[700:], want[700:]) and torch.equal(got[:, :2], want[:, :2])
+    a = make_paged([1, 1], [700, 60], 4, 2, D, 32, seed=5, size=3.0, garbage=False)
+    a["cu_seqlens"] = None
+    want = A.paged_attention(**a)
+    a["v_pages"] = a["v_pages"].clone()
+    a["v_pages"][int(a["block_table"][0, 20]), 3, 1, 7] = 3e38
+    got = A.paged_attention(**a)
+    assert torch.equal(got[1], want[1]) and torch.equal(got[:, :2], want[:, :2]) and torch.isfinite(got.float()).all()
 
 
 def test_many_items_are_weighed_again():
