@@ -206,6 +206,9 @@ SYMBOLS = {
     "alg_row_sumsq": (C.c_int, [C.c_void_p, C.c_int64, C.c_int, C.c_int64, C.c_void_p, C.c_void_p]),
     "alg_gemm_plan": (C.c_int, [C.c_int] * 5 + [C.POINTER(C.c_int)] * 3),
     "alg_selftest_decode_timeout": (C.c_int, [C.POINTER(DecodeArgs), C.c_int, C.c_ulonglong, C.c_void_p, C.c_void_p]),
+    "alg_selftest_packed_timeout": (C.c_int, [C.POINTER(PackedAttnArgs), C.c_int, C.c_ulonglong, C.c_void_p]),
+    "alg_selftest_packed_bwd_timeout": (C.c_int, [C.POINTER(PackedAttnBwdArgs), C.c_int, C.c_ulonglong, C.c_void_p]),
+    "alg_selftest_paged_timeout": (C.c_int, [C.POINTER(PagedAttnArgs), C.c_int, C.c_ulonglong, C.c_void_p]),
     "alg_selftest_bounded_wait": (C.c_int, [C.c_void_p, C.c_ulonglong, C.c_void_p, C.c_void_p]),
     "alg_rms_norm_fwd":(C.c_int, [C.c_void_p, C.c_void_p, C.c_void_p, C.c_int64, C.c_int, C.c_float, C.c_void_p]),
     "alg_alu_glu_fwd": (C.c_int, [C.c_void_p, C.c_void_p, C.c_void_p, C.c_int64, C.c_int, C.c_int64, C.c_int64, C.c_float,

@@ -226,7 +226,7 @@ paged_token_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_consta
     if (threadIdx.x == 0) plan.heads_open[blockIdx.x] = TokenHead{0, 0, 0, 0};
     return;
   }
-  const BoundedWait bw{&ctl->abort_flag, 1000000000ull};
+  const BoundedWait bw{&ctl->abort_flag, p.limits.budget_ns};
   auto run = [&](auto again) {                   // the stretch; again: the second time, in a copy of its own that costs the first nothing
     constexpr bool SECOND = decltype(again)::value;
     Walk w;
@@ -249,6 +249,7 @@ paged_token_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_consta
           const int c0 = t * pieces;
           if (c0 >= held + 32) { held += 32; number = ahead; ahead = number_at(held + 32 + lane); }
           const int stage = tiles % STAGES;
+          if (tiles >= p.limits.max_loads) { ok = false; break; }
           if (!__all_sync(0xffffffffu, bw.wait(&ctl->empty[stage], (uint32_t(tiles / STAGES) & 1u) ^ 1u))) { ok = false; break; }
           unsigned char* dst = smem + size_t(stage) * 2 * TILE_BYTES;
           const int live = min(pieces, chunks - c0);

@@ -94,6 +94,12 @@ struct RaggedBlocks {
 
 struct Strides2 { int64_t t, h; };
 
+// How long a wait may last, and how many tiles a CTA loads: all of them, but for the self-tests of the waits.
+struct WaitLimits {
+  unsigned long long budget_ns = 1000000000ull;
+  int max_loads = 0x7fffffff;
+};
+
 struct RaggedParams {
   RaggedSeqs seqs;
   RaggedPlan plan;
@@ -114,6 +120,7 @@ struct RaggedParams {
   float scale, inv_c;
   int zero_tail;            // rows of no sequence are written as zeros
   int* status;
+  WaitLimits limits;
 };
 
 // One token a sequence (paged_token.cu).
@@ -199,6 +206,7 @@ struct RaggedBwdParams {
   int S, tokens, H, Hkv, G, D, log2n, chunks;
   float scale, inv_c, n_f, y_fast;
   int* status;
+  WaitLimits limits;
 };
 size_t ragged_bwd_workspace_bytes(int S, int tokens, int H);
 int launch_ragged_backward(const RaggedBwdParams& p, void* workspace, cudaStream_t stream);

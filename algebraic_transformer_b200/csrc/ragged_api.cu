@@ -40,6 +40,12 @@ bool may_split(int64_t keys, int tokens, int H, int Hkv) {
   return keys > 16 * 128 && blocks * Hkv < int64_t(8) * sm_count();
 }
 
+bool limits_ok(const int* status, const WaitLimits& limits) {
+  if (status == nullptr || limits.max_loads < 0) { set_error("selftest: status word and a tile count required"); return false; }
+  if (limits.budget_ns == 0 || limits.budget_ns > 1000000000ull) { set_error("selftest: budget must be in (0, 1 s]"); return false; }
+  return true;
+}
+
 }  // namespace
 }  // namespace alg
 
@@ -52,7 +58,9 @@ size_t alg_packed_attn_workspace_bytes(const alg_packed_attn_args* a) {
   return ragged_plan_bytes(a->sequences, a->tokens, a->Hkv, a->H / a->Hkv, a->D, may_split(a->tokens, a->tokens, a->H, a->Hkv));
 }
 
-int alg_packed_attn_fwd(const alg_packed_attn_args* a, void* stream_) {
+}  // extern "C"
+
+static int packed_call(const alg_packed_attn_args* a, const WaitLimits& limits, void* stream_) {
   cudaStream_t stream = static_cast<cudaStream_t>(stream_);
   if (a == nullptr || a->q == nullptr || a->k == nullptr || a->v == nullptr || a->o == nullptr || a->cu_seqlens == nullptr) {
     set_error("packed attention: null tensor argument");
@@ -85,7 +93,17 @@ int alg_packed_attn_fwd(const alg_packed_attn_args* a, void* stream_) {
   p.inv_c = 1.0f / a->c;
   p.zero_tail = a->zero_tail != 0;
   p.status = a->status;
+  p.limits = limits;
   return launch_ragged_attention(p, stream);
+}
+
+extern "C" {
+
+int alg_packed_attn_fwd(const alg_packed_attn_args* a, void* stream) { return packed_call(a, WaitLimits{}, stream); }
+
+int alg_selftest_packed_timeout(const alg_packed_attn_args* a, int max_loads, unsigned long long budget_ns, void* stream) {
+  const WaitLimits limits{budget_ns, max_loads};
+  return a != nullptr && !limits_ok(a->status, limits) ? ALG_ERR_INVALID : packed_call(a, limits, stream);
 }
 
 size_t alg_packed_attn_bwd_workspace_bytes(const alg_packed_attn_bwd_args* a) {
@@ -93,7 +111,9 @@ size_t alg_packed_attn_bwd_workspace_bytes(const alg_packed_attn_bwd_args* a) {
   return ragged_bwd_workspace_bytes(a->sequences, a->tokens, a->H);
 }
 
-int alg_packed_attn_bwd(const alg_packed_attn_bwd_args* a, void* stream) {
+}  // extern "C"
+
+static int packed_bwd_call(const alg_packed_attn_bwd_args* a, const WaitLimits& limits, void* stream) {
   if (a == nullptr || a->q == nullptr || a->k == nullptr || a->v == nullptr || a->o == nullptr || a->o_rest == nullptr || a->d_o == nullptr ||
       a->stat == nullptr || a->cu_seqlens == nullptr || a->dq == nullptr || a->dk == nullptr || a->dv == nullptr) {
     set_error("packed attention backward: null tensor argument");
@@ -133,7 +153,17 @@ int alg_packed_attn_bwd(const alg_packed_attn_bwd_args* a, void* stream) {
   p.inv_c = 1.0f / a->c;
   p.n_f = float(a->n);
   p.status = a->status;
+  p.limits = limits;
   return launch_ragged_backward(p, a->workspace, static_cast<cudaStream_t>(stream));
+}
+
+extern "C" {
+
+int alg_packed_attn_bwd(const alg_packed_attn_bwd_args* a, void* stream) { return packed_bwd_call(a, WaitLimits{}, stream); }
+
+int alg_selftest_packed_bwd_timeout(const alg_packed_attn_bwd_args* a, int max_loads, unsigned long long budget_ns, void* stream) {
+  const WaitLimits limits{budget_ns, max_loads};
+  return a != nullptr && !limits_ok(a->status, limits) ? ALG_ERR_INVALID : packed_bwd_call(a, limits, stream);
 }
 
 }  // extern "C"
@@ -160,7 +190,9 @@ size_t alg_paged_attn_workspace_bytes(const alg_paged_attn_args* a) {
                            may_split(int64_t(a->table_width) * a->page_size, a->tokens, a->H, a->Hkv));
 }
 
-int alg_paged_attn_fwd(const alg_paged_attn_args* a, void* stream_) {
+}  // extern "C"
+
+static int paged_call(const alg_paged_attn_args* a, const WaitLimits& limits, void* stream_) {
   cudaStream_t stream = static_cast<cudaStream_t>(stream_);
   if (a == nullptr || a->q == nullptr || a->k_pages == nullptr || a->v_pages == nullptr || a->o == nullptr || a->kv_lens == nullptr ||
       a->block_table == nullptr) {
@@ -197,10 +229,20 @@ int alg_paged_attn_fwd(const alg_paged_attn_args* a, void* stream_) {
   p.scale = float(1.0 / (sqrt(double(a->D)) * double(a->c)));
   p.inv_c = 1.0f / a->c;
   p.status = a->status;
+  p.limits = limits;
   if (a->cu_seqlens == nullptr) return launch_paged_token(p, a->workspace, stream);
   ragged_plan_carve(&p.plan, a->workspace, a->sequences, a->tokens, a->Hkv, p.G, a->D, may_split(keys, a->tokens, a->H, a->Hkv), false);
   p.zero_tail = a->zero_tail != 0;
   return launch_ragged_attention(p, stream);
+}
+
+extern "C" {
+
+int alg_paged_attn_fwd(const alg_paged_attn_args* a, void* stream) { return paged_call(a, WaitLimits{}, stream); }
+
+int alg_selftest_paged_timeout(const alg_paged_attn_args* a, int max_loads, unsigned long long budget_ns, void* stream) {
+  const WaitLimits limits{budget_ns, max_loads};
+  return a != nullptr && !limits_ok(a->status, limits) ? ALG_ERR_INVALID : paged_call(a, limits, stream);
 }
 
 int alg_paged_append(const alg_paged_append_args* a, void* stream_) {

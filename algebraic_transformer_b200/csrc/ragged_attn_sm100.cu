@@ -29,12 +29,14 @@
 // FMA 34 %, tensor 20 % in the first): the chain scores -> weights -> P V -> next scores through tensor memory and barriers is what it
 // waits for; with the weights' arithmetic left out it still takes 72 of 92 us, 356 of 427.
 //
-// Every mbarrier wait is bounded; a wait that runs out reports ALG_DEV_TIMEOUT.
+// Every mbarrier wait is bounded; a wait that runs out reports ALG_DEV_TIMEOUT, and the rows of the items that its CTA had not finished, and of those
+// that no CTA had taken by then, are NaN.
 #include "common.cuh"
 #include "launchers.h"
 #include "ragged.cuh"
 #include "sm100_ptx.cuh"
 
+#include <limits.h>
 #include <math.h>
 
 #include <algorithm>
@@ -403,7 +405,7 @@ ragged_attn_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_consta
   tc_fence_after();
   griddep_wait();                                       // the plan, and q, k, v of the kernels ahead
   const uint32_t tmem_base = ctl->tmem_base;
-  const BoundedWait bw{&ctl->abort_flag, 1000000000ull};
+  const BoundedWait bw{&ctl->abort_flag, p.limits.budget_ns};
 
   // the k-th work item of this CTA; false at the end of the work or of the waiting
   auto work_at = [&](int k, Work& w) -> bool {
@@ -415,6 +417,21 @@ ragged_attn_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_consta
     __syncwarp();
     if (lane == 0) mbar_arrive(&ctl->work_empty[k % RING]);
   };
+  // item `next` of the list; false behind its end
+  auto item_at = [&](int next, Work& w) -> bool {
+    w.n1 = -1;
+    if (next >= p.plan.header->items * p.Hkv) return false;
+    const RaggedItem it = p.plan.items[next / p.Hkv];
+    w.index = next;
+    w.head = next % p.Hkv;
+    w.row0 = it.row0; w.Lq = it.Lq; w.Lk = it.Lk; w.seq = it.seq; w.k0 = it.k0; w.slot = it.slot; w.n1 = it.nk;
+    const bool two = it.Lq - it.t0 > TT;
+    w.has0 = two ? 1 : 0;
+    w.tok0 = it.t0;
+    w.tok1 = two ? it.t0 + TT : it.t0;
+    w.n0 = two ? min(max(ragged_tiles(it.Lq, it.Lk, it.t0 + TT) - it.k0, 0), it.nk) : 0;
+    return true;
+  };
   // the oldest item that has not been looked at; all roles are done with it
   auto note = [&] {
     const int k = ctl->noted++ % RING;
@@ -423,11 +440,11 @@ ragged_attn_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_consta
     ctl->again = ctl->work[k].index;
   };
 
+  int undone = 0;                                       // weight warps: items of the first pass that they have finished
   auto run = [&](auto again) {                          // the list; again: the noted items, in a copy of its own that costs the first nothing
     constexpr bool SECOND = decltype(again)::value;
     if (warp == 0) {
       if (lane == 0) {
-        const int total = p.plan.header->items * p.Hkv;
         // the next item: the CTA's own number first, then from the counter; shown to the other roles.  It is asked for when the loads of
         // the item before have been issued, which is as late as can be without a pause, so that longest-first holds to the end
         auto fetch = [&](int k, Work& w) -> bool {
@@ -437,22 +454,12 @@ ragged_attn_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_consta
             if (k >= RING) note();
             next = k == 0 ? int(blockIdx.x) : int(gridDim.x) + atomicAdd(&p.plan.header->counter, 1);
           } else {
-            next = ctl->again < 0 ? total : ctl->again;
-            if (next < total) ctl->again = p.plan.again[next];
+            next = ctl->again < 0 ? INT_MAX : ctl->again;
+            if (ctl->again >= 0) ctl->again = p.plan.again[next];
           }
-          w.n1 = -1;
-          if (next < total) {
-            w.index = next;
+          if (item_at(next, w)) {
             ctl->overflowed[k % RING] = 0;
             ++ctl->taken;
-            const RaggedItem it = p.plan.items[next / p.Hkv];
-            w.head = next % p.Hkv;
-            w.row0 = it.row0; w.Lq = it.Lq; w.Lk = it.Lk; w.seq = it.seq; w.k0 = it.k0; w.slot = it.slot; w.n1 = it.nk;
-            const bool two = it.Lq - it.t0 > TT;
-            w.has0 = two ? 1 : 0;
-            w.tok0 = it.t0;
-            w.tok1 = two ? it.t0 + TT : it.t0;
-            w.n0 = two ? min(max(ragged_tiles(it.Lq, it.Lk, it.t0 + TT) - it.k0, 0), it.nk) : 0;
           }
           ctl->work[k % RING] = w;
           mbar_arrive(&ctl->work_full[k % RING]);
@@ -460,11 +467,13 @@ ragged_attn_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_consta
         };
         RingCursor<C::NKV> cur;
         int items0 = 0;                                   // items in which query tile 0 took part
+        int loads = 0;                                    // K and V tiles
         Work w;
         bool ok = true;
         for (int k = 0; ok && fetch(k, w); ++k) {
           auto load_kv = [&](int idx) {                   // K_0, V_0, K_1, V_1, ... of this item
             const int buf = cur.slot;
+            if (loads++ == p.limits.max_loads) return false;
             if (!bw.wait(&ctl->kv_empty[buf], cur.phase ^ 1u)) return false;
             const CUtensorMap* tm = (idx & 1) ? &tm_v : &tm_k;
             unsigned char* dst = smem + C::KV_OFF + buf * C::TILE_BYTES;
@@ -675,7 +684,8 @@ ragged_attn_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_consta
       }
       Work w;
       bool ok = true;
-      for (int k = 0; ok && work_at(k, w); ++k) {
+      int k = 0;
+      for (; ok && work_at(k, w); ++k) {
         const int nk = t == 0 ? w.n0 : w.n1;
         const int tok = (t == 0 ? w.tok0 : w.tok1) + tok_r;
         const bool live = tok_r < TT && tok < w.Lq && (t == 1 || w.has0 != 0);
@@ -807,13 +817,42 @@ ragged_attn_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_consta
         }
         work_done(k);
       }
+      if (!SECOND) undone = k;
     }
     tc_fence_before();
     __syncthreads();
     tc_fence_after();
   };
   run(std::false_type{});
-  if (threadIdx.x == 0 && ctl->abort_flag == 0) {
+  if (ctl->abort_flag != 0) {                           // a wait ran out: NaN to the rows that have no result and will get none
+    auto spoil = [&](const Work& w) {
+      if (warp < FIRST_WEIGHT_WARP) return;
+      const int t = (warp - FIRST_WEIGHT_WARP) >> 2, r = (warp & 3) * 32 + lane, tok_r = r / p.G, head = w.head * p.G + r - tok_r * p.G;
+      const int tok = (t == 0 ? w.tok0 : w.tok1) + tok_r;
+      if (tok_r >= TT || tok >= w.Lq || (t == 0 && w.has0 == 0)) return;
+      const float nan = __int_as_float(0x7fc00000);
+      if (w.slot >= 0) {
+        float* dst = p.plan.slots + ((int64_t(w.slot) * p.Hkv + w.head) * 256 + t * BQ + r) * (D + 4);
+        *reinterpret_cast<float4*>(dst + D) = make_float4(nan, 0.f, 0.f, 0.f);
+        return;
+      }
+      const int64_t row = int64_t(w.row0) + tok;
+      for (int c = 0; c < D; c += 8) {
+        const uint4 v = make_uint4(0x7fc07fc0u, 0x7fc07fc0u, 0x7fc07fc0u, 0x7fc07fc0u);
+        *reinterpret_cast<uint4*>(static_cast<__nv_bfloat16*>(p.o) + row * p.os.t + head * p.os.h + c) = v;
+        if (HILO) *reinterpret_cast<uint4*>(static_cast<__nv_bfloat16*>(p.o_lo) + (row * p.H + head) * D + c) = v;
+      }
+      if (p.stat != nullptr) p.stat[int64_t(head) * p.seqs.tokens + row] = nan;
+    };
+    for (int k = undone; k < ctl->taken; ++k) spoil(ctl->work[k % RING]);
+    for (;;) {
+      __syncthreads();
+      if (threadIdx.x == 0) item_at(int(gridDim.x) + atomicAdd(&p.plan.header->counter, 1), ctl->work[0]);
+      __syncthreads();
+      if (ctl->work[0].n1 < 0) break;
+      spoil(ctl->work[0]);
+    }
+  } else if (threadIdx.x == 0) {
     while (ctl->noted < ctl->taken) note();
     if (ctl->again >= 0) {                              // every load, product and arrival of the first pass has been waited for
       for (uint64_t* bar = ctl->q_full; bar < ctl->work_empty + RING; ++bar) mbar_inval(bar);

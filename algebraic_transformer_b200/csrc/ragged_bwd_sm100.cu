@@ -170,7 +170,7 @@ __device__ __forceinline__ void bwd_block(unsigned char* smem, Control* ctl, con
                                           const CUtensorMap* tm_v, const CUtensorMap* tm_do, const RaggedBwdParams& p, const int4& block, int h) {
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const uint32_t tmem_base = ctl->tmem_base;
-  const BoundedWait bw{&ctl->abort_flag, 1000000000ull};
+  const BoundedWait bw{&ctl->abort_flag, p.limits.budget_ns};
   constexpr bool DB = C::double_s(MODE);
   auto sbuf = [](int j) { return DB ? (j & 1) : 0; };
   auto sphase = [](int j) -> uint32_t { return DB ? ((j >> 1) & 1u) : (j & 1u); };
@@ -229,6 +229,7 @@ __device__ __forceinline__ void bwd_block(unsigned char* smem, Control* ctl, con
     bool ok = true;
     int g = 0, jq = 0;                                       // head of the group, step of the head
     for (int j = 0; j < nsteps; ++j) {
+      if (j >= p.limits.max_loads) { ok = false; break; }
       const int slot = j % C::NS;
       // The clearing of a head's last tiles comes behind the next step's loads, which then do not wait for the landing; but where the
       // slot for these is not free yet it comes first: what frees the slot may be waiting for the cleared tiles.
@@ -455,11 +456,11 @@ __device__ __forceinline__ void bwd_block(unsigned char* smem, Control* ctl, con
     const bool sunk = MODE == 0 && p.dsink != nullptr;
     const bool ok = p.log2n == 4 ? (sunk ? steps(integral_constant<int, 4>{}, std::true_type{}) : steps(integral_constant<int, 4>{}, std::false_type{}))
                                  : (sunk ? steps(integral_constant<int, 0>{}, std::true_type{}) : steps(integral_constant<int, 0>{}, std::false_type{}));
+    constexpr int CPT = D / C::NG;                             // accumulator columns per thread
     if (ok && bw.wait(&ctl->acc_full, 0)) {
       tc_fence_after();
       if (sunk)                                                // the ring has been read to its end
         reinterpret_cast<float2*>(smem + C::RING_OFF)[group * BT + r] = live ? make_float2(row_delta, row_sum) : make_float2(0.f, 0.f);
-      constexpr int CPT = D / C::NG;                           // accumulator columns per thread
       const int64_t at = int64_t(base) + row;
       __nv_bfloat16* out0 = ((MODE == 0) ? p.dq + at * p.dqs.t + h * p.dqs.h : p.dv + at * p.dvs.t + h * p.dvs.h) + group * CPT;
       __nv_bfloat16* out1 = (MODE == 1) ? p.dk + at * p.dks.t + h * p.dks.h + group * CPT : nullptr;
@@ -484,6 +485,14 @@ __device__ __forceinline__ void bwd_block(unsigned char* smem, Control* ctl, con
                              pack_bf16(__uint_as_float(a[8 * i + 6]) * fac, __uint_as_float(a[8 * i + 7]) * fac));
           }
         }
+      }
+    } else if (live) {                                         // a wait ran out: NaN, no plausible row
+      const int64_t at = int64_t(base) + row;
+#pragma unroll 1
+      for (int c = group * CPT; c < (group + 1) * CPT; c += 8) {
+        const uint4 nan = make_uint4(0x7fc07fc0u, 0x7fc07fc0u, 0x7fc07fc0u, 0x7fc07fc0u);
+        *reinterpret_cast<uint4*>((MODE == 0 ? p.dq + at * p.dqs.t + h * p.dqs.h : p.dv + at * p.dvs.t + h * p.dvs.h) + c) = nan;
+        if (MODE == 1) *reinterpret_cast<uint4*>(p.dk + at * p.dks.t + h * p.dks.h + c) = nan;
       }
     }
   }

@@ -269,6 +269,8 @@ ALG_API int alg_attn_decode_status(const alg_decode_args* args, int* status, voi
  * o_rest: (tokens, H, D) dense bf16, what the rounding to o left over (the products then carry 16 bits of the weights).
  * A key or value that is NaN or infinite reaches the queries of its own sequence only; among these it may
  * reach earlier ones of the same 128-row tile.
+ * status: ALG_DEV_TIMEOUT if a wait of the kernel ran out.  With or without the word, rows of o, stat and o_rest that have no result for
+ * it are NaN; so are rows of the gradients, and all of dsink, in the backward, and rows of o over pages.
  * ---------------------------------------------------------------------------------- */
 typedef struct {
   const void* q;
@@ -663,6 +665,11 @@ ALG_API int alg_selftest_bounded_wait(int* status, unsigned long long budget_ns,
  * `*status` and NaN in the rows concerned. */
 ALG_API int alg_selftest_decode_timeout(const alg_decode_args* args, int max_loads, unsigned long long budget_ns, int* status,
                                         void* stream);
+/* The same for the packed and paged operators, whose status word is in their arguments (here it may not be NULL): a CTA loads
+ * `max_loads` tiles at most (K and V tiles; of the backward, and of one token a sequence, pairs of tiles). */
+ALG_API int alg_selftest_packed_timeout(const alg_packed_attn_args* args, int max_loads, unsigned long long budget_ns, void* stream);
+ALG_API int alg_selftest_packed_bwd_timeout(const alg_packed_attn_bwd_args* args, int max_loads, unsigned long long budget_ns, void* stream);
+ALG_API int alg_selftest_paged_timeout(const alg_paged_attn_args* args, int max_loads, unsigned long long budget_ns, void* stream);
 
 /* fp32 -> bf16 cast of the embedding shard (the reference casts E per call,
  * src/algebraic/kernels/fused_head.py:165; model.py:225). */
