@@ -56,7 +56,7 @@ template <int D, int RB> struct Cfg {
 };
 
 template <int RB> struct __align__(16) Control {
-  uint64_t full[MAX_STAGES], empty[MAX_STAGES];
+  uint64_t full[MAX_STAGES], empty[MAX_STAGES], never;
   int abort_flag, overflowed, start_seq, start_len;
   int64_t start_base;                           // units ahead of the first sequence
   int64_t warp_units[MAX_CWARPS + 1];
@@ -175,6 +175,7 @@ paged_token_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_consta
     fence_barrier_init();
   };
   if (threadIdx.x == 0) {
+    mbar_init(&ctl->never, 1);
     init_barriers();
     ctl->abort_flag = ctl->overflowed = 0;
   }
@@ -226,7 +227,7 @@ paged_token_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_consta
     if (threadIdx.x == 0) plan.heads_open[blockIdx.x] = TokenHead{0, 0, 0, 0};
     return;
   }
-  const BoundedWait bw{&ctl->abort_flag, p.limits.budget_ns};
+  const BoundedWait bw{&ctl->abort_flag, 1000000000ull};
   auto run = [&](auto again) {                   // the stretch; again: the second time, in a copy of its own that costs the first nothing
     constexpr bool SECOND = decltype(again)::value;
     Walk w;
@@ -249,7 +250,7 @@ paged_token_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_consta
           const int c0 = t * pieces;
           if (c0 >= held + 32) { held += 32; number = ahead; ahead = number_at(held + 32 + lane); }
           const int stage = tiles % STAGES;
-          if (tiles >= p.limits.max_loads) { ok = false; break; }
+          if (tiles >= p.limits.max_loads) { ok = wait_in_vain(&ctl->abort_flag, &ctl->never, p.limits.budget_ns); break; }
           if (!__all_sync(0xffffffffu, bw.wait(&ctl->empty[stage], (uint32_t(tiles / STAGES) & 1u) ^ 1u))) { ok = false; break; }
           unsigned char* dst = smem + size_t(stage) * 2 * TILE_BYTES;
           const int live = min(pieces, chunks - c0);

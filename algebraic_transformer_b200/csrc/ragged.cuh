@@ -94,7 +94,7 @@ struct RaggedBlocks {
 
 struct Strides2 { int64_t t, h; };
 
-// How long a wait may last, and how many tiles a CTA loads: all of them, but for the self-tests of the waits.
+// For the self-tests of the waits: how many tiles a CTA loads (all of them as a rule) before its loading warp waits in vain, and how long.
 struct WaitLimits {
   unsigned long long budget_ns = 1000000000ull;
   int max_loads = 0x7fffffff;

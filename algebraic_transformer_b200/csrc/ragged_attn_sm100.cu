@@ -79,7 +79,7 @@ struct Work {
 struct __align__(16) Control {
   uint64_t q_full[2], q_ready[2], q_free[2], kv_full[MAX_NKV], kv_empty[MAX_NKV];
   uint64_t s_full[2], p_half[2], p_full[2], o_full[2], o_free[2];
-  uint64_t q_norm_full[2], v_here, v_clean, work_full[RING], work_empty[RING];
+  uint64_t q_norm_full[2], v_here, v_clean, never, work_full[RING], work_empty[RING];
   Work work[RING];
   float q_norm[2][2];             // largest squared row norm of a query tile, of this item and the next one
   int overflowed[RING];           // a row of the item came out infinite or NaN
@@ -355,6 +355,27 @@ template <int NKV> struct RingCursor {
   __device__ __forceinline__ void next() { if (++slot == NKV) { slot = 0; phase ^= 1u; } }
 };
 
+// NaN to this thread's row of an item that has no result and will get none; a weight warp's threads.
+template <int D, bool HILO> __device__ __noinline__ void spoil_row(const RaggedParams& p, const Work& w, int warp, int lane) {
+  const int t = (warp - FIRST_WEIGHT_WARP) >> 2, r = (warp & 3) * 32 + lane, tok_r = r / p.G, head = w.head * p.G + r - tok_r * p.G;
+  const int tok = (t == 0 ? w.tok0 : w.tok1) + tok_r;
+  if (tok_r >= p.tile_tokens || tok >= w.Lq || (t == 0 && w.has0 == 0)) return;
+  const float nan = __int_as_float(0x7fc00000);
+  if (w.slot >= 0) {
+    float* dst = p.plan.slots + ((int64_t(w.slot) * p.Hkv + w.head) * 256 + t * BQ + r) * (D + 4);
+    *reinterpret_cast<float4*>(dst + D) = make_float4(nan, 0.f, 0.f, 0.f);
+    return;
+  }
+  const int64_t row = int64_t(w.row0) + tok;
+#pragma unroll 1
+  for (int c = 0; c < D; c += 8) {
+    const uint4 v = make_uint4(0x7fc07fc0u, 0x7fc07fc0u, 0x7fc07fc0u, 0x7fc07fc0u);
+    *reinterpret_cast<uint4*>(static_cast<__nv_bfloat16*>(p.o) + row * p.os.t + head * p.os.h + c) = v;
+    if (HILO) *reinterpret_cast<uint4*>(static_cast<__nv_bfloat16*>(p.o_lo) + (row * p.H + head) * D + c) = v;
+  }
+  if (p.stat != nullptr) p.stat[int64_t(head) * p.seqs.tokens + row] = nan;
+}
+
 template <int D, int LOG2N, bool HILO, bool PAGED>
 __global__ void __launch_bounds__(NTHREADS, 1)
 ragged_attn_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant__ CUtensorMap tm_k,
@@ -376,7 +397,7 @@ ragged_attn_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_consta
     }
     for (int i = 0; i < MAX_NKV; ++i) { mbar_init(&ctl->kv_full[i], 1); mbar_init(&ctl->kv_empty[i], 1); }
     for (int i = 0; i < RING; ++i) { mbar_init(&ctl->work_full[i], 1); mbar_init(&ctl->work_empty[i], ITEM_READERS); }
-    mbar_init(&ctl->v_here, 1); mbar_init(&ctl->v_clean, 1);
+    mbar_init(&ctl->v_here, 1); mbar_init(&ctl->v_clean, 1); mbar_init(&ctl->never, 1);
     fence_barrier_init();
   };
   if (threadIdx.x == 0) {
@@ -405,7 +426,7 @@ ragged_attn_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_consta
   tc_fence_after();
   griddep_wait();                                       // the plan, and q, k, v of the kernels ahead
   const uint32_t tmem_base = ctl->tmem_base;
-  const BoundedWait bw{&ctl->abort_flag, p.limits.budget_ns};
+  const BoundedWait bw{&ctl->abort_flag, 1000000000ull};
 
   // the k-th work item of this CTA; false at the end of the work or of the waiting
   auto work_at = [&](int k, Work& w) -> bool {
@@ -417,10 +438,10 @@ ragged_attn_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_consta
     __syncwarp();
     if (lane == 0) mbar_arrive(&ctl->work_empty[k % RING]);
   };
-  // item `next` of the list; false behind its end
-  auto item_at = [&](int next, Work& w) -> bool {
+  // item `next` of the list of `total`; false behind its end
+  auto item_at = [&](int next, int total, Work& w) -> bool {
     w.n1 = -1;
-    if (next >= p.plan.header->items * p.Hkv) return false;
+    if (next >= total) return false;
     const RaggedItem it = p.plan.items[next / p.Hkv];
     w.index = next;
     w.head = next % p.Hkv;
@@ -445,6 +466,7 @@ ragged_attn_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_consta
     constexpr bool SECOND = decltype(again)::value;
     if (warp == 0) {
       if (lane == 0) {
+        const int total = p.plan.header->items * p.Hkv;
         // the next item: the CTA's own number first, then from the counter; shown to the other roles.  It is asked for when the loads of
         // the item before have been issued, which is as late as can be without a pause, so that longest-first holds to the end
         auto fetch = [&](int k, Work& w) -> bool {
@@ -457,7 +479,7 @@ ragged_attn_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_consta
             next = ctl->again < 0 ? INT_MAX : ctl->again;
             if (ctl->again >= 0) ctl->again = p.plan.again[next];
           }
-          if (item_at(next, w)) {
+          if (item_at(next, total, w)) {
             ctl->overflowed[k % RING] = 0;
             ++ctl->taken;
           }
@@ -467,13 +489,12 @@ ragged_attn_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_consta
         };
         RingCursor<C::NKV> cur;
         int items0 = 0;                                   // items in which query tile 0 took part
-        int loads = 0;                                    // K and V tiles
+        int left = p.limits.max_loads;                    // K and V tiles that it may load
         Work w;
         bool ok = true;
         for (int k = 0; ok && fetch(k, w); ++k) {
           auto load_kv = [&](int idx) {                   // K_0, V_0, K_1, V_1, ... of this item
             const int buf = cur.slot;
-            if (loads++ == p.limits.max_loads) return false;
             if (!bw.wait(&ctl->kv_empty[buf], cur.phase ^ 1u)) return false;
             const CUtensorMap* tm = (idx & 1) ? &tm_v : &tm_k;
             unsigned char* dst = smem + C::KV_OFF + buf * C::TILE_BYTES;
@@ -506,9 +527,13 @@ ragged_attn_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_consta
                           w.row0 + (t == 0 ? w.tok0 : w.tok1), pn);
             return true;
           };
-          if (k == 0) ok = load_q(0) && load_kv(0) && load_q(1) && load_kv(1);
+          const int loads = min(2 * w.n1, left);
+          left -= loads;
+          if (loads < 2) ok = false;
+          else if (k == 0) ok = load_q(0) && load_kv(0) && load_q(1) && load_kv(1);
           else ok = load_kv(0) && load_q(0) && load_kv(1) && load_q(1);
-          for (int idx = 2; idx < 2 * w.n1 && ok; ++idx) ok = load_kv(idx);
+          for (int idx = 2; idx < loads && ok; ++idx) ok = load_kv(idx);
+          if (loads < 2 * w.n1) ok = wait_in_vain(&ctl->abort_flag, &ctl->never, p.limits.budget_ns);
           if (w.n0 > 0) ++items0;
         }
       }
@@ -825,29 +850,11 @@ ragged_attn_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_consta
   };
   run(std::false_type{});
   if (ctl->abort_flag != 0) {                           // a wait ran out: NaN to the rows that have no result and will get none
-    auto spoil = [&](const Work& w) {
-      if (warp < FIRST_WEIGHT_WARP) return;
-      const int t = (warp - FIRST_WEIGHT_WARP) >> 2, r = (warp & 3) * 32 + lane, tok_r = r / p.G, head = w.head * p.G + r - tok_r * p.G;
-      const int tok = (t == 0 ? w.tok0 : w.tok1) + tok_r;
-      if (tok_r >= TT || tok >= w.Lq || (t == 0 && w.has0 == 0)) return;
-      const float nan = __int_as_float(0x7fc00000);
-      if (w.slot >= 0) {
-        float* dst = p.plan.slots + ((int64_t(w.slot) * p.Hkv + w.head) * 256 + t * BQ + r) * (D + 4);
-        *reinterpret_cast<float4*>(dst + D) = make_float4(nan, 0.f, 0.f, 0.f);
-        return;
-      }
-      const int64_t row = int64_t(w.row0) + tok;
-      for (int c = 0; c < D; c += 8) {
-        const uint4 v = make_uint4(0x7fc07fc0u, 0x7fc07fc0u, 0x7fc07fc0u, 0x7fc07fc0u);
-        *reinterpret_cast<uint4*>(static_cast<__nv_bfloat16*>(p.o) + row * p.os.t + head * p.os.h + c) = v;
-        if (HILO) *reinterpret_cast<uint4*>(static_cast<__nv_bfloat16*>(p.o_lo) + (row * p.H + head) * D + c) = v;
-      }
-      if (p.stat != nullptr) p.stat[int64_t(head) * p.seqs.tokens + row] = nan;
-    };
+    auto spoil = [&](const Work& w) { if (warp >= FIRST_WEIGHT_WARP) spoil_row<D, HILO>(p, w, warp, lane); };
     for (int k = undone; k < ctl->taken; ++k) spoil(ctl->work[k % RING]);
     for (;;) {
       __syncthreads();
-      if (threadIdx.x == 0) item_at(int(gridDim.x) + atomicAdd(&p.plan.header->counter, 1), ctl->work[0]);
+      if (threadIdx.x == 0) item_at(int(gridDim.x) + atomicAdd(&p.plan.header->counter, 1), p.plan.header->items * p.Hkv, ctl->work[0]);
       __syncthreads();
       if (ctl->work[0].n1 < 0) break;
       spoil(ctl->work[0]);

@@ -59,6 +59,7 @@ template <int D, int BS, int CTAS> struct Cfg {
 
 struct __align__(16) Control {
   uint64_t clean[MAX_STEPS];      // the slot's foreign rows are zeroed
+  uint64_t never;                 // at which nothing arrives
   uint64_t res_full, full[MAX_STEPS], empty[MAX_STEPS], vec_full[MAX_STEPS], s_full[2], dp_full, p_done[2], ds_done, acc_full;
   uint32_t tmem_base;
   int abort_flag;
@@ -170,7 +171,7 @@ __device__ __forceinline__ void bwd_block(unsigned char* smem, Control* ctl, con
                                           const CUtensorMap* tm_v, const CUtensorMap* tm_do, const RaggedBwdParams& p, const int4& block, int h) {
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const uint32_t tmem_base = ctl->tmem_base;
-  const BoundedWait bw{&ctl->abort_flag, p.limits.budget_ns};
+  const BoundedWait bw{&ctl->abort_flag, 1000000000ull};
   constexpr bool DB = C::double_s(MODE);
   auto sbuf = [](int j) { return DB ? (j & 1) : 0; };
   auto sphase = [](int j) -> uint32_t { return DB ? ((j >> 1) & 1u) : (j & 1u); };
@@ -228,8 +229,8 @@ __device__ __forceinline__ void bwd_block(unsigned char* smem, Control* ctl, con
     if (MODE == 1) fetch(0, 0);
     bool ok = true;
     int g = 0, jq = 0;                                       // head of the group, step of the head
-    for (int j = 0; j < nsteps; ++j) {
-      if (j >= p.limits.max_loads) { ok = false; break; }
+    const int loads = min(nsteps, p.limits.max_loads);
+    for (int j = 0; j < loads; ++j) {
       const int slot = j % C::NS;
       // The clearing of a head's last tiles comes behind the next step's loads, which then do not wait for the landing; but where the
       // slot for these is not free yet it comes first: what frees the slot may be waiting for the cleared tiles.
@@ -261,7 +262,8 @@ __device__ __forceinline__ void bwd_block(unsigned char* smem, Control* ctl, con
       __syncwarp();
       if (to_clear && !clear(j - 1)) { ok = false; break; }
     }
-    if (ok && foreign) clear(nsteps - 1);
+    if (loads < nsteps) BoundedWait{&ctl->abort_flag, p.limits.budget_ns}.wait(&ctl->never, 0);     // in vain
+    else if (ok && foreign) clear(nsteps - 1);
   } else if (warp == 1) {
     // the whole warp runs the loop and one elected lane issues (cheaper per issue than a lane-0 branch)
     auto wait_all = [&](uint64_t* bar, uint32_t parity) { return __all_sync(0xffffffffu, bw.wait(bar, parity)) != 0; };
@@ -456,11 +458,11 @@ __device__ __forceinline__ void bwd_block(unsigned char* smem, Control* ctl, con
     const bool sunk = MODE == 0 && p.dsink != nullptr;
     const bool ok = p.log2n == 4 ? (sunk ? steps(integral_constant<int, 4>{}, std::true_type{}) : steps(integral_constant<int, 4>{}, std::false_type{}))
                                  : (sunk ? steps(integral_constant<int, 0>{}, std::true_type{}) : steps(integral_constant<int, 0>{}, std::false_type{}));
-    constexpr int CPT = D / C::NG;                             // accumulator columns per thread
     if (ok && bw.wait(&ctl->acc_full, 0)) {
       tc_fence_after();
       if (sunk)                                                // the ring has been read to its end
         reinterpret_cast<float2*>(smem + C::RING_OFF)[group * BT + r] = live ? make_float2(row_delta, row_sum) : make_float2(0.f, 0.f);
+      constexpr int CPT = D / C::NG;                           // accumulator columns per thread
       const int64_t at = int64_t(base) + row;
       __nv_bfloat16* out0 = ((MODE == 0) ? p.dq + at * p.dqs.t + h * p.dqs.h : p.dv + at * p.dvs.t + h * p.dvs.h) + group * CPT;
       __nv_bfloat16* out1 = (MODE == 1) ? p.dk + at * p.dks.t + h * p.dks.h + group * CPT : nullptr;
@@ -486,15 +488,21 @@ __device__ __forceinline__ void bwd_block(unsigned char* smem, Control* ctl, con
           }
         }
       }
-    } else if (live) {                                         // a wait ran out: NaN, no plausible row
-      const int64_t at = int64_t(base) + row;
-#pragma unroll 1
-      for (int c = group * CPT; c < (group + 1) * CPT; c += 8) {
-        const uint4 nan = make_uint4(0x7fc07fc0u, 0x7fc07fc0u, 0x7fc07fc0u, 0x7fc07fc0u);
-        *reinterpret_cast<uint4*>((MODE == 0 ? p.dq + at * p.dqs.t + h * p.dqs.h : p.dv + at * p.dvs.t + h * p.dvs.h) + c) = nan;
-        if (MODE == 1) *reinterpret_cast<uint4*>(p.dk + at * p.dks.t + h * p.dks.h + c) = nan;
-      }
     }
+  }
+}
+
+// A wait ran out: NaN to the block's rows, whatever they hold.
+template <int D>
+__device__ __forceinline__ void spoil_block(const RaggedBwdParams& p, const int4& block, int h, bool keys) {
+  const uint4 nan = make_uint4(0x7fc07fc0u, 0x7fc07fc0u, 0x7fc07fc0u, 0x7fc07fc0u);
+#pragma unroll 1
+  for (int i = threadIdx.x; i < BT * (D / 8); i += blockDim.x) {
+    const int row = block.z + i / (D / 8), col = i % (D / 8) * 8;
+    if (row >= block.y) continue;
+    const int64_t at = int64_t(block.x) + row;
+    *reinterpret_cast<uint4*>((keys ? p.dv + at * p.dvs.t + h * p.dvs.h : p.dq + at * p.dqs.t + h * p.dqs.h) + col) = nan;
+    if (keys) *reinterpret_cast<uint4*>(p.dk + at * p.dks.t + h * p.dks.h + col) = nan;
   }
 }
 
@@ -573,7 +581,7 @@ ragged_bwd_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constan
 
   if (threadIdx.x == 0) {
     tma_prefetch_desc(&tm_q); tma_prefetch_desc(&tm_k); tma_prefetch_desc(&tm_v); tma_prefetch_desc(&tm_do);
-    mbar_init(&ctl->res_full, 1);
+    mbar_init(&ctl->res_full, 1); mbar_init(&ctl->never, 1);
     for (int i = 0; i < C::NS; ++i) { mbar_init(&ctl->full[i], 1); mbar_init(&ctl->empty[i], 1); mbar_init(&ctl->vec_full[i], 1); mbar_init(&ctl->clean[i], 1); }
     for (int i = 0; i < 2; ++i) { mbar_init(&ctl->s_full[i], 1); mbar_init(&ctl->p_done[i], C::EW_WARPS); }
     mbar_init(&ctl->dp_full, 1);
@@ -595,6 +603,7 @@ ragged_bwd_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constan
   tc_fence_before();
   __syncthreads();
   if (ctl->abort_flag != 0) {
+    spoil_block<D>(p, block, idx % heads, keys);
     if (threadIdx.x == 0) {
       if (p.status != nullptr) atomicExch(p.status, ALG_DEV_TIMEOUT);
       const uint64_t t0 = global_timer_ns();                 // let issued loads land before shared memory is released

@@ -71,6 +71,11 @@ struct BoundedWait {
   }
 };
 
+// For the self-tests of the waits: one that runs out, on a barrier at which nothing arrives, and raises the flag.
+static __device__ __noinline__ bool wait_in_vain(volatile int* abort_flag, uint64_t* never, uint64_t budget_ns) {
+  return BoundedWait{abort_flag, budget_ns}.wait(never, 0);
+}
+
 // --------------------------------------------------------------------------------- TMA
 __device__ __forceinline__ void tma_prefetch_desc(const CUtensorMap* m) {
   asm volatile("prefetch.tensormap [%0];" ::"l"(reinterpret_cast<uint64_t>(m)) : "memory");

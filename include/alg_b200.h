@@ -666,7 +666,8 @@ ALG_API int alg_selftest_bounded_wait(int* status, unsigned long long budget_ns,
 ALG_API int alg_selftest_decode_timeout(const alg_decode_args* args, int max_loads, unsigned long long budget_ns, int* status,
                                         void* stream);
 /* The same for the packed and paged operators, whose status word is in their arguments (here it may not be NULL): a CTA loads
- * `max_loads` tiles at most (K and V tiles; of the backward, and of one token a sequence, pairs of tiles). */
+ * `max_loads` tiles at most (K and V tiles; of the backward, and of one token a sequence, pairs of tiles), then its loading warp waits in
+ * vain for `budget_ns`, which ends the waits of its other warps too. */
 ALG_API int alg_selftest_packed_timeout(const alg_packed_attn_args* args, int max_loads, unsigned long long budget_ns, void* stream);
 ALG_API int alg_selftest_packed_bwd_timeout(const alg_packed_attn_bwd_args* args, int max_loads, unsigned long long budget_ns, void* stream);
 ALG_API int alg_selftest_paged_timeout(const alg_paged_attn_args* args, int max_loads, unsigned long long budget_ns, void* stream);
