@@ -11,8 +11,8 @@ namespace {
 
 bool aligned16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15) == 0; }
 
-// Rows of `count` vectors must start on 16-byte boundaries, apart from one another; a single one may have any stride, which is
-// replaced by one the copies accept.
+// Rows of `count` vectors must start on 16-byte boundaries, apart from one another where they are written (written_apart); a single one may
+// have any stride, which is replaced by one the copies accept.
 bool stride_ok(int64_t* s, int64_t count, int64_t dense) {
   if (count <= 1) { *s = dense; return true; }
   return *s > 0 && *s % 8 == 0 && *s < (int64_t(1) << 38);
@@ -21,6 +21,22 @@ bool strides_ok(Strides2* s, const int64_t given[2], int64_t rows, int64_t heads
   *s = {given[0], given[1]};
   return stride_ok(&s->t, rows, int64_t(heads) * D) && stride_ok(&s->h, heads, D);
 }
+
+// No two rows of a tensor that is written share an element: each axis steps over all that the axes of smaller strides span.
+bool written_apart(int D, int64_t n0, int64_t s0, int64_t n1, int64_t s1, int64_t n2 = 1, int64_t s2 = 0) {
+  int64_t count[3] = {n0, n1, n2}, stride[3] = {s0, s1, s2}, span = D;
+  for (int round = 0; round < 3; ++round) {
+    int axis = -1;                                     // the smallest stride that is left
+    for (int i = 0; i < 3; ++i)
+      if (count[i] > 1 && (axis < 0 || stride[i] < stride[axis])) axis = i;
+    if (axis < 0) break;
+    if (stride[axis] < span) return false;
+    span += stride[axis] * (count[axis] - 1);
+    count[axis] = 1;
+  }
+  return true;
+}
+bool written_apart(const Strides2& s, int64_t rows, int64_t heads, int D) { return written_apart(D, rows, s.t, heads, s.h); }
 
 int check_link(const char* what, int H, int Hkv, int D, int n, float c) {
   if (D != 64 && D != 128) { set_error("%s: head_dim must be 64 or 128, got %d", what, D); return ALG_ERR_UNSUPPORTED; }
@@ -72,8 +88,9 @@ static int packed_call(const alg_packed_attn_args* a, const WaitLimits& limits, 
   RaggedParams p{};
   if (!strides_ok(&p.qs, a->q_stride, a->tokens, a->H, a->D) || !strides_ok(&p.ks, a->k_stride, a->tokens, a->Hkv, a->D) ||
       !strides_ok(&p.vs, a->v_stride, a->tokens, a->Hkv, a->D) || !strides_ok(&p.os, a->o_stride, a->tokens, a->H, a->D) ||
-      !aligned16(a->q) || !aligned16(a->k) || !aligned16(a->v) || !aligned16(a->o) || !aligned16(a->o_rest)) {
-    set_error("packed attention: rows must start on 16-byte boundaries and lie apart");
+      !aligned16(a->q) || !aligned16(a->k) || !aligned16(a->v) || !aligned16(a->o) || !aligned16(a->o_rest) ||
+      !written_apart(p.os, a->tokens, a->H, a->D)) {
+    set_error("packed attention: rows must start on 16-byte boundaries, those that are written lie apart");
     return ALG_ERR_INVALID;
   }
   const size_t need = alg_packed_attn_workspace_bytes(a);
@@ -128,8 +145,9 @@ static int packed_bwd_call(const alg_packed_attn_bwd_args* a, const WaitLimits& 
       !strides_ok(&p.gs, a->do_stride, a->tokens, a->H, a->D) || !strides_ok(&p.dqs, a->dq_stride, a->tokens, a->H, a->D) ||
       !strides_ok(&p.dks, a->dk_stride, a->tokens, a->Hkv, a->D) || !strides_ok(&p.dvs, a->dv_stride, a->tokens, a->Hkv, a->D) ||
       !aligned16(a->q) || !aligned16(a->k) || !aligned16(a->v) || !aligned16(a->o) || !aligned16(a->o_rest) || !aligned16(a->d_o) ||
-      !aligned16(a->dq) || !aligned16(a->dk) || !aligned16(a->dv)) {
-    set_error("packed attention backward: rows must start on 16-byte boundaries and lie apart");
+      !aligned16(a->dq) || !aligned16(a->dk) || !aligned16(a->dv) || !written_apart(p.dqs, a->tokens, a->H, a->D) ||
+      !written_apart(p.dks, a->tokens, a->Hkv, a->D) || !written_apart(p.dvs, a->tokens, a->Hkv, a->D)) {
+    set_error("packed attention backward: rows must start on 16-byte boundaries, those that are written lie apart");
     return ALG_ERR_INVALID;
   }
   const size_t need = alg_packed_attn_bwd_workspace_bytes(a);
@@ -207,8 +225,8 @@ static int paged_call(const alg_paged_attn_args* a, const WaitLimits& limits, vo
   if (!strides_ok(&p.qs, a->q_stride, a->tokens, a->H, a->D) || !strides_ok(&p.ks, a->k_stride + 1, a->page_size, a->Hkv, a->D) ||
       !strides_ok(&p.vs, a->v_stride + 1, a->page_size, a->Hkv, a->D) || !strides_ok(&p.os, a->o_stride, a->tokens, a->H, a->D) ||
       !stride_ok(&kp, a->pages, page_elems) || !stride_ok(&vp, a->pages, page_elems) || !aligned16(a->q) || !aligned16(a->k_pages) ||
-      !aligned16(a->v_pages) || !aligned16(a->o)) {
-    set_error("paged attention: rows must start on 16-byte boundaries and lie apart");
+      !aligned16(a->v_pages) || !aligned16(a->o) || !written_apart(p.os, a->tokens, a->H, a->D)) {
+    set_error("paged attention: rows must start on 16-byte boundaries, those that are written lie apart");
     return ALG_ERR_INVALID;
   }
   const size_t need = alg_paged_attn_workspace_bytes(a);
@@ -269,8 +287,10 @@ int alg_paged_append(const alg_paged_append_args* a, void* stream_) {
       !strides_ok(&p.kps, a->kp_stride + 1, a->page_size, a->Hkv, a->D) || !strides_ok(&p.vps, a->vp_stride + 1, a->page_size, a->Hkv, a->D) ||
       !stride_ok(&p.k_page, a->pages, page_elems) || !stride_ok(&p.v_page, a->pages, page_elems) || !aligned16(a->q) || !aligned16(a->k) ||
       !aligned16(a->v) || !aligned16(a->q_out) || !aligned16(a->k_pages) || !aligned16(a->v_pages) || !aligned16(a->cos) || !aligned16(a->sin) ||
-      !aligned16(a->q_gain) || !aligned16(a->k_gain)) {
-    set_error("paged append: rows, gains and tables must start on 16-byte boundaries, rows lie apart");
+      !aligned16(a->q_gain) || !aligned16(a->k_gain) || !written_apart(p.os, a->tokens, a->H, a->D) ||
+      !written_apart(a->D, a->pages, p.k_page, a->page_size, p.kps.t, a->Hkv, p.kps.h) ||
+      !written_apart(a->D, a->pages, p.v_page, a->page_size, p.vps.t, a->Hkv, p.vps.h)) {
+    set_error("paged append: rows, gains and tables must start on 16-byte boundaries, rows that are written lie apart");
     return ALG_ERR_INVALID;
   }
   if (a->tokens == 0) return ALG_OK;
