@@ -56,7 +56,8 @@ template <int D, int RB> struct Cfg {
 };
 
 template <int RB> struct __align__(16) Control {
-  uint64_t full[MAX_STAGES], empty[MAX_STAGES], never;
+  struct { uint64_t full[MAX_STAGES], empty[MAX_STAGES]; } bars[2];             // of the first time over the stretch and of the second
+  uint64_t never;
   int abort_flag, overflowed, start_seq, start_len;
   int64_t start_base;                           // units ahead of the first sequence
   int64_t warp_units[MAX_CWARPS + 1];
@@ -170,14 +171,13 @@ paged_token_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_consta
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int heads = plan.heads;                  // key heads times row groups
 
-  auto init_barriers = [&] {
-    for (int s = 0; s < STAGES; ++s) { mbar_init(&ctl->full[s], 1); mbar_init(&ctl->empty[s], 1); }
+  if (threadIdx.x == 0 || threadIdx.x == 32) {
+    for (int s = 0; s < STAGES; ++s) { mbar_init(&ctl->bars[threadIdx.x >> 5].full[s], 1); mbar_init(&ctl->bars[threadIdx.x >> 5].empty[s], 1); }
+    if (threadIdx.x == 0) {
+      mbar_init(&ctl->never, 1);
+      ctl->abort_flag = ctl->overflowed = 0;
+    }
     fence_barrier_init();
-  };
-  if (threadIdx.x == 0) {
-    mbar_init(&ctl->never, 1);
-    init_barriers();
-    ctl->abort_flag = ctl->overflowed = 0;
   }
   if (threadIdx.x == C::CONSUMERS) { tma_prefetch_desc(&tm_k); tma_prefetch_desc(&tm_v); }
   griddep_wait();
@@ -230,6 +230,7 @@ paged_token_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_consta
   const BoundedWait bw{&ctl->abort_flag, 1000000000ull};
   auto run = [&](auto again) {                   // the stretch; again: the second time, in a copy of its own that costs the first nothing
     constexpr bool SECOND = decltype(again)::value;
+    auto& bar = ctl->bars[SECOND ? 1 : 0];
     Walk w;
     w.at = begin; w.end = min(begin + per, total);
     w.s = ctl->start_seq; w.len = ctl->start_len; w.base = ctl->start_base;
@@ -251,17 +252,17 @@ paged_token_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_consta
           if (c0 >= held + 32) { held += 32; number = ahead; ahead = number_at(held + 32 + lane); }
           const int stage = tiles % STAGES;
           if (tiles >= p.limits.max_loads) { ok = wait_in_vain(&ctl->abort_flag, &ctl->never, p.limits.budget_ns); break; }
-          if (!__all_sync(0xffffffffu, bw.wait(&ctl->empty[stage], (uint32_t(tiles / STAGES) & 1u) ^ 1u))) { ok = false; break; }
+          if (!__all_sync(0xffffffffu, bw.wait(&bar.empty[stage], (uint32_t(tiles / STAGES) & 1u) ^ 1u))) { ok = false; break; }
           unsigned char* dst = smem + size_t(stage) * 2 * TILE_BYTES;
           const int live = min(pieces, chunks - c0);
-          if (lane == 0) mbar_arrive_expect_tx(&ctl->full[stage], uint32_t(live * rows) * (D * 2) * 2);
+          if (lane == 0) mbar_arrive_expect_tx(&bar.full[stage], uint32_t(live * rows) * (D * 2) * 2);
           __syncwarp();
           // a lane a copy: of K or V, a panel, a piece of a page
           const int piece = lane / (2 * C::PANELS), pn = (lane >> 1) % C::PANELS, v = lane & 1;
           const int page = __shfl_sync(0xffffffffu, number, (c0 + piece - held) & 31);
           if (piece < live) {
             const int row = (k0 + ((c0 + piece) << log2_rows)) & (p.page - 1);
-            tma_load_5d(dst + v * TILE_BYTES + pn * PANEL + piece * rows * 128, v ? &tm_v : &tm_k, &ctl->full[stage], 0, row, pn, h, page);
+            tma_load_5d(dst + v * TILE_BYTES + pn * PANEL + piece * rows * 128, v ? &tm_v : &tm_k, &bar.full[stage], 0, row, pn, h, page);
           }
           __syncwarp();
         }
@@ -310,7 +311,7 @@ paged_token_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_consta
         bool shifted = SECOND, begun = false;
         for (int t = (warp + CWARPS - tiles % CWARPS) % CWARPS; t < n && ok; t += CWARPS) {
           const int number = tiles + t, stage = number % STAGES;
-          if (!__all_sync(0xffffffffu, bw.wait(&ctl->full[stage], uint32_t(number / STAGES) & 1u))) { ok = false; break; }
+          if (!__all_sync(0xffffffffu, bw.wait(&bar.full[stage], uint32_t(number / STAGES) & 1u))) { ok = false; break; }
           const uint32_t sk = ring + uint32_t(stage) * (2 * TILE_BYTES), sv = sk + TILE_BYTES;
           float sc[4][4];
 #pragma unroll
@@ -430,7 +431,7 @@ paged_token_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_consta
             else product(std::false_type{});
           }
           __syncwarp();
-          if (lane == 0) mbar_arrive(&ctl->empty[stage]);
+          if (lane == 0) mbar_arrive(&bar.empty[stage]);
         }
         tiles += n;
         // ---- the warps' states together: each leaves its own in shared memory, every thread adds up its columns of a row
@@ -514,14 +515,9 @@ paged_token_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_consta
     }
   };
   run(std::false_type{});
-  if (__syncthreads_or(threadIdx.x == 0 && ctl->abort_flag == 0 && ctl->overflowed != 0)) {
-    if (threadIdx.x == 0) {                      // every load and arrival of the first time has been waited for
-      for (int s = 0; s < STAGES; ++s) { mbar_inval(&ctl->full[s]); mbar_inval(&ctl->empty[s]); }
-      init_barriers();
-    }
-    __syncthreads();
-    run(std::true_type{});
-  }
+  // by every thread's own word, and before any of them starts again
+  const bool overflowed = __syncthreads_or(ctl->overflowed != 0), ended = __syncthreads_or(ctl->abort_flag != 0);
+  if (overflowed && !ended) run(std::true_type{});
   __syncthreads();
   if (ctl->abort_flag != 0 && threadIdx.x == 0) {
     if (p.status != nullptr) atomicExch(p.status, ALG_DEV_TIMEOUT);

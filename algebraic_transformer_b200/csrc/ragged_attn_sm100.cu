@@ -76,10 +76,13 @@ struct Work {
   int index;                      // its place in the list, times Hkv, plus the head
 };
 
-struct __align__(16) Control {
+struct Barriers {
   uint64_t q_full[2], q_ready[2], q_free[2], kv_full[MAX_NKV], kv_empty[MAX_NKV];
   uint64_t s_full[2], p_half[2], p_full[2], o_full[2], o_free[2];
   uint64_t q_norm_full[2], v_here, v_clean, never, work_full[RING], work_empty[RING];
+};
+struct __align__(16) Control {
+  Barriers bars[2];               // of the first pass and of the second (one set, invalidated and set up again, kept the phase of its last barrier)
   Work work[RING];
   float q_norm[2][2];             // largest squared row norm of a query tile, of this item and the next one
   int overflowed[RING];           // a row of the item came out infinite or NaN
@@ -388,20 +391,20 @@ ragged_attn_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_consta
   Control* ctl = reinterpret_cast<Control*>(smem + C::CTL_OFF);
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
 
-  auto init_barriers = [&] {
+  if (lane == 0 && (warp == 0 || warp == 3)) {
+    Barriers* bar = &ctl->bars[warp == 0 ? 0 : 1];
     for (int w = 0; w < 2; ++w) {
-      mbar_init(&ctl->q_full[w], 1); mbar_init(&ctl->q_ready[w], 1); mbar_init(&ctl->q_free[w], NORMS ? 5 : 1);
-      mbar_init(&ctl->s_full[w], 1); mbar_init(&ctl->p_half[w], 4); mbar_init(&ctl->p_full[w], 4);
-      mbar_init(&ctl->o_full[w], 1); mbar_init(&ctl->o_free[w], 4);
-      mbar_init(&ctl->q_norm_full[w], 1);
+      mbar_init(&bar->q_full[w], 1); mbar_init(&bar->q_ready[w], 1); mbar_init(&bar->q_free[w], NORMS ? 5 : 1);
+      mbar_init(&bar->s_full[w], 1); mbar_init(&bar->p_half[w], 4); mbar_init(&bar->p_full[w], 4);
+      mbar_init(&bar->o_full[w], 1); mbar_init(&bar->o_free[w], 4);
+      mbar_init(&bar->q_norm_full[w], 1);
     }
-    for (int i = 0; i < MAX_NKV; ++i) { mbar_init(&ctl->kv_full[i], 1); mbar_init(&ctl->kv_empty[i], 1); }
-    for (int i = 0; i < RING; ++i) { mbar_init(&ctl->work_full[i], 1); mbar_init(&ctl->work_empty[i], ITEM_READERS); }
-    mbar_init(&ctl->v_here, 1); mbar_init(&ctl->v_clean, 1); mbar_init(&ctl->never, 1);
+    for (int i = 0; i < C::NKV; ++i) { mbar_init(&bar->kv_full[i], 1); mbar_init(&bar->kv_empty[i], 1); }
+    for (int i = 0; i < RING; ++i) { mbar_init(&bar->work_full[i], 1); mbar_init(&bar->work_empty[i], ITEM_READERS); }
+    mbar_init(&bar->v_here, 1); mbar_init(&bar->v_clean, 1); mbar_init(&bar->never, 1);
     fence_barrier_init();
-  };
+  }
   if (threadIdx.x == 0) {
-    init_barriers();
     ctl->abort_flag = 0;
     ctl->taken = ctl->noted = 0;
     ctl->again = -1;
@@ -428,16 +431,6 @@ ragged_attn_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_consta
   const uint32_t tmem_base = ctl->tmem_base;
   const BoundedWait bw{&ctl->abort_flag, 1000000000ull};
 
-  // the k-th work item of this CTA; false at the end of the work or of the waiting
-  auto work_at = [&](int k, Work& w) -> bool {
-    if (!__all_sync(0xffffffffu, bw.wait(&ctl->work_full[k % RING], uint32_t(k / RING) & 1u))) return false;
-    w = ctl->work[k % RING];
-    return w.n1 >= 0;
-  };
-  auto work_done = [&](int k) {
-    __syncwarp();
-    if (lane == 0) mbar_arrive(&ctl->work_empty[k % RING]);
-  };
   // item `next` of the list of `total`; false behind its end
   auto item_at = [&](int next, int total, Work& w) -> bool {
     w.n1 = -1;
@@ -464,13 +457,24 @@ ragged_attn_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_consta
   int undone = 0;                                       // weight warps: items of the first pass that they have finished
   auto run = [&](auto again) {                          // the list; again: the noted items, in a copy of its own that costs the first nothing
     constexpr bool SECOND = decltype(again)::value;
+    Barriers* const bar = &ctl->bars[SECOND ? 1 : 0];
+    // the k-th work item of this CTA; false at the end of the work or of the waiting
+    auto work_at = [&](int k, Work& w) -> bool {
+      if (!__all_sync(0xffffffffu, bw.wait(&bar->work_full[k % RING], uint32_t(k / RING) & 1u))) return false;
+      w = ctl->work[k % RING];
+      return w.n1 >= 0;
+    };
+    auto work_done = [&](int k) {
+      __syncwarp();
+      if (lane == 0) mbar_arrive(&bar->work_empty[k % RING]);
+    };
     if (warp == 0) {
       if (lane == 0) {
         const int total = p.plan.header->items * p.Hkv;
         // the next item: the CTA's own number first, then from the counter; shown to the other roles.  It is asked for when the loads of
         // the item before have been issued, which is as late as can be without a pause, so that longest-first holds to the end
         auto fetch = [&](int k, Work& w) -> bool {
-          if (k >= RING && !bw.wait(&ctl->work_empty[k % RING], uint32_t(k / RING - 1) & 1u)) return false;
+          if (k >= RING && !bw.wait(&bar->work_empty[k % RING], uint32_t(k / RING - 1) & 1u)) return false;
           int next;
           if (!SECOND) {
             if (k >= RING) note();
@@ -484,7 +488,7 @@ ragged_attn_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_consta
             ++ctl->taken;
           }
           ctl->work[k % RING] = w;
-          mbar_arrive(&ctl->work_full[k % RING]);
+          mbar_arrive(&bar->work_full[k % RING]);
           return w.n1 >= 0;
         };
         RingCursor<C::NKV> cur;
@@ -495,24 +499,24 @@ ragged_attn_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_consta
         for (int k = 0; ok && fetch(k, w); ++k) {
           auto load_kv = [&](int idx) {                   // K_0, V_0, K_1, V_1, ... of this item
             const int buf = cur.slot;
-            if (!bw.wait(&ctl->kv_empty[buf], cur.phase ^ 1u)) return false;
+            if (!bw.wait(&bar->kv_empty[buf], cur.phase ^ 1u)) return false;
             const CUtensorMap* tm = (idx & 1) ? &tm_v : &tm_k;
             unsigned char* dst = smem + C::KV_OFF + buf * C::TILE_BYTES;
             const int key0 = (w.k0 + (idx >> 1)) * BKEY;
             if (PAGED) {
               const int rows = min(p.page, BKEY), live = min(BKEY, w.Lk - key0);      // keys of the tile that the sequence has
               const int loads = live > 0 ? (live + rows - 1) / rows : 0;
-              mbar_arrive_expect_tx(&ctl->kv_full[buf], uint32_t(loads * rows) * (D * 2));
+              mbar_arrive_expect_tx(&bar->kv_full[buf], uint32_t(loads * rows) * (D * 2));
               const int* pages = p.table + w.seq * p.table_stride;
               for (int i = 0; i < loads; ++i) {
                 const int key = key0 + i * rows;
                 const int number = __ldg(pages + (key >> p.log2_page));    // outside the pool: the copy fills zeros
                 for (int pn = 0; pn < C::PANELS; ++pn)
-                  tma_load_5d(dst + pn * PANEL_BYTES + i * rows * 128, tm, &ctl->kv_full[buf], 0, key & (p.page - 1), pn, w.head, number);
+                  tma_load_5d(dst + pn * PANEL_BYTES + i * rows * 128, tm, &bar->kv_full[buf], 0, key & (p.page - 1), pn, w.head, number);
               }
             } else {
-              mbar_arrive_expect_tx(&ctl->kv_full[buf], C::TILE_BYTES);
-              tma_load_4d(dst, tm, &ctl->kv_full[buf], 0, w.row0 + key0, 0, w.head);
+              mbar_arrive_expect_tx(&bar->kv_full[buf], C::TILE_BYTES);
+              tma_load_4d(dst, tm, &bar->kv_full[buf], 0, w.row0 + key0, 0, w.head);
             }
             cur.next();
             return true;
@@ -520,10 +524,10 @@ ragged_attn_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_consta
           auto load_q = [&](int t) {                      // after the previous item's last S_t has read the tile
             if (t == 0 && w.n0 == 0) return true;
             const int before = t == 0 ? items0 : k;
-            if (before > 0 && !bw.wait(&ctl->q_free[t], uint32_t(before - 1) & 1u)) return false;
-            mbar_arrive_expect_tx(&ctl->q_full[t], uint32_t(p.G * TT) * (D * 2));
+            if (before > 0 && !bw.wait(&bar->q_free[t], uint32_t(before - 1) & 1u)) return false;
+            mbar_arrive_expect_tx(&bar->q_full[t], uint32_t(p.G * TT) * (D * 2));
             for (int pn = 0; pn < C::PANELS; ++pn)
-              tma_load_4d(smem + t * C::TILE_BYTES + pn * PANEL_BYTES, &tm_q, &ctl->q_full[t], 0, w.head * p.G,
+              tma_load_4d(smem + t * C::TILE_BYTES + pn * PANEL_BYTES, &tm_q, &bar->q_full[t], 0, w.head * p.G,
                           w.row0 + (t == 0 ? w.tok0 : w.tok1), pn);
             return true;
           };
@@ -533,7 +537,7 @@ ragged_attn_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_consta
           else if (k == 0) ok = load_q(0) && load_kv(0) && load_q(1) && load_kv(1);
           else ok = load_kv(0) && load_q(0) && load_kv(1) && load_q(1);
           for (int idx = 2; idx < loads && ok; ++idx) ok = load_kv(idx);
-          if (loads < 2 * w.n1) ok = wait_in_vain(&ctl->abort_flag, &ctl->never, p.limits.budget_ns);
+          if (loads < 2 * w.n1) ok = wait_in_vain(&ctl->abort_flag, &bar->never, p.limits.budget_ns);
           if (w.n0 > 0) ++items0;
         }
       }
@@ -542,8 +546,8 @@ ragged_attn_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_consta
       using Cur = RingCursor<C::NKV>;
       Cur cur;
       int t0 = 0, t1 = 0, items0 = 0, cleans = 0;         // score tiles of query tile 0 / 1 in earlier items; items of tile 0
-      auto wait_all = [&](uint64_t* bar, uint32_t parity) { return __all_sync(0xffffffffu, bw.wait(bar, parity)) != 0; };
-      auto kv_wait = [&](const Cur& c) { return wait_all(&ctl->kv_full[c.slot], c.phase); };
+      auto wait_all = [&](uint64_t* word, uint32_t parity) { return __all_sync(0xffffffffu, bw.wait(word, parity)) != 0; };
+      auto kv_wait = [&](const Cur& c) { return wait_all(&bar->kv_full[c.slot], c.phase); };
       const uint32_t q_lo0 = sw128_desc_lo(q_addr, 16), k_lo0 = sw128_desc_lo(kv_addr, 16), v_lo0 = sw128_desc_lo(kv_addr, PANEL_BYTES);
       auto issue_s = [&](int t, int slot) {               // S_t = Q_t K^T
         const uint32_t qa = q_lo0 + t * (C::TILE_BYTES >> 4), ka = k_lo0 + slot * (C::TILE_BYTES >> 4);
@@ -566,17 +570,17 @@ ragged_attn_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_consta
       };
       // P of query tile t, tile j of nt, then the next scores into its place
       auto serve = [&](int t, int j, int nt, int before, int items, int v_slot, int k_slot) -> bool {
-        if (!wait_all(&ctl->p_half[t], uint32_t(before + j) & 1u)) return false;
-        if (j == 0 && items > 0 && !wait_all(&ctl->o_free[t], uint32_t(items - 1) & 1u)) return false;   // the last output has been read
+        if (!wait_all(&bar->p_half[t], uint32_t(before + j) & 1u)) return false;
+        if (j == 0 && items > 0 && !wait_all(&bar->o_free[t], uint32_t(items - 1) & 1u)) return false;   // the last output has been read
         tc_fence_after();
         if (elect_one()) issue_pv(t, v_slot, 0, j == 0);
         __syncwarp();
-        if (!wait_all(&ctl->p_full[t], uint32_t(before + j) & 1u)) return false;
+        if (!wait_all(&bar->p_full[t], uint32_t(before + j) & 1u)) return false;
         tc_fence_after();
         if (elect_one()) {
           issue_pv(t, v_slot, 1, false);
-          if (j + 1 < nt) { issue_s(t, k_slot); umma_commit(&ctl->s_full[t]); }    // behind P V: may overwrite P
-          else umma_commit(&ctl->o_full[t]);
+          if (j + 1 < nt) { issue_s(t, k_slot); umma_commit(&bar->s_full[t]); }    // behind P V: may overwrite P
+          else umma_commit(&bar->o_full[t]);
         }
         __syncwarp();
         return true;
@@ -588,13 +592,13 @@ ragged_attn_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_consta
         work_done(k);
         const int n0 = w.n0, n1 = w.n1;
         const bool foreign = (w.k0 + n1) * BKEY > w.Lk;   // the last V tile has rows of no key of this sequence
-        if ((n0 > 0 && !wait_all(&ctl->q_ready[0], uint32_t(items0) & 1u)) || !kv_wait(cur)) { ok = false; break; }
+        if ((n0 > 0 && !wait_all(&bar->q_ready[0], uint32_t(items0) & 1u)) || !kv_wait(cur)) { ok = false; break; }
         tc_fence_after();
-        if (n0 > 0 && elect_one()) { issue_s(0, cur.slot); umma_commit(&ctl->s_full[0]); }
+        if (n0 > 0 && elect_one()) { issue_s(0, cur.slot); umma_commit(&bar->s_full[0]); }
         __syncwarp();
-        if (!wait_all(&ctl->q_ready[1], uint32_t(k) & 1u)) { ok = false; break; }
+        if (!wait_all(&bar->q_ready[1], uint32_t(k) & 1u)) { ok = false; break; }
         tc_fence_after();
-        if (elect_one()) { issue_s(1, cur.slot); umma_commit(&ctl->s_full[1]); }
+        if (elect_one()) { issue_s(1, cur.slot); umma_commit(&bar->s_full[1]); }
         __syncwarp();
         cur.next();
         for (int j = 0; j < n1 && ok; ++j) {
@@ -604,8 +608,8 @@ ragged_attn_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_consta
           if (j + 1 < n1) cur.next();
           if (!kv_wait(vc) || (j + 1 < n1 && !kv_wait(kc))) { ok = false; break; }
           if (foreign && j + 1 == n1) {                   // the weights of this step take longer than the clearing
-            if (lane == 0) mbar_arrive(&ctl->v_here);
-            if (!wait_all(&ctl->v_clean, uint32_t(cleans) & 1u)) { ok = false; break; }
+            if (lane == 0) mbar_arrive(&bar->v_here);
+            if (!wait_all(&bar->v_clean, uint32_t(cleans) & 1u)) { ok = false; break; }
           }
           if (j < n0 && !serve(0, j, n0, t0, items0, vc.slot, kc.slot)) { ok = false; break; }
           if (!serve(1, j, n1, t1, k, vc.slot, kc.slot)) { ok = false; break; }
@@ -624,7 +628,7 @@ ragged_attn_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_consta
         work_done(k);
         for (int t = 0; t < 2 && ok; ++t) {
           if (t == 0 && w.n0 == 0) continue;
-          if (!__all_sync(0xffffffffu, bw.wait(&ctl->q_full[t], uint32_t(t == 0 ? items0 : k) & 1u))) { ok = false; break; }
+          if (!__all_sync(0xffffffffu, bw.wait(&bar->q_full[t], uint32_t(t == 0 ? items0 : k) & 1u))) { ok = false; break; }
           if (sc.pow2 != 1.0f) {
             uint4* tile = reinterpret_cast<uint4*>(smem + t * C::TILE_BYTES);
 #pragma unroll 8
@@ -637,7 +641,7 @@ ragged_attn_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_consta
             fence_async_shared();
           }
           __syncwarp();
-          if (lane == 0) mbar_arrive(&ctl->q_ready[t]);
+          if (lane == 0) mbar_arrive(&bar->q_ready[t]);
         }
         if (NORMS) {                                      // beside the first products
           for (int t = 0; t < 2 && ok; ++t) {
@@ -645,8 +649,8 @@ ragged_attn_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_consta
             const float norm = largest_row_norm<D>(smem + t * C::TILE_BYTES, lane);
             if (lane == 0) {
               ctl->q_norm[t][(t == 0 ? items0 : k) & 1] = norm;
-              mbar_arrive(&ctl->q_norm_full[t]);
-              mbar_arrive(&ctl->q_free[t]);               // with the weight warps' words that the last scores are there
+              mbar_arrive(&bar->q_norm_full[t]);
+              mbar_arrive(&bar->q_free[t]);               // with the weight warps' words that the last scores are there
             }
           }
         }
@@ -661,7 +665,7 @@ ragged_attn_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_consta
         work_done(k);
         const int live = max(w.Lk - (w.k0 + w.n1 - 1) * BKEY, 0);
         if (live < BKEY) {
-          if (!__all_sync(0xffffffffu, bw.wait(&ctl->v_here, uint32_t(cleans) & 1u))) { ok = false; break; }
+          if (!__all_sync(0xffffffffu, bw.wait(&bar->v_here, uint32_t(cleans) & 1u))) { ok = false; break; }
           unsigned char* tile = smem + C::KV_OFF + (slot + 2 * w.n1 - 1) % C::NKV * C::TILE_BYTES;
           const uint4 zero = make_uint4(0u, 0u, 0u, 0u);
           for (int pn = 0; pn < C::PANELS; ++pn) {
@@ -670,7 +674,7 @@ ragged_attn_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_consta
           }
           fence_async_shared();
           __syncwarp();
-          if (lane == 0) mbar_arrive(&ctl->v_clean);
+          if (lane == 0) mbar_arrive(&bar->v_clean);
           ++cleans;
         }
         slot = (slot + 2 * w.n1) % C::NKV;
@@ -728,24 +732,24 @@ ragged_attn_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_consta
         shifted = SECOND || __any_sync(0xffffffffu, m_run != 0.f);
         float2 la = make_float2(0.f, 0.f), lb = make_float2(0.f, 0.f);
         for (int j = 0; j < nk && ok; ++j) {
-          if (!__all_sync(0xffffffffu, bw.wait(&ctl->s_full[t], uint32_t(tiles + j) & 1u))) { ok = false; break; }
+          if (!__all_sync(0xffffffffu, bw.wait(&bar->s_full[t], uint32_t(tiles + j) & 1u))) { ok = false; break; }
           tc_fence_after();
           if (releaser) {
             if (t == 1) {
-              if (j > 0) { mbar_arrive(&ctl->kv_empty[rel.slot]); rel.next(); }    // V_{j-1}
-              mbar_arrive(&ctl->kv_empty[rel.slot]); rel.next();                   // K_j
+              if (j > 0) { mbar_arrive(&bar->kv_empty[rel.slot]); rel.next(); }    // V_{j-1}
+              mbar_arrive(&bar->kv_empty[rel.slot]); rel.next();                   // K_j
             }
-            if (!NORMS && j == nk - 1) mbar_arrive(&ctl->q_free[t]);
+            if (!NORMS && j == nk - 1) mbar_arrive(&bar->q_free[t]);
           }
           const int lim = limit - j * BKEY;
           const bool masked = limit0 - j * BKEY < BKEY - 1;                        // uniform over the group
           if (NORMS && j == 0) {
-            if (!__all_sync(0xffffffffu, bw.wait(&ctl->q_norm_full[t], uint32_t(items) & 1u))) { ok = false; break; }
+            if (!__all_sync(0xffffffffu, bw.wait(&bar->q_norm_full[t], uint32_t(items) & 1u))) { ok = false; break; }
             trusted = ctl->q_norm[t][items & 1] < q_limit;
           }
           // Every warp's word that the last scores are there and that it has read the norm: with one warp's word alone the next norm, and the one
           // after, could come while another warp still waits for this one, in an item of one key tile
-          if (NORMS && j == nk - 1 && lane == 0) mbar_arrive(&ctl->q_free[t]);
+          if (NORMS && j == nk - 1 && lane == 0) mbar_arrive(&bar->q_free[t]);
           if (!SECOND && !shifted && !trusted) {
             const float sum = tile_square_sum(s_taddr);   // by all lanes: the loads are the whole warp's
             if (!__all_sync(0xffffffffu, !live || sum <= sc.y_fast * sc.y_fast)) {
@@ -754,7 +758,7 @@ ragged_attn_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_consta
             }
           }
           if (!SECOND && !shifted) {
-            weigh_tile<LOG2N, HILO>(s_taddr, &ctl->p_half[t], &ctl->p_full[t], sc.kappa, p.log2n, lim, masked, la, lb);
+            weigh_tile<LOG2N, HILO>(s_taddr, &bar->p_half[t], &bar->p_full[t], sc.kappa, p.log2n, lim, masked, la, lb);
           } else {
             l += (la.x + la.y) + (lb.x + lb.y);
             la = make_float2(0.f, 0.f); lb = make_float2(0.f, 0.f);
@@ -779,7 +783,7 @@ ragged_attn_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_consta
             }
             if (l > 0.f) l *= alpha;
             m_run = m_new;
-            weigh_tile_shifted<HILO>(s_taddr, &ctl->p_half[t], &ctl->p_full[t], sc.m, rho_any(-m_run) * sc.inv_m, p.log2n, lim, la, lb);
+            weigh_tile_shifted<HILO>(s_taddr, &bar->p_half[t], &bar->p_full[t], sc.m, rho_any(-m_run) * sc.inv_m, p.log2n, lim, la, lb);
           }
         }
         if (!ok) break;
@@ -795,9 +799,9 @@ ragged_attn_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_consta
         if (SECOND) write = live && nk > 0 && (partial ? any_not_finite<D>(dst) : any_not_finite<D>(orow));
         if (dst != nullptr && write) *reinterpret_cast<float4*>(dst + D) = make_float4(nk > 0 && live ? l : 0.f, m_run, 0.f, 0.f);
         if (nk > 0) {
-          if (!__all_sync(0xffffffffu, bw.wait(&ctl->o_full[t], uint32_t(items) & 1u))) { ok = false; break; }
+          if (!__all_sync(0xffffffffu, bw.wait(&bar->o_full[t], uint32_t(items) & 1u))) { ok = false; break; }
           ++items;
-          if (releaser && t == 1) { mbar_arrive(&ctl->kv_empty[rel.slot]); rel.next(); }     // the item's last V tile
+          if (releaser && t == 1) { mbar_arrive(&bar->kv_empty[rel.slot]); rel.next(); }     // the item's last V tile
           tc_fence_after();
           __nv_bfloat16* lrow = HILO ? static_cast<__nv_bfloat16*>(p.o_lo) + (row * p.H + head) * D : nullptr;
           float most = 0.f;                               // largest number of the row, as it is written
@@ -807,7 +811,7 @@ ragged_attn_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_consta
             tmem_ld_32x32(o_taddr + c, o);
             tmem_ld_wait_for(o);
             if (c == D - 32) {                            // O is in registers: the next item may overwrite it
-              warp_arrive(&ctl->o_free[t]);
+              warp_arrive(&bar->o_free[t]);
             }
             if (!partial) {
 #pragma unroll
@@ -861,10 +865,6 @@ ragged_attn_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_consta
     }
   } else if (threadIdx.x == 0) {
     while (ctl->noted < ctl->taken) note();
-    if (ctl->again >= 0) {                              // every load, product and arrival of the first pass has been waited for
-      for (uint64_t* bar = ctl->q_full; bar < ctl->work_empty + RING; ++bar) mbar_inval(bar);
-      init_barriers();
-    }
   }
   if (__syncthreads_or(threadIdx.x == 0 && ctl->abort_flag == 0 && ctl->again >= 0)) run(std::true_type{});
 
