@@ -269,8 +269,10 @@ ALG_API int alg_attn_decode_status(const alg_decode_args* args, int* status, voi
  * o_rest: (tokens, H, D) dense bf16, what the rounding to o left over (the products then carry 16 bits of the weights).
  * A key or value that is NaN or infinite reaches the queries of its own sequence only; among these it may
  * reach earlier ones of the same 128-row tile.
+ * An infinite value makes what the rows that see it get infinite or NaN, by form.
  * status: ALG_DEV_TIMEOUT if a wait of the kernel ran out.  With or without the word, rows of o, stat and o_rest that have no result for
- * it are NaN; so are rows of the gradients, and all of dsink, in the backward, and rows of o over pages.
+ * it are NaN (infinite, perhaps, where they were being weighed again); so are rows of the gradients in the backward, with the dsink of
+ * their head, and rows of o over pages.
  * ---------------------------------------------------------------------------------- */
 typedef struct {
   const void* q;
