@@ -9,7 +9,8 @@
 // heads, v heads in turn), LPR = D / 8 lanes a row, 16 bytes a lane, all loads issued ahead of the walk from the token to its
 // sequence and page, which is the latency to hide: a 32-way search in cu_seqlens (two loads for up to 1024
 // sequences), length, table entry.
-// Measured: 24 prompts of 300 to 2001, 16 heads of 128 (152 MB): 36.9 us, 4.1 TB/s.  Eight rows a warp instead of four 40.1, two 41.9,
+// Measured: 6043 new tokens of 24 sequences, 16 heads of 128 (152 MB): 37.2 us, 4.1 TB/s; a warp lives for one load, one walk and one store, and
+// nothing of the next token is asked for ahead (qk_prep.cu, the same arithmetic without a walk: 5.1 TB/s).  Eight rows a warp instead of four 40.1, two 41.9,
 // eight warps a CTA 41.5; held to fewer registers for 8, 10 or 12 CTAs an SM 37.9, 48, 60.7.
 #include "common.cuh"
 #include "ragged.cuh"

@@ -14,8 +14,8 @@
 //   output   A = the weights straight from the scores' registers, as two bf16 that carry 16 bits of them, B = V through
 //            ldmatrix.trans.  Up to 8 rows: both halves in one product, rows 0-7 and 8-15; up to 16: two products.  More
 //            query heads to a key head go as several groups of 16, which read the keys again, from L2.
-// Measured: four sequences of 20000 to 60001 keys, 16 heads on 2 of 128 (170 MB): 37 us, 4.6 TB/s; 64 sequences of 70 to 4001, 24 heads
-// on 8 of 64 (108 MB): 31.4 us, 3.4 TB/s.  The stream itself goes at 5.3 (head_dim 64) to 6.3 TB/s; some 8 us are launch, line, first tile
+// Measured: four sequences of 22978 to 60001 keys, 16 heads on 2 of 128 (170 MB): 37 us, 4.6 TB/s; 64 sequences of 81 to 4001, 24 heads
+// on 8 of 64 (108 MB): 32 us, 3.4 TB/s.  The stream itself goes at 5.3 (head_dim 64) to 6.3 TB/s; some 8 us are launch, line, first tile
 // and merge.  A head alone takes 1.7 us in its CTA, the latency of a tile and of the warps' meeting: 1024 sequences of 64 keys, 55 us, are bound
 // by that (asking for the next head's q and page numbers ahead of the meeting did not help).
 // Unshifted weights go up to 2^64, and with them the sum of finite values may leave the range.  Where a row of a CTA's stretch comes out infinite
@@ -303,7 +303,7 @@ paged_token_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_consta
 #pragma unroll
         for (int c = 0; c < D / 8; ++c) acc[c][0] = acc[c][1] = acc[c][2] = acc[c][3] = 0.f;
         // weights are (rho(x) rho(-m_ref))^n: unshifted (m_ref = 0) until a score of the warp's rows leaves the range in which that is safe
-        // (|x| <= x_fast keeps them within 2^+-64 and the cancellation of x + sqrt(1 + x^2) below 2e-4), max-shifted from then on
+        // (|x| <= x_fast keeps them within 2^+-64 and the cancellation of x + sqrt(1 + x^2) below 3.3e-4 of a weight), max-shifted from then on
         float m_ref[NR];
         float2 l_part[NR];
 #pragma unroll

@@ -148,8 +148,9 @@ __device__ __forceinline__ float ragged_sink(const float* sink, int head, float 
   return b > 1e30f ? 1e30f : b < -1e30f ? -1e30f : b;
 }
 
-// |x| up to which weights may go unshifted: rho(x)^n <= 2^64, and x + sqrt(1 + x^2) loses no more than n x^2 2^-23 < 2e-4 of a
-// weight to cancellation
+// |x| up to which weights may go unshifted: rho(x)^n <= 2^64, and the cancellation of x + sqrt(1 + x^2) stays small.  At x < 0 the root, off
+// by |x| (2^-22.9 + 2^-25) for the approximate reciprocal root and the rounding of 1 + x^2, leaves rho = 1 / (2 |x|) or more, so that a
+// weight loses 2 n x^2 (2^-22.9 + 2^-25) of itself at most: 3.3e-4, at n = 16
 inline float ragged_fast_range(int n) {
   const double rho = pow(2.0, 64.0 / n), x = 0.5 * (rho - 1.0 / rho);
   return float(x < 8.0 ? x : 8.0);

@@ -12,7 +12,7 @@
 //     Keys past the sequence's end are masked by the causal limit, but 0 times the NaN or infinity that a
 //     foreign V row may hold is NaN: one warp zeroes those rows of a sequence's last V tile in shared memory;
 //   - any scores: a warp takes a tile unshifted where all its |x| <= x_fast (which keeps the weights within 2^+-64 and the
-//     cancellation of y + sqrt(kappa + y^2) below 2e-4).  For packed keys the largest row norms of the call's keys (ragged_plan.cu) and
+//     cancellation of y + sqrt(kappa + y^2) below 3.3e-4 of a weight).  For packed keys the largest row norms of the call's keys (ragged_plan.cu) and
 //     of the item's queries settle that as a rule; else the scores are looked at ahead of their weights: a sum of squares, then the largest.  A
 //     score out of range, or a NaN, sends the warp to the max-shifted form with the cancellation-free rho for the rest of the item;
 //   - values of any size: unshifted weights go up to 2^64 and may take the sum of finite values out of range.  A row that comes out
@@ -21,13 +21,14 @@
 //
 // Roles: warp 0 takes the work and runs the TMA loads, warp 1 issues the MMAs, warp 2 scales Q in shared memory and takes its row norms, warp 3 clears the
 // foreign V rows, warps 4..7 and 8..11 weigh query tile 0 and 1, a thread a row.  An item of one tile runs as tile 1.
-// HILO (training): the weights go to the second product as two bf16 halves and the output is stored as two, since the
-// gradient of the sinks is a float32 sum of what the output's rounding would leave of its digits.
+// HILO (training): the weights go to the second product as two bf16 halves and the output is stored as two, for delta = dO . o, which the
+// backward takes from dP where p has nearly all of a row: with 8 bits of either, dq and dk are off by 0.0029 (normalised rows), 0.0048 (scores four
+// times as large) and 0.0052 (nine times) of their norm against 64 bits, with 16 bits by 0.0024 throughout, which is the rounding of dS.
 //
-// Measured, with the plan ahead: 24 prompts of 17 to 2001 tokens, 16 heads on 4 of 64: 92 us; two of 5000 and 8192, 16 on 2 of 128: 427 us,
-// 948 TFLOP/s; 2048 new tokens on two caches of 20000 and 30001 keys, 16 on 4 of 128: 676 us, 903 TFLOP/s.  No pipe is full (MUFU 37 %,
+// Measured, with the plan ahead: 24 prompts of 19 to 2001 tokens, 16 heads on 4 of 64: 95 us; two of 5623 and 8192, 16 on 2 of 128: 431 us,
+// 937 TFLOP/s; chunks of 620 and 2048 tokens on caches of 24784 and 30001 keys, 16 on 4 of 128: 681 us, 897 TFLOP/s.  No pipe is full (MUFU 37 %,
 // FMA 34 %, tensor 20 % in the first): the chain scores -> weights -> P V -> next scores through tensor memory and barriers is what it
-// waits for; with the weights' arithmetic left out it still takes 72 of 92 us, 356 of 427.
+// waits for; with the weights' arithmetic left out it still took 72 of 92 us, 356 of 427.
 //
 // Every mbarrier wait is bounded; a wait that runs out reports ALG_DEV_TIMEOUT, and the rows of the items that its CTA had not finished, and of those
 // that no CTA had taken by then, are NaN.

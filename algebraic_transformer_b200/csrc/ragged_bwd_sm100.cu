@@ -19,9 +19,9 @@
 //     and l_i = p_sink,i + sum_j p_ij from the weights in fp32, a row's share is p_sink delta / l^2 (l is 1 but for the statistic's last bits),
 //     and blocks' shares are added in a fixed order by the block that arrives last.
 // Bound as the batched backward is: the element-wise phases, a tensor-memory load and an mbarrier between every two products.  Measured
-// with the forward (three sequences of 901 to 4096, 16 heads of 128): 838 us, 510 TFLOP/s of 3.5 times the forward's products, the
-// forward's second half of the weights not counted; of it 5 % are the sinks' sums.  20 sequences of 60 to 1024, 12 heads on 4 of 64: the GPU's
-// part is 140 us, the call's 181 (autograd's host side).
+// with the forward (sequences of 2314, 2770 and 4096, 16 heads of 128): 830 us, 515 TFLOP/s of 3.5 times the forward's products, the
+// forward's second half of the weights not counted; of it 5 % are the sinks' sums.  20 sequences of 72 to 1024, 12 heads on 4 of 64: the GPU's
+// part is 140 us, the call's 176 to 182 (autograd's host side).
 #include "common.cuh"
 #include "ragged.cuh"
 #include "sm100_ptx.cuh"
