@@ -763,10 +763,11 @@ ragged_attn_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_consta
           } else {
             l += (la.x + la.y) + (lb.x + lb.y);
             la = make_float2(0.f, 0.f); lb = make_float2(0.f, 0.f);
-            // the reference moves to the row's largest score so far; with nothing weighed yet it may also fall
+            // the reference moves to the row's largest score so far; with nothing weighed yet it may also fall, to the sink's own where there is
+            // one: at zero, weights of 2^-126 and less would be lost beside a sink's of 2^-64
             const float top = tile_row_max(s_taddr, sc.m, lim);
             float m_new = m_run;
-            if (lim >= 0 && top > -INFINITY) m_new = l > 0.f ? fmaxf(m_run, top) : top;
+            if (lim >= 0 && top > -INFINITY) m_new = j == 0 ? (whole_sink ? fmaxf(ragged_sink(p.sink, head, p.inv_c), top) : top) : l > 0.f ? fmaxf(m_run, top) : top;
             const float alpha = m_new != m_run ? pow2n_rt(rho_any(m_run) * rho_any(-m_new), p.log2n) : 1.0f;
             // O of the earlier tiles is at rest (these scores were issued behind their product): rescale it where a reference moved
             if (__any_sync(0xffffffffu, j > 0 && alpha != 1.0f)) {
