@@ -3,6 +3,7 @@
 import pytest
 import torch
 
+import algebraic_transformer_b200 as A
 from algebraic_transformer_b200 import _lib as L
 import ragged_reference as R
 from test_gpu_packed_attention import make
@@ -69,3 +70,35 @@ def test_paged(H, Hkv, D, single):
                 R.assert_close(o[rows], ref, spread, err)
             first = o.clone()
         assert torch.equal(o, first)
+
+
+def test_replayed_with_values_of_other_sizes():
+    """One captured call, whose values need no second pass, then one, then none."""
+    lens = [700, 3, 2300, 90]
+    q, k, v, sink, cu = make(lens, 4, 2, 64, seed=8, size=3.0)
+    paged = make_paged([20, 1, 60, 7], [400, 30, 2500, 9], 4, 2, 128, 32, seed=9, size=3.0, garbage=False)
+    single = dict(make_paged([1] * 4, [400, 30, 2500, 9], 6, 2, 64, 16, seed=9, size=3.0, garbage=False), cu_seqlens=None)
+
+    def calls():
+        return (A.packed_attention(q, k, v, cu, sink), *A.packed_attention(q, k, v, cu, sink, return_stat=True), A.paged_attention(**paged),
+                A.paged_attention(**single))
+
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        calls()
+    torch.cuda.current_stream().wait_stream(side)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        outs = calls()
+    values = [v, paged["v_pages"], single["v_pages"]]
+    plain = [t.clone() for t in values]
+    for scale in (1.0, 2.0 ** 100, 1.0, 2.0 ** 66):
+        for t, p in zip(values, plain):
+            t.copy_(p * scale)
+        for t in outs:
+            t.fill_(float("nan"))
+        graph.replay()
+        torch.cuda.synchronize()
+        for got, want in zip(outs, calls()):
+            assert torch.isfinite(got).all() and torch.equal(got, want)
